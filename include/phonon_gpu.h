@@ -498,6 +498,96 @@ int pgpu_attention_static(void *stream, const float *q, const pgpu_paged_kv *kv,
                           int streams, int heads, int max_splits, float *out,
                           uint16_t *out_split, int *status);
 
+/* -- 8-bit paged KV cache (pgpu_kv8.hip). A block of 16 positions of one head
+ * holds its keys and its values as whole numbers q in [-127, 127] with one
+ * fp32 scale each: s = max|x| / 127 (fp32 division) rounded up to 12
+ * significant bits, at least 2^-126; q = x / s rounded to nearest, ties to
+ * even; the stored value is q * s (exact). 12 bits make q independent of the
+ * precision it is computed in: (q + 1/2) s is an fp32 number, so x / s is
+ * never rounded onto a tie that x is not on. |x| up to 3.4e38. The block that holds a
+ * stream's newest position stays in fp32 in the stream's open slot, so
+ * nothing is quantised twice and the stored bits do not depend on how rows
+ * were dealt to calls: a block is stored when its 16th row is written, and
+ * its rows stay in the slot until the next block's first row replaces them.
+ * Reads take a stream's newest block from its slot, earlier ones from the
+ * blocks. -- */
+/* Bytes of a (block, head): keys [16 positions][head_dim]; then values
+ * [position / 4][dim % 16][dim / 16][position % 4], the operand order of the
+ * attention's matrix instructions. */
+typedef struct {
+    int8_t *values; /* (dev) [layers][blocks][heads][2][16 * head_dim]; 16-byte aligned */
+    float *scales;  /* (dev) [layers][blocks][heads][keys, values]; 8-byte aligned */
+    float *open;    /* (dev) [layers][slots][heads][2][16][head_dim]; 16-byte aligned */
+    int layers, heads, head_dim; /* heads 1..256; head_dim 64 or 128 */
+    size_t blocks, slots;        /* blocks up to INT32_MAX */
+} pgpu_kv8;
+/* The rows of a call. Stream s has the rows offsets[s] .. offsets[s + 1] - 1
+ * (offsets NULL: row s alone, rows = streams, max_rows = 1), at positions
+ * first[s], first[s] + 1, ...; first[s] < 0: the stream is an empty place of
+ * the batch and is passed over. Its block of positions [16 i, 16 i + 16) is
+ * tables[s * table_stride + i], its open slot slots[s]. Streams of one call
+ * have slots of their own, and blocks that are written are no other stream's.
+ * `max_rows` bounds the rows of a stream and `rows` every row index. A
+ * stream outside its bounds (offsets, table, slot, more than max_rows rows)
+ * is left out, a block id outside the cache likewise, and status bit 2 set. */
+typedef struct {
+    const int32_t *tables;  /* (dev) [streams][table_stride] */
+    int table_stride;
+    const int32_t *slots;   /* (dev) [streams] */
+    const int32_t *first;   /* (dev) [streams] */
+    const int32_t *offsets; /* (dev) [streams + 1] or NULL */
+    int streams;            /* 1..65535 */
+    int rows, max_rows;
+} pgpu_kv8_rows;
+/* Writes rows of keys and values, row r's head h at k[r * row_stride + h *
+ * head_dim] (row_stride a multiple of 4, k and v 16-byte aligned): quantises
+ * the blocks that become full and leaves the newest block's rows in the open
+ * slot. A first row inside a block continues the rows that the slot holds. A
+ * non-finite value sets status bit 1 and makes its block's scale NaN. */
+int pgpu_kv8_write(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,
+                   const float *k, const float *v, size_t row_stride, int *status);
+/* One pass over projected rows [rows][row_stride]: heads * group query heads,
+ * then heads key heads, then heads value heads. Queries and keys are divided
+ * by their head's root mean square (sqrt(mean x^2 + epsilon)) and multiplied
+ * by q_weight / k_weight [head_dim] (NULL: not normalised), and each pair (2i,
+ * 2i + 1) is turned by its position's angle, rope[position][i] = (cos, sin);
+ * in 64 bits, rounded to fp32 once, so that the 8-bit keys do not depend on a
+ * summation order. Queries, times q_scale, go to q_out [rows][heads * group *
+ * head_dim]; keys and values as in pgpu_kv8_write. */
+int pgpu_kv8_rotate_write(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,
+                          const float *qkv, size_t row_stride, int group, const float *q_weight,
+                          const float *k_weight, float epsilon, const float *rope,
+                          int rope_positions, float q_scale, float *q_out, int *status);
+/* Reads rows back as fp32 (the layout of pgpu_kv8_write). lengths[s] (dev):
+ * the positions that stream s holds; a row at or past it sets status bit 2
+ * and leaves its stream out. */
+int pgpu_kv8_read(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,
+                  const int32_t *lengths, float *k, float *v, size_t row_stride, int *status);
+/* For callers that append rows to the open slots themselves (a slot is a
+ * block of a pgpu_paged_kv pool when heads = 8 and head_dim = 64): of every
+ * stream whose newest position positions[s] is its block's last, stores the
+ * slot's 16 rows as block tables[s][positions[s] / 16], in layers
+ * [first_layer, first_layer + layers). positions[s] < 0: passed over. */
+int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer, int layers,
+                   const int32_t *tables, int table_stride, const int32_t *slots,
+                   const int32_t *positions, int streams, int *status);
+/* Causal attention over the cache: row r's query head h (group query heads to
+ * a key head, 1..16; q[r * q_stride + h * head_dim]) attends the keys of
+ * positions 0 .. its own, softmax(scale q k) v, into out[r * out_stride + h *
+ * head_dim]. The cache already holds the call's rows; each stream's newest
+ * position is that of its last row here. One row a stream, or runs of rows.
+ * `max_positions` bounds every position + 1 (a stream past it is left out,
+ * status bit 2). A stream with first < 0 gets zero rows. Strides multiples of
+ * 4, pointers 16-byte aligned. `work` (dev): pgpu_kv8_attention_bytes(kv,
+ * rows, group, max_positions) bytes that no other call uses at the same time;
+ * they need no clearing. */
+size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows, int group,
+                                int max_positions);
+int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,
+                       const float *q, size_t q_stride, int group, float scale,
+                       int max_positions, float *out, size_t out_stride, void *work,
+                       size_t work_bytes, int *status);
+
 /* -- flow head launches (pgpu_head.hip); BF16 matrices -- */
 /* One launch of three independent parts: silu_split = split fragments of
  * SiLU((cond_w . c + cond_bias) + tsum) (tsum optional); if eos_w (16 rows,

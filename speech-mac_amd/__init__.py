@@ -97,6 +97,18 @@ class PgpuAttentionScratch(ctypes.Structure):
     _fields_ = [("part_acc", _vp), ("part_ml", _vp), ("max_streams", _i), ("max_splits", _i)]
 
 
+class PgpuKv8(ctypes.Structure):
+    """pgpu_kv8 (phonon_gpu.h): the 8-bit paged KV cache."""
+    _fields_ = [("values", _vp), ("scales", _vp), ("open", _vp), ("layers", _i), ("heads", _i),
+                ("head_dim", _i), ("blocks", _sz), ("slots", _sz)]
+
+
+class PgpuKv8Rows(ctypes.Structure):
+    """pgpu_kv8_rows (phonon_gpu.h): the rows of a call."""
+    _fields_ = [("tables", _vp), ("table_stride", _i), ("slots", _vp), ("first", _vp),
+                ("offsets", _vp), ("streams", _i), ("rows", _i), ("max_rows", _i)]
+
+
 class PgpuGemmInput(ctypes.Structure):
     _fields_ = [("split", _vp), ("ln_rows", _vp), ("ln_weight", _vp), ("ln_bias", _vp),
                 ("ln_epsilon", _f), ("attn_acc", _vp), ("attn_ml", _vp),
@@ -129,6 +141,8 @@ _mp = ctypes.POINTER(PgpuMatrix)
 _kvp = ctypes.POINTER(PgpuPagedKv)
 _scp = ctypes.POINTER(PgpuAttentionScratch)
 _gip = ctypes.POINTER(PgpuGemmInput)
+_k8p = ctypes.POINTER(PgpuKv8)
+_k8r = ctypes.POINTER(PgpuKv8Rows)
 _pp = ctypes.POINTER(_vp)
 
 # Every function declared in include/*.h: name -> (restype, argtypes).
@@ -343,6 +357,14 @@ EXPORTS = {
                                   _vp, _i]),
     "pgpu_mimi_attention": (_i, [_vp, _vp, _i, ctypes.c_longlong, _vp, _vp, _i, _i, _vp,
                                  _vp]),
+    "pgpu_kv8_write": (_i, [_vp, _k8p, _i, _k8r, _vp, _vp, _sz, _vp]),
+    "pgpu_kv8_rotate_write": (_i, [_vp, _k8p, _i, _k8r, _vp, _sz, _i, _vp, _vp, _f, _vp, _i, _f,
+                                   _vp, _vp]),
+    "pgpu_kv8_read": (_i, [_vp, _k8p, _i, _k8r, _vp, _vp, _vp, _sz, _vp]),
+    "pgpu_kv8_close": (_i, [_vp, _k8p, _i, _i, _vp, _i, _vp, _vp, _i, _vp]),
+    "pgpu_kv8_attention_bytes": (_sz, [_k8p, _k8r, _i, _i]),
+    "pgpu_kv8_attention": (_i, [_vp, _k8p, _i, _k8r, _vp, _sz, _i, _f, _i, _vp, _sz, _vp, _sz,
+                                _vp]),
     "pgpu_head_flow_schedule": (_i, [_vp, _i, _i, _i, _i]),
     "pgpu_head_flow_launch": (_i, [_vp, _vp]),
     "pgpu_head_flow_reset": (_i, [_vp, _vp, _sz, _vp]),
