@@ -369,7 +369,327 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 kv, Kv8Rows rows, const in
 
 // ----------------------------------------------------------------- attention
 
-// One wave per (row, query head), a block of 16 keys at a time: lane l takes
+// The sums are taken on the int8 matrix instruction v_mfma_i32_16x16x64_i8:
+// the cache's bytes are its operands as they are stored, nothing is converted.
+// A query (and the weights of 64 keys) becomes a fixed-point number of 22 to 23
+// bits below its largest element, split into three signed bytes that stand in
+// three rows of the other operand: products and sums are exact, and
+//   (hi * 2^16 + mid * 2^8 + lo) * step
+// has the precision of fp32. Four queries fill the 16 rows (row 4 j + t: byte t
+// of query j); a lone query stands there four times, which costs nothing.
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kKv8Waves = 4;  // 64 keys each
+
+__device__ inline float row16_max(float v) {
+    // v_max of the lane 8, 4, 2, 1 apart within each row of 16.
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                     0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, false)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                     0, __builtin_bit_cast(int, v), 0x124, 0xf, 0xf, false)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                     0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, false)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                     0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, false)));
+    return v;
+}
+
+// Fixed point below `top` (>= 0, the largest magnitude): the power of two that
+// takes it into [2^21, 2^22). Below 2^-105 the step stays at 2^-126.
+__device__ inline int fix_exponent(float top) {
+    return min(126, 148 - (int)(fbits(top) >> 23));
+}
+__device__ inline float power_of_2(int e) { return bitsf((uint32_t)(127 + e) << 23); }
+// The three bytes of the number (bits 0..23), each signed: n = sum of
+// byte t * 256^t, |n| <= 2^22.
+__device__ inline uint32_t fix_bytes(float x, float mul) {
+    return ((uint32_t)(int)rintf(x * mul) + 0x808080u) ^ 0x808080u;
+}
+// Which byte of a number stands in row t of its query: the highest in row 0.
+// Row 3 repeats the lowest byte; nothing reads its sums.
+__device__ inline uint32_t row_byte(int t) { return t < 2 ? 2u - t : 0u; }
+// Byte b of four numbers -> a word; sel = b | (4 + b) << 8.
+__device__ inline uint32_t pick4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t sel) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, sel),
+                                 __builtin_amdgcn_perm(b, a, sel), 0x05040100u);
+}
+__device__ inline float fix_sum(i32x4 c) {
+    return fmaf((float)(c.x * 256 + c.y), 256.0f, (float)c.z);
+}
+
+template <int P>
+__device__ inline uint32_t quad_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, P * 0x55, 0xf, 0xf, false);
+}
+
+__device__ inline i32x4 stream_load16(const int8_t *p) {
+    return __builtin_nontemporal_load((const i32x4 *)p);
+}
+
+// LDS between the lanes of one wave: nothing is moved across it.
+__device__ inline void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+struct Kv8Decode {
+    const float *q;
+    size_t q_stride;
+    int group;
+    float scale;  // of the scores, times log2 e
+    int max_positions, splits;
+    float *part_acc, *part_ml;  // slot (row * query heads + head) * splits + split
+    float *out;                 // splits = 1: the rows themselves (else NULL)
+    size_t out_stride;
+};
+
+template <int D>
+struct Kv8DecodeShared {
+    __align__(16) uint32_t digits[kKv8Waves][16][16];  // [row][group of lanes, block]
+    __align__(16) float own[kKv8Waves][4][16];         // weights of the newest block
+    float acc[kKv8Waves][4][D];
+    float m[kKv8Waves][4], l[kKv8Waves][4];
+};
+
+// One row a stream. A work-group takes 256 keys of one (stream, key head), a
+// wave 64 of them: 4 blocks, whose bytes it requests together (8 or 16 KB),
+// then passes over 4 queries of the group at a time. Bound by the cache's
+// bytes; no wave waits for another before the joint of the four.
+template <int D>
+__global__ __launch_bounds__(64 * kKv8Waves) void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a,
+                                                               int *status) {
+    constexpr int KB = D / 64, T = D / 16;
+    __shared__ Kv8DecodeShared<D> sh;
+    const int head = blockIdx.x, split = blockIdx.y, s = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
+    const int b0 = (split * kKv8Waves + wave) * 4;
+    int ids[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+        ids[t] = rows.tables[(size_t)s * rows.table_stride + min(b0 + t, rows.table_stride - 1)];
+    const Kv8Span span = kv8_span(kv, rows, s, a.max_positions,
+                                  threadIdx.x == 0 && head == 0 && split == 0, status);
+    const int width = kv.heads * a.group;  // query heads
+    const int p = span.first;
+    if (!span.live) {
+        if (a.out && p < 0 && span.count > 0)
+            for (int e = threadIdx.x; e < a.group * D; e += 64 * kKv8Waves)
+                a.out[(size_t)s * a.out_stride + (size_t)head * a.group * D + e] = 0.0f;
+        return;
+    }
+    if (split * 256 > p) return;
+    const int newest = p / kBlockPos, closed = min(max(newest - b0, 0), 4);
+    const int own = newest - b0;  // 0..3: the newest block is this wave's
+    const bool mine = own >= 0 && own < 4;
+
+    i32x4 kr[4][KB], vr[4][KB];
+    float2 sc[4];
+    bool wild = false;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        if (t < closed) {
+            wild |= (unsigned)ids[t] >= kv.blocks;
+            const unsigned id = (unsigned)ids[t] < kv.blocks ? (unsigned)ids[t] : 0u;
+            const int8_t *tile = kv.values + kv8_tile<D>(kv, id, head);
+            sc[t] = *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
+#pragma unroll
+            for (int n = 0; n < KB; n++) kr[t][n] = stream_load16(tile + i * D + n * 64 + g * 16);
+#pragma unroll
+            for (int n = 0; n < KB; n++)
+                vr[t][n] = stream_load16(tile + kBlockPos * D + lane * (D / 4) + n * 16);
+        } else {
+            sc[t] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int n = 0; n < KB; n++) kr[t][n] = vr[t][n] = i32x4{0, 0, 0, 0};
+        }
+    }
+    if (wild && lane == 0) atomicOr(status, 2);
+    const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
+
+    for (int j0 = 0; j0 < a.group; j0 += 4) {
+        // Row i of the operand: byte i % 4 of query j0 + i / 4.
+        const float *q = a.q + (size_t)s * a.q_stride +
+                         ((size_t)head * a.group + min(j0 + (i >> 2), a.group - 1)) * D;
+        float4 x[KB][4];
+        float top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < KB; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float4 v = *(const float4 *)(q + n * 64 + g * 16 + k * 4);
+                x[n][k] = v;
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
+                                       fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
+        top = xor16_32_max(top);
+        const int e = fix_exponent(top);
+        const float mul = power_of_2(e);
+        const uint32_t byte = row_byte(i & 3), sel = byte | (4u + byte) << 8;
+        i32x4 qd[KB];
+#pragma unroll
+        for (int n = 0; n < KB; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                qd[n][k] = (int)pick4(fix_bytes(x[n][k].x, mul), fix_bytes(x[n][k].y, mul),
+                                      fix_bytes(x[n][k].z, mul), fix_bytes(x[n][k].w, mul), sel);
+        // From here on this lane's query is j0 + g (rows 4 g .. 4 g + 3).
+        const float step = __shfl(a.scale * power_of_2(-e), g * 4);
+
+        // Scores, in units of log 2: lane (g, i) key i of each block.
+        float score[4], m = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            i32x4 c = {0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < KB; n++)
+                c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[n], kr[t][n], c, 0, 0, 0);
+            score[t] = t < closed ? fix_sum(c) * (step * sc[t].x) : -INFINITY;
+        }
+        if (mine) {
+            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < KB; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float4 y = *(const float4 *)(slot + i * D + n * 64 + g * 16 + k * 4);
+                    const float4 v = (i & 3) ? make_float4(0.f, 0.f, 0.f, 0.f) : x[n][k];
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x, y.x, c, 0, 0, 0);
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.y, y.y, c, 0, 0, 0);
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, y.z, c, 0, 0, 0);
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, y.w, c, 0, 0, 0);
+                }
+            const float v = newest * kBlockPos + i <= p ? c.x * a.scale : -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                if (t == own) score[t] = v;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) m = fmaxf(m, score[t]);
+        m = row16_max(m);
+        float w[4], l = 0.0f, last = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            w[t] = score[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(score[t] - m);
+            l += w[t];
+            if (mine && t == own) last = w[t];
+        }
+        l = row16_sum(l);
+
+        // The weights times their blocks' value scales, in fixed point below
+        // the largest of the query's 64; byte t of four keys in a row's word.
+        float big = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            w[t] *= sc[t].y;
+            big = fmaxf(big, w[t]);
+        }
+        const int f = fix_exponent(row16_max(big));
+        const float mul2 = power_of_2(f), back = power_of_2(-f);
+        i32x4 word;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint32_t u = fix_bytes(w[t], mul2);
+            word[t] = (int)pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u),
+                                 quad_lane<3>(u), sel);
+        }
+        *(i32x4 *)&sh.digits[wave][g * 4 + (i & 3)][(i >> 2) * 4] = word;
+        if (mine) sh.own[wave][g][i] = last;
+        wave_lds_fence();
+        const i32x4 pd = *(const i32x4 *)&sh.digits[wave][i][g * 4];
+        float acc[T];
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const i32x4 v = {vr[0][t / 4][t % 4], vr[1][t / 4][t % 4], vr[2][t / 4][t % 4],
+                             vr[3][t / 4][t % 4]};
+            const i32x4 c =
+                __builtin_amdgcn_mfma_i32_16x16x64_i8(pd, v, i32x4{0, 0, 0, 0}, 0, 0, 0);
+            acc[t] = fix_sum(c) * back;
+        }
+        if (mine) {
+            float4 y = *(const float4 *)&sh.own[wave][i >> 2][g * 4];
+            if (i & 3) y = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float wk[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    // Rows past the position may hold anything.
+                    const bool in = newest * kBlockPos + g * 4 + k <= p;
+                    const float v = slot[kBlockPos * D + (g * 4 + k) * D + t * 16 + i];
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(wk[k], in ? v : 0.0f, c, 0, 0, 0);
+                }
+                acc[t] += c.x;
+            }
+        }
+        const int live = min(4, a.group - j0);  // queries of this pass
+        if (g < live) {
+#pragma unroll
+            for (int t = 0; t < T; t++) sh.acc[wave][g][t * 16 + i] = acc[t];
+            if (i == 0) {
+                sh.m[wave][g] = m;
+                sh.l[wave][g] = l;
+            }
+        }
+        bool bad = !(top < INFINITY);
+        __syncthreads();
+        for (int e2 = threadIdx.x; e2 < live * D; e2 += 64 * kKv8Waves) {
+            const int j = e2 / D, d = e2 % D;
+            float mx = -INFINITY;
+            for (int n = 0; n < kKv8Waves; n++) mx = fmaxf(mx, sh.m[n][j]);
+            float total = 0.0f, o = 0.0f;
+            for (int n = 0; n < kKv8Waves; n++) {
+                if (sh.l[n][j] == 0.0f) continue;  // a wave past the context
+                const float c = __builtin_amdgcn_exp2f(sh.m[n][j] - mx);
+                total = fmaf(sh.l[n][j], c, total);
+                o = fmaf(sh.acc[n][j][d], c, o);
+            }
+            const size_t qh = (size_t)head * a.group + j0 + j;
+            if (a.out) {
+                o = o / total;
+                a.out[(size_t)s * a.out_stride + qh * D + d] = o;
+                bad |= !isfinite(o);
+            } else {
+                const size_t at = ((size_t)s * width + qh) * a.splits + split;
+                a.part_acc[at * D + d] = o;
+                if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(mx, total);
+            }
+        }
+        flag_nonfinite(status, bad);
+        __syncthreads();
+    }
+}
+
+// The splits of a row's query head joined, one wave for 64 dims.
+template <int D>
+__global__ __launch_bounds__(64) void k_kv8_join(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
+    const int s = blockIdx.z, qh = blockIdx.y, d = blockIdx.x * 64 + threadIdx.x;
+    const Kv8Span span = kv8_span(kv, rows, s, a.max_positions, false, status);
+    if (span.count == 0 || (!span.live && span.first >= 0)) return;
+    float *dst = a.out + (size_t)s * a.out_stride + (size_t)qh * D + d;
+    if (!span.live) {
+        *dst = 0.0f;
+        return;
+    }
+    const int n = span.first / 256 + 1;
+    const size_t at = ((size_t)s * kv.heads * a.group + qh) * a.splits;
+    float mx = -INFINITY;
+    for (int j = 0; j < n; j++) mx = fmaxf(mx, a.part_ml[(at + j) * 2]);
+    float total = 0.0f, o = 0.0f;
+    for (int j = 0; j < n; j++) {
+        const float c = __builtin_amdgcn_exp2f(a.part_ml[(at + j) * 2] - mx);
+        total = fmaf(a.part_ml[(at + j) * 2 + 1], c, total);
+        o = fmaf(a.part_acc[(at + j) * D + d], c, o);
+    }
+    o = o / total;
+    *dst = o;
+    flag_nonfinite(status, !isfinite(o));
+}
+
+// Runs of rows: one wave per (row, query head), a block of 16 keys at a time: lane l takes
 // key l % 16 and the quarter l / 16 of the dims for the score, then dims l
 // (and l + 64) of the values.
 template <int D>
@@ -589,8 +909,19 @@ extern "C" int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer,
     return launch_ok("pgpu_kv8_close");
 }
 
-extern "C" size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *, const pgpu_kv8_rows *, int, int) {
-    return 0;
+namespace {
+
+// Splits of 256 keys that positions below max_positions lie in.
+int splits_of(int max_positions) { return (max_positions - 1) / 256 + 1; }
+
+}  // namespace
+
+extern "C" size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows,
+                                           int group, int max_positions) {
+    if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
+    if (rows->offsets || splits_of(max_positions) == 1) return 0;
+    return (size_t)rows->rows * kv->heads * group * splits_of(max_positions) *
+           (kv->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
@@ -605,14 +936,50 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
         out_stride < width || max_positions <= 0 || !__builtin_isfinite(scale))
         return bad_arguments("pgpu_kv8_attention");
     if (rows->rows == 0) return 1;
-    const dim3 grid(rows->max_rows, kv->heads * group, rows->streams);
+    const size_t need = pgpu_kv8_attention_bytes(kv, rows, group, max_positions);
+    if (need && (!work || !aligned(work, 16) || work_bytes < need))
+        return bad_arguments("pgpu_kv8_attention (workspace)");
+    const Kv8 c = layer_of(kv, layer);
+    const Kv8Rows r = rows_of(rows);
+    const int wide = kv->heads * group;
+    if (rows->offsets) {
+        const dim3 grid(rows->max_rows, wide, rows->streams);
+        if (kv->head_dim == 64)
+            hipLaunchKernelGGL(k_kv8_attend<64>, grid, dim3(64), 0, (hipStream_t)stream, c, r, q,
+                               q_stride, group, scale, max_positions, out, out_stride, status);
+        else
+            hipLaunchKernelGGL(k_kv8_attend<128>, grid, dim3(64), 0, (hipStream_t)stream, c, r, q,
+                               q_stride, group, scale, max_positions, out, out_stride, status);
+        return launch_ok("pgpu_kv8_attention");
+    }
+    const int splits = splits_of(max_positions);
+    const size_t parts = (size_t)rows->rows * wide * splits;
+    Kv8Decode a = {};
+    a.q = q;
+    a.q_stride = q_stride;
+    a.group = group;
+    a.scale = scale * 1.44269504f;
+    a.max_positions = max_positions;
+    a.splits = splits;
+    a.part_acc = (float *)work;
+    a.part_ml = (float *)work + parts * kv->head_dim;
+    a.out = splits == 1 ? out : nullptr;
+    a.out_stride = out_stride;
+    const dim3 grid(kv->heads, splits, rows->streams), joint(kv->head_dim / 64, wide, rows->streams);
     if (kv->head_dim == 64)
-        hipLaunchKernelGGL(k_kv8_attend<64>, grid, dim3(64), 0, (hipStream_t)stream,
-                           layer_of(kv, layer), rows_of(rows), q, q_stride, group, scale,
-                           max_positions, out, out_stride, status);
+        hipLaunchKernelGGL(k_kv8_decode<64>, grid, dim3(64 * kKv8Waves), 0, (hipStream_t)stream, c,
+                           r, a, status);
     else
-        hipLaunchKernelGGL(k_kv8_attend<128>, grid, dim3(64), 0, (hipStream_t)stream,
-                           layer_of(kv, layer), rows_of(rows), q, q_stride, group, scale,
-                           max_positions, out, out_stride, status);
+        hipLaunchKernelGGL(k_kv8_decode<128>, grid, dim3(64 * kKv8Waves), 0, (hipStream_t)stream,
+                           c, r, a, status);
+    if (!launch_ok("pgpu_kv8_attention")) return 0;
+    if (splits == 1) return 1;
+    a.out = out;
+    if (kv->head_dim == 64)
+        hipLaunchKernelGGL(k_kv8_join<64>, joint, dim3(64), 0, (hipStream_t)stream, c, r, a,
+                           status);
+    else
+        hipLaunchKernelGGL(k_kv8_join<128>, joint, dim3(64), 0, (hipStream_t)stream, c, r, a,
+                           status);
     return launch_ok("pgpu_kv8_attention");
 }
