@@ -1,6 +1,8 @@
 // 8-bit paged KV cache: quantised writes (with the heads' norm and rotation in
 // the same pass), reads, and causal attention over it. The formats and the
 // rules of the stored values are in phonon_gpu.h.
+#include <type_traits>
+
 #include "pgpu_common.hpp"
 #include "phonon_gpu.h"
 
@@ -663,109 +665,377 @@ __global__ __launch_bounds__(64 * kKv8Waves) void k_kv8_decode(Kv8 kv, Kv8Rows r
     }
 }
 
-// The splits of a row's query head joined, one wave for 64 dims.
+// Runs of rows: a work-group of 4 waves takes 4 tiles of 16 rows of one query
+// head each (the query heads of a key head side by side), and passes over the
+// keys 64 at a time: each wave turns one block's bytes into fp16 (exact) in
+// LDS, where all four read them, while the next 64 keys' bytes are on their
+// way. Scores are taken keys by rows (K Q^T), so that a lane holds 16 of its
+// row's scores and the weights are the next product's operand as they stand
+// (O^T = V^T P^T). A query and a weight are two fp16 terms (22 bits), each
+// product with the cache's whole numbers exact in fp32. The running maximum is
+// a whole number (in units of log 2), so that rescaling is exact and rare; the
+// weights carry their block's value scale relative to 2^unit, the largest power
+// of two below a scale so far, and 2^14 to keep their low terms normal.
+struct Kv8Run {
+    const float *q;
+    size_t q_stride;
+    int group;
+    float scale;  // of the scores, times log2 e
+    int max_positions, splits, chunks;  // 64-key chunks of a split
+    float *part_acc, *part_ml;
+    float *out;  // splits = 1: the rows themselves
+    size_t out_stride;
+};
+
 template <int D>
-__global__ __launch_bounds__(64) void k_kv8_join(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
-    const int s = blockIdx.z, qh = blockIdx.y, d = blockIdx.x * 64 + threadIdx.x;
-    const Kv8Span span = kv8_span(kv, rows, s, a.max_positions, false, status);
-    if (span.count == 0 || (!span.live && span.first >= 0)) return;
-    float *dst = a.out + (size_t)s * a.out_stride + (size_t)qh * D + d;
+struct Kv8RunShared {
+    f16x8 k[2][4][D / 32][64];      // [buffer][block][step][lane]
+    f16x8 v[2][2][D / 16][64];      // [buffer][pair of blocks][16 dims][lane]
+    float2 scale[2][4];
+};
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+// Four signed bytes -> fp16: 0x6400 | (byte ^ 0x80) is 1152 + byte.
+__device__ inline f16x4 bytes_f16(int x) {
+    const uint32_t u = (uint32_t)x ^ 0x80808080u;
+    const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off;
+    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
+    return f16x4{a.x, a.y, b.x, b.y};
+}
+
+// x -> two fp16 terms, both truncated: hi + lo has 22 bits of it.
+__device__ inline void split_pair(float x, float y, f16x2 &hi, f16x2 &lo) {
+    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.0f, x),
+                                                              fmaf((float)hi.y, -1.0f, y)));
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a, int *status) {
+    constexpr int KB = D / 64, KS = D / 32, T = D / 16;
+    constexpr float kNone = -3.0e38f;  // the maximum of no scores
+    __shared__ Kv8RunShared<D> sh;
+    const int s = blockIdx.z, head = blockIdx.y % kv.heads, split = blockIdx.y / kv.heads;
+    const int bx = gridDim.x - 1 - blockIdx.x;  // the longest rows first
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
+    const Kv8Span span = kv8_span(kv, rows, s, a.max_positions,
+                                  threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+    const int tiles = (span.count + 15) / 16 * a.group;
+    if (bx * 4 >= tiles) return;
+    const int tile = bx * 4 + wave, r0 = tile / a.group * 16;
+    const int qh = head * a.group + tile % a.group;
+    const int live = tile < tiles ? min(16, span.count - r0) : 0;  // rows of this wave
+    const size_t row = (size_t)(span.row0 + (live > 0 ? r0 + min(i, live - 1) : 0));
+    if (!span.live) {
+        if (span.first < 0 && split == 0 && i < live) {
+            float *dst = a.out + row * a.out_stride + (size_t)qh * D;
+            for (int t = 0; t < T; t++)
+                *(float4 *)(dst + t * 16 + g * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        return;
+    }
+    const int end = span.first + span.count, newest = (end - 1) / kBlockPos;
+    const int top = span.first + min(span.count, ((min(bx * 4 + 3, tiles - 1)) / a.group + 1) * 16) - 1;
+    const int keys = min(newest * kBlockPos, top + 1);  // of blocks, to be seen by some row here
+    const int c0 = split * a.chunks, c1 = min(c0 + a.chunks, (keys + 63) / 64);
+    const bool last_split = newest / 4 >= c0 && newest / 4 < c0 + a.chunks;
+    if (c0 * 64 > top) return;
+    const int p0 = span.first + r0, p = i < live ? p0 + i : -1;  // this lane's row
+    const int wave_top = p0 + live - 1;
+    const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
+
+    // The wave's queries, two terms, scaled to a largest element in [2^14, 2^15).
+    const float *q = a.q + row * a.q_stride + (size_t)qh * D;
+    f16x8 qhi[KS], qlo[KS];
+    float qs, biggest = 0.0f;
+    {
+        float4 x[KB][4];
+#pragma unroll
+        for (int n = 0; n < KB; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float4 v = *(const float4 *)(q + n * 64 + g * 16 + k * 4);
+                x[n][k] = v;
+                biggest = fmaxf(biggest, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
+                                               fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
+        biggest = xor16_32_max(biggest);
+        const int e = min(126, 141 - (int)(fbits(biggest) >> 23));
+        const float mul = copysignf(power_of_2(e), a.scale);
+        qs = fabsf(a.scale) * power_of_2(-e);
+#pragma unroll
+        for (int n = 0; n < KB; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                f16x2 h0, l0, h1, l1;
+                split_pair(x[n][k].x * mul, x[n][k].y * mul, h0, l0);
+                split_pair(x[n][k].z * mul, x[n][k].w * mul, h1, l1);
+                const int ks = n * 2 + k / 2, o = k % 2 * 4;
+                qhi[ks][o] = h0.x, qhi[ks][o + 1] = h0.y, qhi[ks][o + 2] = h1.x, qhi[ks][o + 3] = h1.y;
+                qlo[ks][o] = l0.x, qlo[ks][o + 1] = l0.y, qlo[ks][o + 2] = l1.x, qlo[ks][o + 3] = l1.y;
+            }
+    }
+
+    // Block 4 c + wave of chunk c: requested, then turned into LDS.
+    i32x4 kr[KB], vr[KB];
+    float2 sc;
+    bool wild = false;
+    const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
+    auto request = [&](int c) {
+        const int b = c * 4 + wave;
+        if (b * kBlockPos < keys) {
+            const int raw = table[b];
+            wild |= (unsigned)raw >= kv.blocks;
+            const unsigned id = (unsigned)raw < kv.blocks ? (unsigned)raw : 0u;
+            const int8_t *tl = kv.values + kv8_tile<D>(kv, id, head);
+            sc = *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
+#pragma unroll
+            for (int n = 0; n < KB; n++) {
+                kr[n] = *(const i32x4 *)(tl + i * D + n * 64 + g * 16);
+                vr[n] = *(const i32x4 *)(tl + kBlockPos * D + lane * (D / 4) + n * 16);
+            }
+        } else {
+            sc = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int n = 0; n < KB; n++) kr[n] = vr[n] = i32x4{0, 0, 0, 0};
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int n = 0; n < KB; n++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const f16x4 x = bytes_f16(kr[n][k * 2]), y = bytes_f16(kr[n][k * 2 + 1]);
+                sh.k[buf][wave][n * 2 + k][lane] =
+                    __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            *((f16x4 *)&sh.v[buf][wave >> 1][t][lane] + (wave & 1)) =
+                bytes_f16(vr[t / 4][t % 4]);
+        if (lane == 0) sh.scale[buf][wave] = sc;
+    };
+
+    float m = kNone, l = 0.0f;  // l: of this lane's keys
+    f32x4 acc[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int unit = -100;  // acc holds the values' sums / 2^(unit - 14)
+
+    auto attend = [&](int buf, int c, auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        float2 bs[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) bs[t] = sh.scale[buf][t];
+        f32x4 w[4];
+        float mx = kNone;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const f16x8 kk = sh.k[buf][t][k][lane];
+                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qhi[k], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qlo[k], x, 0, 0, 0);
+            }
+            const float f = bs[t].x * qs;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                w[t][r] = x[r] * f;
+                if (MASK) {
+                    const int key = c * 64 + t * 16 + g * 4 + r;
+                    w[t][r] = key <= p && key < keys ? w[t][r] : -INFINITY;
+                }
+                mx = fmaxf(mx, w[t][r]);
+            }
+        }
+        mx = xor16_32_max(mx);
+        // A whole number; not below the last one.
+        const float mn = fmaxf(m, ceilf(mx));
+        int up = unit;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {  // NaN (a block that was not finite) does not count
+            const int n = (int)(fbits(bs[t].y) >> 23) - 127;
+            up = max(up, n < 128 ? n : -100);
+        }
+        up = __builtin_amdgcn_readfirstlane(up);
+        if (up != unit || __any(mn != m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - mn);
+            l *= shrink;
+            const float both = shrink * __builtin_amdgcn_exp2f((float)(unit - up));
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[t][r] *= both;
+            m = mn;
+            unit = up;
+        }
+        f16x8 hi[2], lo[2];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            // 2^(14 - unit) times the scale: below 2^15.
+            const float f = ldexpf(bs[t].y, 14 - unit);
+            float x[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float e = __builtin_amdgcn_exp2f(w[t][r] - m);
+                l += e;
+                x[r] = e * f;
+                if (MASK) x[r] = w[t][r] == -INFINITY ? 0.0f : x[r];
+            }
+            f16x2 h0, l0, h1, l1;
+            split_pair(x[0], x[1], h0, l0);
+            split_pair(x[2], x[3], h1, l1);
+            const int o = t % 2 * 4;
+            hi[t / 2][o] = h0.x, hi[t / 2][o + 1] = h0.y, hi[t / 2][o + 2] = h1.x, hi[t / 2][o + 3] = h1.y;
+            lo[t / 2][o] = l0.x, lo[t / 2][o + 1] = l0.y, lo[t / 2][o + 2] = l1.x, lo[t / 2][o + 3] = l1.y;
+        }
+#pragma unroll
+        for (int t = 0; t < T; t++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const f16x8 v = sh.v[buf][n][t][lane];
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[n], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[n], acc[t], 0, 0, 0);
+            }
+    };
+
+    if (c0 < c1) {
+        request(c0);
+        stage(0);
+        __syncthreads();
+        for (int c = c0; c < c1; c++) {
+            const int buf = (c - c0) & 1;
+            if (c + 1 < c1) request(c + 1);
+            if (live > 0 && c * 64 <= wave_top) {
+                if (c * 64 + 63 <= p0 && c * 64 + 64 <= keys && live == 16)
+                    attend(buf, c, std::false_type{});
+                else
+                    attend(buf, c, std::true_type{});
+            }
+            if (c + 1 < c1) stage(buf ^ 1);
+            __syncthreads();
+        }
+    }
+    if (wild && lane == 0) atomicOr(status, 2);
+    if (live == 0) return;
+
+    // The newest block, in fp32 on the fp32 matrix instruction.
+    const float back = __builtin_amdgcn_exp2f((float)(unit - 14));
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[t][r] *= back;
+    if (last_split && wave_top >= newest * kBlockPos) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < KB; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float4 y = *(const float4 *)(slot + i * D + n * 64 + g * 16 + k * 4);
+                const float4 z = *(const float4 *)(q + n * 64 + g * 16 + k * 4);
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(y.x, z.x, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(y.y, z.y, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(y.z, z.z, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(y.w, z.w, x, 0, 0, 0);
+            }
+        // Values [key 4 g + r][16 t + i]; rows past the last may hold anything.
+        // A value that is not finite makes its key's weight NaN for the rows that
+        // see it, and is left out of the product, where it would reach all rows.
+        float v[T][4];
+        uint32_t odd = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const bool in = newest * kBlockPos + g * 4 + r < end;
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                const float y = slot[kBlockPos * D + (g * 4 + r) * D + t * 16 + i];
+                const bool fine = isfinite(y);
+                v[t][r] = in && fine ? y : 0.0f;
+                if (in && !fine) odd |= 1u << r;
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) odd |= (uint32_t)__shfl_xor((int)odd, o);
+        float mx = kNone;
+        f32x4 w;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            w[r] = newest * kBlockPos + g * 4 + r <= p ? x[r] * a.scale : -INFINITY;
+            mx = fmaxf(mx, w[r]);
+        }
+        mx = xor16_32_max(mx);
+        // The last maximum as it is: a row of one key gets that key's value.
+        const float mn = fmaxf(m, mx), shrink = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= shrink;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const bool seen = w[r] != -INFINITY;
+            w[r] = seen ? __builtin_amdgcn_exp2f(w[r] - m) : 0.0f;
+            if (seen && (odd >> r & 1)) w[r] = __builtin_nanf("");
+            l += w[r];
+        }
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[t][r] *= shrink;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][r], w[r], acc[t], 0, 0, 0);
+        }
+    }
+    l = xor16_32_sum(l);
+    bool bad = false;
+    if (i < live) {
+        const size_t at = (row * kv.heads * a.group + qh) * a.splits + split;
+        float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
+        const float f = a.splits == 1 ? 1.0f / l : 1.0f;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const float4 o = make_float4(acc[t][0] * f, acc[t][1] * f, acc[t][2] * f, acc[t][3] * f);
+            bad |= !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w));
+            *(float4 *)(dst + t * 16 + g * 4) = o;
+        }
+        if (a.splits > 1 && g == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(m, l);
+        bad |= !(biggest < INFINITY);
+    }
+    flag_nonfinite(status, bad);
+}
+
+// The splits of a row's query head joined, one wave for 64 dims. `keys`: of a split.
+template <int D>
+__global__ __launch_bounds__(64) void k_kv8_join(Kv8 kv, Kv8Rows rows, const float *part_acc,
+                                                 const float *part_ml, int group,
+                                                 int max_positions, int splits, int keys,
+                                                 float *out, size_t out_stride, int *status) {
+    const int s = blockIdx.z, i = blockIdx.y, qh = blockIdx.x / (D / 64);
+    const int d = blockIdx.x % (D / 64) * 64 + threadIdx.x;
+    const Kv8Span span = kv8_span(kv, rows, s, max_positions, false, status);
+    if (i >= span.count || (!span.live && span.first >= 0)) return;
+    const size_t row = (size_t)(span.row0 + i);
+    float *dst = out + row * out_stride + (size_t)qh * D + d;
     if (!span.live) {
         *dst = 0.0f;
         return;
     }
-    const int n = span.first / 256 + 1;
-    const size_t at = ((size_t)s * kv.heads * a.group + qh) * a.splits;
+    const int n = (span.first + i) / keys + 1;
+    const size_t at = (row * kv.heads * group + qh) * splits;
     float mx = -INFINITY;
-    for (int j = 0; j < n; j++) mx = fmaxf(mx, a.part_ml[(at + j) * 2]);
+    for (int j = 0; j < n; j++) mx = fmaxf(mx, part_ml[(at + j) * 2]);
     float total = 0.0f, o = 0.0f;
     for (int j = 0; j < n; j++) {
-        const float c = __builtin_amdgcn_exp2f(a.part_ml[(at + j) * 2] - mx);
-        total = fmaf(a.part_ml[(at + j) * 2 + 1], c, total);
-        o = fmaf(a.part_acc[(at + j) * D + d], c, o);
+        const float c = __builtin_amdgcn_exp2f(part_ml[(at + j) * 2] - mx);
+        total = fmaf(part_ml[(at + j) * 2 + 1], c, total);
+        o = fmaf(part_acc[(at + j) * D + d], c, o);
     }
     o = o / total;
     *dst = o;
     flag_nonfinite(status, !isfinite(o));
-}
-
-// Runs of rows: one wave per (row, query head), a block of 16 keys at a time: lane l takes
-// key l % 16 and the quarter l / 16 of the dims for the score, then dims l
-// (and l + 64) of the values.
-template <int D>
-__global__ __launch_bounds__(64) void k_kv8_attend(Kv8 kv, Kv8Rows rows, const float *q,
-                                                   size_t q_stride, int group, float scale,
-                                                   int max_positions, float *out,
-                                                   size_t out_stride, int *status) {
-    constexpr int N = D / 64;
-    const int s = blockIdx.z, qh = blockIdx.y, i = blockIdx.x, lane = threadIdx.x;
-    const Kv8Span span = kv8_span(kv, rows, s, max_positions,
-                                  lane == 0 && i == 0 && qh == 0, status);
-    if (i >= span.count) return;
-    const size_t row = (size_t)(span.row0 + i);
-    float *dst = out + row * out_stride + qh * D + lane;
-    if (!span.live) {
-        if (span.first < 0)
-            for (int n = 0; n < N; n++) dst[n * 64] = 0.0f;
-        return;
-    }
-    const int head = qh / group, key = lane & 15, part = lane >> 4;
-    const int p = span.first + i, newest = (span.first + span.count - 1) / kBlockPos;
-    const float *qr = q + row * q_stride + qh * D + part * (D / 4);
-    float w[D / 4];
-#pragma unroll
-    for (int d = 0; d < D / 4; d++) w[d] = qr[d] * scale;
-    float m = -INFINITY, l = 0.0f, acc[N] = {};
-    for (int b = 0; b <= p / kBlockPos; b++) {
-        float dot = 0.0f, val[N][kBlockPos];
-        if (b == newest) {
-            const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) *
-                                              (2 * kBlockPos * D);
-            for (int d = 0; d < D / 4; d++)
-                dot = fmaf(w[d], slot[key * D + part * (D / 4) + d], dot);
-            for (int n = 0; n < N; n++)
-                for (int j = 0; j < kBlockPos; j++)
-                    val[n][j] = slot[kBlockPos * D + j * D + n * 64 + lane];
-        } else {
-            const int id = rows.tables[(size_t)s * rows.table_stride + b];
-            if ((unsigned)id >= kv.blocks) {
-                if (lane == 0) atomicOr(status, 2);
-                return;
-            }
-            const int8_t *tile = kv.values + kv8_tile<D>(kv, (unsigned)id, head);
-            const float2 sc =
-                *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
-            for (int d = 0; d < D / 4; d++)
-                dot = fmaf(w[d], (float)tile[key * D + part * (D / 4) + d], dot);
-            dot *= sc.x;
-            for (int n = 0; n < N; n++)
-                for (int j = 0; j < kBlockPos; j++)
-                    val[n][j] =
-                        sc.y * (float)tile[kBlockPos * D + kv8_value_at<D>(j, n * 64 + lane)];
-        }
-        dot = xor16_32_sum(dot);
-        const int keys = min(kBlockPos, p + 1 - b * kBlockPos);
-        float top = key < keys ? dot : -INFINITY;
-        for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float mx = fmaxf(m, top), keep = expf(m - mx);
-        m = mx;
-        l *= keep;
-        for (int n = 0; n < N; n++) acc[n] *= keep;
-        for (int j = 0; j < kBlockPos; j++) {
-            // Rows past the position may hold anything: skipped, not weighted.
-            if (j >= keys) break;
-            const float e = expf(__shfl(dot, j) - m);
-            l += e;
-            for (int n = 0; n < N; n++) acc[n] = fmaf(e, val[n][j], acc[n]);
-        }
-    }
-    bool bad = false;
-    for (int n = 0; n < N; n++) {
-        const float o = acc[n] / l;
-        dst[n * 64] = o;
-        bad |= !isfinite(o);
-    }
-    flag_nonfinite(status, bad);
 }
 
 }  // namespace pgpu
@@ -911,17 +1181,66 @@ extern "C" int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer,
 
 namespace {
 
-// Splits of 256 keys that positions below max_positions lie in.
-int splits_of(int max_positions) { return (max_positions - 1) / 256 + 1; }
+// How an attention call deals its work: splits of `keys` keys.
+struct Deal {
+    int splits, keys, tiles;
+};
+
+Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_positions) {
+    Deal d;
+    if (!r->offsets) {
+        d.keys = 64 * kKv8Waves;
+        d.splits = (max_positions - 1) / d.keys + 1;
+        d.tiles = 1;
+        return d;
+    }
+    // Work-groups without splits; where they are few, each row's keys are dealt
+    // out until there are about two for every CU, 256 keys at least to each.
+    d.tiles = ((r->max_rows + 15) / 16 * group + 3) / 4;
+    const size_t groups = (size_t)d.tiles * kv->heads * r->streams;
+    const int chunks = (max_positions - 1) / 64 + 1;
+    int want = groups >= 512 ? 1 : (int)(512 / groups);
+    if (want > chunks / 4) want = chunks / 4 < 1 ? 1 : chunks / 4;
+    const int each = (chunks + want - 1) / want;
+    d.keys = each * 64;
+    d.splits = (chunks + each - 1) / each;
+    return d;
+}
+
+template <int D>
+int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal &d,
+           const Kv8Decode &a, int *status) {
+    hipStream_t st = (hipStream_t)stream;
+    const int wide = c.heads * a.group;
+    float *out = a.out;
+    if (r.offsets) {
+        const Kv8Run run = {a.q, a.q_stride, a.group, a.scale, a.max_positions, d.splits,
+                            d.keys / 64, a.part_acc, a.part_ml, out, a.out_stride};
+        hipLaunchKernelGGL(k_kv8_run<D>, dim3(d.tiles, c.heads * d.splits, streams), dim3(256), 0,
+                           st, c, r, run, status);
+    } else {
+        Kv8Decode one = a;
+        if (d.splits > 1) one.out = nullptr;
+        hipLaunchKernelGGL(k_kv8_decode<D>, dim3(c.heads, d.splits, streams),
+                           dim3(64 * kKv8Waves), 0, st, c, r, one, status);
+    }
+    if (!launch_ok("pgpu_kv8_attention")) return 0;
+    if (d.splits == 1) return 1;
+    hipLaunchKernelGGL(k_kv8_join<D>, dim3(wide * (D / 64), r.max_rows, streams), dim3(64), 0, st,
+                       c, r, a.part_acc, a.part_ml, a.group, a.max_positions, d.splits, d.keys,
+                       out, a.out_stride, status);
+    return launch_ok("pgpu_kv8_attention");
+}
 
 }  // namespace
 
 extern "C" size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows,
                                            int group, int max_positions) {
     if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
-    if (rows->offsets || splits_of(max_positions) == 1) return 0;
-    return (size_t)rows->rows * kv->heads * group * splits_of(max_positions) *
-           (kv->head_dim + 2) * sizeof(float);
+    if (rows->rows == 0) return 0;
+    const Deal d = deal_of(kv, rows, group, max_positions);
+    if (d.splits == 1) return 0;
+    return (size_t)rows->rows * kv->heads * group * d.splits * (kv->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
@@ -936,50 +1255,20 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
         out_stride < width || max_positions <= 0 || !__builtin_isfinite(scale))
         return bad_arguments("pgpu_kv8_attention");
     if (rows->rows == 0) return 1;
+    const Deal d = deal_of(kv, rows, group, max_positions);
+    // Grid limits; a cache's worst case is far inside them.
+    if (d.splits > 65535 || (size_t)kv->heads * d.splits > 65535 || rows->max_rows > 65535)
+        return bad_arguments("pgpu_kv8_attention");
     const size_t need = pgpu_kv8_attention_bytes(kv, rows, group, max_positions);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv8_attention (workspace)");
+    const Kv8Decode a = {q, q_stride, group, scale * 1.44269504f, max_positions, d.splits,
+                         (float *)work,
+                         (float *)work + (size_t)rows->rows * kv->heads * group * d.splits *
+                                             kv->head_dim,
+                         out, out_stride};
     const Kv8 c = layer_of(kv, layer);
-    const Kv8Rows r = rows_of(rows);
-    const int wide = kv->heads * group;
-    if (rows->offsets) {
-        const dim3 grid(rows->max_rows, wide, rows->streams);
-        if (kv->head_dim == 64)
-            hipLaunchKernelGGL(k_kv8_attend<64>, grid, dim3(64), 0, (hipStream_t)stream, c, r, q,
-                               q_stride, group, scale, max_positions, out, out_stride, status);
-        else
-            hipLaunchKernelGGL(k_kv8_attend<128>, grid, dim3(64), 0, (hipStream_t)stream, c, r, q,
-                               q_stride, group, scale, max_positions, out, out_stride, status);
-        return launch_ok("pgpu_kv8_attention");
-    }
-    const int splits = splits_of(max_positions);
-    const size_t parts = (size_t)rows->rows * wide * splits;
-    Kv8Decode a = {};
-    a.q = q;
-    a.q_stride = q_stride;
-    a.group = group;
-    a.scale = scale * 1.44269504f;
-    a.max_positions = max_positions;
-    a.splits = splits;
-    a.part_acc = (float *)work;
-    a.part_ml = (float *)work + parts * kv->head_dim;
-    a.out = splits == 1 ? out : nullptr;
-    a.out_stride = out_stride;
-    const dim3 grid(kv->heads, splits, rows->streams), joint(kv->head_dim / 64, wide, rows->streams);
-    if (kv->head_dim == 64)
-        hipLaunchKernelGGL(k_kv8_decode<64>, grid, dim3(64 * kKv8Waves), 0, (hipStream_t)stream, c,
-                           r, a, status);
-    else
-        hipLaunchKernelGGL(k_kv8_decode<128>, grid, dim3(64 * kKv8Waves), 0, (hipStream_t)stream,
-                           c, r, a, status);
-    if (!launch_ok("pgpu_kv8_attention")) return 0;
-    if (splits == 1) return 1;
-    a.out = out;
-    if (kv->head_dim == 64)
-        hipLaunchKernelGGL(k_kv8_join<64>, joint, dim3(64), 0, (hipStream_t)stream, c, r, a,
-                           status);
-    else
-        hipLaunchKernelGGL(k_kv8_join<128>, joint, dim3(64), 0, (hipStream_t)stream, c, r, a,
-                           status);
-    return launch_ok("pgpu_kv8_attention");
+    return kv->head_dim == 64
+               ? attend<64>(stream, c, rows_of(rows), rows->streams, d, a, status)
+               : attend<128>(stream, c, rows_of(rows), rows->streams, d, a, status);
 }
