@@ -23,6 +23,13 @@ struct Kv8Rows {
     int rows, max_rows;
 };
 
+// Memory that no work-group of a launch writes, at an address that is the same
+// for a wave: read through the scalar cache.
+template <typename T>
+__device__ inline T uniform_load(const T *p) {
+    return *(const __attribute__((address_space(4))) T *)p;
+}
+
 // A stream's rows, checked: uniform over the work-group.
 struct Kv8Span {
     int first, count, row0, slot;
@@ -34,10 +41,10 @@ struct Kv8Span {
 __device__ inline Kv8Span kv8_span(const Kv8 &kv, const Kv8Rows &r, int s, int limit, bool speak,
                                    int *status) {
     Kv8Span x;
-    x.first = r.first[s];
-    x.slot = r.slots[s];
-    x.row0 = r.offsets ? r.offsets[s] : s;
-    const int end = r.offsets ? r.offsets[s + 1] : s + 1;
+    x.first = uniform_load(r.first + s);
+    x.slot = uniform_load(r.slots + s);
+    x.row0 = r.offsets ? uniform_load(r.offsets + s) : s;
+    const int end = r.offsets ? uniform_load(r.offsets + s + 1) : s + 1;
     // 64 bits: any int32 may stand in the arrays.
     const long long count = (long long)end - x.row0;
     const bool wild = x.row0 < 0 || count < 0 || end > r.rows || count > r.max_rows;
@@ -382,8 +389,6 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 kv, Kv8Rows rows, const in
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kKv8Waves = 4;  // 64 keys each
-
 __device__ inline float row16_max(float v) {
     // v_max of the lane 8, 4, 2, 1 apart within each row of 16.
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
@@ -420,6 +425,10 @@ __device__ inline float fix_sum(i32x4 c) {
     return fmaf((float)(c.x * 256 + c.y), 256.0f, (float)c.z);
 }
 
+__device__ inline float lane_value(float v, int lane) {
+    return bitsf((uint32_t)__builtin_amdgcn_readlane((int)fbits(v), lane));
+}
+
 template <int P>
 __device__ inline uint32_t quad_lane(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, P * 0x55, 0xf, 0xf, false);
@@ -441,82 +450,97 @@ struct Kv8Decode {
     size_t q_stride;
     int group;
     float scale;  // of the scores, times log2 e
-    int max_positions, splits;
+    int max_positions, splits, steps;  // a split: steps * W * 64 keys
     float *part_acc, *part_ml;  // slot (row * query heads + head) * splits + split
     float *out;                 // splits = 1: the rows themselves (else NULL)
     size_t out_stride;
 };
 
-template <int D>
+template <int D, int W, int Q>
 struct Kv8DecodeShared {
-    __align__(16) uint32_t digits[kKv8Waves][16][16];  // [row][group of lanes, block]
-    __align__(16) float own[kKv8Waves][4][16];         // weights of the newest block
-    float acc[kKv8Waves][4][D];
-    float m[kKv8Waves][4], l[kKv8Waves][4];
+    __align__(16) uint32_t digits[W][16][16];  // [row][group of lanes, block]
+    __align__(16) float own[W][4][16];         // weights of the newest block
+    float acc[W][Q][D];
+    float m[W][Q], l[W][Q];
 };
 
-// One row a stream. A work-group takes 256 keys of one (stream, key head), a
-// wave 64 of them: 4 blocks, whose bytes it requests together (8 or 16 KB),
-// then passes over 4 queries of the group at a time. Bound by the cache's
-// bytes; no wave waits for another before the joint of the four.
-template <int D>
-__global__ __launch_bounds__(64 * kKv8Waves) void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a,
-                                                               int *status) {
-    constexpr int KB = D / 64, T = D / 16;
-    __shared__ Kv8DecodeShared<D> sh;
-    const int head = blockIdx.x, split = blockIdx.y, s = blockIdx.z;
+// One row a stream. A work-group of W waves takes a split's keys of one
+// (stream, key head) for Q (1 or 4) of its queries, W * 64 keys a step: a wave's
+// 64 are 4 blocks, whose bytes it requests together (8 or 16 KB), the next
+// step's as soon as the registers are free: keys after the scores, values
+// after their product. Bound by the cache's bytes; no wave waits for another
+// before the joint of all W.
+//
+// Values: the 16 bytes that a lane (g, i) holds of a block are 4 positions (4 g
+// ..) of the dims i, 16 + i, 32 + i and 48 + i. They are an operand as they are
+// too: row 4 T + t of the other one has byte t of the weights in word T and
+// zeros elsewhere, so that its sums are those of dims 16 T + i.
+template <int D, int W, int Q>
+__global__ __launch_bounds__(64 * W, D == 64 ? (Q == 1 ? 6 : 5) : (Q == 1 ? 4 : 3))
+void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
+    constexpr int KB = D / 64;
+    __shared__ Kv8DecodeShared<D, W, Q> sh;
+    // Heads vary fastest: with 8 of them a head's passes stay on one XCD.
+    const int head = blockIdx.x % kv.heads, j0 = blockIdx.x / kv.heads * Q;
+    const int split = blockIdx.y, s = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
-    const int b0 = (split * kKv8Waves + wave) * 4;
+    int b0 = (split * a.steps * W + wave) * 4;  // the wave's blocks: b0 .. b0 + 3
+    const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
     int ids[4];
 #pragma unroll
     for (int t = 0; t < 4; t++)
-        ids[t] = rows.tables[(size_t)s * rows.table_stride + min(b0 + t, rows.table_stride - 1)];
+        ids[t] = uniform_load(table + min(b0 + t, rows.table_stride - 1));
     const Kv8Span span = kv8_span(kv, rows, s, a.max_positions,
-                                  threadIdx.x == 0 && head == 0 && split == 0, status);
-    const int width = kv.heads * a.group;  // query heads
+                                  threadIdx.x == 0 && blockIdx.x == 0 && split == 0, status);
+    const int live = min(Q, a.group - j0);  // queries of this work-group
     const int p = span.first;
     if (!span.live) {
         if (a.out && p < 0 && span.count > 0)
-            for (int e = threadIdx.x; e < a.group * D; e += 64 * kKv8Waves)
-                a.out[(size_t)s * a.out_stride + (size_t)head * a.group * D + e] = 0.0f;
+            for (int e = threadIdx.x; e < live * D; e += 64 * W)
+                a.out[(size_t)s * a.out_stride + ((size_t)head * a.group + j0) * D + e] = 0.0f;
         return;
     }
-    if (split * 256 > p) return;
-    const int newest = p / kBlockPos, closed = min(max(newest - b0, 0), 4);
-    const int own = newest - b0;  // 0..3: the newest block is this wave's
-    const bool mine = own >= 0 && own < 4;
+    if (split * a.steps * W * 64 > p) return;
+    const int newest = p / kBlockPos;
 
     i32x4 kr[4][KB], vr[4][KB];
-    float2 sc[4];
+    float ks[4], vs[4];
     bool wild = false;
+    // The closed blocks among b .. b + 3.
+    auto load = [&](int b, bool values) {
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-        if (t < closed) {
-            wild |= (unsigned)ids[t] >= kv.blocks;
-            const unsigned id = (unsigned)ids[t] < kv.blocks ? (unsigned)ids[t] : 0u;
-            const int8_t *tile = kv.values + kv8_tile<D>(kv, id, head);
-            sc[t] = *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
+        for (int t = 0; t < 4; t++) {
+            if (b + t < newest) {
+                wild |= (unsigned)ids[t] >= kv.blocks;
+                const unsigned id = (unsigned)ids[t] < kv.blocks ? (unsigned)ids[t] : 0u;
+                const int8_t *tile = kv.values + kv8_tile<D>(kv, id, head);
+                const float *sc = kv.scales + ((size_t)id * kv.heads + head) * 2;
+                (values ? vs : ks)[t] = uniform_load(sc + values);
 #pragma unroll
-            for (int n = 0; n < KB; n++) kr[t][n] = stream_load16(tile + i * D + n * 64 + g * 16);
+                for (int n = 0; n < KB; n++)
+                    (values ? vr : kr)[t][n] =
+                        stream_load16(values ? tile + kBlockPos * D + lane * (D / 4) + n * 16
+                                             : tile + i * D + n * 64 + g * 16);
+            } else {
+                (values ? vs : ks)[t] = 0.0f;
 #pragma unroll
-            for (int n = 0; n < KB; n++)
-                vr[t][n] = stream_load16(tile + kBlockPos * D + lane * (D / 4) + n * 16);
-        } else {
-            sc[t] = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int n = 0; n < KB; n++) kr[t][n] = vr[t][n] = i32x4{0, 0, 0, 0};
+                for (int n = 0; n < KB; n++) (values ? vr : kr)[t][n] = i32x4{0, 0, 0, 0};
+            }
         }
-    }
-    if (wild && lane == 0) atomicOr(status, 2);
+    };
+    load(b0, false);
+    load(b0, true);
     const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
 
-    for (int j0 = 0; j0 < a.group; j0 += 4) {
-        // Row i of the operand: byte i % 4 of query j0 + i / 4.
-        const float *q = a.q + (size_t)s * a.q_stride +
-                         ((size_t)head * a.group + min(j0 + (i >> 2), a.group - 1)) * D;
+    // Row i of the operand: byte i % 4 of query j0 + i / 4.
+    const float *q = a.q + (size_t)s * a.q_stride +
+                     ((size_t)head * a.group + min(j0 + (i >> 2), a.group - 1)) * D;
+    const uint32_t byte = row_byte(i & 3), sel = byte | (4u + byte) << 8;
+    i32x4 qd[KB];
+    float step, top = 0.0f;
+    {
         float4 x[KB][4];
-        float top = 0.0f;
 #pragma unroll
         for (int n = 0; n < KB; n++)
 #pragma unroll
@@ -529,8 +553,6 @@ __global__ __launch_bounds__(64 * kKv8Waves) void k_kv8_decode(Kv8 kv, Kv8Rows r
         top = xor16_32_max(top);
         const int e = fix_exponent(top);
         const float mul = power_of_2(e);
-        const uint32_t byte = row_byte(i & 3), sel = byte | (4u + byte) << 8;
-        i32x4 qd[KB];
 #pragma unroll
         for (int n = 0; n < KB; n++)
 #pragma unroll
@@ -538,131 +560,157 @@ __global__ __launch_bounds__(64 * kKv8Waves) void k_kv8_decode(Kv8 kv, Kv8Rows r
                 qd[n][k] = (int)pick4(fix_bytes(x[n][k].x, mul), fix_bytes(x[n][k].y, mul),
                                       fix_bytes(x[n][k].z, mul), fix_bytes(x[n][k].w, mul), sel);
         // From here on this lane's query is j0 + g (rows 4 g .. 4 g + 3).
-        const float step = __shfl(a.scale * power_of_2(-e), g * 4);
+        step = __shfl(a.scale * power_of_2(-e), g * 4);
+    }
+    // This lane's query is j0 + g in m and l; acc: dims lane, 64 + lane of each.
+    float m = -INFINITY, l = 0.0f, acc[Q][KB];
+#pragma unroll
+    for (int j = 0; j < Q; j++)
+#pragma unroll
+        for (int k = 0; k < KB; k++) acc[j][k] = 0.0f;
 
+    for (int n = 0; n < a.steps && b0 < newest; n++, b0 += 4 * W) {
+        const int closed = newest - b0;  // blocks from b0 on
+        const bool more = n + 1 < a.steps && b0 + 4 * W < newest;
+        if (more)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                ids[t] = uniform_load(table + min(b0 + 4 * W + t, rows.table_stride - 1));
         // Scores, in units of log 2: lane (g, i) key i of each block.
-        float score[4], m = -INFINITY;
+        float w[4], mx = m;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             i32x4 c = {0, 0, 0, 0};
 #pragma unroll
-            for (int n = 0; n < KB; n++)
-                c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[n], kr[t][n], c, 0, 0, 0);
-            score[t] = t < closed ? fix_sum(c) * (step * sc[t].x) : -INFINITY;
+            for (int k = 0; k < KB; k++)
+                c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[k], kr[t][k], c, 0, 0, 0);
+            w[t] = t < closed ? fix_sum(c) * (step * ks[t]) : -INFINITY;
+            mx = fmaxf(mx, w[t]);
         }
-        if (mine) {
-            f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < KB; n++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float4 y = *(const float4 *)(slot + i * D + n * 64 + g * 16 + k * 4);
-                    const float4 v = (i & 3) ? make_float4(0.f, 0.f, 0.f, 0.f) : x[n][k];
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x, y.x, c, 0, 0, 0);
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.y, y.y, c, 0, 0, 0);
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, y.z, c, 0, 0, 0);
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, y.w, c, 0, 0, 0);
-                }
-            const float v = newest * kBlockPos + i <= p ? c.x * a.scale : -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-                if (t == own) score[t] = v;
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++) m = fmaxf(m, score[t]);
-        m = row16_max(m);
-        float w[4], l = 0.0f, last = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            w[t] = score[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(score[t] - m);
-            l += w[t];
-            if (mine && t == own) last = w[t];
-        }
-        l = row16_sum(l);
-
+        if (more) load(b0 + 4 * W, false);
+        mx = row16_max(mx);
+        const float shrink = __builtin_amdgcn_exp2f(m - mx);  // m = -inf: 0
+        m = mx;
+        float sum = 0.0f, big = 0.0f;
         // The weights times their blocks' value scales, in fixed point below
         // the largest of the query's 64; byte t of four keys in a row's word.
-        float big = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            w[t] *= sc[t].y;
+            w[t] = __builtin_amdgcn_exp2f(w[t] - m);
+            sum += w[t];
+            w[t] *= vs[t];
             big = fmaxf(big, w[t]);
         }
+        l = fmaf(l, shrink, row16_sum(sum));
         const int f = fix_exponent(row16_max(big));
-        const float mul2 = power_of_2(f), back = power_of_2(-f);
+        const float mul = power_of_2(f), back = power_of_2(-f);
         i32x4 word;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const uint32_t u = fix_bytes(w[t], mul2);
+            const uint32_t u = fix_bytes(w[t], mul);
             word[t] = (int)pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u),
                                  quad_lane<3>(u), sel);
         }
         *(i32x4 *)&sh.digits[wave][g * 4 + (i & 3)][(i >> 2) * 4] = word;
-        if (mine) sh.own[wave][g][i] = last;
         wave_lds_fence();
-        const i32x4 pd = *(const i32x4 *)&sh.digits[wave][i][g * 4];
-        float acc[T];
 #pragma unroll
-        for (int t = 0; t < T; t++) {
-            const i32x4 v = {vr[0][t / 4][t % 4], vr[1][t / 4][t % 4], vr[2][t / 4][t % 4],
-                             vr[3][t / 4][t % 4]};
-            const i32x4 c =
-                __builtin_amdgcn_mfma_i32_16x16x64_i8(pd, v, i32x4{0, 0, 0, 0}, 0, 0, 0);
-            acc[t] = fix_sum(c) * back;
-        }
-        if (mine) {
-            float4 y = *(const float4 *)&sh.own[wave][i >> 2][g * 4];
-            if (i & 3) y = make_float4(0.f, 0.f, 0.f, 0.f);
-            const float wk[4] = {y.x, y.y, y.z, y.w};
+        for (int j = 0; j < Q; j++) {
+            const i32x4 pd = *(const i32x4 *)&sh.digits[wave][j * 4 + (i & 3)][g * 4];
+            i32x4 c[KB];
 #pragma unroll
-            for (int t = 0; t < T; t++) {
-                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < KB; k++) c[k] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    // Rows past the position may hold anything.
-                    const bool in = newest * kBlockPos + g * 4 + k <= p;
-                    const float v = slot[kBlockPos * D + (g * 4 + k) * D + t * 16 + i];
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(wk[k], in ? v : 0.0f, c, 0, 0, 0);
-                }
-                acc[t] += c.x;
-            }
-        }
-        const int live = min(4, a.group - j0);  // queries of this pass
-        if (g < live) {
+            for (int t = 0; t < 4; t++) {
+                const int x = pd[t], z = i >> 2;
+                const i32x4 row = {z == 0 ? x : 0, z == 1 ? x : 0, z == 2 ? x : 0, z == 3 ? x : 0};
 #pragma unroll
-            for (int t = 0; t < T; t++) sh.acc[wave][g][t * 16 + i] = acc[t];
-            if (i == 0) {
-                sh.m[wave][g] = m;
-                sh.l[wave][g] = l;
+                for (int k = 0; k < KB; k++)
+                    c[k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(row, vr[t][k], c[k], 0, 0, 0);
             }
+            const float one = Q == 1 ? back : lane_value(back, j * 16);
+            const float less = Q == 1 ? shrink : lane_value(shrink, j * 16);
+#pragma unroll
+            for (int k = 0; k < KB; k++) acc[j][k] = fmaf(fix_sum(c[k]), one, acc[j][k] * less);
         }
-        bool bad = !(top < INFINITY);
-        __syncthreads();
-        for (int e2 = threadIdx.x; e2 < live * D; e2 += 64 * kKv8Waves) {
-            const int j = e2 / D, d = e2 % D;
-            float mx = -INFINITY;
-            for (int n = 0; n < kKv8Waves; n++) mx = fmaxf(mx, sh.m[n][j]);
-            float total = 0.0f, o = 0.0f;
-            for (int n = 0; n < kKv8Waves; n++) {
-                if (sh.l[n][j] == 0.0f) continue;  // a wave past the context
-                const float c = __builtin_amdgcn_exp2f(sh.m[n][j] - mx);
-                total = fmaf(sh.l[n][j], c, total);
-                o = fmaf(sh.acc[n][j][d], c, o);
-            }
-            const size_t qh = (size_t)head * a.group + j0 + j;
-            if (a.out) {
-                o = o / total;
-                a.out[(size_t)s * a.out_stride + qh * D + d] = o;
-                bad |= !isfinite(o);
-            } else {
-                const size_t at = ((size_t)s * width + qh) * a.splits + split;
-                a.part_acc[at * D + d] = o;
-                if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(mx, total);
-            }
-        }
-        flag_nonfinite(status, bad);
-        __syncthreads();
+        if (more) load(b0 + 4 * W, true);
+        wave_lds_fence();
     }
+    // The newest block, in fp32: by the wave after the one whose blocks end there,
+    // which has had a step less.
+    if (newest / (a.steps * W * 4) == split && (newest / 4 + 1) % W == wave) {
+        f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KB * 4; k++) {
+            const int d = k / 4 * 64 + g * 16 + k % 4 * 4;
+            const float4 y = *(const float4 *)(slot + i * D + d);
+            float4 v = *(const float4 *)(q + d);
+            if (i & 3) v = make_float4(0.f, 0.f, 0.f, 0.f);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x, y.x, c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.y, y.y, c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, y.z, c, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, y.w, c, 0, 0, 0);
+        }
+        float w = newest * kBlockPos + i <= p ? c.x * a.scale : -INFINITY;
+        const float mx = row16_max(fmaxf(m, w)), shrink = __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        w = __builtin_amdgcn_exp2f(w - m);
+        l = fmaf(l, shrink, row16_sum(w));
+        sh.own[wave][g][i] = w;
+        wave_lds_fence();
+        // Rows past the position may hold anything: left out.
+#pragma unroll
+        for (int j = 0; j < Q; j++) {
+            const float less = Q == 1 ? shrink : lane_value(shrink, j * 16);
+#pragma unroll
+            for (int k = 0; k < KB; k++) acc[j][k] *= less;
+        }
+#pragma unroll
+        for (int n = 0; n < kBlockPos; n++)
+            if (newest * kBlockPos + n <= p)
+#pragma unroll
+                for (int k = 0; k < KB; k++) {
+                    const float v = slot[kBlockPos * D + n * D + k * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < Q; j++)
+                        acc[j][k] = fmaf(sh.own[wave][j][n], v, acc[j][k]);
+                }
+    }
+    if (wild && lane == 0) atomicOr(status, 2);
+#pragma unroll
+    for (int j = 0; j < Q; j++)
+#pragma unroll
+        for (int k = 0; k < KB; k++) sh.acc[wave][j][k * 64 + lane] = acc[j][k];
+    if (g < Q && i == 0) {
+        sh.m[wave][g] = m;
+        sh.l[wave][g] = l;
+    }
+    bool bad = !(top < INFINITY);
+    __syncthreads();
+    for (int e = threadIdx.x; e < live * D; e += 64 * W) {
+        const int j = e / D, d = e % D;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < W; n++) mx = fmaxf(mx, sh.m[n][j]);
+        float total = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int n = 0; n < W; n++) {
+            // A wave past the context: l = 0, m = -inf, acc = 0.
+            const float c = __builtin_amdgcn_exp2f(sh.m[n][j] - mx);
+            total = fmaf(sh.l[n][j], c, total);
+            o = fmaf(sh.acc[n][j][d], c, o);
+        }
+        const size_t qh = (size_t)head * a.group + j0 + j;
+        if (a.out) {
+            o = o / total;
+            a.out[(size_t)s * a.out_stride + qh * D + d] = o;
+            bad |= !isfinite(o);
+        } else {
+            const size_t at = ((size_t)s * kv.heads * a.group + qh) * a.splits + split;
+            a.part_acc[at * D + d] = o;
+            if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(mx, total);
+        }
+    }
+    flag_nonfinite(status, bad);
 }
 
 // Runs of rows: a work-group of 4 waves takes 4 tiles of 16 rows of one query
@@ -1025,14 +1073,28 @@ __global__ __launch_bounds__(64) void k_kv8_join(Kv8 kv, Kv8Rows rows, const flo
     }
     const int n = (span.first + i) / keys + 1;
     const size_t at = (row * kv.heads * group + qh) * splits;
-    float mx = -INFINITY;
-    for (int j = 0; j < n; j++) mx = fmaxf(mx, part_ml[(at + j) * 2]);
-    float total = 0.0f, o = 0.0f;
-    for (int j = 0; j < n; j++) {
-        const float c = __builtin_amdgcn_exp2f(part_ml[(at + j) * 2] - mx);
-        total = fmaf(part_ml[(at + j) * 2 + 1], c, total);
-        o = fmaf(part_acc[(at + j) * D + d], c, o);
+    // Lane j has split j's maximum and sum (and j + 64's, ...).
+    float mx = -INFINITY, total = 0.0f, o = 0.0f;
+    for (int j = threadIdx.x; j < n; j += 64) mx = fmaxf(mx, part_ml[(at + j) * 2]);
+    mx = wave_max(mx);
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int j = j0 + threadIdx.x;
+        const float2 ml = j < n ? *(const float2 *)(part_ml + (at + j) * 2)
+                                : make_float2(-INFINITY, 0.0f);
+        const float c = __builtin_amdgcn_exp2f(ml.x - mx);
+        total = fmaf(ml.y, c, total);
+        const int last = min(64, n - j0);
+        for (int k = 0; k < last; k += 8) {
+            float x[8];  // eight rows on their way at once
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                x[u] = part_acc[(at + j0 + min(k + u, last - 1)) * D + d];
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (k + u < last) o = fmaf(x[u], lane_value(c, k + u), o);
+        }
     }
+    total = wave_sum(total);
     o = o / total;
     *dst = o;
     flag_nonfinite(status, !isfinite(o));
@@ -1183,15 +1245,33 @@ namespace {
 
 // How an attention call deals its work: splits of `keys` keys.
 struct Deal {
-    int splits, keys, tiles;
+    int splits, keys, tiles, waves, steps;
 };
 
 Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_positions) {
     Deal d;
     if (!r->offsets) {
-        d.keys = 64 * kKv8Waves;
+        // A stream's keys whole in one work-group of W waves, where that is few
+        // steps of W * 64 keys or there are work-groups to fill the chip; else
+        // dealt to work-groups of 4 waves, more keys to each the more of them
+        // there are. us, whole / dealt (8 heads of 64): 1 stream of 2011 keys 8.6 /
+        // 10.7, of 8187 19.7 / 10.4; 16 of up to 2048 10.7 / 11.2, of up to 8187
+        // 26.6 / 19.2; 64 of up to 2048 16.3 / 18.6, of up to 8187 52.3 / 49.6; 128
+        // of up to 2048 32.5 / 37.3. W = 4, 8, 16: 1 stream of 700 keys 7.8, 7.8, 7.6,
+        // of 2011 13.5, 9.5, 8.6; 64 of up to 2048 18.2, 16.3, 18.0; 256 of up to
+        // 600 24.4, 29.4, 51.4. (16 waves of 4 queries would not fit the registers.)
+        d.tiles = group == 1 ? 1 : (group + 3) / 4;
+        const size_t groups = (size_t)kv->heads * d.tiles * r->streams;
+        const int units = (max_positions - 1) / 64 + 1;
+        d.waves = groups > 768 ? 4 : groups > 256 || group > 1 ? 8 : 16;
+        d.steps = (units + d.waves - 1) / d.waves;
+        if (d.steps > (groups < 128 ? 2 : groups < 1024 ? 4 : 8)) {
+            d.waves = 4;
+            d.steps = (groups < 64 ? 1 : groups < 256 ? 2 : 4) * 64 / kv->head_dim;
+            if (d.steps < 1) d.steps = 1;
+        }
+        d.keys = 64 * d.waves * d.steps;
         d.splits = (max_positions - 1) / d.keys + 1;
-        d.tiles = 1;
         return d;
     }
     // Work-groups without splits; where they are few, each row's keys are dealt
@@ -1220,9 +1300,22 @@ int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal
                            st, c, r, run, status);
     } else {
         Kv8Decode one = a;
+        one.steps = d.steps;
         if (d.splits > 1) one.out = nullptr;
-        hipLaunchKernelGGL(k_kv8_decode<D>, dim3(c.heads, d.splits, streams),
-                           dim3(64 * kKv8Waves), 0, st, c, r, one, status);
+        const dim3 grid(c.heads * d.tiles, d.splits, streams);
+#define KV8_DECODE(W, Q)                                                                        \
+    hipLaunchKernelGGL((k_kv8_decode<D, W, Q>), grid, dim3(64 * W), 0, st, c, r, one, status)
+        if (a.group == 1 && d.waves == 4)
+            KV8_DECODE(4, 1);
+        else if (a.group == 1 && d.waves == 8)
+            KV8_DECODE(8, 1);
+        else if (a.group == 1)
+            KV8_DECODE(16, 1);
+        else if (d.waves == 4)
+            KV8_DECODE(4, 4);
+        else
+            KV8_DECODE(8, 4);
+#undef KV8_DECODE
     }
     if (!launch_ok("pgpu_kv8_attention")) return 0;
     if (d.splits == 1) return 1;
@@ -1262,7 +1355,7 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
     const size_t need = pgpu_kv8_attention_bytes(kv, rows, group, max_positions);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv8_attention (workspace)");
-    const Kv8Decode a = {q, q_stride, group, scale * 1.44269504f, max_positions, d.splits,
+    const Kv8Decode a = {q, q_stride, group, scale * 1.44269504f, max_positions, d.splits, 1,
                          (float *)work,
                          (float *)work + (size_t)rows->rows * kv->heads * group * d.splits *
                                              kv->head_dim,
