@@ -754,20 +754,39 @@ __device__ inline f16x4 bytes_f16(int x) {
     return f16x4{a.x, a.y, b.x, b.y};
 }
 
-// x -> two fp16 terms, both truncated: hi + lo has 22 bits of it.
+// x, y -> two fp16 terms, both truncated: hi + lo has 22 bits of them. The
+// remainder is one v_fma_mix_f32, which reads an fp16 half as it stands.
 __device__ inline void split_pair(float x, float y, f16x2 &hi, f16x2 &lo) {
-    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
-    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, -1.0f, x),
-                                                              fmaf((float)hi.y, -1.0f, y)));
+    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+    const uint32_t u = __builtin_bit_cast(uint32_t, h);
+    float rx, ry;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rx) : "v"(u), "v"(x));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(ry) : "v"(u), "v"(y));
+    hi = __builtin_bit_cast(f16x2, h);
+    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(rx, ry));
+}
+
+// Pairs of terms -> an operand of 8.
+__device__ inline f16x8 join_pairs(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
+    const i32x4 x = {__builtin_bit_cast(int, a), __builtin_bit_cast(int, b),
+                     __builtin_bit_cast(int, c), __builtin_bit_cast(int, d)};
+    return __builtin_bit_cast(f16x8, x);
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a, int *status) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a, int *status) {
     constexpr int KB = D / 64, KS = D / 32, T = D / 16;
     constexpr float kNone = -3.0e38f;  // the maximum of no scores
     __shared__ Kv8RunShared<D> sh;
-    const int s = blockIdx.z, head = blockIdx.y % kv.heads, split = blockIdx.y / kv.heads;
-    const int bx = gridDim.x - 1 - blockIdx.x;  // the longest rows first
+    // Heads fastest (with 8 of them a head's keys stay in one XCD's L2), the
+    // longest rows first, and every second 256 work-groups the other way round: a
+    // CU, which gets each 256th, has long and short ones.
+    const int s = blockIdx.z, head = blockIdx.x % kv.heads, split = blockIdx.x / kv.heads;
+    const int turn = max(1, 256 / (int)gridDim.x), lap = blockIdx.y / turn;
+    int bx = blockIdx.y;
+    if (lap & 1) bx = min((lap + 1) * turn, (int)gridDim.y) - 1 - (bx - lap * turn);
+    bx = gridDim.y - 1 - bx;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
     const Kv8Span span = kv8_span(kv, rows, s, a.max_positions,
@@ -818,13 +837,16 @@ __global__ __launch_bounds__(256) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a,
 #pragma unroll
         for (int n = 0; n < KB; n++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                f16x2 h0, l0, h1, l1;
-                split_pair(x[n][k].x * mul, x[n][k].y * mul, h0, l0);
-                split_pair(x[n][k].z * mul, x[n][k].w * mul, h1, l1);
-                const int ks = n * 2 + k / 2, o = k % 2 * 4;
-                qhi[ks][o] = h0.x, qhi[ks][o + 1] = h0.y, qhi[ks][o + 2] = h1.x, qhi[ks][o + 3] = h1.y;
-                qlo[ks][o] = l0.x, qlo[ks][o + 1] = l0.y, qlo[ks][o + 2] = l1.x, qlo[ks][o + 3] = l1.y;
+            for (int k = 0; k < 2; k++) {
+                f16x2 h[4], o[4];
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const float4 v = x[n][k * 2 + z];
+                    split_pair(v.x * mul, v.y * mul, h[z * 2], o[z * 2]);
+                    split_pair(v.z * mul, v.w * mul, h[z * 2 + 1], o[z * 2 + 1]);
+                }
+                qhi[n * 2 + k] = join_pairs(h[0], h[1], h[2], h[3]);
+                qlo[n * 2 + k] = join_pairs(o[0], o[1], o[2], o[3]);
             }
     }
 
@@ -881,32 +903,34 @@ __global__ __launch_bounds__(256) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a,
         for (int t = 0; t < 4; t++) bs[t] = sh.scale[buf][t];
         f32x4 w[4];
         float mx = kNone;
+        auto hidden = [&](int t, int r) {
+            const int key = c * 64 + t * 16 + g * 4 + r;
+            return key > p || key >= keys;
+        };
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const f16x8 kk = sh.k[buf][t][k][lane];
-                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qhi[k], x, 0, 0, 0);
-                x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qlo[k], x, 0, 0, 0);
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qhi[k], w[t], 0, 0, 0);
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qlo[k], w[t], 0, 0, 0);
             }
-            const float f = bs[t].x * qs;
+            if (MASK)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                w[t][r] = x[r] * f;
-                if (MASK) {
-                    const int key = c * 64 + t * 16 + g * 4 + r;
-                    w[t][r] = key <= p && key < keys ? w[t][r] : -INFINITY;
-                }
-                mx = fmaxf(mx, w[t][r]);
-            }
+                for (int r = 0; r < 4; r++)
+                    if (hidden(t, r)) w[t][r] = -INFINITY;
+            // The factor is not negative; a NaN (a block that was not finite, or a
+            // scale of 0 times a hidden key) does not count.
+            mx = fmaxf(mx, fmaxf(fmaxf(w[t][0], w[t][1]), fmaxf(w[t][2], w[t][3])) *
+                               (bs[t].x * qs));
         }
         mx = xor16_32_max(mx);
         // A whole number; not below the last one.
         const float mn = fmaxf(m, ceilf(mx));
         int up = unit;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {  // NaN (a block that was not finite) does not count
+        for (int t = 0; t < 4; t++) {  // NaN does not count here either
             const int n = (int)(fbits(bs[t].y) >> 23) - 127;
             up = max(up, n < 128 ? n : -100);
         }
@@ -922,33 +946,33 @@ __global__ __launch_bounds__(256) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a,
             m = mn;
             unit = up;
         }
-        f16x8 hi[2], lo[2];
+        f16x2 hi[4][2], lo[4][2];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             // 2^(14 - unit) times the scale: below 2^15.
-            const float f = ldexpf(bs[t].y, 14 - unit);
+            const float f = bs[t].x * qs, z = ldexpf(bs[t].y, 14 - unit);
             float x[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float e = __builtin_amdgcn_exp2f(w[t][r] - m);
-                l += e;
-                x[r] = e * f;
-                if (MASK) x[r] = w[t][r] == -INFINITY ? 0.0f : x[r];
+                const float e = __builtin_amdgcn_exp2f(fmaf(w[t][r], f, -m));
+                const bool hide = MASK && hidden(t, r);
+                l += hide ? 0.0f : e;
+                x[r] = hide ? 0.0f : e * z;
             }
-            f16x2 h0, l0, h1, l1;
-            split_pair(x[0], x[1], h0, l0);
-            split_pair(x[2], x[3], h1, l1);
-            const int o = t % 2 * 4;
-            hi[t / 2][o] = h0.x, hi[t / 2][o + 1] = h0.y, hi[t / 2][o + 2] = h1.x, hi[t / 2][o + 3] = h1.y;
-            lo[t / 2][o] = l0.x, lo[t / 2][o + 1] = l0.y, lo[t / 2][o + 2] = l1.x, lo[t / 2][o + 3] = l1.y;
+            split_pair(x[0], x[1], hi[t][0], lo[t][0]);
+            split_pair(x[2], x[3], hi[t][1], lo[t][1]);
         }
+        const f16x8 ph[2] = {join_pairs(hi[0][0], hi[0][1], hi[1][0], hi[1][1]),
+                             join_pairs(hi[2][0], hi[2][1], hi[3][0], hi[3][1])};
+        const f16x8 pl[2] = {join_pairs(lo[0][0], lo[0][1], lo[1][0], lo[1][1]),
+                             join_pairs(lo[2][0], lo[2][1], lo[3][0], lo[3][1])};
 #pragma unroll
         for (int t = 0; t < T; t++)
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 const f16x8 v = sh.v[buf][n][t][lane];
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[n], acc[t], 0, 0, 0);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[n], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[n], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[n], acc[t], 0, 0, 0);
             }
     };
 
@@ -1296,7 +1320,7 @@ int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal
     if (r.offsets) {
         const Kv8Run run = {a.q, a.q_stride, a.group, a.scale, a.max_positions, d.splits,
                             d.keys / 64, a.part_acc, a.part_ml, out, a.out_stride};
-        hipLaunchKernelGGL(k_kv8_run<D>, dim3(d.tiles, c.heads * d.splits, streams), dim3(256), 0,
+        hipLaunchKernelGGL(k_kv8_run<D>, dim3(c.heads * d.splits, d.tiles, streams), dim3(256), 0,
                            st, c, r, run, status);
     } else {
         Kv8Decode one = a;
