@@ -774,6 +774,13 @@ __device__ inline f16x8 join_pairs(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
     return __builtin_bit_cast(f16x8, x);
 }
 
+// The largest of three; NaN does not count.
+__device__ inline float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a, int *status) {
     constexpr int KB = D / 64, KS = D / 32, T = D / 16;
@@ -783,10 +790,15 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     // longest rows first, and every second 256 work-groups the other way round: a
     // CU, which gets each 256th, has long and short ones.
     const int s = blockIdx.z, head = blockIdx.x % kv.heads, split = blockIdx.x / kv.heads;
-    const int turn = max(1, 256 / (int)gridDim.x), lap = blockIdx.y / turn;
-    int bx = blockIdx.y;
-    if (lap & 1) bx = min((lap + 1) * turn, (int)gridDim.y) - 1 - (bx - lap * turn);
-    bx = gridDim.y - 1 - bx;
+    const int plane = gridDim.x * gridDim.y;
+    int bx = gridDim.y - 1 - blockIdx.y;
+    if (plane <= 256) {
+        if ((int)((size_t)blockIdx.z * plane / 256) & 1) bx = blockIdx.y;
+    } else {
+        const int turn = max(1, 256 / (int)gridDim.x), lap = blockIdx.y / turn;
+        if (lap & 1)
+            bx = gridDim.y - min((lap + 1) * turn, (int)gridDim.y) + (blockIdx.y - lap * turn);
+    }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
     const Kv8Span span = kv8_span(kv, rows, s, a.max_positions,
@@ -806,7 +818,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
         return;
     }
     const int end = span.first + span.count, newest = (end - 1) / kBlockPos;
-    const int top = span.first + min(span.count, ((min(bx * 4 + 3, tiles - 1)) / a.group + 1) * 16) - 1;
+    const int top = span.first + min(span.count, (min(bx * 4 + 3, tiles - 1) / a.group + 1) * 16) - 1;
     const int keys = min(newest * kBlockPos, top + 1);  // of blocks, to be seen by some row here
     const int c0 = split * a.chunks, c1 = min(c0 + a.chunks, (keys + 63) / 64);
     const bool last_split = newest / 4 >= c0 && newest / 4 < c0 + a.chunks;
@@ -832,8 +844,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             }
         biggest = xor16_32_max(biggest);
         const int e = min(126, 141 - (int)(fbits(biggest) >> 23));
-        const float mul = copysignf(power_of_2(e), a.scale);
-        qs = fabsf(a.scale) * power_of_2(-e);
+        // The factor of the scores stays above 0, for a scale of 0 too.
+        const float mul = a.scale == 0.0f ? 0.0f : copysignf(power_of_2(e), a.scale);
+        qs = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * power_of_2(-e);
 #pragma unroll
         for (int n = 0; n < KB; n++)
 #pragma unroll
@@ -850,28 +863,39 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             }
     }
 
-    // Block 4 c + wave of chunk c: requested, then turned into LDS.
+    // Chunk c: its bytes requested, then turned into LDS; wave w takes block w.
+    // The block's id and scales of chunk c0 + j wait in lane j (j below 64, then
+    // the next 64): no chunk waits for its own.
     i32x4 kr[KB], vr[KB];
-    float2 sc;
+    int id_of = 0;
+    float2 scale_of = make_float2(1.0f, 0.0f), sc;
     bool wild = false;
     const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
+    auto look_up = [&](int c) {
+        const int b = (c + lane) * 4 + wave;
+        const bool in = c + lane < c1 && b * kBlockPos < keys;
+        const int raw = in ? table[b] : 0;
+        wild |= (unsigned)raw >= kv.blocks;
+        id_of = (unsigned)raw < kv.blocks ? raw : 0;
+        scale_of = make_float2(1.0f, 0.0f);
+        if (in) {
+            scale_of = *(const float2 *)(kv.scales + ((size_t)id_of * kv.heads + head) * 2);
+            // A block whose values were not finite: its scores say so instead, to
+            // the rows that see it.
+            if (scale_of.y != scale_of.y) scale_of = make_float2(scale_of.y, 0.0f);
+        }
+    };
     auto request = [&](int c) {
-        const int b = c * 4 + wave;
-        if (b * kBlockPos < keys) {
-            const int raw = table[b];
-            wild |= (unsigned)raw >= kv.blocks;
-            const unsigned id = (unsigned)raw < kv.blocks ? (unsigned)raw : 0u;
-            const int8_t *tl = kv.values + kv8_tile<D>(kv, id, head);
-            sc = *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
+        const int j = (c - c0) & 63;
+        if (j == 0) look_up(c);
+        const unsigned id = (unsigned)__builtin_amdgcn_readlane(id_of, j);
+        sc = make_float2(lane_value(scale_of.x, j), lane_value(scale_of.y, j));
+        // Past the keys: block 0's bytes, whose keys are hidden and whose scale is 0.
+        const int8_t *tl = kv.values + kv8_tile<D>(kv, id, head);
 #pragma unroll
-            for (int n = 0; n < KB; n++) {
-                kr[n] = *(const i32x4 *)(tl + i * D + n * 64 + g * 16);
-                vr[n] = *(const i32x4 *)(tl + kBlockPos * D + lane * (D / 4) + n * 16);
-            }
-        } else {
-            sc = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int n = 0; n < KB; n++) kr[n] = vr[n] = i32x4{0, 0, 0, 0};
+        for (int n = 0; n < KB; n++) {
+            kr[n] = *(const i32x4 *)(tl + i * D + n * 64 + g * 16);
+            vr[n] = *(const i32x4 *)(tl + kBlockPos * D + lane * (D / 4) + n * 16);
         }
     };
     auto stage = [&](int buf) {
@@ -885,8 +909,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             }
 #pragma unroll
         for (int t = 0; t < T; t++)
-            *((f16x4 *)&sh.v[buf][wave >> 1][t][lane] + (wave & 1)) =
-                bytes_f16(vr[t / 4][t % 4]);
+            *((f16x4 *)&sh.v[buf][wave >> 1][t][lane] + (wave & 1)) = bytes_f16(vr[t / 4][t % 4]);
         if (lane == 0) sh.scale[buf][wave] = sc;
     };
 
@@ -896,17 +919,13 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     int unit = -100;  // acc holds the values' sums / 2^(unit - 14)
 
-    auto attend = [&](int buf, int c, auto masked) {
-        constexpr bool MASK = decltype(masked)::value;
+    auto attend = [&](int buf, int c, bool masked) {
         float2 bs[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) bs[t] = sh.scale[buf][t];
         f32x4 w[4];
-        float mx = kNone;
-        auto hidden = [&](int t, int r) {
-            const int key = c * 64 + t * 16 + g * 4 + r;
-            return key > p || key >= keys;
-        };
+        // The last key that this lane's row sees, from its own first one on.
+        const int last = min(p, keys - 1) - c * 64 - g * 4;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -916,25 +935,30 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
                 w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qhi[k], w[t], 0, 0, 0);
                 w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qlo[k], w[t], 0, 0, 0);
             }
-            if (MASK)
+        }
+        if (masked)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    if (hidden(t, r)) w[t][r] = -INFINITY;
-            // The factor is not negative; a NaN (a block that was not finite, or a
-            // scale of 0 times a hidden key) does not count.
-            mx = fmaxf(mx, fmaxf(fmaxf(w[t][0], w[t][1]), fmaxf(w[t][2], w[t][3])) *
-                               (bs[t].x * qs));
+                    if (t * 16 + r > last) w[t][r] = -INFINITY;
+        float f[4], mx = kNone;
+#pragma unroll
+        for (int t = 0; t < 4; t += 2) {
+            // A factor is not negative; NaN (a block that was not finite, or a
+            // factor that fell to 0 times a hidden key) does not count.
+            f[t] = bs[t].x * qs, f[t + 1] = bs[t + 1].x * qs;
+            mx = max3(mx, max3(max3(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]) * f[t],
+                      max3(max3(w[t + 1][0], w[t + 1][1], w[t + 1][2]), w[t + 1][3],
+                           w[t + 1][3]) * f[t + 1]);
         }
         mx = xor16_32_max(mx);
         // A whole number; not below the last one.
         const float mn = fmaxf(m, ceilf(mx));
-        int up = unit;
+        uint32_t high = 0;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {  // NaN does not count here either
-            const int n = (int)(fbits(bs[t].y) >> 23) - 127;
-            up = max(up, n < 128 ? n : -100);
-        }
-        up = __builtin_amdgcn_readfirstlane(up);
+        for (int t = 0; t < 4; t++) high = max(high, fbits(bs[t].y));
+        const int up = max(unit, (int)(__builtin_amdgcn_readfirstlane(high) >> 23) - 127);
         if (up != unit || __any(mn != m)) {
             const float shrink = __builtin_amdgcn_exp2f(m - mn);
             l *= shrink;
@@ -946,21 +970,26 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             m = mn;
             unit = up;
         }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], f[t], -m));
+        if (masked)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (t * 16 + r > last) w[t][r] = 0.0f;
         f16x2 hi[4][2], lo[4][2];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             // 2^(14 - unit) times the scale: below 2^15.
-            const float f = bs[t].x * qs, z = ldexpf(bs[t].y, 14 - unit);
-            float x[4];
+            const float z = ldexpf(bs[t].y, 14 - unit);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(w[t][r], f, -m));
-                const bool hide = MASK && hidden(t, r);
-                l += hide ? 0.0f : e;
-                x[r] = hide ? 0.0f : e * z;
-            }
-            split_pair(x[0], x[1], hi[t][0], lo[t][0]);
-            split_pair(x[2], x[3], hi[t][1], lo[t][1]);
+            for (int r = 0; r < 4; r++) l += w[t][r];
+            split_pair(w[t][0] * z, w[t][1] * z, hi[t][0], lo[t][0]);
+            split_pair(w[t][2] * z, w[t][3] * z, hi[t][1], lo[t][1]);
         }
         const f16x8 ph[2] = {join_pairs(hi[0][0], hi[0][1], hi[1][0], hi[1][1]),
                              join_pairs(hi[2][0], hi[2][1], hi[3][0], hi[3][1])};
@@ -983,12 +1012,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
         for (int c = c0; c < c1; c++) {
             const int buf = (c - c0) & 1;
             if (c + 1 < c1) request(c + 1);
-            if (live > 0 && c * 64 <= wave_top) {
-                if (c * 64 + 63 <= p0 && c * 64 + 64 <= keys && live == 16)
-                    attend(buf, c, std::false_type{});
-                else
-                    attend(buf, c, std::true_type{});
-            }
+            if (live > 0 && c * 64 <= wave_top)
+                attend(buf, c, c * 64 + 63 > p0 || c * 64 + 64 > keys || live < 16);
             if (c + 1 < c1) stage(buf ^ 1);
             __syncthreads();
         }
@@ -1269,7 +1294,7 @@ namespace {
 
 // How an attention call deals its work: splits of `keys` keys.
 struct Deal {
-    int splits, keys, tiles, waves, steps;
+    int splits, keys, tiles, waves, steps;  // tiles: work-groups for a stream and head
 };
 
 Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_positions) {
