@@ -729,7 +729,7 @@ struct Kv8Run {
     size_t q_stride;
     int group;
     float scale;  // of the scores, times log2 e
-    int max_positions, splits, chunks;  // 64-key chunks of a split
+    int max_positions, splits;
     float *part_acc, *part_ml;
     float *out;  // splits = 1: the rows themselves
     size_t out_stride;
@@ -820,9 +820,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     const int end = span.first + span.count, newest = (end - 1) / kBlockPos;
     const int top = span.first + min(span.count, (min(bx * 4 + 3, tiles - 1) / a.group + 1) * 16) - 1;
     const int keys = min(newest * kBlockPos, top + 1);  // of blocks, to be seen by some row here
-    const int c0 = split * a.chunks, c1 = min(c0 + a.chunks, (keys + 63) / 64);
-    const bool last_split = newest / 4 >= c0 && newest / 4 < c0 + a.chunks;
-    if (c0 * 64 > top) return;
+    // Splits take the chunks in turn, so that each has its share of every row's keys.
+    const int c0 = split, stride = a.splits, c1 = (keys + 63) / 64;
     const int p0 = span.first + r0, p = i < live ? p0 + i : -1;  // this lane's row
     const int wave_top = p0 + live - 1;
     const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
@@ -864,7 +863,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     }
 
     // Chunk c: its bytes requested, then turned into LDS; wave w takes block w.
-    // The block's id and scales of chunk c0 + j wait in lane j (j below 64, then
+    // The block's id and scales of the j-th chunk wait in lane j (j below 64, then
     // the next 64): no chunk waits for its own.
     i32x4 kr[KB], vr[KB];
     int id_of = 0;
@@ -872,8 +871,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     bool wild = false;
     const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
     auto look_up = [&](int c) {
-        const int b = (c + lane) * 4 + wave;
-        const bool in = c + lane < c1 && b * kBlockPos < keys;
+        const int at = c + lane * stride, b = at * 4 + wave;
+        const bool in = at < c1 && b * kBlockPos < keys;
         const int raw = in ? table[b] : 0;
         wild |= (unsigned)raw >= kv.blocks;
         id_of = (unsigned)raw < kv.blocks ? raw : 0;
@@ -885,8 +884,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             if (scale_of.y != scale_of.y) scale_of = make_float2(scale_of.y, 0.0f);
         }
     };
-    auto request = [&](int c) {
-        const int j = (c - c0) & 63;
+    auto request = [&](int c, int n) {
+        const int j = n & 63;
         if (j == 0) look_up(c);
         const unsigned id = (unsigned)__builtin_amdgcn_readlane(id_of, j);
         sc = make_float2(lane_value(scale_of.x, j), lane_value(scale_of.y, j));
@@ -1006,15 +1005,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     };
 
     if (c0 < c1) {
-        request(c0);
+        request(c0, 0);
         stage(0);
         __syncthreads();
-        for (int c = c0; c < c1; c++) {
-            const int buf = (c - c0) & 1;
-            if (c + 1 < c1) request(c + 1);
+        for (int c = c0, n = 0; c < c1; c += stride, n++) {
+            const int buf = n & 1;
+            const bool more = c + stride < c1;
+            if (more) request(c + stride, n + 1);
             if (live > 0 && c * 64 <= wave_top)
                 attend(buf, c, c * 64 + 63 > p0 || c * 64 + 64 > keys || live < 16);
-            if (c + 1 < c1) stage(buf ^ 1);
+            if (more) stage(buf ^ 1);
             __syncthreads();
         }
     }
@@ -1027,7 +1027,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     for (int t = 0; t < T; t++)
 #pragma unroll
         for (int r = 0; r < 4; r++) acc[t][r] *= back;
-    if (last_split && wave_top >= newest * kBlockPos) {
+    if (split == newest / 4 % stride && wave_top >= newest * kBlockPos) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < KB; n++)
@@ -1104,49 +1104,55 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     flag_nonfinite(status, bad);
 }
 
-// The splits of a row's query head joined, one wave for 64 dims. `keys`: of a split.
+// The splits of a row's query head joined: D / 4 lanes for each, 4 dims a lane.
+// `keys`: of a split, or 0: every split has keys of every row, or says that it has
+// none. Eight splits' parts are on their way at once.
 template <int D>
-__global__ __launch_bounds__(64) void k_kv8_join(Kv8 kv, Kv8Rows rows, const float *part_acc,
-                                                 const float *part_ml, int group,
-                                                 int max_positions, int splits, int keys,
-                                                 float *out, size_t out_stride, int *status) {
-    const int s = blockIdx.z, i = blockIdx.y, qh = blockIdx.x / (D / 64);
-    const int d = blockIdx.x % (D / 64) * 64 + threadIdx.x;
+__global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const float *part_acc,
+                                                  const float *part_ml, int group,
+                                                  int max_positions, int splits, int keys,
+                                                  float *out, size_t out_stride, int *status) {
+    const int s = blockIdx.z, wide = kv.heads * group;
+    const size_t e = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int d = (int)(e % (D / 4)) * 4, qh = (int)(e / (D / 4) % wide);
+    const size_t i = e / (D / 4) / wide;
     const Kv8Span span = kv8_span(kv, rows, s, max_positions, false, status);
-    if (i >= span.count || (!span.live && span.first >= 0)) return;
-    const size_t row = (size_t)(span.row0 + i);
+    if (i >= (size_t)span.count || (!span.live && span.first >= 0)) return;
+    const size_t row = span.row0 + i;
     float *dst = out + row * out_stride + (size_t)qh * D + d;
     if (!span.live) {
-        *dst = 0.0f;
+        *(float4 *)dst = make_float4(0.f, 0.f, 0.f, 0.f);
         return;
     }
-    const int n = (span.first + i) / keys + 1;
-    const size_t at = (row * kv.heads * group + qh) * splits;
-    // Lane j has split j's maximum and sum (and j + 64's, ...).
-    float mx = -INFINITY, total = 0.0f, o = 0.0f;
-    for (int j = threadIdx.x; j < n; j += 64) mx = fmaxf(mx, part_ml[(at + j) * 2]);
-    mx = wave_max(mx);
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        const int j = j0 + threadIdx.x;
-        const float2 ml = j < n ? *(const float2 *)(part_ml + (at + j) * 2)
-                                : make_float2(-INFINITY, 0.0f);
-        const float c = __builtin_amdgcn_exp2f(ml.x - mx);
-        total = fmaf(ml.y, c, total);
-        const int last = min(64, n - j0);
-        for (int k = 0; k < last; k += 8) {
-            float x[8];  // eight rows on their way at once
+    const int n = keys ? (span.first + (int)i) / keys + 1 : splits;
+    const size_t at = (row * wide + qh) * splits;
+    float mx = -INFINITY;
+    for (int j = 0; j < n; j += 8)
 #pragma unroll
-            for (int u = 0; u < 8; u++)
-                x[u] = part_acc[(at + j0 + min(k + u, last - 1)) * D + d];
+        for (int k = 0; k < 8; k++) mx = fmaxf(mx, part_ml[(at + min(j + k, n - 1)) * 2]);
+    float total = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < n; j += 8) {
+        float2 ml[8];
+        float4 x[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++)
-                if (k + u < last) o = fmaf(x[u], lane_value(c, k + u), o);
+        for (int k = 0; k < 8; k++) {
+            ml[k] = *(const float2 *)(part_ml + (at + min(j + k, n - 1)) * 2);
+            x[k] = *(const float4 *)(part_acc + (at + min(j + k, n - 1)) * D + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float c = j + k < n ? __builtin_amdgcn_exp2f(ml[k].x - mx) : 0.0f;
+            total = fmaf(ml[k].y, c, total);
+            o.x = fmaf(x[k].x, c, o.x);
+            o.y = fmaf(x[k].y, c, o.y);
+            o.z = fmaf(x[k].z, c, o.z);
+            o.w = fmaf(x[k].w, c, o.w);
         }
     }
-    total = wave_sum(total);
-    o = o / total;
-    *dst = o;
-    flag_nonfinite(status, !isfinite(o));
+    o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
+    *(float4 *)dst = o;
+    flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
 }
 
 }  // namespace pgpu
@@ -1328,11 +1334,9 @@ Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_posi
     d.tiles = ((r->max_rows + 15) / 16 * group + 3) / 4;
     const size_t groups = (size_t)d.tiles * kv->heads * r->streams;
     const int chunks = (max_positions - 1) / 64 + 1;
-    int want = groups >= 512 ? 1 : (int)(512 / groups);
-    if (want > chunks / 4) want = chunks / 4 < 1 ? 1 : chunks / 4;
-    const int each = (chunks + want - 1) / want;
-    d.keys = each * 64;
-    d.splits = (chunks + each - 1) / each;
+    d.splits = groups >= 512 ? 1 : (int)(512 / groups);
+    if (d.splits > chunks / 4) d.splits = chunks / 4 < 1 ? 1 : chunks / 4;
+    d.keys = 0;
     return d;
 }
 
@@ -1344,7 +1348,7 @@ int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal
     float *out = a.out;
     if (r.offsets) {
         const Kv8Run run = {a.q, a.q_stride, a.group, a.scale, a.max_positions, d.splits,
-                            d.keys / 64, a.part_acc, a.part_ml, out, a.out_stride};
+                            a.part_acc, a.part_ml, out, a.out_stride};
         hipLaunchKernelGGL(k_kv8_run<D>, dim3(c.heads * d.splits, d.tiles, streams), dim3(256), 0,
                            st, c, r, run, status);
     } else {
@@ -1368,9 +1372,10 @@ int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal
     }
     if (!launch_ok("pgpu_kv8_attention")) return 0;
     if (d.splits == 1) return 1;
-    hipLaunchKernelGGL(k_kv8_join<D>, dim3(wide * (D / 64), r.max_rows, streams), dim3(64), 0, st,
-                       c, r, a.part_acc, a.part_ml, a.group, a.max_positions, d.splits, d.keys,
-                       out, a.out_stride, status);
+    const size_t lanes = (size_t)r.max_rows * wide * (D / 4);
+    hipLaunchKernelGGL(k_kv8_join<D>, dim3((unsigned)((lanes + 255) / 256), 1, streams), dim3(256),
+                       0, st, c, r, a.part_acc, a.part_ml, a.group, a.max_positions, d.splits,
+                       d.keys, out, a.out_stride, status);
     return launch_ok("pgpu_kv8_attention");
 }
 
