@@ -537,7 +537,7 @@ typedef struct {
     const int32_t *first;   /* (dev) [streams] */
     const int32_t *offsets; /* (dev) [streams + 1] or NULL */
     int streams;            /* 1..65535 */
-    int rows, max_rows;
+    int rows, max_rows;     /* max_rows up to 65535 */
 } pgpu_kv8_rows;
 /* Writes rows of keys and values, row r's head h at k[r * row_stride + h *
  * head_dim] (row_stride a multiple of 4, k and v 16-byte aligned): quantises
@@ -577,8 +577,8 @@ int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer, int layers
  * head_dim]. The cache already holds the call's rows; each stream's newest
  * position is that of its last row here. One row a stream, or runs of rows.
  * `max_positions` bounds every position + 1 (a stream past it is left out,
- * status bit 2). A stream with first < 0 gets zero rows. max_rows up to
- * 65535. Strides multiples of 4, pointers 16-byte aligned. `work` (dev): pgpu_kv8_attention_bytes(kv,
+ * status bit 2). A stream with first < 0 gets zero rows. Strides multiples of
+ * 4, pointers 16-byte aligned. `work` (dev): pgpu_kv8_attention_bytes(kv,
  * rows, group, max_positions) bytes that no other call uses at the same time;
  * they need no clearing. */
 size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows, int group,

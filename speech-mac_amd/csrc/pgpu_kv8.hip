@@ -8,6 +8,15 @@
 
 namespace pgpu {
 
+// Rows that a call reads or writes once, past the caches.
+__device__ inline float4 once_load(const float *p) {
+    const f32x4 v = __builtin_nontemporal_load((const f32x4 *)p);
+    return make_float4(v.x, v.y, v.z, v.w);
+}
+__device__ inline void once_store(float *p, float4 v) {
+    __builtin_nontemporal_store(f32x4{v.x, v.y, v.z, v.w}, (f32x4 *)p);
+}
+
 // One layer of the cache, and the rows of a call (pgpu_kv8, pgpu_kv8_rows).
 struct Kv8 {
     int8_t *values;
@@ -77,85 +86,107 @@ __device__ inline float kv8_scale(float top) {
     return fminf(fmaxf(bitsf(bits), 1.17549435e-38f), 0x1.02p+121f);
 }
 
+// Byte b of four numbers -> a word; sel = b | (4 + b) << 8.
+__device__ inline uint32_t pick4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t sel) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, sel),
+                                 __builtin_amdgcn_perm(b, a, sel), 0x05040100u);
+}
+// LDS between the lanes of one wave: nothing is moved across it.
+__device__ inline void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // ------------------------------------------------------------------- writing
 
-// A work-group of 256 threads holds one (block, head): thread u the NV groups
-// of 4 dims at elements 4 (256 i + u) of [16][D], of keys and of values.
+// A wave holds one (block, head): lane (g, c) has rows 4 g .. 4 g + 3 of the 4
+// dims from 4 (c + 16 n) on, n < D / 64: the rows of a byte's word among the
+// values, and the dims of one among the keys.
 template <int D>
 struct Kv8Tile {
-    static constexpr int NV = D / 64;
-    float4 x[2][NV];
+    float4 x[D / 64][4];  // [n][row of the four]
 };
 
 template <int D>
-struct Kv8Shared {
-    float top[2][4];
-    __align__(16) int8_t values[kBlockPos * D];
-};
-
-// The block's 16 rows in x -> the cache. Every thread of the work-group calls
-// it. A non-finite value: a NaN scale, and status bit 1.
-template <int D>
-__device__ inline void kv8_store(const Kv8 &kv, unsigned block, int head, const Kv8Tile<D> &t,
-                                 Kv8Shared<D> &sh, int *status) {
-    constexpr int NV = D / 64;
-    const int u = threadIdx.x, wave = u >> 6;
-    float top[2];
+__device__ inline uint32_t kv8_top(const Kv8Tile<D> &t) {
+    uint32_t top = 0;  // |x| orders like its bits: infinities and NaN come out on top
 #pragma unroll
-    for (int p = 0; p < 2; p++) {
-        float m = 0.0f;
+    for (int n = 0; n < D / 64; n++)
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const float4 v = t.x[p][i];
-            // |x| orders like its bits: infinities and NaN come out on top.
-            m = bitsf(max(max(fbits(m), fbits(v.x) & 0x7fffffffu),
-                          max(fbits(v.y) & 0x7fffffffu,
-                              max(fbits(v.z) & 0x7fffffffu, fbits(v.w) & 0x7fffffffu))));
+        for (int r = 0; r < 4; r++) {
+            const float4 v = t.x[n][r];
+            top = max(max(top, fbits(v.x) & 0x7fffffffu), fbits(v.y) & 0x7fffffffu);
+            top = max(max(top, fbits(v.z) & 0x7fffffffu), fbits(v.w) & 0x7fffffffu);
         }
-        uint32_t b = fbits(m);
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, o));
-        top[p] = bitsf(b);
-    }
-    if ((u & 63) == 0) {
-        sh.top[0][wave] = top[0];
-        sh.top[1][wave] = top[1];
-    }
-    __syncthreads();
-    int8_t *tile = kv.values + kv8_tile<D>(kv, block, head);
-    float scale[2];
-    bool bad = false;
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    return top;
+}
+
+// The block's 16 rows of keys (p = 0) or values (1) -> the cache. `lds`: 16 D
+// bytes of the wave's own. A value that is not finite: a NaN scale, and status
+// bit 1. x / s by the reciprocal, which is off by less than 1.6e-5 below 128;
+// where that could decide a rounding, by the division.
+template <int D>
+__device__ inline void kv8_store(const Kv8 &kv, unsigned block, int head, int p,
+                                 const Kv8Tile<D> &t, uint32_t *lds, int *status) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    int8_t *tile = kv.values + kv8_tile<D>(kv, block, head) + p * kBlockPos * D;
+    const uint32_t top = kv8_top<D>(t);
+    const bool wild = top >= 0x7f800000u;
+    const float s = kv8_scale(bitsf(top)), inverse = 1.0f / s;
 #pragma unroll
-    for (int p = 0; p < 2; p++) {
-        uint32_t b = 0;
-        for (int w = 0; w < 4; w++) b = max(b, fbits(sh.top[p][w]));
-        const bool wild = b >= 0x7f800000u;
-        bad |= wild;
-        const float s = kv8_scale(bitsf(b));
-        scale[p] = wild ? __builtin_nanf("") : s;
+    for (int n = 0; n < D / 64; n++) {
+        float q[4][4], off = 0.0f;  // [row][dim]
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int e = (i * 256 + u) * 4, j = e / D, d = e % D;
-            const float4 v = t.x[p][i];
-            const float f[4] = {v.x, v.y, v.z, v.w};
-            int8_t q[4];
+        for (int r = 0; r < 4; r++) {
+            const float4 x = t.x[n][r];
+            const float f[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                q[k] = wild ? (int8_t)0 : (int8_t)(int)rintf(f[k] / s);
-            if (p == 0) {
-                *(char4 *)(tile + e) = make_char4(q[0], q[1], q[2], q[3]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++) sh.values[kv8_value_at<D>(j, d + k)] = q[k];
+            for (int d = 0; d < 4; d++) {
+                const float y = f[d] * inverse;
+                q[r][d] = rintf(y);
+                off = fmaxf(off, fabsf(y - q[r][d]));
             }
         }
+        if (__any(off > 0.5f - 1.6e-5f))
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float4 x = t.x[n][r];
+                q[r][0] = rintf(x.x / s);
+                q[r][1] = rintf(x.y / s);
+                q[r][2] = rintf(x.z / s);
+                q[r][3] = rintf(x.w / s);
+            }
+        uint32_t u[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int d = 0; d < 4; d++) u[r][d] = wild ? 0u : (uint32_t)(int)q[r][d];
+        // Byte 0 of four numbers -> a word: of a row's dims, or of a dim's rows.
+        if (p == 0) {
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                *(uint32_t *)(tile + (g * 4 + z) * D + n * 64 + c * 4) =
+                    pick4(u[z][0], u[z][1], u[z][2], u[z][3], 0x0400u);
+        } else {
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                lds[kv8_value_at<D>(g * 4, n * 64 + c * 4 + z) / 4] =
+                    pick4(u[0][z], u[1][z], u[2][z], u[3][z], 0x0400u);
+        }
     }
-    __syncthreads();
-    if (u < D) *(int4 *)(tile + kBlockPos * D + u * 16) = *(const int4 *)(sh.values + u * 16);
-    if (u == 0)
-        *(float2 *)(kv.scales + ((size_t)block * kv.heads + head) * 2) =
-            make_float2(scale[0], scale[1]);
-    if (bad && u == 0) atomicOr(status, 1);
+    if (p) {
+        wave_lds_fence();
+#pragma unroll
+        for (int n = 0; n < D / 64; n++)
+            *(uint4 *)(tile + (n * 64 + lane) * 16) = ((const uint4 *)lds)[n * 64 + lane];
+    }
+    if (lane == 0) {
+        kv.scales[((size_t)block * kv.heads + head) * 2 + p] = wild ? __builtin_nanf("") : s;
+        if (wild) atomicOr(status, 1);
+    }
 }
 
 struct Kv8Turn {
@@ -171,208 +202,259 @@ struct Kv8Turn {
     float *q_out;
 };
 
-// 4 dims of a row's head: normalised (weight), turned, scaled; in 64 bits,
-// rounded once. The D / 4 lanes of a row are neighbours in a wave, and all
-// lanes of the wave call it.
+// A row's head in the D / 4 dim groups of 16 lanes (D / 64 to a lane):
+// normalised (weight), turned, scaled; in 64 bits, rounded once. All 16 lanes
+// call it.
 template <int D>
-__device__ inline float4 kv8_turn(float4 x, int d, const float *weight, float epsilon,
-                                  const float *rope_row, float scale) {
-    double y[4] = {x.x, x.y, x.z, x.w};
+__device__ inline void kv8_turn(float4 *x, const float *weight, float epsilon,
+                                const float *rope_row, float scale) {
+    constexpr int N = D / 64;
+    const int c = threadIdx.x & 15;
+    double r = 1.0;
     if (weight) {
-        double sq = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
+        double sq = 0.0;
 #pragma unroll
-        for (int o = 1; o < D / 4; o <<= 1) sq += __shfl_xor(sq, o);
-        const double r = 1.0 / sqrt(sq / D + (double)epsilon);
-        const float4 w = *(const float4 *)(weight + d);
-        y[0] = y[0] * r * w.x;
-        y[1] = y[1] * r * w.y;
-        y[2] = y[2] * r * w.z;
-        y[3] = y[3] * r * w.w;
+        for (int n = 0; n < N; n++) {
+            const double a = x[n].x, b = x[n].y, e = x[n].z, f = x[n].w;
+            sq += a * a + b * b + e * e + f * f;
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) sq += __shfl_xor(sq, o);
+        r = 1.0 / sqrt(sq / D + (double)epsilon);
     }
-    const float4 cs = *(const float4 *)(rope_row + d);
-    const double f = scale;
-    return make_float4((float)((y[0] * cs.x - y[1] * cs.y) * f),
-                       (float)((y[0] * cs.y + y[1] * cs.x) * f),
-                       (float)((y[2] * cs.z - y[3] * cs.w) * f),
-                       (float)((y[2] * cs.w + y[3] * cs.z) * f));
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        double y[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+        if (weight) {
+            const float4 w = *(const float4 *)(weight + n * 64 + c * 4);
+            y[0] = y[0] * r * w.x;
+            y[1] = y[1] * r * w.y;
+            y[2] = y[2] * r * w.z;
+            y[3] = y[3] * r * w.w;
+        }
+        const float4 cs = *(const float4 *)(rope_row + n * 64 + c * 4);
+        const double f = scale;
+        x[n] = make_float4((float)((y[0] * cs.x - y[1] * cs.y) * f),
+                           (float)((y[0] * cs.y + y[1] * cs.x) * f),
+                           (float)((y[2] * cs.z - y[3] * cs.w) * f),
+                           (float)((y[2] * cs.w + y[3] * cs.z) * f));
+    }
 }
 
-// One (block of the call's rows, head) per work-group: y < heads keys and
-// values, past them (rotate) query head y - heads.
+__device__ inline bool fine4(float4 x) {
+    return isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w);
+}
+
+// A wave for each (block of the call's rows, head) of the keys, of the values
+// and (rotate) of the queries; no wave waits for another.
 template <int D, bool ROTATE>
-__global__ __launch_bounds__(256) void k_kv8_write(Kv8 kv, Kv8Rows rows, Kv8Turn a, int *status) {
-    constexpr int NV = D / 64;
-    __shared__ Kv8Shared<D> sh;
-    const int s = blockIdx.z, u = threadIdx.x;
-    const bool queries = ROTATE && (int)blockIdx.y >= kv.heads;
-    const Kv8Span span = kv8_span(kv, rows, s, ROTATE ? a.rope_positions : INT32_MAX - kBlockPos,
-                                  u == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+__global__ __launch_bounds__(256, D == 64 ? 6 : 4) void k_kv8_write(Kv8 kv, Kv8Rows rows,
+                                                                    Kv8Turn a, int *status) {
+    constexpr int N = D / 64;
+    __shared__ __align__(16) uint32_t lds[4][D * 4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int s = blockIdx.z, g = lane >> 4, c = lane & 15;
+    const Kv8Span span = kv8_span(kv, rows, s,
+                                  ROTATE ? a.rope_positions : INT32_MAX - kBlockPos,
+                                  threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
     if (!span.live) return;
     const int end = span.first + span.count;
-    const int block = span.first / kBlockPos + (int)blockIdx.x, newest = (end - 1) / kBlockPos;
-    if (block > newest) return;
-    const int head = queries ? (int)blockIdx.y - kv.heads : (int)blockIdx.y;
+    const int block = span.first / kBlockPos + (int)blockIdx.y, newest = (end - 1) / kBlockPos;
+    const int unit = blockIdx.x * 4 + wave, units = kv.heads * (ROTATE ? 2 + a.group : 2);
+    if (block > newest || unit >= units) return;
     bool bad = false;
 
-    if constexpr (ROTATE) {
-        if (queries) {
-            const int width = kv.heads * a.group * D;
+    if (ROTATE && unit >= 2 * kv.heads) {
+        const int head = unit - 2 * kv.heads, width = kv.heads * a.group * D;
+        float4 x[4][N];
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const int e = (i * 256 + u) * 4, d = e % D, p = block * kBlockPos + e / D;
-                const bool in = p >= span.first && p < end;
-                const size_t row = (size_t)(span.row0 + (in ? p - span.first : 0));
-                float4 x = *(const float4 *)(a.qkv + row * a.row_stride + head * D + d);
-                x = kv8_turn<D>(x, d, a.q_weight, a.epsilon,
-                                a.rope + (size_t)(in ? p : span.first) * D, a.q_scale);
-                if (in) {
-                    *(float4 *)(a.q_out + row * width + head * D + d) = x;
-                    bad |= !(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w));
-                }
-            }
-            flag_nonfinite(status, bad);
-            return;
-        }
-    }
-
-    float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
-    // Rows of block b (the keys and values of this thread's places): the
-    // call's, else what the slot held (only before the call's first row), else 0.
-    auto gather = [&](int b, Kv8Tile<D> &t) {
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int e = (i * 256 + u) * 4, d = e % D, p = b * kBlockPos + e / D;
+        for (int r = 0; r < 4; r++) {
+            const int p = block * kBlockPos + g * 4 + r;
             const bool in = p >= span.first && p < end;
             const size_t row = (size_t)(span.row0 + (in ? p - span.first : 0));
-            if constexpr (ROTATE) {
-                const float *src = a.qkv + row * a.row_stride;
-                float4 k = *(const float4 *)(src + (kv.heads * a.group + head) * D + d);
-                t.x[0][i] = kv8_turn<D>(k, d, a.k_weight, a.epsilon,
-                                        a.rope + (size_t)(in ? p : span.first) * D, 1.0f);
-                t.x[1][i] = *(const float4 *)(src + (kv.heads * (a.group + 1) + head) * D + d);
-            } else {
-                t.x[0][i] = *(const float4 *)(a.qkv + row * a.row_stride + head * D + d);
-                t.x[1][i] = *(const float4 *)(a.v + row * a.row_stride + head * D + d);
-            }
-            if (!in)
 #pragma unroll
-                for (int k = 0; k < 2; k++)
-                    t.x[k][i] = p < span.first ? *(const float4 *)(slot + k * kBlockPos * D + e)
-                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int n = 0; n < N; n++)
+                x[r][n] = once_load(a.qkv + row * a.row_stride + head * D + n * 64 + c * 4);
         }
-    };
-    // The call's rows of block b into the slot.
-    auto keep = [&](int b, const Kv8Tile<D> &t) {
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int e = (i * 256 + u) * 4, p = b * kBlockPos + e / D;
-            if (p < span.first || p >= end) continue;
+        for (int r = 0; r < 4; r++) {
+            const int p = block * kBlockPos + g * 4 + r;
+            if (p < span.first || p >= end) continue;  // the same for the row's 16 lanes
+            const size_t row = (size_t)(span.row0 + p - span.first);
+            kv8_turn<D>(x[r], a.q_weight, a.epsilon, a.rope + (size_t)p * D, a.q_scale);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const float4 x = t.x[k][i];
-                *(float4 *)(slot + k * kBlockPos * D + e) = x;
-                bad |= !(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w));
+            for (int n = 0; n < N; n++) {
+                *(float4 *)(a.q_out + row * width + head * D + n * 64 + c * 4) = x[r][n];
+                bad |= !fine4(x[r][n]);
             }
         }
+        flag_nonfinite(status, bad);
+        return;
+    }
+
+    const int head = unit >> 1, part = unit & 1;  // keys, values
+    float *slot = kv.open + (((size_t)span.slot * kv.heads + head) * 2 + part) * (kBlockPos * D);
+    const float *src = ROTATE ? a.qkv + (size_t)(kv.heads * (a.group + part) + head) * D
+                              : (part ? a.v : a.qkv) + (size_t)head * D;
+    // Rows of block b: the call's, else what the slot held (only before the
+    // call's first row), else 0.
+    auto gather = [&](int b, Kv8Tile<D> &t) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int p = b * kBlockPos + g * 4 + r;
+            const bool held = p < span.first, in = !held && p < end;
+            const float *x = held ? slot + (g * 4 + r) * D
+                                  : src + (size_t)(span.row0 + (in ? p - span.first : 0)) * a.row_stride;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                t.x[n][r] = in || held ? once_load(x + n * 64 + c * 4)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (ROTATE && part == 0)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int p = b * kBlockPos + g * 4 + r;
+                if (p < span.first || p >= end) continue;
+                float4 x[N];
+#pragma unroll
+                for (int n = 0; n < N; n++) x[n] = t.x[n][r];
+                kv8_turn<D>(x, a.k_weight, a.epsilon, a.rope + (size_t)p * D, 1.0f);
+#pragma unroll
+                for (int n = 0; n < N; n++) t.x[n][r] = x[n];
+            }
     };
     Kv8Tile<D> t;
     gather(block, t);
     if ((block + 1) * kBlockPos <= end) {
-        const int id = rows.tables[(size_t)s * rows.table_stride + block];
+        const int id = uniform_load(rows.tables + (size_t)s * rows.table_stride + block);
         if ((unsigned)id < kv.blocks)
-            kv8_store<D>(kv, (unsigned)id, head, t, sh, status);
-        else if (u == 0)
+            kv8_store<D>(kv, (unsigned)id, head, part, t, lds[wave], status);
+        else if (lane == 0)
             atomicOr(status, 2);
     }
-    // The first block's work-group, which reads the slot's earlier rows, also
-    // replaces them: its threads have all read them by then.
-    if (blockIdx.x != 0) return;
-    __syncthreads();
+    // The first block's wave, which reads the slot's earlier rows, also replaces
+    // them, by the call's rows of the newest block.
+    if (blockIdx.y != 0) return;
     if (block != newest) gather(newest, t);
-    keep(newest, t);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int p = newest * kBlockPos + g * 4 + r;
+        if (p < span.first || p >= end) continue;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            *(float4 *)(slot + (g * 4 + r) * D + n * 64 + c * 4) = t.x[n][r];
+            bad |= !fine4(t.x[n][r]);
+        }
+    }
     flag_nonfinite(status, bad);
 }
 
-// The open slots' full blocks -> the cache. Layers and streams in z.
+// The open slots' full blocks -> the cache, a wave for each (head, keys or values,
+// layer, stream).
 template <int D>
 __global__ __launch_bounds__(256) void k_kv8_close(Kv8 kv, size_t layer_values,
                                                    size_t layer_scales, size_t layer_open,
                                                    const int32_t *tables, int table_stride,
                                                    const int32_t *slots, const int32_t *positions,
                                                    int *status) {
-    __shared__ Kv8Shared<D> sh;
-    const int s = blockIdx.z, head = blockIdx.x, layer = blockIdx.y, u = threadIdx.x;
-    const int p = positions[s];
-    if (p < 0 || p % kBlockPos != kBlockPos - 1) return;
+    __shared__ __align__(16) uint32_t lds[4][D * 4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int s = blockIdx.z, layer = blockIdx.y, head = blockIdx.x * 2 + wave / 2, part = wave & 1;
+    const int p = uniform_load(positions + s);
+    if (p < 0 || p % kBlockPos != kBlockPos - 1 || head >= kv.heads) return;
     const int id = p / kBlockPos < table_stride
-                       ? tables[(size_t)s * table_stride + p / kBlockPos] : -1;
-    const int slot = slots[s];
+                       ? uniform_load(tables + (size_t)s * table_stride + p / kBlockPos) : -1;
+    const int slot = uniform_load(slots + s);
     if ((unsigned)id >= kv.blocks || (unsigned)slot >= kv.slots) {
-        if (u == 0) atomicOr(status, 2);
+        if (lane == 0) atomicOr(status, 2);
         return;
     }
     kv.values += layer * layer_values;
     kv.scales += layer * layer_scales;
     const float *src = kv.open + layer * layer_open +
-                       ((size_t)slot * kv.heads + head) * (2 * kBlockPos * D);
+                       (((size_t)slot * kv.heads + head) * 2 + part) * (kBlockPos * D);
     Kv8Tile<D> t;
 #pragma unroll
-    for (int k = 0; k < 2; k++)
+    for (int n = 0; n < D / 64; n++)
 #pragma unroll
-        for (int i = 0; i < D / 64; i++)
-            t.x[k][i] = *(const float4 *)(src + k * kBlockPos * D + (i * 256 + u) * 4);
-    kv8_store<D>(kv, (unsigned)id, head, t, sh, status);
+        for (int r = 0; r < 4; r++)
+            t.x[n][r] = *(const float4 *)(src + ((lane >> 4) * 4 + r) * D + n * 64 + (lane & 15) * 4);
+    kv8_store<D>(kv, (unsigned)id, head, part, t, lds[wave], status);
 }
 
 // ------------------------------------------------------------------- reading
 
+// A wave for each (block of the rows read, head).
 template <int D>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8 kv, Kv8Rows rows, const int32_t *lengths,
                                                   float *k, float *v, size_t row_stride,
                                                   int *status) {
-    constexpr int NV = D / 64;
-    __shared__ __align__(16) int8_t sh[kBlockPos * D];
-    const int s = blockIdx.z, head = blockIdx.y, u = threadIdx.x;
-    const Kv8Span span = kv8_span(kv, rows, s, lengths[s],
-                                  u == 0 && blockIdx.x == 0 && head == 0, status);
-    if (!span.live) return;
+    constexpr int N = D / 64;
+    __shared__ __align__(16) uint32_t lds[4][D * 4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int s = blockIdx.z, head = blockIdx.x * 4 + wave, g = lane >> 4, c = lane & 15;
+    const int length = uniform_load(lengths + s);
+    const Kv8Span span = kv8_span(kv, rows, s, length,
+                                  threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+    if (!span.live || head >= kv.heads) return;
     const int end = span.first + span.count;
-    const int block = span.first / kBlockPos + (int)blockIdx.x;
+    const int block = span.first / kBlockPos + (int)blockIdx.y;
     if (block * kBlockPos >= end) return;
-    const bool open = block == (lengths[s] - 1) / kBlockPos;
-    const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
-    const int8_t *tile = nullptr;
-    float2 scale = make_float2(1.0f, 1.0f);
-    if (!open) {
-        const int id = rows.tables[(size_t)s * rows.table_stride + block];
+    float4 x[N][4], y[N][4];
+    if (block == (length - 1) / kBlockPos) {
+        const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int e = (g * 4 + r) * D + n * 64 + c * 4;
+                x[n][r] = *(const float4 *)(slot + e);
+                y[n][r] = *(const float4 *)(slot + kBlockPos * D + e);
+            }
+    } else {
+        const int id = uniform_load(rows.tables + (size_t)s * rows.table_stride + block);
         if ((unsigned)id >= kv.blocks) {
-            if (u == 0) atomicOr(status, 2);
+            if (lane == 0) atomicOr(status, 2);
             return;
         }
-        tile = kv.values + kv8_tile<D>(kv, (unsigned)id, head);
-        scale = *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
-        if (u < D) *(int4 *)(sh + u * 16) = *(const int4 *)(tile + kBlockPos * D + u * 16);
-        __syncthreads();
+        const int8_t *tile = kv.values + kv8_tile<D>(kv, (unsigned)id, head);
+        const float2 scale = *(const float2 *)(kv.scales + ((size_t)id * kv.heads + head) * 2);
+        uint32_t q[N][4];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                q[n][r] = *(const uint32_t *)(tile + (g * 4 + r) * D + n * 64 + c * 4);
+            ((uint4 *)lds[wave])[n * 64 + lane] =
+                *(const uint4 *)(tile + kBlockPos * D + (n * 64 + lane) * 16);
+        }
+        wave_lds_fence();
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            uint32_t w[4];  // of dim z: the four rows' bytes
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                w[z] = lds[wave][kv8_value_at<D>(g * 4, n * 64 + c * 4 + z) / 4];
+            auto byte = [](uint32_t a, int i) { return (float)(int8_t)(a >> (8 * i)); };
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                x[n][r] = make_float4(byte(q[n][r], 0) * scale.x, byte(q[n][r], 1) * scale.x,
+                                      byte(q[n][r], 2) * scale.x, byte(q[n][r], 3) * scale.x);
+                y[n][r] = make_float4(byte(w[0], r) * scale.y, byte(w[1], r) * scale.y,
+                                      byte(w[2], r) * scale.y, byte(w[3], r) * scale.y);
+            }
+        }
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int e = (i * 256 + u) * 4, j = e / D, d = e % D, p = block * kBlockPos + j;
+    for (int r = 0; r < 4; r++) {
+        const int p = block * kBlockPos + g * 4 + r;
         if (p < span.first || p >= end) continue;
-        float4 x, y;
-        if (open) {
-            x = *(const float4 *)(slot + e);
-            y = *(const float4 *)(slot + kBlockPos * D + e);
-        } else {
-            const char4 q = *(const char4 *)(tile + e);
-            x = make_float4(q.x * scale.x, q.y * scale.x, q.z * scale.x, q.w * scale.x);
-            y = make_float4(sh[kv8_value_at<D>(j, d)] * scale.y,
-                            sh[kv8_value_at<D>(j, d + 1)] * scale.y,
-                            sh[kv8_value_at<D>(j, d + 2)] * scale.y,
-                            sh[kv8_value_at<D>(j, d + 3)] * scale.y);
+        const size_t at = (size_t)(span.row0 + p - span.first) * row_stride + head * D + c * 4;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            once_store(k + at + n * 64, x[n][r]);
+            once_store(v + at + n * 64, y[n][r]);
         }
-        const size_t at = (size_t)(span.row0 + p - span.first) * row_stride + head * D + d;
-        *(float4 *)(k + at) = x;
-        *(float4 *)(v + at) = y;
     }
 }
 
@@ -380,8 +462,8 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 kv, Kv8Rows rows, const in
 
 // The sums are taken on the int8 matrix instruction v_mfma_i32_16x16x64_i8:
 // the cache's bytes are its operands as they are stored, nothing is converted.
-// A query (and the weights of 64 keys) becomes a fixed-point number of 22 to 23
-// bits below its largest element, split into three signed bytes that stand in
+// A query (and the weights of 64 keys) becomes a fixed-point number of 23 bits
+// below its largest element, split into three signed bytes that stand in
 // three rows of the other operand: products and sums are exact, and
 //   (hi * 2^16 + mid * 2^8 + lo) * step
 // has the precision of fp32. Four queries fill the 16 rows (row 4 j + t: byte t
@@ -403,24 +485,21 @@ __device__ inline float row16_max(float v) {
 }
 
 // Fixed point below `top` (>= 0, the largest magnitude): the power of two that
-// takes it into [2^21, 2^22). Below 2^-105 the step stays at 2^-126.
+// takes it above 2^22 / 1.004 and not above 127 * 2^16 + 127 * 2^8 + 127, the
+// largest sum of three signed bytes (0x11000 carries a significand above 1.992
+// into the exponent). Below 2^-104 the step stays at 2^-126.
 __device__ inline int fix_exponent(float top) {
-    return min(126, 148 - (int)(fbits(top) >> 23));
+    return min(126, 149 - (int)((fbits(top) + 0x11000u) >> 23));
 }
 __device__ inline float power_of_2(int e) { return bitsf((uint32_t)(127 + e) << 23); }
 // The three bytes of the number (bits 0..23), each signed: n = sum of
-// byte t * 256^t, |n| <= 2^22.
+// byte t * 256^t.
 __device__ inline uint32_t fix_bytes(float x, float mul) {
     return ((uint32_t)(int)rintf(x * mul) + 0x808080u) ^ 0x808080u;
 }
 // Which byte of a number stands in row t of its query: the highest in row 0.
 // Row 3 repeats the lowest byte; nothing reads its sums.
 __device__ inline uint32_t row_byte(int t) { return t < 2 ? 2u - t : 0u; }
-// Byte b of four numbers -> a word; sel = b | (4 + b) << 8.
-__device__ inline uint32_t pick4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t sel) {
-    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, sel),
-                                 __builtin_amdgcn_perm(b, a, sel), 0x05040100u);
-}
 __device__ inline float fix_sum(i32x4 c) {
     return fmaf((float)(c.x * 256 + c.y), 256.0f, (float)c.z);
 }
@@ -436,13 +515,6 @@ __device__ inline uint32_t quad_lane(uint32_t v) {
 
 __device__ inline i32x4 stream_load16(const int8_t *p) {
     return __builtin_nontemporal_load((const i32x4 *)p);
-}
-
-// LDS between the lanes of one wave: nothing is moved across it.
-__device__ inline void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 struct Kv8Decode {
@@ -926,14 +998,18 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
         // The last key that this lane's row sees, from its own first one on.
         const int last = min(p, keys - 1) - c * 64 - g * 4;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; t++) w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const f16x8 kk = sh.k[buf][t][k][lane];
-                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qhi[k], w[t], 0, 0, 0);
-                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qlo[k], w[t], 0, 0, 0);
-            }
+        for (int k = 0; k < KS; k++) {
+            f16x8 kk[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) kk[t] = sh.k[buf][t][k][lane];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t], qhi[k], w[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t], qlo[k], w[t], 0, 0, 0);
         }
         if (masked)
 #pragma unroll
@@ -995,12 +1071,18 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
         const f16x8 pl[2] = {join_pairs(lo[0][0], lo[0][1], lo[1][0], lo[1][1]),
                              join_pairs(lo[2][0], lo[2][1], lo[3][0], lo[3][1])};
 #pragma unroll
-        for (int t = 0; t < T; t++)
+        for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const f16x8 v = sh.v[buf][n][t][lane];
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[n], acc[t], 0, 0, 0);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[n], acc[t], 0, 0, 0);
+            for (int t0 = 0; t0 < T; t0 += 4) {
+                f16x8 v[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) v[t] = sh.v[buf][n][t0 + t][lane];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], ph[n], acc[t0 + t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], pl[n], acc[t0 + t], 0, 0, 0);
             }
     };
 
@@ -1126,30 +1208,38 @@ __global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const fl
     }
     const int n = keys ? (span.first + (int)i) / keys + 1 : splits;
     const size_t at = (row * wide + qh) * splits;
-    float mx = -INFINITY;
-    for (int j = 0; j < n; j += 8)
+    // Lane j of the D / 4 has split j's maximum and sum, and the next D / 4's.
+    constexpr int L = D / 4;
+    const int lane = threadIdx.x % L;
+    float mx = -INFINITY, total = 0.0f;
+    for (int j = lane; j < n; j += L) mx = fmaxf(mx, part_ml[(at + j) * 2]);
 #pragma unroll
-        for (int k = 0; k < 8; k++) mx = fmaxf(mx, part_ml[(at + min(j + k, n - 1)) * 2]);
-    float total = 0.0f;
+    for (int z = 1; z < L; z <<= 1) mx = fmaxf(mx, __shfl_xor(mx, z));
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = 0; j < n; j += 8) {
-        float2 ml[8];
-        float4 x[8];
+    for (int j0 = 0; j0 < n; j0 += L) {
+        const int last = min(L, n - j0);
+        const float2 ml = lane < last ? *(const float2 *)(part_ml + (at + j0 + lane) * 2)
+                                      : make_float2(-INFINITY, 0.0f);
+        const float c = __builtin_amdgcn_exp2f(ml.x - mx);
+        total = fmaf(ml.y, c, total);
+        for (int j = 0; j < last; j += 8) {
+            float4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            ml[k] = *(const float2 *)(part_ml + (at + min(j + k, n - 1)) * 2);
-            x[k] = *(const float4 *)(part_acc + (at + min(j + k, n - 1)) * D + d);
-        }
+            for (int k = 0; k < 8; k++)
+                x[k] = *(const float4 *)(part_acc + (at + j0 + min(j + k, last - 1)) * D + d);
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float c = j + k < n ? __builtin_amdgcn_exp2f(ml[k].x - mx) : 0.0f;
-            total = fmaf(ml[k].y, c, total);
-            o.x = fmaf(x[k].x, c, o.x);
-            o.y = fmaf(x[k].y, c, o.y);
-            o.z = fmaf(x[k].z, c, o.z);
-            o.w = fmaf(x[k].w, c, o.w);
+            for (int k = 0; k < 8; k++) {
+                const float w = __shfl(c, j + k, L);  // 0 past the last
+                if (j + k >= last) continue;
+                o.x = fmaf(x[k].x, w, o.x);
+                o.y = fmaf(x[k].y, w, o.y);
+                o.z = fmaf(x[k].z, w, o.z);
+                o.w = fmaf(x[k].w, w, o.w);
+            }
         }
     }
+#pragma unroll
+    for (int z = 1; z < L; z <<= 1) total += __shfl_xor(total, z);
     o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
     *(float4 *)dst = o;
     flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
@@ -1174,7 +1264,8 @@ bool cache_ok(const pgpu_kv8 *kv) {
 
 bool rows_ok(const pgpu_kv8_rows *r) {
     return r && r->tables && r->table_stride > 0 && r->slots && r->first && r->streams > 0 &&
-           r->streams <= 65535 && r->rows >= 0 && r->max_rows >= 0 && r->max_rows <= r->rows &&
+           r->streams <= 65535 && r->rows >= 0 && r->max_rows >= 0 && r->max_rows <= 65535 &&
+           r->max_rows <= r->rows &&
            (r->offsets ? (r->max_rows > 0 || r->rows == 0)
                        : (r->rows == r->streams && r->max_rows == 1));
 }
@@ -1203,8 +1294,8 @@ int blocks_of(int max_rows) { return (max_rows + 2 * kBlockPos - 2) / kBlockPos;
 int write_rows(const char *name, void *stream, const pgpu_kv8 *kv, int layer,
                const pgpu_kv8_rows *rows, const Kv8Turn &a, bool rotate, int *status) {
     const Kv8 c = layer_of(kv, layer);
-    const dim3 grid(blocks_of(rows->max_rows), kv->heads * (rotate ? 1 + a.group : 1),
-                    rows->streams);
+    const int units = kv->heads * (rotate ? 2 + a.group : 2);
+    const dim3 grid((units + 3) / 4, blocks_of(rows->max_rows), rows->streams);
     const Kv8Rows r = rows_of(rows);
     if (kv->head_dim == 64 && rotate)
         hipLaunchKernelGGL((k_kv8_write<64, true>), grid, dim3(256), 0, (hipStream_t)stream, c, r,
@@ -1265,7 +1356,7 @@ extern "C" int pgpu_kv8_read(void *stream, const pgpu_kv8 *kv, int layer,
         row_stride < (size_t)kv->heads * kv->head_dim)
         return bad_arguments("pgpu_kv8_read");
     if (rows->rows == 0) return 1;
-    const dim3 grid(blocks_of(rows->max_rows), kv->heads, rows->streams);
+    const dim3 grid((kv->heads + 3) / 4, blocks_of(rows->max_rows), rows->streams);
     if (kv->head_dim == 64)
         hipLaunchKernelGGL(k_kv8_read<64>, grid, dim3(256), 0, (hipStream_t)stream,
                            layer_of(kv, layer), rows_of(rows), lengths, k, v, row_stride, status);
@@ -1284,7 +1375,7 @@ extern "C" int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer,
         return bad_arguments("pgpu_kv8_close");
     const size_t scales = kv->blocks * kv->heads * 2, open = kv->slots * kv->heads * tile_bytes(kv),
                  values = kv->blocks * kv->heads * tile_bytes(kv);
-    const dim3 grid(kv->heads, layers, streams);
+    const dim3 grid((kv->heads + 1) / 2, layers, streams);
     if (kv->head_dim == 64)
         hipLaunchKernelGGL(k_kv8_close<64>, grid, dim3(256), 0, (hipStream_t)stream,
                            layer_of(kv, first_layer), values, scales, open, tables, table_stride,
@@ -1334,8 +1425,10 @@ Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_posi
     d.tiles = ((r->max_rows + 15) / 16 * group + 3) / 4;
     const size_t groups = (size_t)d.tiles * kv->heads * r->streams;
     const int chunks = (max_positions - 1) / 64 + 1;
-    d.splits = groups >= 512 ? 1 : (int)(512 / groups);
-    if (d.splits > chunks / 4) d.splits = chunks / 4 < 1 ? 1 : chunks / 4;
+    d.splits = groups >= 512 ? 1 : (int)(1024 / groups);
+    const int least = r->max_rows <= 16 ? 2 : 4;
+    if (d.splits > chunks / least) d.splits = chunks / least < 1 ? 1 : chunks / least;
+    if (d.splits > 32) d.splits = 32;
     d.keys = 0;
     return d;
 }
@@ -1403,9 +1496,8 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
         return bad_arguments("pgpu_kv8_attention");
     if (rows->rows == 0) return 1;
     const Deal d = deal_of(kv, rows, group, max_positions);
-    // Grid limits; a cache's worst case is far inside them.
-    if (d.splits > 65535 || (size_t)kv->heads * d.splits > 65535 || rows->max_rows > 65535)
-        return bad_arguments("pgpu_kv8_attention");
+    // The grid's limit: 16 million positions of one row a stream.
+    if (d.splits > 65535) return bad_arguments("pgpu_kv8_attention");
     const size_t need = pgpu_kv8_attention_bytes(kv, rows, group, max_positions);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv8_attention (workspace)");
