@@ -61,6 +61,28 @@ int phonon_kv_pool_read(const PhononKvPool *pool, const int32_t *table, size_t t
 /* The pool's device description, for the kernels of phonon_gpu.h. */
 int phonon_kv_pool_view(const PhononKvPool *pool, pgpu_paged_kv *view);
 
+/* A pool that holds its blocks in 8 bits (16 KiB and 128 bytes of scales per
+ * block and layer): pgpu_kv8 of phonon_gpu.h with 8 heads of 64. The block that
+ * a stream is writing stays in fp32 in one of `slots` open slots (64 KiB per
+ * layer), so a stream needs a slot as well as blocks. Blocks are allocated and
+ * released as in any pool; the calls below take its other parts, and the fp32
+ * forms of them (and phonon_kv_pool_fill_normal, _view) refuse it. */
+int phonon_kv_pool_create_q8(size_t layers, size_t blocks, size_t slots, PhononKvPool **pool);
+size_t phonon_kv_pool_free_slots(const PhononKvPool *pool);
+int phonon_kv_pool_alloc_slots(PhononKvPool *pool, size_t count, int32_t *slots);
+int phonon_kv_pool_release_slots(PhononKvPool *pool, size_t count, const int32_t *slots);
+/* phonon_kv_pool_write and _read of one stream. A write appends: positions
+ * below `first` are held already (those of first's block in the slot), and
+ * first + count is the stream's new length. A read gives `length` positions'
+ * newest block from the slot, the others as stored. */
+int phonon_kv_pool_write_q8(PhononKvPool *pool, const int32_t *table, size_t table_len,
+                            int32_t slot, size_t first, size_t count, const float *keys,
+                            const float *values, size_t capacity);
+int phonon_kv_pool_read_q8(const PhononKvPool *pool, const int32_t *table, size_t table_len,
+                           int32_t slot, size_t length, size_t first, size_t count, float *keys,
+                           float *values, size_t capacity);
+int phonon_kv_pool_view_q8(const PhononKvPool *pool, pgpu_kv8 *view);
+
 /* A batch of up to max_streams streams of at most max_positions positions
  * (<= 8192) each, bound to a model and a pool with the model's layer count. */
 int phonon_flow_batch_create(const PhononFlowModel *model, PhononKvPool *pool,
@@ -73,6 +95,14 @@ void phonon_flow_batch_destroy(PhononFlowBatch *batch);
 int phonon_flow_batch_set_streams(PhononFlowBatch *batch, size_t streams,
                                   const size_t *positions, const int32_t *tables,
                                   size_t table_len);
+/* The same over an 8-bit pool; slots[s]: the stream's open slot (its own), which
+ * holds the rows of the block of position positions[s] before it. Steps run phase
+ * by phase, in one group: a step's attention reads each stream's newest block in
+ * fp32 and the earlier ones in 8 bits, and a block is stored by the step of its
+ * last position. */
+int phonon_flow_batch_set_streams_q8(PhononFlowBatch *batch, size_t streams,
+                                     const size_t *positions, const int32_t *tables,
+                                     size_t table_len, const int32_t *slots);
 /* One decode step of every active stream: inputs/outputs host [streams][512].
  * Appends one K/V row per layer at each stream's position, then advances the
  * positions. Returns 0 (positions still advanced, outputs unspecified) if
@@ -98,6 +128,16 @@ int phonon_flow_batch_prefill_device(PhononFlowBatch *batch, size_t streams, con
                                      const size_t *counts, const int32_t *tables,
                                      size_t table_len, const float *inputs, float theta,
                                      float *outputs);
+/* The same over an 8-bit pool, slots[i] being stream i's open slot. Each layer's
+ * rows are written before its attention, so a row attends to every block but its
+ * prompt's newest as it is stored in 8 bits, its own one included: outputs depend
+ * on how a prompt is cut into calls by as much as 8 bits do. (Exact mode 1 sets
+ * the projections' terms; the attention has fp32's precision in every mode.) */
+int phonon_flow_batch_prefill_q8_device(PhononFlowBatch *batch, size_t streams,
+                                        const size_t *first, const size_t *counts,
+                                        const int32_t *tables, size_t table_len,
+                                        const int32_t *slots, const float *inputs, float theta,
+                                        float *outputs);
 /* Arithmetic of phase-by-phase batched prefills: 1 exact: the projections
  * with the decode step's three bf16 split terms and the decode step's split
  * attention and merge, so every output row has the bits of single steps;

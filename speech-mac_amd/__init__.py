@@ -209,6 +209,17 @@ EXPORTS = {
     "phonon_kv_pool_write": (_i, [_vp, _i32p, _sz, _sz, _sz, _fp, _fp, _sz]),
     "phonon_kv_pool_read": (_i, [_vp, _i32p, _sz, _sz, _sz, _fp, _fp, _sz]),
     "phonon_kv_pool_view": (_i, [_vp, _kvp]),
+    "phonon_kv_pool_create_q8": (_i, [_sz, _sz, _sz, _pp]),
+    "phonon_kv_pool_free_slots": (_sz, [_vp]),
+    "phonon_kv_pool_alloc_slots": (_i, [_vp, _sz, _i32p]),
+    "phonon_kv_pool_release_slots": (_i, [_vp, _sz, _i32p]),
+    "phonon_kv_pool_write_q8": (_i, [_vp, _i32p, _sz, ctypes.c_int32, _sz, _sz, _fp, _fp, _sz]),
+    "phonon_kv_pool_read_q8": (_i, [_vp, _i32p, _sz, ctypes.c_int32, _sz, _sz, _sz, _fp, _fp,
+                                    _sz]),
+    "phonon_kv_pool_view_q8": (_i, [_vp, _k8p]),
+    "phonon_flow_batch_set_streams_q8": (_i, [_vp, _sz, _szp, _i32p, _sz, _i32p]),
+    "phonon_flow_batch_prefill_q8_device": (_i, [_vp, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _f,
+                                                 _vp]),
     "phonon_flow_batch_create": (_i, [_vp, _vp, _sz, _sz, _pp]),
     "phonon_flow_batch_destroy": (None, [_vp]),
     "phonon_flow_batch_set_streams": (_i, [_vp, _sz, _szp, _i32p, _sz]),

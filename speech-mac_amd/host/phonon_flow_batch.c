@@ -27,11 +27,18 @@ struct PhononFlowModel {
     size_t allocation_count, device_bytes;
 };
 
-struct PhononKvPool {
-    pgpu_paged_kv kv;
+/* Ids 0 .. count - 1, handed out low ones first. */
+typedef struct {
     int32_t *free_ids;
-    size_t free_count;
+    size_t count, free_count;
     unsigned char *in_use;
+} PhIds;
+
+struct PhononKvPool {
+    pgpu_paged_kv kv;   /* an 8-bit pool's: its open slots, as blocks */
+    int q8;
+    pgpu_kv8 kv8;       /* of an 8-bit pool */
+    PhIds blocks, slots;
 };
 
 struct PhononFlowBatch {
@@ -98,6 +105,17 @@ struct PhononFlowBatch {
         unsigned wait_us;           /* give-up bound of the tasks' waits (0: 1 s) */
     } fl;
     int *status;
+    /* Over an 8-bit pool: each stream's open slot, the tables by which the
+     * projections append to it (every entry the slot), the attention's rows and
+     * workspace; a prefill's projected rows, and zeros for their residual. */
+    struct {
+        int32_t *slots, *slot_tables;
+        float *att, *qkv, *zeros;
+        void *work;
+        size_t work_bytes;
+        const int32_t *pre_slots, *pre_first, *pre_offsets; /* (dev) in pre.stage_dev */
+        size_t pre_streams, pre_rows;
+    } q8;
     pgpu_attention_scratch scratch;
     size_t *host_positions;
     int pos_lag;                    /* one-launch steps the device positions trail
@@ -260,6 +278,51 @@ size_t phonon_flow_model_device_bytes(const PhononFlowModel *model) {
 
 /* ----------------------------------------------------------------- pool -- */
 
+static int ids_init(PhIds *ids, size_t count) {
+    ids->free_ids = malloc(count * sizeof(int32_t));
+    ids->in_use = calloc(count, 1);
+    ids->count = count;
+    ids->free_count = 0;
+    if (!ids->free_ids || !ids->in_use)
+        return 0;
+    for (size_t i = 0; i < count; i++)
+        ids->free_ids[i] = (int32_t)(count - 1 - i);
+    ids->free_count = count;
+    return 1;
+}
+
+static void ids_free(PhIds *ids) {
+    free(ids->free_ids);
+    free(ids->in_use);
+}
+
+static int ids_take(PhIds *ids, size_t count, int32_t *out) {
+    if ((count && !out) || count > ids->free_count)
+        return 0;
+    for (size_t i = 0; i < count; i++) {
+        out[i] = ids->free_ids[--ids->free_count];
+        ids->in_use[out[i]] = 1;
+    }
+    return 1;
+}
+
+static int ids_give(PhIds *ids, size_t count, const int32_t *in) {
+    if (count && !in)
+        return 0;
+    /* All or none: an id given twice is one that is not in use. */
+    size_t n = 0;
+    while (n < count && in[n] >= 0 && (size_t)in[n] < ids->count && ids->in_use[in[n]])
+        ids->in_use[in[n++]] = 0;
+    if (n < count) {
+        while (n)
+            ids->in_use[in[--n]] = 1;
+        return 0;
+    }
+    for (size_t i = 0; i < count; i++)
+        ids->free_ids[ids->free_count++] = in[i];
+    return 1;
+}
+
 int phonon_kv_pool_create(size_t layers, size_t blocks, PhononKvPool **pool) {
     if (!pool)
         return 0;
@@ -275,19 +338,46 @@ int phonon_kv_pool_create(size_t layers, size_t blocks, PhononKvPool **pool) {
     p->kv.blocks = blocks;
     p->kv.layer_stride = blocks * block_floats;
     p->kv.base = pgpu_malloc(layers * p->kv.layer_stride * sizeof(float));
-    p->free_ids = malloc(blocks * sizeof(int32_t));
-    p->in_use = calloc(blocks, 1);
     /* Zeroed so that never-written slots read as finite values. */
-    if (!p->kv.base || !p->free_ids || !p->in_use ||
+    if (!p->kv.base || !ids_init(&p->blocks, blocks) ||
         !pgpu_memset(ph_stream(), p->kv.base, 0, layers * p->kv.layer_stride * sizeof(float)) ||
         !pgpu_stream_sync(ph_stream())) {
         phonon_kv_pool_destroy(p);
         return 0;
     }
-    /* Hand out low ids first. */
-    for (size_t i = 0; i < blocks; i++)
-        p->free_ids[i] = (int32_t)(blocks - 1 - i);
-    p->free_count = blocks;
+    *pool = p;
+    return 1;
+}
+
+int phonon_kv_pool_create_q8(size_t layers, size_t blocks, size_t slots, PhononKvPool **pool) {
+    if (!pool)
+        return 0;
+    *pool = NULL;
+    const size_t block = (size_t)PH_HEADS * 2 * 16 * PH_HEAD; /* elements of a block */
+    if (!layers || layers > 64 || !blocks || blocks > INT32_MAX || !slots || slots > INT32_MAX ||
+        blocks > SIZE_MAX / (layers * block) ||
+        slots > SIZE_MAX / (layers * block * sizeof(float)) || !ph_init())
+        return 0;
+    PhononKvPool *p = calloc(1, sizeof(*p));
+    if (!p)
+        return 0;
+    const size_t values = layers * blocks * block,
+                 scales = layers * blocks * PH_HEADS * 2 * sizeof(float),
+                 open = layers * slots * block * sizeof(float);
+    p->q8 = 1;
+    p->kv8 = (pgpu_kv8){.values = pgpu_malloc(values), .scales = pgpu_malloc(scales),
+                        .open = pgpu_malloc(open), .layers = (int)layers, .heads = PH_HEADS,
+                        .head_dim = PH_HEAD, .blocks = blocks, .slots = slots};
+    p->kv = (pgpu_paged_kv){.base = p->kv8.open, .layers = (int)layers, .blocks = slots,
+                            .layer_stride = slots * block};
+    void *stream = ph_stream();
+    if (!p->kv8.values || !p->kv8.scales || !p->kv8.open || !ids_init(&p->blocks, blocks) ||
+        !ids_init(&p->slots, slots) || !pgpu_memset(stream, p->kv8.values, 0, values) ||
+        !pgpu_memset(stream, p->kv8.scales, 0, scales) ||
+        !pgpu_memset(stream, p->kv8.open, 0, open) || !pgpu_stream_sync(stream)) {
+        phonon_kv_pool_destroy(p);
+        return 0;
+    }
     *pool = p;
     return 1;
 }
@@ -295,45 +385,48 @@ int phonon_kv_pool_create(size_t layers, size_t blocks, PhononKvPool **pool) {
 void phonon_kv_pool_destroy(PhononKvPool *pool) {
     if (!pool)
         return;
-    if (pool->kv.base) {
+    if (pool->kv.base || pool->kv8.values || pool->kv8.scales)
         (void)pgpu_stream_sync(ph_stream());
-        pgpu_free(pool->kv.base);
-    }
-    free(pool->free_ids);
-    free(pool->in_use);
+    pgpu_free(pool->kv.base); /* an 8-bit pool's open slots */
+    pgpu_free(pool->kv8.values);
+    pgpu_free(pool->kv8.scales);
+    ids_free(&pool->blocks);
+    ids_free(&pool->slots);
     free(pool);
 }
 
 size_t phonon_kv_pool_free_blocks(const PhononKvPool *pool) {
-    return pool ? pool->free_count : 0;
+    return pool ? pool->blocks.free_count : 0;
 }
 
 int phonon_kv_pool_alloc(PhononKvPool *pool, size_t count, int32_t *blocks) {
-    if (!pool || (count && !blocks) || count > pool->free_count)
-        return 0;
-    for (size_t i = 0; i < count; i++) {
-        blocks[i] = pool->free_ids[--pool->free_count];
-        pool->in_use[blocks[i]] = 1;
-    }
-    return 1;
+    return pool && ids_take(&pool->blocks, count, blocks);
 }
 
 int phonon_kv_pool_release(PhononKvPool *pool, size_t count, const int32_t *blocks) {
-    if (!pool || (count && !blocks))
-        return 0;
-    for (size_t i = 0; i < count; i++)
-        if (blocks[i] < 0 || (size_t)blocks[i] >= pool->kv.blocks || !pool->in_use[blocks[i]])
-            return 0;
-    for (size_t i = 0; i < count; i++) {
-        pool->in_use[blocks[i]] = 0;
-        pool->free_ids[pool->free_count++] = blocks[i];
-    }
-    return 1;
+    return pool && ids_give(&pool->blocks, count, blocks);
 }
+
+size_t phonon_kv_pool_free_slots(const PhononKvPool *pool) {
+    return pool ? pool->slots.free_count : 0;
+}
+
+int phonon_kv_pool_alloc_slots(PhononKvPool *pool, size_t count, int32_t *slots) {
+    return pool && ids_take(&pool->slots, count, slots);
+}
+
+int phonon_kv_pool_release_slots(PhononKvPool *pool, size_t count, const int32_t *slots) {
+    return pool && ids_give(&pool->slots, count, slots);
+}
+
+static const char kNotQ8[] = "the pool holds fp32 blocks, not 8-bit ones",
+                  kQ8[] = "the pool holds 8-bit blocks: use the _q8 form of the call";
 
 int phonon_kv_pool_fill_normal(PhononKvPool *pool, uint64_t seed) {
     if (!pool)
         return 0;
+    if (pool->q8)
+        return ph_fail(kQ8);
     return pgpu_fill_normal(ph_stream(), pool->kv.base, pool->kv.layers * pool->kv.layer_stride,
                             seed) &&
            pgpu_stream_sync(ph_stream());
@@ -344,7 +437,18 @@ const pgpu_paged_kv *ph_pool_kv(const PhononKvPool *pool) { return &pool->kv; }
 int phonon_kv_pool_view(const PhononKvPool *pool, pgpu_paged_kv *view) {
     if (!pool || !view)
         return 0;
+    if (pool->q8)
+        return ph_fail(kQ8);
     *view = pool->kv;
+    return 1;
+}
+
+int phonon_kv_pool_view_q8(const PhononKvPool *pool, pgpu_kv8 *view) {
+    if (!pool || !view)
+        return 0;
+    if (!pool->q8)
+        return ph_fail(kNotQ8);
+    *view = pool->kv8;
     return 1;
 }
 
@@ -354,6 +458,8 @@ static int pool_copy(const PhononKvPool *pool, const int32_t *table, size_t tabl
     if (!pool || !table || !keys || !values || !count || first + count > capacity ||
         first + count > table_len * 16 || capacity > PHONON_FLOW_MAX_POSITIONS)
         return 0;
+    if (pool->q8)
+        return ph_fail(kQ8);
     for (size_t i = first / 16; i < (first + count + 15) / 16; i++)
         if (table[i] < 0 || (size_t)table[i] >= pool->kv.blocks)
             return 0;
@@ -402,6 +508,71 @@ int phonon_kv_pool_read(const PhononKvPool *pool, const int32_t *table, size_t t
     return pool_copy(pool, table, table_len, first, count, keys, values, capacity, 1);
 }
 
+/* Positions [first, first + count) of every layer between host arrays (the
+ * reference layout) and an 8-bit pool; `length`: the positions that the stream
+ * holds, with those written. A layer at a time through [count][512] rows. */
+static int pool_copy_q8(const PhononKvPool *pool, const int32_t *table, size_t table_len,
+                        int32_t slot, size_t length, size_t first, size_t count, float *keys,
+                        float *values, size_t capacity, int to_host) {
+    if (!pool || !table || !keys || !values || !count || count > capacity ||
+        first > capacity - count || first + count > length || length > table_len * 16 ||
+        capacity > PHONON_FLOW_MAX_POSITIONS)
+        return 0;
+    if (!pool->q8)
+        return ph_fail(kNotQ8);
+    if (slot < 0 || (size_t)slot >= pool->slots.count)
+        return 0;
+    for (size_t i = first / 16; i < (first + count + 15) / 16; i++)
+        if (table[i] < 0 || (size_t)table[i] >= pool->blocks.count)
+            return 0;
+    const size_t bytes = count * PH_WIDTH * sizeof(float);
+    const int32_t host[] = {slot, (int32_t)first, 0, (int32_t)count, (int32_t)length, 0};
+    void *stream = ph_stream();
+    float *dk = pgpu_malloc(bytes), *dv = pgpu_malloc(bytes);
+    int32_t *dt = pgpu_malloc(table_len * sizeof(int32_t)), *dh = pgpu_malloc(sizeof(host));
+    int ok = dk && dv && dt && dh &&
+             pgpu_copy_h2d(stream, dt, table, table_len * sizeof(int32_t)) &&
+             pgpu_copy_h2d(stream, dh, host, sizeof(host));
+    const pgpu_kv8_rows rows = {.tables = dt, .table_stride = (int)table_len, .slots = dh,
+                                .first = dh + 1, .offsets = dh + 2, .streams = 1,
+                                .rows = (int)count, .max_rows = (int)count};
+    int *status = (int *)dh + 5;
+    for (size_t l = 0; ok && l < (size_t)pool->kv8.layers; l++) {
+        float *k = keys + (l * capacity + first) * PH_WIDTH,
+              *v = values + (l * capacity + first) * PH_WIDTH;
+        ok = to_host ? pgpu_kv8_read(stream, &pool->kv8, (int)l, &rows, dh + 4, dk, dv, PH_WIDTH,
+                                     status) &&
+                           pgpu_copy_d2h(stream, k, dk, bytes) &&
+                           pgpu_copy_d2h(stream, v, dv, bytes)
+                     : pgpu_copy_h2d(stream, dk, k, bytes) &&
+                           pgpu_copy_h2d(stream, dv, v, bytes) &&
+                           pgpu_kv8_write(stream, &pool->kv8, (int)l, &rows, dk, dv, PH_WIDTH,
+                                          status);
+    }
+    int st = 1;
+    ok = ok && pgpu_copy_d2h(stream, &st, status, sizeof(int)) && st == 0;
+    (void)pgpu_stream_sync(stream);
+    pgpu_free(dk);
+    pgpu_free(dv);
+    pgpu_free(dt);
+    pgpu_free(dh);
+    return ok;
+}
+
+int phonon_kv_pool_write_q8(PhononKvPool *pool, const int32_t *table, size_t table_len,
+                            int32_t slot, size_t first, size_t count, const float *keys,
+                            const float *values, size_t capacity) {
+    return pool_copy_q8(pool, table, table_len, slot, first + count, first, count, (float *)keys,
+                        (float *)values, capacity, 0);
+}
+
+int phonon_kv_pool_read_q8(const PhononKvPool *pool, const int32_t *table, size_t table_len,
+                           int32_t slot, size_t length, size_t first, size_t count, float *keys,
+                           float *values, size_t capacity) {
+    return pool_copy_q8(pool, table, table_len, slot, length, first, count, keys, values,
+                        capacity, 1);
+}
+
 /* ---------------------------------------------------------------- batch -- */
 
 static void drop_graphs(PhononFlowBatch *b) {
@@ -428,7 +599,9 @@ void phonon_flow_batch_destroy(PhononFlowBatch *b) {
                     b->rows, b->xh, b->positions, b->tables, b->status,
                     b->scratch.part_acc, b->scratch.part_ml, b->pre.stage_dev,
                     b->fl.act, b->fl.part_acc, b->fl.part_ml, b->fl.hidden, b->fl.counters,
-                    b->fl.rows, b->fl.parts, b->fl.mlp_parts, b->fl.schedule};
+                    b->fl.rows, b->fl.parts, b->fl.mlp_parts, b->fl.schedule,
+                    b->q8.slots, b->q8.slot_tables, b->q8.att, b->q8.qkv, b->q8.zeros,
+                    b->q8.work};
     for (size_t i = 0; i < sizeof(bufs) / sizeof(bufs[0]); i++)
         pgpu_free(bufs[i]);
     pgpu_stream_destroy(b->own_stream);
@@ -488,6 +661,12 @@ int ph_batch_create_on(const PhononFlowModel *model, PhononKvPool *pool, size_t 
     b->scratch.part_ml = pgpu_malloc(slots * 2 * sizeof(float));
     b->scratch.max_streams = (int)max_streams;
     b->scratch.max_splits = (int)b->max_splits;
+    if (pool->q8) {
+        b->q8.slots = pgpu_malloc(max_streams * sizeof(int32_t));
+        b->q8.slot_tables = pgpu_malloc(max_streams * b->table_len * sizeof(int32_t));
+        b->q8.att = pgpu_malloc(rows);
+        ok = ok && b->q8.slots && b->q8.slot_tables && b->q8.att;
+    }
     b->host_positions = calloc(max_streams, sizeof(size_t));
     b->fl.cover = calloc(max_streams, sizeof(size_t));
     b->fl.units = calloc(max_streams, sizeof(size_t));
@@ -542,25 +721,29 @@ static void flow_loosen(PhononFlowBatch *b) {
     b->fl.ran = 0;
 }
 
-int phonon_flow_batch_set_streams(PhononFlowBatch *b, size_t streams, const size_t *positions,
-                                  const int32_t *tables, size_t table_len) {
+static int set_streams(PhononFlowBatch *b, size_t streams, const size_t *positions,
+                       const int32_t *tables, size_t table_len, const int32_t *slots) {
     if (!b || !streams || streams > b->max_streams || !positions || !tables ||
         table_len != b->table_len)
         return 0;
     int32_t *pos32 = malloc(streams * sizeof(int32_t));
-    if (!pos32)
-        return 0;
-    for (size_t s = 0; s < streams; s++) {
-        if (positions[s] >= b->max_positions) {
-            free(pos32);
-            return 0;
-        }
+    int32_t *wide = slots ? malloc(streams * table_len * sizeof(int32_t)) : NULL;
+    int ok = pos32 && (wide || !slots);
+    for (size_t s = 0; ok && s < streams; s++) {
+        ok = positions[s] < b->max_positions &&
+             (!slots || (slots[s] >= 0 && (size_t)slots[s] < b->pool->slots.count));
         pos32[s] = (int32_t)positions[s];
+        for (size_t i = 0; wide && ok && i < table_len; i++)
+            wide[s * table_len + i] = slots[s];
     }
-    int ok = pgpu_stream_sync(b->stream) &&
-             pgpu_copy_h2d(b->stream, b->positions, pos32, streams * sizeof(int32_t)) &&
-             pgpu_copy_h2d(b->stream, b->tables, tables, streams * table_len * sizeof(int32_t));
+    ok = ok && pgpu_stream_sync(b->stream) &&
+         pgpu_copy_h2d(b->stream, b->positions, pos32, streams * sizeof(int32_t)) &&
+         pgpu_copy_h2d(b->stream, b->tables, tables, streams * table_len * sizeof(int32_t)) &&
+         (!slots || (pgpu_copy_h2d(b->stream, b->q8.slots, slots, streams * sizeof(int32_t)) &&
+                     pgpu_copy_h2d(b->stream, b->q8.slot_tables, wide,
+                                   streams * table_len * sizeof(int32_t))));
     free(pos32);
+    free(wide);
     if (!ok)
         return 0;
     memcpy(b->host_positions, positions, streams * sizeof(size_t));
@@ -569,6 +752,23 @@ int phonon_flow_batch_set_streams(PhononFlowBatch *b, size_t streams, const size
     b->pre.active = 0;
     flow_loosen(b);
     return 1;
+}
+
+int phonon_flow_batch_set_streams(PhononFlowBatch *b, size_t streams, const size_t *positions,
+                                  const int32_t *tables, size_t table_len) {
+    if (b && b->pool->q8)
+        return ph_fail(kQ8);
+    return set_streams(b, streams, positions, tables, table_len, NULL);
+}
+
+int phonon_flow_batch_set_streams_q8(PhononFlowBatch *b, size_t streams, const size_t *positions,
+                                     const int32_t *tables, size_t table_len,
+                                     const int32_t *slots) {
+    if (!b || !slots)
+        return 0;
+    if (!b->pool->q8)
+        return ph_fail(kNotQ8);
+    return set_streams(b, streams, positions, tables, table_len, slots);
 }
 
 int ph_batch_bind_model(PhononFlowBatch *b, const PhononFlowModel *model) {
@@ -618,6 +818,51 @@ static size_t splits_for(const PhononFlowBatch *b, size_t ahead) {
     return splits < b->max_splits ? splits : b->max_splits;
 }
 
+/* The rows that an 8-bit pool's calls have: one a stream, or the prefill's. */
+static pgpu_kv8_rows q8_rows(const PhononFlowBatch *b) {
+    if (b->pre.active) {
+        return (pgpu_kv8_rows){.tables = b->table_src, .table_stride = (int)b->table_len,
+                               .slots = b->q8.pre_slots, .first = b->q8.pre_first,
+                               .offsets = b->q8.pre_offsets, .streams = (int)b->q8.pre_streams,
+                               .rows = (int)b->streams, .max_rows = (int)b->q8.pre_rows};
+    }
+    return (pgpu_kv8_rows){.tables = b->tables, .table_stride = (int)b->table_len,
+                           .slots = b->q8.slots, .first = b->positions,
+                           .streams = (int)b->streams, .rows = (int)b->streams, .max_rows = 1};
+}
+
+/* Positions that the attention's work is dealt by: b->splits' keys. */
+static int q8_positions(const PhononFlowBatch *b) {
+    const size_t keys = b->splits * PH_SPLIT_KEYS, most = b->table_len * 16;
+    return (int)(keys < most ? keys : most);
+}
+
+/* Room for the attention's parts with b->splits, before any capture. Graphs
+ * hold the workspace's address. */
+static int q8_reserve(PhononFlowBatch *b) {
+    if (!b->pool->q8)
+        return 1;
+    const pgpu_kv8_rows rows = q8_rows(b);
+    const size_t need = pgpu_kv8_attention_bytes(&b->pool->kv8, &rows, 1, q8_positions(b));
+    if (need <= b->q8.work_bytes)
+        return 1;
+    if (!pgpu_stream_sync(b->stream))
+        return 0;
+    drop_graphs(b);
+    pgpu_free(b->q8.work);
+    b->q8.work = pgpu_malloc(need);
+    b->q8.work_bytes = b->q8.work ? need : 0;
+    return b->q8.work != NULL;
+}
+
+/* The attention of a layer of an 8-bit pool into the rows q8.att. */
+static int q8_attention(PhononFlowBatch *b, void *stream, int layer) {
+    const pgpu_kv8_rows rows = q8_rows(b);
+    return pgpu_kv8_attention(stream, &b->pool->kv8, layer, &rows, b->q, PH_WIDTH, 1, 1.0f,
+                              q8_positions(b), b->q8.att, PH_WIDTH, b->q8.work,
+                              b->q8.work_bytes, b->status);
+}
+
 /* Enqueues layers [first, first+count) for streams [s0, s0+n) of the batch
  * (s0 a multiple of 16) on `stream`. Every buffer is used at the group's
  * offset, so groups share no memory and may run concurrently. */
@@ -652,6 +897,30 @@ static int enqueue_prefill(PhononFlowBatch *b, void *stream, size_t first, size_
         const float *norm = m->norms + l * 4 * PH_WIDTH;
         float *next = (l + 1 == first + count) ? output : b->x;
         const int layer = (int)(l + pool_offset);
+        if (b->pool->q8) {
+            /* The projected rows, then rotated and quantised into the cache. */
+            const pgpu_kv8_rows rows = q8_rows(b);
+            if (!pgpu_rows_split_ln(stream, cur, norm, norm + PH_WIDTH, 1e-5f, n, terms, xs,
+                                    b->status) ||
+                !pgpu_prefill_gemm_residual(stream, &m->wide[l * 4], xs, n, terms, b->q8.zeros,
+                                            b->q8.qkv, b->status) ||
+                !pgpu_kv8_rotate_write(stream, &b->pool->kv8, layer, &rows, b->q8.qkv,
+                                       3 * PH_WIDTH, 1, NULL, NULL, 0.0f, rope,
+                                       PHONON_FLOW_MAX_POSITIONS, 0.125f, b->q, b->status) ||
+                !q8_attention(b, stream, layer) ||
+                !pgpu_split_rows(stream, b->q8.att, n, PH_WIDTH, xs, b->status) ||
+                !pgpu_prefill_gemm_residual(stream, &m->wide[l * 4 + 1], xs, n, 3, cur, b->r,
+                                            b->status) ||
+                !pgpu_rows_split_ln(stream, b->r, norm + 2 * PH_WIDTH, norm + 3 * PH_WIDTH,
+                                    1e-5f, n, terms, xs, b->status) ||
+                !pgpu_prefill_gemm_gelu_split(stream, &m->wide[l * 4 + 2], xs, n, terms, b->xh,
+                                              b->status) ||
+                !pgpu_prefill_gemm_residual(stream, &m->wide[l * 4 + 3], b->xh, n, terms, b->r,
+                                            next, b->status))
+                return 0;
+            cur = next;
+            continue;
+        }
         if (!pgpu_rows_split_ln(stream, cur, norm, norm + PH_WIDTH, 1e-5f, n, terms, xs,
                                 b->status) ||
             !pgpu_prefill_gemm_qkv(stream, &m->wide[l * 4], xs, n, terms, &b->pool->kv, layer,
@@ -722,6 +991,22 @@ static int enqueue_group(PhononFlowBatch *b, void *stream, size_t s0, size_t n, 
         const pgpu_gemm_input ln2 = {.ln_rows = r, .ln_weight = norm + 2 * PH_WIDTH,
                                      .ln_bias = norm + 3 * PH_WIDTH, .ln_epsilon = 1e-5f};
         const pgpu_gemm_input hidden = {.split = xh};
+        if (b->pool->q8) {
+            /* The projection appends to the open slots, by tables that lead every
+             * position to its stream's. */
+            const pgpu_gemm_input rows = {.rows = b->q8.att};
+            if (!pgpu_gemm_qkv(stream, &m->qkv[l], &ln1, (int)n, &b->pool->kv, pool_layer,
+                               b->q8.slot_tables, (int)b->table_len, positions, rope, q,
+                               b->status) ||
+                !q8_attention(b, stream, pool_layer) ||
+                !pgpu_gemm_residual(stream, &m->out[l], &rows, (int)n, cur, r, b->status) ||
+                !pgpu_gemm_gelu_split(stream, &m->mlp_in[l], &ln2, (int)n, xh, b->status) ||
+                !pgpu_gemm_residual(stream, &m->mlp_out[l], &hidden, (int)n, r, next,
+                                    b->status))
+                return 0;
+            cur = next;
+            continue;
+        }
         if (!pgpu_gemm_qkv(stream, &m->qkv[l], &ln1, (int)n, &b->pool->kv, pool_layer, tables,
                            (int)b->table_len, positions, rope, q, b->status) ||
             !(b->pre.active
@@ -791,6 +1076,11 @@ static int enqueue_step(PhononFlowBatch *b, const float *input, float *output, f
         if (!pgpu_event_record(b->join[g - 1], b->side[g - 1]) ||
             !pgpu_stream_wait_event(b->stream, b->join[g - 1]))
             return 0;
+    if (b->pool->q8 && !b->pre.active &&
+        !pgpu_kv8_close(b->stream, &b->pool->kv8, 0, (int)b->model->layers, b->tables,
+                        (int)b->table_len, b->q8.slots, b->positions, (int)b->streams,
+                        b->status))
+        return 0;
     return pgpu_advance_positions(b->stream, b->positions, (int)b->streams, 1);
 }
 
@@ -808,7 +1098,8 @@ static size_t flow_ml_group(const PhononFlowBatch *b) {
  * tiles; prefill and larger batches are attention-bound, where the separate
  * attention kernel streams K/V faster). */
 static int flow_usable(const PhononFlowBatch *b, int prefill) {
-    if (!b->flow || b->model->q8 < 0 || b->model->layers > 63 || b->streams > 4096)
+    if (!b->flow || b->model->q8 < 0 || b->model->layers > 63 || b->streams > 4096 ||
+        b->pool->q8)
         return 0;
     const size_t tiles = (b->streams + 15) / 16;
     return b->flow == 2 ||
@@ -1375,23 +1666,82 @@ int ph_batch_set_prefill(PhononFlowBatch *b, size_t streams, const size_t *first
            set_prefill(b, streams, first, counts, tables_dev);
 }
 
-int phonon_flow_batch_prefill_device(PhononFlowBatch *b, size_t streams, const size_t *first,
-                                     const size_t *counts, const int32_t *tables,
-                                     size_t table_len, const float *inputs, float theta,
-                                     float *outputs) {
+/* An 8-bit pool's part of a prefill call: its streams' slots, first positions
+ * and rows staged, and room for the projected rows. */
+static int q8_prefill(PhononFlowBatch *b, size_t streams, const size_t *first,
+                      const size_t *counts, const int32_t *slots) {
+    int32_t *host = malloc((2 * streams + 1) * sizeof(int32_t));
+    if (!host)
+        return 0;
+    int32_t *at = host + streams;
+    at[0] = 0;
+    b->q8.pre_rows = 0;
+    int ok = 1;
+    for (size_t i = 0; i < streams; i++) {
+        host[i] = (int32_t)first[i];
+        at[i + 1] = at[i] + (int32_t)counts[i];
+        if (counts[i] > b->q8.pre_rows)
+            b->q8.pre_rows = counts[i];
+        ok = ok && slots[i] >= 0 && (size_t)slots[i] < b->pool->slots.count;
+    }
+    const size_t bytes = b->padded_streams * 3 * PH_WIDTH * sizeof(float);
+    if (ok && !b->q8.qkv)
+        ok = (b->q8.qkv = pgpu_malloc(bytes)) != NULL;
+    if (ok && !b->q8.zeros)
+        ok = (b->q8.zeros = pgpu_malloc(bytes)) != NULL &&
+             pgpu_memset(b->stream, b->q8.zeros, 0, bytes);
+    ok = ok && (b->q8.pre_slots = stage_put(b, slots, streams * sizeof(int32_t))) &&
+         (b->q8.pre_first = stage_put(b, host, streams * sizeof(int32_t))) &&
+         (b->q8.pre_offsets = stage_put(b, at, (streams + 1) * sizeof(int32_t)));
+    b->q8.pre_streams = streams;
+    free(host);
+    return ok;
+}
+
+static int prefill_device(PhononFlowBatch *b, size_t streams, const size_t *first,
+                          const size_t *counts, const int32_t *tables, size_t table_len,
+                          const int32_t *slots, const float *inputs, float theta,
+                          float *outputs) {
     if (!b || !streams || streams > b->max_streams || !first || !counts || !tables ||
         table_len != b->table_len || !inputs || !outputs || !isfinite(theta) || theta <= 0.0f)
         return 0;
     const size_t total = prefill_total(b, streams, first, counts),
-                 table_bytes = streams * table_len * sizeof(int32_t);
+                 table_bytes = streams * table_len * sizeof(int32_t),
+                 q8_bytes = slots ? (3 * streams + 1) * sizeof(int32_t) + 3 * 256 : 0;
     if (!total || !pgpu_stream_sync(b->stream) ||
-        !stage_begin(b, stage_bytes(total, table_bytes)) ||
-        !(b->table_src = stage_put(b, tables, table_bytes)) ||
-        !set_prefill(b, streams, first, counts, b->table_src))
+        !stage_begin(b, stage_bytes(total, table_bytes + q8_bytes)) ||
+        !(b->table_src = stage_put(b, tables, table_bytes)))
+        return 0;
+    if (slots && !q8_prefill(b, streams, first, counts, slots))
+        return 0;
+    if (!set_prefill(b, streams, first, counts, b->table_src))
         return 0;
     if (flow_usable(b, 1))
         return flow_prepare(b, 1) && enqueue_flow(b, inputs, outputs, theta);
-    return (b->splits = splits_for(b, 0)) > 0 && enqueue_step(b, inputs, outputs, theta);
+    return (b->splits = splits_for(b, 0)) > 0 && q8_reserve(b) &&
+           enqueue_step(b, inputs, outputs, theta);
+}
+
+int phonon_flow_batch_prefill_device(PhononFlowBatch *b, size_t streams, const size_t *first,
+                                     const size_t *counts, const int32_t *tables,
+                                     size_t table_len, const float *inputs, float theta,
+                                     float *outputs) {
+    if (b && b->pool->q8)
+        return ph_fail(kQ8);
+    return prefill_device(b, streams, first, counts, tables, table_len, NULL, inputs, theta,
+                          outputs);
+}
+
+int phonon_flow_batch_prefill_q8_device(PhononFlowBatch *b, size_t streams, const size_t *first,
+                                        const size_t *counts, const int32_t *tables,
+                                        size_t table_len, const int32_t *slots,
+                                        const float *inputs, float theta, float *outputs) {
+    if (!b || !slots)
+        return 0;
+    if (!b->pool->q8)
+        return ph_fail(kNotQ8);
+    return prefill_device(b, streams, first, counts, tables, table_len, slots, inputs, theta,
+                          outputs);
 }
 
 int phonon_flow_batch_set_wait_limit(PhononFlowBatch *b, unsigned microseconds) {
@@ -1411,6 +1761,8 @@ int phonon_flow_batch_set_prefill_exact(PhononFlowBatch *b, int exact) {
 int phonon_flow_batch_set_groups(PhononFlowBatch *b, size_t groups) {
     if (!b || !groups || groups > PH_MAX_GROUPS)
         return 0;
+    if (groups > 1 && b->pool->q8)
+        return ph_fail("a batch over an 8-bit pool runs as one group");
     if (groups > 1) {
         /* each made once; a failure leaves the groups as they were */
         int ok = b->fork || pgpu_event_create(&b->fork);
@@ -1512,6 +1864,8 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
      * and position lag as arguments: it is never captured. */
     if (b->eager || b->time_before || flow) {
         b->splits = splits_for(b, 0);
+        if (!q8_reserve(b))
+            return 0;
         if (!(flow ? enqueue_flow(b, inputs, outputs, theta)
                    : enqueue_step(b, inputs, outputs, theta)))
             return 0;
@@ -1524,6 +1878,9 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
      * context outgrows it. */
     const size_t need = splits_for(b, 0);
     void *exec = NULL;
+    b->splits = splits_for(b, PH_SPLIT_KEYS);
+    if (!q8_reserve(b))
+        return 0;
     for (size_t i = 0; i < 2 && !exec; i++)
         if (b->graphs[i].exec && b->graphs[i].streams == b->streams &&
             b->graphs[i].splits >= need && b->graphs[i].theta == theta &&
@@ -1533,7 +1890,6 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
         const size_t slot = b->graph_victim;
         pgpu_graph_destroy(b->graphs[slot].exec);
         b->graphs[slot].exec = NULL;
-        b->splits = splits_for(b, PH_SPLIT_KEYS);
         if (!ph_rope_table(theta) || !pgpu_graph_begin(b->stream))
             return 0;
         const int enqueued = enqueue_step(b, inputs, outputs, theta);
