@@ -615,3 +615,222 @@ def test_a_prompt_then_frames_together(cache, lib):
         q = model.turn(x[:, :heads * group], w[0], 1e-5, rope[at])
         assert (np.abs(a.q - q) <= 2.0 ** -24 * np.abs(q) + 1e-44).all()
         a.check(a.run())
+
+
+@pytest.mark.parametrize("streams,heads,group,dim,most", [
+    (1, 8, 1, 64, 2000),     # whole streams, 16 waves, two steps
+    (40, 8, 1, 64, 1500),    # 8 waves
+    (100, 8, 1, 64, 700),    # 4 waves
+    (12, 8, 1, 64, 2300),    # dealt, two steps of 4 waves
+    (64, 8, 1, 64, 8192),    # dealt, four steps
+    (3, 2, 1, 64, 8192),     # dealt, a step
+    (30, 8, 4, 64, 900),     # four queries, 8 waves
+    (100, 8, 2, 64, 500),    # four queries' places, two queries
+    (9, 8, 3, 128, 8192),    # wide heads, dealt
+    (20, 4, 1, 128, 800),    # wide heads, whole
+    (3, 3, 9, 128, 1200),    # three passes over the queries
+])
+def test_attention_in_each_way_of_dealing_the_keys(cache, streams, heads, group, dim, most):
+    """How the keys are dealt goes by max_positions and the batch; the contexts
+    themselves are short, and of every offset in a block and a step."""
+    c = cache(streams, heads, dim, positions=700, seed=streams)
+    lengths = [1 + (s * 37 + s * s) % min(690, most - 1) if s % 9 else 1 for s in range(streams)]
+    lengths[-1] = min(690, most - 1)
+    c.fill(lengths)
+    first = [-1 if s % 11 == 5 else n - 1 for s, n in enumerate(lengths)]
+    a = Attend(c, first, None, group, most=most)
+    got = a.run()
+    keep = [s for s in range(streams) if s % max(1, streams // 8) == 0 or s == streams - 1]
+    assert (got[[s for s in range(streams) if first[s] < 0]] == 0).all()
+    assert c.st() == 0
+    for s in keep:
+        if first[s] < 0:
+            continue
+        k, v = (model.seen(x) for x in c.rows[s])
+        want, bound = model.attention(a.q[s:s + 1], k, v, first[s], a.scale)
+        assert (np.abs(got[s:s + 1] - want) <= bound).all(), s
+
+
+@pytest.mark.parametrize("most,heads,group,dim", [(4000, 2, 1, 64), (8192, 8, 2, 64),
+                                                  (2000, 1, 5, 128), (120, 8, 1, 64)])
+def test_runs_in_each_way_of_dealing_the_keys(cache, most, heads, group, dim):
+    counts, before = [40, 1, 17, 3], [70, 0, 33, 100]
+    c = cache(4, heads, dim, positions=120)
+    c.fill(before)
+    c.write(before, counts, *c.random_rows(sum(counts)))
+    a = Attend(c, before, counts, group, most=most)
+    a.check(a.run())
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-30])
+@pytest.mark.parametrize("counts", [None, [20, 33, 1]])
+def test_attention_with_other_scales(cache, scale, counts):
+    """A negative scale turns the order of the scores; with none every key weighs
+    the same."""
+    c = cache(3, 2, 64, positions=100)
+    n = counts or [1] * 3
+    c.fill([50, 0, 63])
+    c.write([50, 0, 63], n, *c.random_rows(sum(n)))
+    a = Attend(c, [50, 0, 63], counts, 2, scale=scale)
+    a.check(a.run())
+
+
+@pytest.mark.parametrize("counts", [None, [40, 3]])
+def test_queries_of_zero_and_of_any_magnitude(cache, counts):
+    c = cache(2, 2, 64, positions=120)
+    n = counts or [1, 1]
+    c.fill([70, 40])
+    c.write([70, 40], n, *c.random_rows(sum(n)))
+    for factor in (0.0, 1e-42, 1e-20, 1e20):
+        a = Attend(c, [70, 40], counts, 2, scale=0.125 / max(factor, 1e-3) if factor > 1 else 0.125)
+        a.q = (a.q * np.float32(factor)).astype(np.float32)
+        a.dq.upload(a.q.reshape(a.total, -1))
+        a.check(a.run())
+
+
+def test_a_cache_past_32_bits(lib, pkg):
+    """Blocks whose bytes start past 2^32, in layer 1 of 2."""
+    heads, dim, blocks = 8, 64, 300000
+    tile, slot = 2 * 16 * dim, 2 * 16 * dim
+    assert blocks * heads * tile > 2 ** 32
+    big = [pkg.DeviceBuffer(lib, n) for n in (2 * blocks * heads * tile, 2 * blocks * heads * 8,
+                                              2 * 2 * heads * slot * 4)]
+    try:
+        kv = pkg.PgpuKv8(*(b.ptr for b in big), 2, heads, dim, blocks, 2)
+        table = np.array([[blocks - 1, 5, blocks - 7, 262144], [blocks - 2, 1, 2, 3]], np.int32)
+        n = [60, 33]
+        rng = np.random.default_rng(8)
+        k, v = (rng.standard_normal((sum(n), heads, dim)).astype(np.float32) for _ in range(2))
+        host = dict(tables=table, slots=np.array([1, 0], np.int32), first=np.zeros(2, np.int32),
+                    offsets=np.array([0, 60, 93], np.int32), status=np.zeros(1, np.int32),
+                    lengths=np.array(n, np.int32), last=np.array(n, np.int32) - 1, k=k, v=v,
+                    q=rng.standard_normal((2, heads, dim)).astype(np.float32))
+        dev = {}
+        for name, a in host.items():
+            dev[name] = pkg.DeviceBuffer(lib, a.nbytes)
+            dev[name].upload(a)
+        out, bk, bv = (pkg.DeviceBuffer(lib, x) for x in (2 * 2048, k.nbytes, k.nbytes))
+        rows = pkg.PgpuKv8Rows(dev["tables"].ptr, 4, dev["slots"].ptr, dev["first"].ptr,
+                               dev["offsets"].ptr, 2, 93, 60)
+        one = pkg.PgpuKv8Rows(dev["tables"].ptr, 4, dev["slots"].ptr, dev["last"].ptr, None, 2, 2, 1)
+        kp = ctypes.byref(kv)
+        assert lib.pgpu_kv8_write(None, kp, 1, ctypes.byref(rows), dev["k"].ptr, dev["v"].ptr, 512,
+                                  dev["status"].ptr)
+        assert lib.pgpu_kv8_read(None, kp, 1, ctypes.byref(rows), dev["lengths"].ptr, bk.ptr,
+                                 bv.ptr, 512, dev["status"].ptr)
+        assert lib.pgpu_kv8_attention(None, kp, 1, ctypes.byref(one), dev["q"].ptr, 512, 1, 0.125,
+                                      64, out.ptr, 512, None, 0, dev["status"].ptr)
+        assert dev["status"].download((1,), np.int32)[0] == 0
+        gk, gv, go = bk.download(k.shape), bv.download(v.shape), out.download((2, heads, dim))
+        for s, lo in ((0, 0), (1, 60)):
+            wk, wv = model.seen(k[lo:lo + n[s]]), model.seen(v[lo:lo + n[s]])
+            assert np.array_equal(gk[lo:lo + n[s]], wk) and np.array_equal(gv[lo:lo + n[s]], wv)
+            want, bound = model.attention(host["q"][s:s + 1], wk, wv, n[s] - 1, 0.125)
+            assert (np.abs(go[s:s + 1] - want) <= bound).all()
+    finally:
+        for b in big:
+            b.free()
+
+
+def test_two_streams_at_once(cache, lib):
+    """Two calls on HIP streams of their own, each with its workspace, give the
+    bits that they give alone."""
+    c = cache(4, 8, 64, positions=2400)
+    c.fill([2300, 5, 900, 60])
+    c.write(c.lengths(), [30, 1, 70, 16], *c.random_rows(117))
+    calls = [Attend(c, [2300, 5, 900, 60], [30, 1, 70, 16], 1),
+             Attend(c, [n - 1 for n in c.lengths()], None, 2, most=8192, seed=9)]
+    want = [a.run() for a in calls]
+    streams = [ctypes.c_void_p(), ctypes.c_void_p()]
+    for s in streams:
+        assert lib.pgpu_stream_create(ctypes.byref(s))
+    try:
+        for _ in range(4):
+            for a, s in zip(calls, streams):
+                a.dout.upload(a.mark)
+            for _ in range(3):
+                for a, s in zip(calls, streams):
+                    assert a.enqueue(s)
+            for s in streams:
+                assert lib.pgpu_stream_sync(s)
+            for a, w in zip(calls, want):
+                assert np.array_equal(a.result(), w)
+    finally:
+        for s in streams:
+            lib.pgpu_stream_destroy(s)
+
+
+def test_frames_from_one_graph(cache, lib):
+    """A frame's rotated append, its attention and the advance of the positions
+    captured once, and replayed over block borders with the program's own work
+    between; the cache and every result against the model."""
+    heads, group, dim, frames = 2, 2, 64, 40
+    c = cache(3, heads, dim, positions=160)
+    rng = c.rng
+    angle = np.arange(160)[:, None] * 10000.0 ** (-2 * np.arange(dim // 2) / dim)
+    rope = np.stack([np.cos(angle), np.sin(angle)], -1).astype(np.float32)
+    drope = c.up(rope)
+    c.fill([100, 15, 0])
+    width = heads * dim * (2 + group)
+    a = Attend(c, [100, 15, 0], None, group, most=160)
+    dx = c.up(np.zeros((3, width), np.float32))
+    stream, exec_ = ctypes.c_void_p(), ctypes.c_void_p()
+    assert lib.pgpu_stream_create(ctypes.byref(stream))
+    try:
+        assert lib.pgpu_graph_begin_global(stream)
+        ok = lib.pgpu_kv8_rotate_write(stream, ctypes.byref(c.kv), 1, ctypes.byref(a.rows), dx.ptr,
+                                       width, group, None, None, 0.0, drope.ptr, 160, 1.0,
+                                       a.dq.ptr, c.status.ptr) and a.enqueue(stream) and \
+            lib.pgpu_advance_positions(stream, a.rows.first, 3, 1)
+        ended = lib.pgpu_graph_end(stream, ctypes.byref(exec_))
+        assert ok and ended, c.pkg.last_error(lib)
+        for frame in range(frames):
+            first = c.lengths()
+            qkv = rng.standard_normal((3, width)).astype(np.float32)
+            dx.upload(qkv)
+            assert lib.pgpu_graph_launch(exec_, stream) and lib.pgpu_stream_sync(stream)
+            x = qkv.reshape(3, -1, dim)
+            at = np.asarray(first)
+            k = model.turn(x[:, heads * group:-heads], None, 0.0, rope[at]).astype(np.float32)
+            c.note(first, [1] * 3, k, x[:, -heads:])
+            a.first, a.q = first, a.dq.download(a.q.shape)
+            a.check(a.result())
+            if frame % 7 == 0:
+                check_contents(c)
+    finally:
+        lib.pgpu_graph_destroy(exec_)
+        lib.pgpu_stream_destroy(stream)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_is_not_finite_stays_with_the_rows_that_see_it(cache, which, bad):
+    """A key or value of the newest block, and one of a stored block: rows of the
+    same run before it come out whole, those that see it do not come out finite,
+    and it is said."""
+    c = cache(2, 2, 64, positions=120)
+    c.fill([30, 0])
+    k, v = c.random_rows(50 + 90)
+    c.write([30, 0], [50, 90], k, v)
+    assert c.st() == 0
+    clean = [[x.copy() for x in r] for r in c.rows]
+    opened = c.open.download(c.open0.shape)
+    opened[1, c.slot[0], :, which, 75 - 64, 7] = bad            # newest block of stream 0
+    opened[1, c.slot[1], :, which, 85 - 80, 7] = bad            # and of stream 1
+    c.open.upload(opened)
+    scales = c.scales.download(c.scales0.shape)
+    scales[1, c.table[1, 40 // 16], :, which] = np.nan          # block 2 of stream 1
+    c.scales.upload(scales)
+    a = Attend(c, [30, 0], [50, 90], 2)
+    got = a.run()
+    assert c.st() == 1
+    at = 0
+    for s, (first, n, ends) in enumerate(((30, 50, 75), (0, 90, 32))):
+        kk, vv = (model.seen(x) for x in clean[s])
+        fine = ends - first
+        want, bound = model.attention(a.q[at:at + fine], kk[:ends], vv[:ends], first, a.scale)
+        assert (np.abs(got[at:at + fine] - want) <= bound).all()
+        rest = np.isfinite(got[at + fine:at + n]).reshape(n - fine, -1)
+        if s == 1 or which == 1 or np.isnan(bad):
+            assert not rest.all(1).any()
+        at += n
