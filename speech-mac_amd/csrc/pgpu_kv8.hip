@@ -1192,51 +1192,52 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     flag_nonfinite(status, bad);
 }
 
-// The splits of a row's query head joined: D / 4 lanes for each, 4 dims a lane.
-// `keys`: of a split, or 0: every split has keys of every row, or says that it has
-// none. Eight splits' parts are on their way at once.
-template <int D>
+// The splits of a row's query head joined: D / 4 lanes for 4 dims each, times G
+// that share the splits. `keys`: of a split, or 0: every split has keys of every
+// row, or says that it has none. Eight splits' parts are on their way at once.
+template <int D, int G>
 __global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const float *part_acc,
                                                   const float *part_ml, int group,
                                                   int max_positions, int splits, int keys,
                                                   float *out, size_t out_stride, int *status) {
+    constexpr int L = D / 4, M = L * G;
     const int s = blockIdx.z, wide = kv.heads * group;
-    const size_t e = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int d = (int)(e % (D / 4)) * 4, qh = (int)(e / (D / 4) % wide);
-    const size_t i = e / (D / 4) / wide;
+    const size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int lane = (int)(e % M), share = lane / L, d = lane % L * 4;
+    const int qh = (int)(e / M % wide);
+    const size_t i = e / M / wide;
     const Kv8Span span = kv8_span(kv, rows, s, max_positions, false, status);
     if (i >= (size_t)span.count || (!span.live && span.first >= 0)) return;
     const size_t row = span.row0 + i;
     float *dst = out + row * out_stride + (size_t)qh * D + d;
     if (!span.live) {
-        *(float4 *)dst = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (share == 0) *(float4 *)dst = make_float4(0.f, 0.f, 0.f, 0.f);
         return;
     }
     const int n = keys ? (span.first + (int)i) / keys + 1 : splits;
     const size_t at = (row * wide + qh) * splits;
-    // Lane j of the D / 4 has split j's maximum and sum, and the next D / 4's.
-    constexpr int L = D / 4;
-    const int lane = threadIdx.x % L;
+    // Lane j of the M has split j's maximum and sum, and the next M's.
     float mx = -INFINITY, total = 0.0f;
-    for (int j = lane; j < n; j += L) mx = fmaxf(mx, part_ml[(at + j) * 2]);
+    for (int j = lane; j < n; j += M) mx = fmaxf(mx, part_ml[(at + j) * 2]);
 #pragma unroll
-    for (int z = 1; z < L; z <<= 1) mx = fmaxf(mx, __shfl_xor(mx, z));
+    for (int z = 1; z < M; z <<= 1) mx = fmaxf(mx, __shfl_xor(mx, z));
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = 0; j0 < n; j0 += L) {
-        const int last = min(L, n - j0);
+    for (int j0 = 0; j0 < n; j0 += M) {
+        const int last = min(M, n - j0);
         const float2 ml = lane < last ? *(const float2 *)(part_ml + (at + j0 + lane) * 2)
                                       : make_float2(-INFINITY, 0.0f);
         const float c = __builtin_amdgcn_exp2f(ml.x - mx);
         total = fmaf(ml.y, c, total);
-        for (int j = 0; j < last; j += 8) {
+        for (int j = 0; j < last; j += 8 * G) {
             float4 x[8];
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                x[k] = *(const float4 *)(part_acc + (at + j0 + min(j + k, last - 1)) * D + d);
+                x[k] = *(const float4 *)(part_acc +
+                                         (at + j0 + min(j + k * G + share, last - 1)) * D + d);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float w = __shfl(c, j + k, L);  // 0 past the last
-                if (j + k >= last) continue;
+                const float w = __shfl(c, min(j + k * G + share, M - 1), M);
+                if (j + k * G + share >= last) continue;
                 o.x = fmaf(x[k].x, w, o.x);
                 o.y = fmaf(x[k].y, w, o.y);
                 o.z = fmaf(x[k].z, w, o.z);
@@ -1245,7 +1246,15 @@ __global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const fl
         }
     }
 #pragma unroll
-    for (int z = 1; z < L; z <<= 1) total += __shfl_xor(total, z);
+    for (int z = 1; z < M; z <<= 1) total += __shfl_xor(total, z);
+#pragma unroll
+    for (int z = L; z < M; z <<= 1) {
+        o.x += __shfl_xor(o.x, z);
+        o.y += __shfl_xor(o.y, z);
+        o.z += __shfl_xor(o.z, z);
+        o.w += __shfl_xor(o.w, z);
+    }
+    if (share) return;
     o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
     *(float4 *)dst = o;
     flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
@@ -1403,21 +1412,24 @@ struct Deal {
 Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_positions) {
     Deal d;
     if (!r->offsets) {
-        // A stream's keys whole in one work-group of W waves, where that is few
-        // steps of W * 64 keys or there are work-groups to fill the chip; else
-        // dealt to work-groups of 4 waves, more keys to each the more of them
-        // there are. us, whole / dealt (8 heads of 64): 1 stream of 2011 keys 8.6 /
-        // 10.7, of 8187 19.7 / 10.4; 16 of up to 2048 10.7 / 11.2, of up to 8187
-        // 26.6 / 19.2; 64 of up to 2048 16.3 / 18.6, of up to 8187 52.3 / 49.6; 128
-        // of up to 2048 32.5 / 37.3. W = 4, 8, 16: 1 stream of 700 keys 7.8, 7.8, 7.6,
-        // of 2011 13.5, 9.5, 8.6; 64 of up to 2048 18.2, 16.3, 18.0; 256 of up to
-        // 600 24.4, 29.4, 51.4. (16 waves of 4 queries would not fit the registers.)
+        // A stream's keys whole in one work-group of W waves (no parts to be joined),
+        // except where few work-groups have many keys each: those are dealt to
+        // work-groups of 4 waves, more keys to each the more of them there are.
+        // us, whole / dealt (heads of 64, 8 of them; contexts of one stream as said,
+        // of several up to that): 1 stream of 2011 keys 8.6 / 10.7, of 8187 19.7 /
+        // 10.4; 4 of 2560 11.3 / 11.6; 16 of 2560 11.5 / 13.3, of 4096 15.7 / 14.3, of
+        // 8187 26.6 / 19.2; 24 of 4096 16.2 / 17.3; 48 of 4096 25.1 / 24.9; 64 of 2048
+        // 16.3 / 18.6, of 4096 26.9 / 28.8, of 8187 53.8 / 49.6; 128 of 4096 52.7 / 53.5.
+        // W = 4, 8, 16: 1 stream of 2011 keys 13.5, 9.5, 8.6; 32 of 4096 28.0, 19.3, 17.7;
+        // 64 of 2048 18.2, 16.3, 18.0; 128 of 2048 32.5, 34.9, 39.5, of 4096 54.2, 52.7,
+        // 59.8; 256 of 600 24.4, 29.4, 51.4. (16 waves of 4 queries would not fit the
+        // registers.)
         d.tiles = group == 1 ? 1 : (group + 3) / 4;
         const size_t groups = (size_t)kv->heads * d.tiles * r->streams;
         const int units = (max_positions - 1) / 64 + 1;
-        d.waves = groups > 768 ? 4 : groups > 256 || group > 1 ? 8 : 16;
+        d.waves = groups > 768 ? (units > 36 ? 8 : 4) : groups > 256 || group > 1 ? 8 : 16;
         d.steps = (units + d.waves - 1) / d.waves;
-        if (d.steps > (groups < 128 ? 2 : groups < 1024 ? 4 : 8)) {
+        if (units > (groups < 192 ? 3 * d.waves : 96 * 64 / kv->head_dim)) {
             d.waves = 4;
             d.steps = (groups < 64 ? 1 : groups < 256 ? 2 : 4) * 64 / kv->head_dim;
             if (d.steps < 1) d.steps = 1;
@@ -1471,10 +1483,19 @@ int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal
     }
     if (!launch_ok("pgpu_kv8_attention")) return 0;
     if (d.splits == 1) return 1;
-    const size_t lanes = (size_t)r.max_rows * wide * (D / 4);
-    hipLaunchKernelGGL(k_kv8_join<D>, dim3((unsigned)((lanes + 255) / 256), 1, streams), dim3(256),
-                       0, st, c, r, a.part_acc, a.part_ml, a.group, a.max_positions, d.splits,
-                       d.keys, out, a.out_stride, status);
+    // Many splits of few rows: a wave for each, spread over the CUs (4 streams of up
+    // to 8187 keys, 32 splits: 11.8 us in all, 13.6 with 16 lanes to a head; a run of
+    // 16 rows after 8000 12.0 and 14.9); else few splits of many rows.
+    const size_t items = (size_t)r.max_rows * wide;
+    if (d.splits >= 8 && items * streams <= 4096)
+        hipLaunchKernelGGL((k_kv8_join<D, 256 / D>), dim3((unsigned)items, 1, streams), dim3(64), 0,
+                           st, c, r, a.part_acc, a.part_ml, a.group, a.max_positions, d.splits,
+                           d.keys, out, a.out_stride, status);
+    else
+        hipLaunchKernelGGL((k_kv8_join<D, 1>),
+                           dim3((unsigned)((items * (D / 4) + 255) / 256), 1, streams), dim3(256),
+                           0, st, c, r, a.part_acc, a.part_ml, a.group, a.max_positions, d.splits,
+                           d.keys, out, a.out_stride, status);
     return launch_ok("pgpu_kv8_attention");
 }
 
