@@ -1,8 +1,6 @@
 // 8-bit paged KV cache: quantised writes (with the heads' norm and rotation in
 // the same pass), reads, and causal attention over it. The formats and the
 // rules of the stored values are in phonon_gpu.h.
-#include <type_traits>
-
 #include "pgpu_common.hpp"
 #include "phonon_gpu.h"
 
@@ -584,7 +582,7 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
 
     i32x4 kr[4][KB], vr[4][KB];
     float ks[4], vs[4];
-    bool wild = false;
+    bool wild = false, spoiled = false;
     // The closed blocks among b .. b + 3.
     auto load = [&](int b, bool values) {
 #pragma unroll
@@ -676,6 +674,8 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
         for (int t = 0; t < 4; t++) {
             w[t] = __builtin_amdgcn_exp2f(w[t] - m);
             sum += w[t];
+            // A block whose values were not finite: fixed point cannot say so.
+            spoiled |= vs[t] != vs[t];
             w[t] *= vs[t];
             big = fmaxf(big, w[t]);
         }
@@ -754,6 +754,7 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
                 }
     }
     if (wild && lane == 0) atomicOr(status, 2);
+    if (spoiled) l = __builtin_nanf("");
 #pragma unroll
     for (int j = 0; j < Q; j++)
 #pragma unroll
@@ -827,8 +828,10 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 __device__ inline f16x4 bytes_f16(int x) {
     const uint32_t u = (uint32_t)x ^ 0x80808080u;
     const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off;
-    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
+    const uint32_t low = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const uint32_t high = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    const f16x2 a = __builtin_bit_cast(f16x2, low) + off;
+    const f16x2 b = __builtin_bit_cast(f16x2, high) + off;
     return f16x4{a.x, a.y, b.x, b.y};
 }
 
@@ -860,7 +863,8 @@ __device__ inline float max3(float a, float b, float c) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a, int *status) {
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a,
+                                                                  int *status) {
     constexpr int KB = D / 64, KS = D / 32, T = D / 16;
     constexpr float kNone = -3.0e38f;  // the maximum of no scores
     __shared__ Kv8RunShared<D> sh;
@@ -962,8 +966,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             if (scale_of.y != scale_of.y) scale_of = make_float2(scale_of.y, 0.0f);
         }
     };
-    auto request = [&](int c, int n) {
-        const int j = n & 63;
+    auto request = [&](int c, int nth) {
+        const int j = nth & 63;
         if (j == 0) look_up(c);
         const unsigned id = (unsigned)__builtin_amdgcn_readlane(id_of, j);
         sc = make_float2(lane_value(scale_of.x, j), lane_value(scale_of.y, j));
@@ -1085,10 +1089,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
                 for (int t = 0; t < 4; t++) v[t] = sh.v[buf][n][t0 + t][lane];
 #pragma unroll
                 for (int t = 0; t < 4; t++)
-                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], ph[n], acc[t0 + t], 0, 0, 0);
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], ph[n],
+                                                                         acc[t0 + t], 0, 0, 0);
 #pragma unroll
                 for (int t = 0; t < 4; t++)
-                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], pl[n], acc[t0 + t], 0, 0, 0);
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], pl[n],
+                                                                         acc[t0 + t], 0, 0, 0);
             }
     };
 
@@ -1106,7 +1112,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             __syncthreads();
         }
     }
-    if (wild && lane == 0) atomicOr(status, 2);
+    if (__any(wild) && lane == 0) atomicOr(status, 2);
     if (live == 0) return;
 
     // The newest block, in fp32 on the fp32 matrix instruction.

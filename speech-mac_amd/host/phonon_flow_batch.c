@@ -419,6 +419,19 @@ int phonon_kv_pool_release_slots(PhononKvPool *pool, size_t count, const int32_t
     return pool && ids_give(&pool->slots, count, slots);
 }
 
+/* Whether these are slots of the pool, each once: a slot is one stream's. */
+static int slots_fit(const PhononKvPool *pool, const int32_t *slots, size_t count) {
+    unsigned char *seen = calloc(pool->slots.count, 1);
+    int ok = seen != NULL;
+    for (size_t i = 0; ok && i < count; i++) {
+        ok = slots[i] >= 0 && (size_t)slots[i] < pool->slots.count && !seen[slots[i]];
+        if (ok)
+            seen[slots[i]] = 1;
+    }
+    free(seen);
+    return ok || ph_fail("open slots: one outside the pool, or one given to two streams");
+}
+
 static const char kNotQ8[] = "the pool holds fp32 blocks, not 8-bit ones",
                   kQ8[] = "the pool holds 8-bit blocks: use the _q8 form of the call";
 
@@ -726,12 +739,13 @@ static int set_streams(PhononFlowBatch *b, size_t streams, const size_t *positio
     if (!b || !streams || streams > b->max_streams || !positions || !tables ||
         table_len != b->table_len)
         return 0;
+    if (slots && !slots_fit(b->pool, slots, streams))
+        return 0;
     int32_t *pos32 = malloc(streams * sizeof(int32_t));
     int32_t *wide = slots ? malloc(streams * table_len * sizeof(int32_t)) : NULL;
     int ok = pos32 && (wide || !slots);
     for (size_t s = 0; ok && s < streams; s++) {
-        ok = positions[s] < b->max_positions &&
-             (!slots || (slots[s] >= 0 && (size_t)slots[s] < b->pool->slots.count));
+        ok = positions[s] < b->max_positions;
         pos32[s] = (int32_t)positions[s];
         for (size_t i = 0; wide && ok && i < table_len; i++)
             wide[s * table_len + i] = slots[s];
@@ -1676,13 +1690,12 @@ static int q8_prefill(PhononFlowBatch *b, size_t streams, const size_t *first,
     int32_t *at = host + streams;
     at[0] = 0;
     b->q8.pre_rows = 0;
-    int ok = 1;
+    int ok = slots_fit(b->pool, slots, streams);
     for (size_t i = 0; i < streams; i++) {
         host[i] = (int32_t)first[i];
         at[i + 1] = at[i] + (int32_t)counts[i];
         if (counts[i] > b->q8.pre_rows)
             b->q8.pre_rows = counts[i];
-        ok = ok && slots[i] >= 0 && (size_t)slots[i] < b->pool->slots.count;
     }
     const size_t bytes = b->padded_streams * 3 * PH_WIDTH * sizeof(float);
     if (ok && !b->q8.qkv)

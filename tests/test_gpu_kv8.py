@@ -834,3 +834,59 @@ def test_what_is_not_finite_stays_with_the_rows_that_see_it(cache, which, bad):
         if s == 1 or which == 1 or np.isnan(bad):
             assert not rest.all(1).any()
         at += n
+
+
+@pytest.mark.parametrize("group", [1, 3])
+def test_a_stored_block_that_was_not_finite_reaches_its_stream_s_row_alone(cache, group):
+    """A NaN scale of keys or values of a block at the front, inside a step and in
+    a later step: that stream's row does not come out finite, the others do."""
+    c = cache(4, 2, 64, positions=700)
+    c.fill([600, 690, 650, 40])
+    a = Attend(c, [n - 1 for n in c.lengths()], None, group)
+    want = a.run()
+    a.check(want)
+    fine = c.scales.download(c.scales0.shape)
+    for which in (0, 1):
+        scales = fine.copy()
+        for s, b in ((0, 0), (1, 41), (2, 7)):
+            scales[1, c.table[s, b], :, which] = np.nan
+        c.scales.upload(scales)
+        got = a.run()
+        assert c.st() == 1
+        assert not np.isfinite(got[:3]).any()
+        assert np.array_equal(got[3], want[3])
+    c.scales.upload(fine)
+
+
+def test_runs_flag_what_they_cannot_cover(cache):
+    """Block ids outside the cache at the front and in a later chunk, a slot
+    outside it, and rows past max_positions: said, and the other streams whole."""
+    c = cache(3, 2, 64, positions=400)
+    c.fill([300, 200, 100])
+    counts = [20, 90, 33]
+    c.write(c.lengths(), counts, *c.random_rows(sum(counts)))
+    a = Attend(c, [300, 200, 100], counts, 2)
+    want = a.run()
+    a.check(want)
+    for s, b in ((0, 0), (1, 7), (0, 13), (2, 5)):
+        table = c.table.copy()
+        table[s, b] = [c.blocks, -1][b % 2]
+        c.tables.upload(table)
+        got = a.run()
+        assert c.st() == 2, (s, b)
+        at = np.concatenate([[0], np.cumsum(counts)])
+        for o in range(3):
+            if o != s:
+                assert np.array_equal(got[at[o]:at[o + 1]], want[at[o]:at[o + 1]])
+    c.tables.upload(c.table)
+    slot = c.slot.copy()
+    slot[2] = -1
+    c.slotd.upload(slot)
+    a.dout.upload(a.mark)
+    got = a.run()
+    assert c.st() == 2 and (got[110:] == 5.5).all() and np.array_equal(got[:110], want[:110])
+    c.slotd.upload(c.slot)
+    b = Attend(c, [300, 200, 100], counts, 2, most=300)
+    got = b.run()
+    assert c.st() == 2 and (got[:20] == 5.5).all()
+    assert np.allclose(got[20:], want[20:], rtol=0, atol=1e-5)

@@ -235,6 +235,14 @@ def test_calls_refuse_the_other_kind_of_pool(server, lib, pkg):
     bad = np.array([0, sv.n + 2], np.int32)
     assert not lib.phonon_flow_batch_set_streams_q8(sv.batch, 2, pos.ctypes.data_as(szp), t,
                                                     sv.stride, i32(bad))
+    both = np.array([sv.slots[0], sv.slots[0]], np.int32)  # one slot for two streams
+    assert not lib.phonon_flow_batch_set_streams_q8(sv.batch, 2, pos.ctypes.data_as(szp), t,
+                                                    sv.stride, i32(both))
+    assert b"two streams" in lib.pgpu_last_error()
+    two = np.ones(2, np.uintp)
+    assert not lib.phonon_flow_batch_prefill_q8_device(
+        sv.batch, 2, pos.ctypes.data, two.ctypes.data, sv.tables.ctypes.data, sv.stride,
+        both.ctypes.data, d.ptr, 10000.0, d.ptr)
     assert not lib.phonon_kv_pool_write_q8(sv.pool, t, sv.stride, sv.n + 2, 0, 4, f32(buf),
                                            f32(buf), MOST)
     assert not lib.phonon_kv_pool_write_q8(sv.pool, t, 1, int(sv.slots[0]), 3, 14, f32(buf),
