@@ -1445,13 +1445,18 @@ Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_posi
         return d;
     }
     // Work-groups without splits; where they are few, each row's keys are dealt
-    // out until there are about two for every CU, 256 keys at least to each.
+    // out until there are about two for every CU, in chunks of 64 and as many at
+    // least to each as pay for the join. us, by the least chunks to a split (heads
+    // of 64, 8 of them): 2 / 4 / whole: 100 rows behind 1000 keys 11.9 / 14.3 / 23.9,
+    // 300 behind 200 12.9 / 14.4 / 14.2, 4 streams of 256 behind 256 17.1 / 16.2 /
+    // 13.8, 1024 rows 20.5 / 18.6 / 21.7, 2 streams of 256 rows 13.1 / 10.1 / 9.9, 16
+    // streams of 16 rows behind 240 12.7 / 9.3 / 9.2, behind 1000 15.5 / 15.1 / 21.2.
     d.tiles = ((r->max_rows + 15) / 16 * group + 3) / 4;
     const size_t groups = (size_t)d.tiles * kv->heads * r->streams;
     const int chunks = (max_positions - 1) / 64 + 1;
     d.splits = groups >= 512 ? 1 : (int)(1024 / groups);
-    const int least = r->max_rows <= 16 ? 2 : 4;
-    if (d.splits > chunks / least) d.splits = chunks / least < 1 ? 1 : chunks / least;
+    const int least = chunks <= 6 ? chunks : groups <= 64 ? 2 : chunks < 12 ? chunks : 4;
+    if (d.splits > chunks / least) d.splits = chunks / least;
     if (d.splits > 32) d.splits = 32;
     d.keys = 0;
     return d;
