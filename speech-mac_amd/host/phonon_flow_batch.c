@@ -529,7 +529,7 @@ static int pool_copy_q8(const PhononKvPool *pool, const int32_t *table, size_t t
                         float *values, size_t capacity, int to_host) {
     if (!pool || !table || !keys || !values || !count || count > capacity ||
         first > capacity - count || first + count > length || length > table_len * 16 ||
-        capacity > PHONON_FLOW_MAX_POSITIONS)
+        capacity > PHONON_FLOW_MAX_POSITIONS || length > PHONON_FLOW_MAX_POSITIONS)
         return 0;
     if (!pool->q8)
         return ph_fail(kNotQ8);
@@ -1864,6 +1864,9 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
                                   float *outputs) {
     if (!b || !b->streams || !inputs || !outputs)
         return 0;
+    /* It would write the prefill's rows again. */
+    if (b->pool->q8 && b->pre.active)
+        return ph_fail("a step over an 8-bit pool after a prefill: set the streams first");
     for (size_t s = 0; s < b->streams; s++)
         if (b->host_positions[s] >= b->max_positions)
             return 0;

@@ -271,3 +271,30 @@ def test_calls_refuse_the_other_kind_of_pool(server, lib, pkg):
     assert lib.phonon_kv_pool_release_slots(sv.pool, 1, i32(twice))
     assert not lib.phonon_kv_pool_release_slots(sv.pool, 1, i32(twice))
     assert lib.phonon_kv_pool_free_slots(sv.pool) == free + 1
+
+
+def test_a_step_after_a_prefill_needs_its_streams(server, lib, pkg):
+    """The prefill's rows are the batch's streams until they are set: a step
+    would write them again. It is refused, and what the pool holds stays."""
+    sv = server(2)
+    sv.hold([5, 16])
+    counts = np.array([20, 3], np.uintp)
+    x = sv.rng.standard_normal((23, 512)).astype(np.float32)
+    d = pkg.DeviceBuffer(lib, x.nbytes)
+    d.upload(x)
+    out = pkg.DeviceBuffer(lib, x.nbytes)
+    first = sv.lengths.astype(np.uintp)
+    assert lib.phonon_flow_batch_prefill_q8_device(
+        sv.batch, 2, first.ctypes.data, counts.ctypes.data, sv.tables.ctypes.data, sv.stride,
+        sv.slots.ctypes.data, d.ptr, 10000.0, out.ptr), pkg.last_error(lib)
+    assert lib.phonon_flow_batch_sync(sv.batch)
+    sv.lengths += counts.astype(int)
+    before = [sv.held(s) for s in range(2)]
+    assert not lib.phonon_flow_batch_step_device(sv.batch, d.ptr, 10000.0, out.ptr)
+    assert b"set the streams" in lib.pgpu_last_error()
+    for s in range(2):
+        for a, b in zip(before[s], sv.held(s)):
+            assert np.array_equal(a, b)
+    sv.set()
+    y = sv.step(x[:2])
+    assert np.isfinite(y).all()
