@@ -1426,6 +1426,11 @@ Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_posi
         // 10.4; 4 of 2560 11.3 / 11.6; 16 of 2560 11.5 / 13.3, of 4096 15.7 / 14.3, of
         // 8187 26.6 / 19.2; 24 of 4096 16.2 / 17.3; 48 of 4096 25.1 / 24.9; 64 of 2048
         // 16.3 / 18.6, of 4096 26.9 / 28.8, of 8187 53.8 / 49.6; 128 of 4096 52.7 / 53.5.
+        // Steps of a dealt work-group, 1 / 2 / 3 / 4: 4 streams of 8187 10.9 / 13.0 / 13.1
+        // / 14.8, 16 20.6 / 19.2 / 21.0 / 20.8, 64 54.4 / 49.4 / 49.5 / 49.7; heads of 128
+        // with 4 queries each, 16 streams of 4096 27.1 / 27.1 / 27.3 / 24.7, 24 of 8187
+        // 58.4 / 58.4 / 50.9 / 56.9, 64 of 4096 74.7 / 72.5 / 69.6 / 80.5, 128 148 / 142 /
+        // 133 / 145.
         // W = 4, 8, 16: 1 stream of 2011 keys 13.5, 9.5, 8.6; 32 of 4096 28.0, 19.3, 17.7;
         // 64 of 2048 18.2, 16.3, 18.0; 128 of 2048 32.5, 34.9, 39.5, of 4096 54.2, 52.7,
         // 59.8; 256 of 600 24.4, 29.4, 51.4. (16 waves of 4 queries would not fit the
@@ -1437,8 +1442,7 @@ Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_posi
         d.steps = (units + d.waves - 1) / d.waves;
         if (units > (groups < 192 ? 3 * d.waves : 96 * 64 / kv->head_dim)) {
             d.waves = 4;
-            d.steps = (groups < 64 ? 1 : groups < 256 ? 2 : 4) * 64 / kv->head_dim;
-            if (d.steps < 1) d.steps = 1;
+            d.steps = groups < 64 ? 1 : groups < 192 ? 128 / kv->head_dim : 3;
         }
         d.keys = 64 * d.waves * d.steps;
         d.splits = (max_positions - 1) / d.keys + 1;
