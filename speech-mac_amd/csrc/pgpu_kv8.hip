@@ -511,14 +511,25 @@ __device__ inline uint32_t quad_lane(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, P * 0x55, 0xf, 0xf, false);
 }
 
-// Bytes of the cache for one row a stream, read once: past the caches where a
-// load instruction takes whole lines (heads of 64: 64 streams of up to 2048 keys
-// 16.3 us against 19.6, 256 of up to 8187 179 against 202). A wide head's comes
-// in two instructions, the second of which finds its lines (35.7 against 43.8).
-template <int D>
+// Bytes of the cache for one row a stream, read once: past the caches, which pays
+// where a load instruction takes whole lines (64 streams of up to 2048 keys 16.3 us
+// against 19.6, 256 of up to 8187 179 against 202; heads of 128, 48 streams of up to
+// 4096 keys 46.6 against 55.5, and 55.9 with half lines and the caches).
 __device__ inline i32x4 stream_load16(const int8_t *p) {
-    if (D == 64) return __builtin_nontemporal_load((const i32x4 *)p);
-    return *(const i32x4 *)p;
+    return __builtin_nontemporal_load((const i32x4 *)p);
+}
+
+// Lanes 0..3 of 8 get the first half of lane ^ 7 as their second one, and the
+// others the second half of lane ^ 7 as their first.
+template <int KB>
+__device__ inline void trade_halves(i32x4 (&x)[KB]) {
+    if constexpr (KB == 2)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int a = x[0][e], b = x[1][e];
+            x[0][e] = __builtin_amdgcn_update_dpp(a, b, 0x141, 0xf, 0xa, false);
+            x[1][e] = __builtin_amdgcn_update_dpp(b, a, 0x141, 0xf, 0x5, false);
+        }
 }
 
 struct Kv8Decode {
@@ -545,15 +556,20 @@ struct Kv8DecodeShared {
 // 64 are 4 blocks, whose bytes it requests together (8 or 16 KB), the next
 // step's as soon as the registers are free: keys after the scores, values
 // after their product. Bound by the cache's bytes; no wave waits for another
-// before the joint of all W.
+// before the joint of all W. A step's requests are the same whatever it holds, and
+// the last step stands apart, so that the compiler counts what is in flight and a
+// step waits for its own bytes only (with branches between them it waited for all:
+// 64 streams of 2900 keys, heads of 128 with 4 queries, 62.8 us against 54.8). 256
+// streams of up to 8187 keys, heads of 64: 172 us for 1.10 GB, the rate of a plain
+// read (6.2 TB/s).
 //
 // Values: the 16 bytes that a lane (g, i) holds of a block are 4 positions (4 g
 // ..) of the dims i, 16 + i, 32 + i and 48 + i. They are an operand as they are
 // too: row 4 T + t of the other one has byte t of the weights in word T and
 // zeros elsewhere, so that its sums are those of dims 16 T + i.
 template <int D, int W, int Q>
-__global__ __launch_bounds__(64 * W, D == 64 ? (Q == 1 ? 6 : 5) : (Q == 1 ? 4 : 3))
-void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
+__global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, Kv8Rows rows,
+                                                                        Kv8Decode a, int *status) {
     constexpr int KB = D / 64;
     __shared__ Kv8DecodeShared<D, W, Q> sh;
     // Heads vary fastest: with 8 of them a head's passes stay on one XCD.
@@ -580,49 +596,62 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
     if (split * a.steps * W * 64 > p) return;
     const int newest = p / kBlockPos;
 
+    // Where this lane's 16 bytes are: a key's 16 KB from dim 16 KB g on, and the
+    // block's values from 16 KB lane on. Two instructions of a wide head each take
+    // whole lines: lane and lane ^ 7 have both halves of the one's, then of the
+    // other's, and trade.
+    int key_at[KB], value_at[KB];
+#pragma unroll
+    for (int n = 0; n < KB; n++) {
+        const int flip = D == 64 || (lane & 7) / 4 == n ? 0 : 7, half = (lane & 7) / 4;
+        key_at[n] = (i ^ flip) * D + g * (D / 4) + (D == 64 ? 0 : half * 16);
+        value_at[n] = (lane ^ flip) * (D / 4) + (D == 64 ? 0 : half * 16);
+    }
     i32x4 kr[4][KB], vr[4][KB];
     float ks[4], vs[4];
     bool wild = false, spoiled = false;
-    // The closed blocks among b .. b + 3.
+    // Blocks b .. b + 3; block 0 for one that is not closed, so that every step
+    // requests alike and waits for no more than it needs.
     auto load = [&](int b, bool values) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            if (b + t < newest) {
-                wild |= (unsigned)ids[t] >= kv.blocks;
-                const unsigned id = (unsigned)ids[t] < kv.blocks ? (unsigned)ids[t] : 0u;
-                const int8_t *tile = kv.values + kv8_tile<D>(kv, id, head);
-                const float *sc = kv.scales + ((size_t)id * kv.heads + head) * 2;
-                (values ? vs : ks)[t] = uniform_load(sc + values);
+            const unsigned raw = b + t < newest ? (unsigned)ids[t] : 0u;
+            wild |= raw >= kv.blocks;
+            const unsigned id = raw < kv.blocks ? raw : 0u;
+            const int8_t *tile = kv.values + kv8_tile<D>(kv, id, head);
+            const float *sc = kv.scales + ((size_t)id * kv.heads + head) * 2;
+            (values ? vs : ks)[t] = uniform_load(sc + values);
 #pragma unroll
-                for (int n = 0; n < KB; n++)
-                    (values ? vr : kr)[t][n] =
-                        stream_load16<D>(values ? tile + kBlockPos * D + lane * (D / 4) + n * 16
-                                             : tile + i * D + n * 64 + g * 16);
-            } else {
-                (values ? vs : ks)[t] = 0.0f;
-#pragma unroll
-                for (int n = 0; n < KB; n++) (values ? vr : kr)[t][n] = i32x4{0, 0, 0, 0};
-            }
+            for (int n = 0; n < KB; n++)
+                (values ? vr : kr)[t][n] = stream_load16(
+                    tile + (values ? kBlockPos * D + value_at[n] : key_at[n]));
         }
     };
-    load(b0, false);
-    load(b0, true);
     const float *slot = kv.open + ((size_t)span.slot * kv.heads + head) * (2 * kBlockPos * D);
 
     // Row i of the operand: byte i % 4 of query j0 + i / 4.
     const float *q = a.q + (size_t)s * a.q_stride +
                      ((size_t)head * a.group + min(j0 + (i >> 2), a.group - 1)) * D;
+    float4 x[KB][4];
+#pragma unroll
+    for (int n = 0; n < KB; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[n][k] = *(const float4 *)(q + g * (D / 4) + n * 16 + k * 4);
+    // The order of the requests is the order in which they are waited for.
+    __builtin_amdgcn_sched_barrier(0);
+    load(b0, false);
+    __builtin_amdgcn_sched_barrier(0);
+    load(b0, true);
+    __builtin_amdgcn_sched_barrier(0);
     const uint32_t byte = row_byte(i & 3), sel = byte | (4u + byte) << 8;
     i32x4 qd[KB];
     float step, top = 0.0f;
     {
-        float4 x[KB][4];
 #pragma unroll
         for (int n = 0; n < KB; n++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float4 v = *(const float4 *)(q + n * 64 + g * 16 + k * 4);
-                x[n][k] = v;
+                const float4 v = x[n][k];
                 top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
                                        fmaxf(fabsf(v.z), fabsf(v.w))));
             }
@@ -645,9 +674,8 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
 #pragma unroll
         for (int k = 0; k < KB; k++) acc[j][k] = 0.0f;
 
-    for (int n = 0; n < a.steps && b0 < newest; n++, b0 += 4 * W) {
+    auto attend = [&](bool more) {
         const int closed = newest - b0;  // blocks from b0 on
-        const bool more = n + 1 < a.steps && b0 + 4 * W < newest;
         if (more)
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -657,6 +685,7 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             i32x4 c = {0, 0, 0, 0};
+            trade_halves<KB>(kr[t]);
 #pragma unroll
             for (int k = 0; k < KB; k++)
                 c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[k], kr[t][k], c, 0, 0, 0);
@@ -674,9 +703,10 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
         for (int t = 0; t < 4; t++) {
             w[t] = __builtin_amdgcn_exp2f(w[t] - m);
             sum += w[t];
+            const float v = t < closed ? vs[t] : 0.0f;
             // A block whose values were not finite: fixed point cannot say so.
-            spoiled |= vs[t] != vs[t];
-            w[t] *= vs[t];
+            spoiled |= v != v;
+            w[t] *= v;
             big = fmaxf(big, w[t]);
         }
         l = fmaf(l, shrink, row16_sum(sum));
@@ -691,6 +721,8 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
         }
         *(i32x4 *)&sh.digits[wave][g * 4 + (i & 3)][(i >> 2) * 4] = word;
         wave_lds_fence();
+#pragma unroll
+        for (int t = 0; t < 4; t++) trade_halves<KB>(vr[t]);
 #pragma unroll
         for (int j = 0; j < Q; j++) {
             const i32x4 pd = *(const i32x4 *)&sh.digits[wave][j * 4 + (i & 3)][g * 4];
@@ -710,9 +742,14 @@ void k_kv8_decode(Kv8 kv, Kv8Rows rows, Kv8Decode a, int *status) {
 #pragma unroll
             for (int k = 0; k < KB; k++) acc[j][k] = fmaf(fix_sum(c[k]), one, acc[j][k] * less);
         }
-        if (more) load(b0 + 4 * W, true);
+        b0 += 4 * W;
+        if (more) load(b0, true);
         wave_lds_fence();
-    }
+    };
+    // The last step apart: no branch stands between a request and its wait.
+    int steps = b0 < newest ? min(a.steps, (newest - b0 - 1) / (4 * W) + 1) : 0;
+    for (; steps > 1; steps--) attend(true);
+    if (steps > 0) attend(false);
     // The newest block, in fp32: by the wave after the one whose blocks end there,
     // which has had a step less.
     if (newest / (a.steps * W * 4) == split && (newest / 4 + 1) % W == wave) {
@@ -1421,28 +1458,29 @@ Deal deal_of(const pgpu_kv8 *kv, const pgpu_kv8_rows *r, int group, int max_posi
         // A stream's keys whole in one work-group of W waves (no parts to be joined),
         // except where few work-groups have many keys each: those are dealt to
         // work-groups of 4 waves, more keys to each the more of them there are.
-        // us, whole / dealt (heads of 64, 8 of them; contexts of one stream as said,
-        // of several up to that): 1 stream of 2011 keys 8.6 / 10.7, of 8187 19.7 /
-        // 10.4; 4 of 2560 11.3 / 11.6; 16 of 2560 11.5 / 13.3, of 4096 15.7 / 14.3, of
-        // 8187 26.6 / 19.2; 24 of 4096 16.2 / 17.3; 48 of 4096 25.1 / 24.9; 64 of 2048
-        // 16.3 / 18.6, of 4096 26.9 / 28.8, of 8187 53.8 / 49.6; 128 of 4096 52.7 / 53.5.
-        // Steps of a dealt work-group, 1 / 2 / 3 / 4: 4 streams of 8187 10.9 / 13.0 / 13.1
-        // / 14.8, 16 20.6 / 19.2 / 21.0 / 20.8, 64 54.4 / 49.4 / 49.5 / 49.7; heads of 128
-        // with 4 queries each, 16 streams of 4096 27.1 / 27.1 / 27.3 / 24.7, 24 of 8187
-        // 58.4 / 58.4 / 50.9 / 56.9, 64 of 4096 74.7 / 72.5 / 69.6 / 80.5, 128 148 / 142 /
-        // 133 / 145.
-        // W = 4, 8, 16: 1 stream of 2011 keys 13.5, 9.5, 8.6; 32 of 4096 28.0, 19.3, 17.7;
-        // 64 of 2048 18.2, 16.3, 18.0; 128 of 2048 32.5, 34.9, 39.5, of 4096 54.2, 52.7,
-        // 59.8; 256 of 600 24.4, 29.4, 51.4. (16 waves of 4 queries would not fit the
-        // registers.)
+        // us, whole / dealt (8 heads of 64; contexts of one stream as said, of several
+        // up to that): 1 stream of 2048 keys 10.1 / 11.1, of 8187 22.4 / 10.2; 16 of
+        // 2048 10.7 / 11.8, of 4096 16.2 / 14.0; 32 of 4096 18.4 / 19.4, 64 26.6 / 27.7,
+        // of 6000 41.6 / 40.1; 128 of 4096 52.3 / 52.4, of 6000 81.3 / 75.6. Heads of
+        // 128: 1 stream of 2048 16.0 / 11.5, 16 of 2900 22.7 / 19.1, 64 39.4 / 43.8, of
+        // 8187 102 / 92.
+        // Steps of a dealt work-group, 1 / 2 / 3 / 4: 4 streams of 8187 11.9 / 11.7 / 12.9
+        // / 12.5, 16 19.6 / 19.4 / 20.9 / 21.4, 256 191 / 182 / 180 / 181; heads of 128
+        // with 4 queries each, 24 of 8187 46.9 / 42.8 / 41.5 / 45.6, 48 of 4096 49.9 / 47.7
+        // / 47.1 / 52.0, 128 126 / 124 / 115 / 127.
+        // W = 4, 8, 16: 1 stream of 2048 keys 12.5, 10.4, 10.1; 32 of 4096 23.1, 18.5,
+        // 18.4; 64 of 2048 17.6, 17.0, 19.5; 128 33.1, 36.6, 41.2, of 4096 56.0, 53.8,
+        // 61.1; 256 of 600 24.2, 31.0, 57.6; heads of 128, 1 of 600 8.9, 8.6, 10.8, 64 of
+        // 2048 31.5, 31.7, 35.1. (16 waves of 4 queries would not fit the registers.)
         d.tiles = group == 1 ? 1 : (group + 3) / 4;
         const size_t groups = (size_t)kv->heads * d.tiles * r->streams;
         const int units = (max_positions - 1) / 64 + 1;
-        d.waves = groups > 768 ? (units > 36 ? 8 : 4) : groups > 256 || group > 1 ? 8 : 16;
+        const bool wide = kv->head_dim != 64;
+        d.waves = groups > 768 ? (units > 36 ? 8 : 4) : groups > 256 || group > 1 || wide ? 8 : 16;
         d.steps = (units + d.waves - 1) / d.waves;
-        if (units > (groups < 192 ? 3 * d.waves : 96 * 64 / kv->head_dim)) {
+        if (units > (groups < 192 ? 3 * d.waves : wide ? 48 : 80)) {
             d.waves = 4;
-            d.steps = groups < 64 ? 1 : groups < 192 ? 128 / kv->head_dim : 3;
+            d.steps = groups < 64 ? 1 : groups < 192 ? (wide ? 1 : 2) : 3;
         }
         d.keys = 64 * d.waves * d.steps;
         d.splits = (max_positions - 1) / d.keys + 1;
@@ -1488,9 +1526,9 @@ int attend(void *stream, const Kv8 &c, const Kv8Rows &r, int streams, const Deal
             KV8_DECODE(4, 1);
         else if (a.group == 1 && d.waves == 8)
             KV8_DECODE(8, 1);
-        else if (a.group == 1)
-            KV8_DECODE(16, 1);
-        else if (d.waves == 4)
+        else if (a.group == 1) {
+            if constexpr (D == 64) KV8_DECODE(16, 1);
+        } else if (d.waves == 4)
             KV8_DECODE(4, 4);
         else
             KV8_DECODE(8, 4);
