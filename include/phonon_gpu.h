@@ -553,7 +553,7 @@ int pgpu_kv8_write(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_r
  * 2i + 1) is turned by its position's angle, rope[position][i] = (cos, sin);
  * in 64 bits, rounded to fp32 once, so that the 8-bit keys do not depend on a
  * summation order. Queries, times q_scale, go to q_out [rows][heads * group *
- * head_dim]; keys and values as in pgpu_kv8_write. */
+ * head_dim], which must not overlap qkv; keys and values as in pgpu_kv8_write. */
 int pgpu_kv8_rotate_write(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,
                           const float *qkv, size_t row_stride, int group, const float *q_weight,
                           const float *k_weight, float epsilon, const float *rope,
@@ -578,9 +578,9 @@ int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer, int layers
  * position is that of its last row here. One row a stream, or runs of rows.
  * `max_positions` bounds every position + 1 (a stream past it is left out,
  * status bit 2). A stream with first < 0 gets zero rows. Strides multiples of
- * 4, pointers 16-byte aligned. `work` (dev): pgpu_kv8_attention_bytes(kv,
- * rows, group, max_positions) bytes that no other call uses at the same time;
- * they need no clearing. */
+ * 4, pointers 16-byte aligned; out must not overlap q. `work` (dev):
+ * pgpu_kv8_attention_bytes(kv, rows, group, max_positions) bytes that no other
+ * call uses at the same time; they need no clearing. */
 size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows, int group,
                                 int max_positions);
 int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,
