@@ -621,8 +621,8 @@ def test_a_prompt_then_frames_together(cache, lib):
     (1, 8, 1, 64, 2000),     # whole streams, 16 waves, two steps
     (40, 8, 1, 64, 1500),    # 8 waves
     (100, 8, 1, 64, 700),    # 4 waves
-    (12, 8, 1, 64, 2300),    # dealt, two steps of 4 waves
-    (64, 8, 1, 64, 8192),    # dealt, four steps
+    (12, 8, 1, 64, 2300),    # 16 waves, three steps
+    (64, 8, 1, 64, 8192),    # dealt, three steps
     (3, 2, 1, 64, 8192),     # dealt, a step
     (30, 8, 4, 64, 900),     # four queries, 8 waves
     (100, 8, 2, 64, 500),    # four queries' places, two queries
@@ -649,6 +649,38 @@ def test_attention_in_each_way_of_dealing_the_keys(cache, streams, heads, group,
         k, v = (model.seen(x) for x in c.rows[s])
         want, bound = model.attention(a.q[s:s + 1], k, v, first[s], a.scale)
         assert (np.abs(got[s:s + 1] - want) <= bound).all(), s
+
+
+@pytest.mark.parametrize("streams,heads,group,dim,most", [
+    (12, 8, 1, 64, 4096),    # dealt, two steps of 4 waves
+    (3, 3, 1, 128, 2000),    # wide heads, dealt, a step
+    (26, 8, 1, 128, 4000),   # dealt, three steps
+    (26, 8, 4, 128, 4000),
+    (100, 8, 1, 128, 700),   # whole, 4 waves
+    (40, 8, 2, 128, 1500),   # whole, 8 waves, three steps
+])
+def test_attention_of_wide_heads_and_dealt_steps(cache, streams, heads, group, dim, most):
+    """Contexts that end in every block of a step, at its borders and in its first
+    block: a step's last blocks are not there, and a wave may have no step."""
+    c = cache(streams, heads, dim, positions=1300 if streams < 30 else 330)
+    lengths = [(1, 16, 17, 63, 64, 65, 113, 255, 256, 257, 321, 511, 513, 767, 769, 1025, 1281)
+               [s % 17] for s in range(streams)]
+    lengths = [min(n, 1300 if streams < 30 else 330) for n in lengths]
+    c.fill(lengths)
+    a = Attend(c, [n - 1 for n in lengths], None, group, most=most)
+    a.check(a.run())
+
+
+@pytest.mark.parametrize("streams,heads,most", [(9, 8, 700), (9, 8, 1000), (2, 2, 1000), (2, 2, 380)])
+def test_runs_dealt_by_their_number(cache, streams, heads, most):
+    """More or fewer than 64 work-groups, with 11, 16 and 6 chunks of keys."""
+    c = cache(streams, heads, 64, positions=380)
+    before = [(0, 300, 129, 64)[s % 4] for s in range(streams)]
+    counts = [(80, 5, 16, 37)[s % 4] for s in range(streams)]
+    c.fill(before)
+    c.write(before, counts, *c.random_rows(sum(counts)))
+    a = Attend(c, before, counts, 1, most=most)
+    a.check(a.run())
 
 
 @pytest.mark.parametrize("most,heads,group,dim", [(4000, 2, 1, 64), (8192, 8, 2, 64),
