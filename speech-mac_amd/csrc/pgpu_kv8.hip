@@ -565,8 +565,8 @@ struct Kv8DecodeShared {
 // the last step stands apart, so that the compiler counts what is in flight and a
 // step waits for its own bytes only (with branches between them it waited for all:
 // 64 streams of 2900 keys, heads of 128 with 4 queries, 62.8 us against 54.8). 256
-// streams of up to 8187 keys, heads of 64: 172 us for 1.10 GB, the rate of a plain
-// read (6.2 TB/s).
+// streams of up to 8187 keys, heads of 64: 169 us for 1.10 GB, the rate of a plain
+// read (6.5 TB/s).
 //
 // Values: the 16 bytes that a lane (g, i) holds of a block are 4 positions (4 g
 // ..) of the dims i, 16 + i, 32 + i and 48 + i. They are an operand as they are
