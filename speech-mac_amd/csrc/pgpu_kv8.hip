@@ -865,8 +865,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
 // a whole number (in units of log 2), so that rescaling is exact and rare; the
 // weights carry their block's value scale relative to 2^unit, the largest power
 // of two below a scale so far, and 2^14 to keep their low terms normal. Bound by
-// vector instructions: a run of 8187 rows over 8 heads of 64 takes 167 us (0.41
-// PFLOP/s of the formula's, 0.82 with the terms'), 254 instructions a tile and chunk in
+// vector instructions: a run of 8187 rows over 8 heads of 64 takes 165 us (0.42
+// PFLOP/s of the formula's, 0.83 with the terms'), 249 instructions a tile and chunk in
 // 69% of the cycles, the matrix cores busy in 32%. Tiles of 16 rows keep 4 waves a SIMD
 // (two tiles a wave, half the waves: 244); a work-group of 8 waves, which would share
 // the conversion by twice the rows, waits at its barriers (192). Short runs are bound
@@ -928,6 +928,17 @@ __device__ inline float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
+}
+
+// The largest over lanes 16 and 32 apart, without the quieting of NaN that fmaxf adds
+// to each operand (8187 rows 164.9 us, 166.8 with it).
+__device__ inline float quarters_max(float v) {
+    auto x = __builtin_amdgcn_permlane16_swap(fbits(v), fbits(v), false, false);
+    v = max3(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]),
+             __builtin_bit_cast(float, (uint32_t)x[1]));
+    x = __builtin_amdgcn_permlane32_swap(fbits(v), fbits(v), false, false);
+    return max3(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]),
+                __builtin_bit_cast(float, (uint32_t)x[1]));
 }
 
 template <int D>
@@ -1105,9 +1116,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
                       max3(max3(w[t + 1][0], w[t + 1][1], w[t + 1][2]), w[t + 1][3],
                            w[t + 1][3]) * f[t + 1]);
         }
-        mx = xor16_32_max(mx);
         // A whole number; not below the last one.
-        const float mn = fmaxf(m, ceilf(mx));
+        const float least = ceilf(quarters_max(mx)), mn = max3(m, least, least);
         uint32_t high = 0;
 #pragma unroll
         for (int t = 0; t < 4; t++) high = max(high, fbits(bs[t].y));
