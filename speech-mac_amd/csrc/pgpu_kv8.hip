@@ -862,9 +862,12 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
 // row's scores and the weights are the next product's operand as they stand
 // (O^T = V^T P^T). A query and a weight are two fp16 terms (22 bits), each
 // product with the cache's whole numbers exact in fp32. The running maximum is
-// a whole number (in units of log 2), so that rescaling is exact and rare; the
-// weights carry their block's value scale relative to 2^unit, the largest power
-// of two below a scale so far, and 2^14 to keep their low terms normal. Bound by
+// a whole number (in units of log 2), so that rescaling is exact and rare. The
+// weights carry their block's value scale times 2^lift, which keeps them below
+// 2^15 and their low terms normal: with every scale so far within 2^4 of the first
+// block's, one lift for all rows; else each row's own, from the largest weight
+// times scale among the keys that it sees (so no row loses bits to a block that it
+// does not see or hardly weighs). Bound by
 // vector instructions: a run of 8187 rows over 8 heads of 64 takes 165 us (0.42
 // PFLOP/s of the formula's, 0.83 with the terms'), 249 instructions a tile and chunk in
 // 69% of the cycles, the matrix cores busy in 32%. Tiles of 16 rows keep 4 waves a SIMD
@@ -1031,18 +1034,26 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     float2 scale_of = make_float2(1.0f, 0.0f), sc;
     bool wild = false;
     const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
+    constexpr int kNear = 4;
+    auto exponent = [](float x) { return (int)(fbits(x) >> 23 & 255u) - 127; };
+    int usual = 0;  // the value scale's of this work-group's first block
     auto look_up = [&](int c) {
         const int at = c + lane * stride, b = at * 4 + wave;
         const bool in = at < c1 && b * kBlockPos < keys;
-        const int raw = in ? table[b] : 0;
+        const int raw = in ? table[b] : 0, front = table[c0 * 4];
         wild |= (unsigned)raw >= kv.blocks;
         id_of = (unsigned)raw < kv.blocks ? raw : 0;
+        usual = exponent(kv.scales[((size_t)((unsigned)front < kv.blocks ? front : 0) * kv.heads +
+                                    head) * 2 + 1]);
         scale_of = make_float2(1.0f, 0.0f);
         if (in) {
             scale_of = *(const float2 *)(kv.scales + ((size_t)id_of * kv.heads + head) * 2);
             // A block whose values were not finite: its scores say so instead, to
             // the rows that see it.
             if (scale_of.y != scale_of.y) scale_of = make_float2(scale_of.y, 0.0f);
+            // The sign says that it is far from the first block's.
+            if (scale_of.y != 0.0f && abs(exponent(scale_of.y) - usual) > kNear)
+                scale_of.y = -scale_of.y;
         }
     };
     auto request = [&](int c, int nth) {
@@ -1077,7 +1088,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     f32x4 acc[T];
 #pragma unroll
     for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int unit = -100;  // acc holds the values' sums / 2^(unit - 14)
+    // acc holds the values' sums times 2^lift. A scale within 2^kNear: below 2^15.
+    int lift = 0;
+    bool apart = false;  // a scale so far was not
 
     auto attend = [&](int buf, int c, bool masked) {
         float2 bs[4];
@@ -1118,20 +1131,36 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
         }
         // A whole number; not below the last one.
         const float least = ceilf(quarters_max(mx)), mn = max3(m, least, least);
-        uint32_t high = 0;
+        uint32_t signs = 0;
 #pragma unroll
-        for (int t = 0; t < 4; t++) high = max(high, fbits(bs[t].y));
-        const int up = max(unit, (int)(__builtin_amdgcn_readfirstlane(high) >> 23) - 127);
-        if (up != unit || __any(mn != m)) {
+        for (int t = 0; t < 4; t++) signs |= fbits(bs[t].y);
+        apart |= (int)__builtin_amdgcn_readfirstlane(signs) < 0;
+        if (apart || __any(mn != m)) {
             const float shrink = __builtin_amdgcn_exp2f(m - mn);
             l *= shrink;
-            const float both = shrink * __builtin_amdgcn_exp2f((float)(unit - up));
+            float both = shrink;
+            if (apart) {
+                // The exponent that no weight times scale of this row passes; and not so
+                // far below a scale that it sees that 2^lift times that overflows.
+                float large = kNone, seen = kNone;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const float e = (float)(exponent(bs[t].y) + 1);
+                    const float best = max3(max3(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
+                    large = max3(large, fmaf(best, f[t], e), large);
+                    if (!masked || t * 16 <= last) seen = fmaxf(seen, e);
+                }
+                large = ceilf(quarters_max(large)) - mn;
+                const float next = fminf(fminf((float)lift + (mn - m), 14.0f - large),
+                                         100.0f - quarters_max(seen));
+                both = __builtin_amdgcn_exp2f((m - mn) + (next - (float)lift));
+                lift = (int)next;
+            }
 #pragma unroll
             for (int t = 0; t < T; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) acc[t][r] *= both;
             m = mn;
-            unit = up;
         }
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -1147,8 +1176,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
         f16x2 hi[4][2], lo[4][2];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            // 2^(14 - unit) times the scale: below 2^15.
-            const float z = ldexpf(bs[t].y, 14 - unit);
+            const float z = ldexpf(fabsf(bs[t].y), lift);
 #pragma unroll
             for (int r = 0; r < 4; r++) l += w[t][r];
             split_pair(w[t][0] * z, w[t][1] * z, hi[t][0], lo[t][0]);
@@ -1178,6 +1206,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
 
     if (c0 < c1) {
         request(c0, 0);
+        lift = 14 - usual - kNear;
         stage(0);
         __syncthreads();
         for (int c = c0, n = 0; c < c1; c += stride, n++) {
@@ -1194,11 +1223,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     if (live == 0) return;
 
     // The newest block, in fp32 on the fp32 matrix instruction.
-    const float back = __builtin_amdgcn_exp2f((float)(unit - 14));
 #pragma unroll
     for (int t = 0; t < T; t++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) acc[t][r] *= back;
+        for (int r = 0; r < 4; r++) acc[t][r] = ldexpf(acc[t][r], -lift);
     if (split == newest / 4 % stride && wave_top >= newest * kBlockPos) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
