@@ -132,7 +132,7 @@ int phonon_flow_batch_prefill_device(PhononFlowBatch *batch, size_t streams, con
  * rows are written before its attention, so a row attends to every block but its
  * prompt's newest as it is stored in 8 bits, its own one included: outputs depend
  * on how a prompt is cut into calls by as much as 8 bits do. (Exact mode 1 sets
- * the projections' terms; the attention has fp32's precision in every mode.) A step
+ * the projections' terms; the attention is pgpu_kv8_attention in every mode.) A step
  * before the streams are set anew is refused: it would write these rows again. */
 int phonon_flow_batch_prefill_q8_device(PhononFlowBatch *batch, size_t streams,
                                         const size_t *first, const size_t *counts,

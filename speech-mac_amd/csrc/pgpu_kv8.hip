@@ -465,12 +465,15 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 kv, Kv8Rows rows, const in
 
 // The sums are taken on the int8 matrix instruction v_mfma_i32_16x16x64_i8:
 // the cache's bytes are its operands as they are stored, nothing is converted.
-// A query (and the weights of 64 keys) becomes a fixed-point number of 23 bits
-// below its largest element, split into three signed bytes that stand in
-// three rows of the other operand: products and sums are exact, and
-//   (hi * 2^16 + mid * 2^8 + lo) * step
-// has the precision of fp32. Four queries fill the 16 rows (row 4 j + t: byte t
-// of query j); a lone query stands there four times, which costs nothing.
+// A query (and the weights of 64 keys) becomes a fixed-point number of 30 bits
+// below its largest element, split into four signed bytes that stand in
+// four rows of the other operand: products and sums are exact, and
+//   ((b3 * 2^8 + b2) * 2^16 + (b1 * 2^8 + b0)) * step
+// is rounded to fp32. An element down to 2^-7 of the largest keeps all its 24
+// bits, a smaller one what is above 2^-31 of the largest (three bytes lost 2^-23 of
+// it: 2^-9 of dims that lie 2^14 below one of the block's). Four queries fill the 16
+// rows (row 4 j + t: byte 3 - t of query j); a lone query stands there four times,
+// which costs nothing.
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -488,23 +491,22 @@ __device__ inline float row16_max(float v) {
 }
 
 // Fixed point below `top` (>= 0, the largest magnitude): the power of two that
-// takes it above 2^22 / 1.004 and not above 127 * 2^16 + 127 * 2^8 + 127, the
-// largest sum of three signed bytes (0x11000 carries a significand above 1.992
-// into the exponent). Below 2^-104 the step stays at 2^-126.
+// takes it above 2^30 / 1.004 and not above 127 * (2^24 + 2^16 + 2^8 + 1), the
+// largest sum of four signed bytes (0x11000 carries a significand above 1.992
+// into the exponent). Below 2^-96 the step stays at 2^-126.
 __device__ inline int fix_exponent(float top) {
-    return min(126, 149 - (int)((fbits(top) + 0x11000u) >> 23));
+    return min(126, 157 - (int)((fbits(top) + 0x11000u) >> 23));
 }
 __device__ inline float power_of_2(int e) { return bitsf((uint32_t)(127 + e) << 23); }
-// The three bytes of the number (bits 0..23), each signed: n = sum of
-// byte t * 256^t.
+// The four bytes of the number, each signed: n = sum of byte t * 256^t.
 __device__ inline uint32_t fix_bytes(float x, float mul) {
-    return ((uint32_t)(int)rintf(x * mul) + 0x808080u) ^ 0x808080u;
+    return ((uint32_t)(int)rintf(x * mul) + 0x80808080u) ^ 0x80808080u;
 }
 // Which byte of a number stands in row t of its query: the highest in row 0.
-// Row 3 repeats the lowest byte; nothing reads its sums.
-__device__ inline uint32_t row_byte(int t) { return t < 2 ? 2u - t : 0u; }
+__device__ inline uint32_t row_byte(int t) { return 3u - t; }
+// At most 128 products of 2^14 to a byte: two bytes' sums together stay below 2^30.
 __device__ inline float fix_sum(i32x4 c) {
-    return fmaf((float)(c.x * 256 + c.y), 256.0f, (float)c.z);
+    return fmaf((float)(c.x * 256 + c.y), 65536.0f, (float)(c.z * 256 + c.w));
 }
 
 __device__ inline float lane_value(float v, int lane) {

@@ -105,3 +105,37 @@ def test_a_large_block_with_a_small_weight(cache, behind):
     a.q[:, :, 0] = 4.0
     a.dq.upload(a.q.reshape(a.total, -1))
     check(c, a, a.run())
+
+
+@pytest.mark.parametrize("behind", [0.0, 5.0, 21.0, 250.0])
+@pytest.mark.parametrize("heads,group,dim", [(2, 1, 64), (1, 4, 128)])
+def test_one_row_beside_a_large_block_of_little_weight(cache, behind, heads, group, dim):
+    c = cache(1, heads, dim, positions=400)
+    k, v = c.random_rows(400)
+    k *= np.float32(0.1)
+    k[32:48, :, 0] = -2 * behind
+    v[32:48] *= np.float32(2.0 ** 40)
+    c.write([0], [400], k, v)
+    for most in (400, 8192):  # whole, and dealt
+        a = Attend(c, [399], None, group, most=most)
+        a.q[:, :, 0] = 0.5 * dim ** 0.5
+        a.dq.upload(a.q.reshape(a.total, -1))
+        check(c, a, a.run())
+
+
+@pytest.mark.parametrize("power", [4, 10, 14, 17])
+@pytest.mark.parametrize("heads,group,dim", [(2, 1, 64), (1, 4, 128)])
+@pytest.mark.parametrize("runs", [False, True])
+def test_dims_beside_a_far_larger_one(cache, power, heads, group, dim, runs):
+    """One element of the values, and one of the queries over a key channel of next to
+    nothing, 2^power above the others: the other dims are held by their own size."""
+    c = cache(2, heads, dim, positions=300)
+    k, v = (x.reshape(2, 300, heads, dim) for x in c.random_rows(600))
+    v[0, 40::64, :, 5] = 2.0 ** power
+    k[1, :, :, 7] *= np.float32(2.0 ** -power)
+    c.write([0, 0], [300, 300], k.reshape(-1, heads, dim), v.reshape(-1, heads, dim))
+    first, counts = ([0, 200], [300, 100]) if runs else ([299, 299], None)
+    a = Attend(c, first, counts, group)
+    a.q[counts[0] if runs else 1:, :, 7] = 2.0 ** power
+    a.dq.upload(a.q.reshape(a.total, -1))
+    check(c, a, a.run())
