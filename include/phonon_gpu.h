@@ -577,15 +577,18 @@ int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer, int layers
  * head_dim]. The cache already holds the call's rows; each stream's newest
  * position is that of its last row here. One row a stream, or runs of rows.
  * `max_positions` bounds every position + 1 (a stream past it is left out,
- * status bit 2). A stream with first < 0 gets zero rows. Strides multiples of
- * 4, pointers 16-byte aligned; out must not overlap q. A run holds a query's
- * elements and a key's weight times its block's value scale in two fp16 terms: to
- * 2^-21 of themselves, or 2^-28 of the largest that the row sees (blocks whose value
- * scales differ by up to 2^86). One row a stream holds them to 2^-31 of the largest
- * element of the query, or of the weighted scales of 64 keys (magnitudes from 2^-96
- * on); what it multiplies and sums of them is exact. `work` (dev):
- * pgpu_kv8_attention_bytes(kv, rows, group, max_positions) bytes that no other
- * call uses at the same time; they need no clearing. */
+ * status bit 2). A block whose id is outside the cache weighs nothing (status
+ * bit 2; a row that is left no key gets zeros). A stream with first < 0 gets
+ * zero rows. Strides multiples of 4, pointers 16-byte aligned; out must not
+ * overlap q.
+ * A run holds a query's elements and a key's weight times its block's value
+ * scale in two fp16 terms: to 2^-21 of themselves, or 2^-28 of the largest that
+ * the row sees (blocks whose value scales differ by up to 2^86). One row a
+ * stream holds them to 2^-31 of the largest element of the query, or of the
+ * weighted scales of 64 keys (magnitudes from 2^-96 on); what it multiplies and
+ * sums of them is exact.
+ * `work` (dev): pgpu_kv8_attention_bytes(kv, rows, group, max_positions) bytes
+ * that no other call uses at the same time; they need no clearing. */
 size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows, int group,
                                 int max_positions);
 int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,

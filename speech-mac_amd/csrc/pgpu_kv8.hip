@@ -477,6 +477,8 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8 kv, Kv8Rows rows, const in
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+constexpr float kNone = -3.0e38f;  // the maximum of no scores
+
 __device__ inline float row16_max(float v) {
     // v_max of the lane 8, 4, 2, 1 apart within each row of 16.
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
@@ -617,14 +619,19 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
     i32x4 kr[4][KB], vr[4][KB];
     float ks[4], vs[4];
     bool wild = false, spoiled = false;
-    // Blocks b .. b + 3; block 0 for one that is not closed, so that every step
-    // requests alike and waits for no more than it needs.
+    unsigned on = 0;  // bit t: block t of the step whose keys were requested counts
+    // Blocks b .. b + 3; block 0 for one that is not closed or not in the cache, so
+    // that every step requests alike and waits for no more than it needs.
     auto load = [&](int b, bool values) {
+        if (!values) on = 0;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const unsigned raw = b + t < newest ? (unsigned)ids[t] : 0u;
-            wild |= raw >= kv.blocks;
-            const unsigned id = raw < kv.blocks ? raw : 0u;
+            const bool closed = b + t < newest, in = (unsigned)ids[t] < kv.blocks;
+            const unsigned id = closed && in ? (unsigned)ids[t] : 0u;
+            if (!values) {
+                wild |= closed && !in;
+                on |= (closed && in ? 1u : 0u) << t;
+            }
             const int8_t *tile = kv.values + kv8_tile<D>(kv, id, head);
             const float *sc = kv.scales + ((size_t)id * kv.heads + head) * 2;
             (values ? vs : ks)[t] = uniform_load(sc + values);
@@ -676,14 +683,14 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
         step = __shfl(a.scale * power_of_2(-e), g * 4);
     };
     // This lane's query is j0 + g in m and l; acc: dims lane, 64 + lane of each.
-    float m = -INFINITY, l = 0.0f, acc[Q][KB];
+    float m = kNone, l = 0.0f, acc[Q][KB];
 #pragma unroll
     for (int j = 0; j < Q; j++)
 #pragma unroll
         for (int k = 0; k < KB; k++) acc[j][k] = 0.0f;
 
     auto attend = [&](bool more) {
-        const int closed = newest - b0;  // blocks from b0 on
+        const unsigned count = on;
         if (more)
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -697,12 +704,12 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
 #pragma unroll
             for (int k = 0; k < KB; k++)
                 c = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[k], kr[t][k], c, 0, 0, 0);
-            w[t] = t < closed ? fix_sum(c) * (step * ks[t]) : -INFINITY;
+            w[t] = count >> t & 1 ? fix_sum(c) * (step * ks[t]) : -INFINITY;
             mx = fmaxf(mx, w[t]);
         }
         if (more) load(b0 + 4 * W, false);
         mx = row16_max(mx);
-        const float shrink = __builtin_amdgcn_exp2f(m - mx);  // m = -inf: 0
+        const float shrink = __builtin_amdgcn_exp2f(m - mx);  // m = kNone: 0
         m = mx;
         float sum = 0.0f, big = 0.0f;
         // The weights times their blocks' value scales, in fixed point below
@@ -711,7 +718,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
         for (int t = 0; t < 4; t++) {
             w[t] = __builtin_amdgcn_exp2f(w[t] - m);
             sum += w[t];
-            const float v = t < closed ? vs[t] : 0.0f;
+            const float v = count >> t & 1 ? vs[t] : 0.0f;
             // A block whose values were not finite: fixed point cannot say so.
             spoiled |= v != v;
             w[t] *= v;
@@ -837,7 +844,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
         float total = 0.0f, o = 0.0f;
 #pragma unroll
         for (int n = 0; n < W; n++) {
-            // A wave past the context: l = 0, m = -inf, acc = 0.
+            // A wave past the context: l = 0, m = kNone, acc = 0.
             const float c = __builtin_amdgcn_exp2f(sh.m[n][j] - mx);
             total = fmaf(sh.l[n][j], c, total);
             o = fmaf(sh.acc[n][j][d], c, o);
@@ -950,7 +957,6 @@ template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Rows rows, Kv8Run a,
                                                                   int *status) {
     constexpr int KB = D / 64, KS = D / 32, T = D / 16;
-    constexpr float kNone = -3.0e38f;  // the maximum of no scores
     __shared__ Kv8RunShared<D> sh;
     // Heads fastest (with 8 of them a head's keys stay in one XCD's L2), the
     // longest rows first, and every second 256 work-groups the other way round: a
@@ -1056,6 +1062,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             // The sign says that it is far from the first block's.
             if (scale_of.y != 0.0f && abs(exponent(scale_of.y) - usual) > kNear)
                 scale_of.y = -scale_of.y;
+            // A block that is not in the cache is left out: its scores, which are NaN
+            // to the maximum, become -inf.
+            if ((unsigned)raw >= kv.blocks) scale_of = make_float2(__builtin_nanf(""), -0.0f);
         }
     };
     auto request = [&](int c, int nth) {
@@ -1151,6 +1160,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
                     const float best = max3(max3(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
                     large = max3(large, fmaf(best, f[t], e), large);
                     if (!masked || t * 16 <= last) seen = fmaxf(seen, e);
+                    if (fbits(bs[t].y) == 0x80000000u) {  // no block
+                        w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        f[t] = 1.0f;
+                    }
                 }
                 large = ceilf(quarters_max(large)) - mn;
                 const float next = fminf(fminf((float)lift + (mn - m), 14.0f - large),
@@ -1293,7 +1306,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     if (i < live) {
         const size_t at = (row * kv.heads * a.group + qh) * a.splits + split;
         float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
-        const float f = a.splits == 1 ? 1.0f / l : 1.0f;
+        // l = 0: every block that the row sees was left out.
+        const float f = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int t = 0; t < T; t++) {
             const float4 o = make_float4(acc[t][0] * f, acc[t][1] * f, acc[t][2] * f, acc[t][3] * f);
@@ -1370,7 +1384,8 @@ __global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const fl
         o.w += __shfl_xor(o.w, z);
     }
     if (share) return;
-    o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
+    // A sum of 0: every block that the row sees was left out.
+    if (total != 0.0f) o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
     *(float4 *)dst = o;
     flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
 }
