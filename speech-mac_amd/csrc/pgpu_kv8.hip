@@ -679,8 +679,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
             for (int k = 0; k < 4; k++)
                 qd[n][k] = (int)pick4(fix_bytes(x[n][k].x, mul), fix_bytes(x[n][k].y, mul),
                                       fix_bytes(x[n][k].z, mul), fix_bytes(x[n][k].w, mul), sel);
-        // From here on this lane's query is j0 + g (rows 4 g .. 4 g + 3).
-        step = __shfl(a.scale * power_of_2(-e), g * 4);
+        // From here on this lane's query is j0 + g (rows 4 g .. 4 g + 3). Fixed point
+        // cannot say that it is infinite.
+        step = __shfl(top < INFINITY ? a.scale * power_of_2(-e) : __builtin_nanf(""), g * 4);
     };
     // This lane's query is j0 + g in m and l; acc: dims lane, 64 + lane of each.
     float m = kNone, l = 0.0f, acc[Q][KB];
@@ -801,6 +802,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
             c = __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, y.w, c, 0, 0, 0);
         }
         float w = newest * kBlockPos + i <= p ? c.x * a.scale : -INFINITY;
+        // An infinite query's scores may all be -inf.
+        if (!(__shfl(xor16_32_max(top), g * 4) < INFINITY)) w = __builtin_nanf("");
         const float mx = row16_max(fmaxf(m, w)), shrink = __builtin_amdgcn_exp2f(m - mx);
         m = mx;
         w = __builtin_amdgcn_exp2f(w - m);

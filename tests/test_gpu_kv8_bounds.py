@@ -34,3 +34,49 @@ def test_a_block_outside_the_cache_weighs_nothing(cache, counts, group, dim, mos
         c.scales.upload(changed)
         a = Attend(c, [300 - x for x in n], counts, group, most=most)
         check(c, a, a.run(), LOST, 2)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("counts", [None, [20, 33]])
+@pytest.mark.parametrize("group,dim", [(1, 64), (4, 128)])
+def test_a_query_that_is_not_finite(cache, counts, group, dim, bad):
+    """Its row does not come out finite, whatever the newest block's keys make of it
+    in fp32, and is said; the other rows and heads come out as without it."""
+    c = cache(2, 2, dim, positions=200)
+    k, v = c.random_rows(400)
+    k[:, :, 3] = np.abs(k[:, :, 3]) + 0.5  # infinite scores are of one sign
+    c.write([0, 0], [193, 199], k[:392], v[:392])
+    n = counts or [1, 1]
+    for most in (200, 8192):
+        a = Attend(c, [193 - n[0], 199 - n[1]], counts, group, most=most)
+        want = a.run()
+        assert c.st() == 0
+        row = n[0] - 1  # the newest block has its key alone
+        q = a.q.copy()
+        q[row, 0, 3] = bad
+        a.dq.upload(q.reshape(a.total, -1))
+        got = a.run()
+        assert c.st() == 1
+        assert not np.isfinite(got[row, 0]).any()
+        got[row, 0] = want[row, 0]
+        assert np.array_equal(got[:, ::group], want[:, ::group])
+
+
+@pytest.mark.parametrize("most", [64, 8192])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_a_query_that_is_not_finite_over_a_first_block(cache, bad, most):
+    c = cache(2, 2, 64, positions=30)
+    k, v = c.random_rows(14)
+    k[:, :, 3] = np.abs(k[:, :, 3]) + 0.5
+    c.write([0, 0], [3, 11], k, v)
+    a = Attend(c, [2, 10], None, 1, most=most)
+    want = a.run()
+    assert c.st() == 0
+    q = a.q.copy()
+    q[0, 1, 3] = bad
+    a.dq.upload(q.reshape(a.total, -1))
+    got = a.run()
+    assert c.st() == 1
+    assert not np.isfinite(got[0, 1]).any()
+    got[0, 1] = want[0, 1]
+    assert np.array_equal(got, want)
