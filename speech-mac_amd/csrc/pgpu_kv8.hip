@@ -1309,7 +1309,14 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     if (i < live) {
         const size_t at = (row * kv.heads * a.group + qh) * a.splits + split;
         float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
-        // l = 0: every block that the row sees was left out.
+        // A sum of 0 over keys that the row sees: their blocks were left out, which
+        // gives zeros, or all scores are -inf, which does not come out finite.
+        if (l == 0.0f && p >= c0 * 64) {
+            bool lost = false;
+            for (int b = 0; b < newest && b * kBlockPos <= p; b++)
+                lost |= (unsigned)table[b] >= kv.blocks;
+            if (!lost) l = __builtin_nanf("");
+        }
         const float f = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int t = 0; t < T; t++) {
@@ -1387,8 +1394,8 @@ __global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const fl
         o.w += __shfl_xor(o.w, z);
     }
     if (share) return;
-    // A sum of 0: every block that the row sees was left out.
-    if (total != 0.0f) o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
+    // A sum of 0 in a run: every block that the row sees was left out.
+    if (keys || total != 0.0f) o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
     *(float4 *)dst = o;
     flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
 }

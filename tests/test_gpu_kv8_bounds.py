@@ -80,3 +80,20 @@ def test_a_query_that_is_not_finite_over_a_first_block(cache, bad, most):
     assert not np.isfinite(got[0, 1]).any()
     got[0, 1] = want[0, 1]
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("most", [64, 300, 8192])
+@pytest.mark.parametrize("counts", [None, [20, 33]])
+def test_scores_that_are_all_minus_infinity(cache, counts, most):
+    """Products of large finite keys and queries that pass fp32: no weights are left,
+    and that is said."""
+    c = cache(2, 2, 64, positions=60)
+    k, v = c.random_rows(120)
+    k = -np.abs(k) * np.float32(1e20)
+    c.write([0, 0], [55, 60], k[:115], v[:115])
+    n = counts or [1, 1]
+    a = Attend(c, [55 - n[0], 60 - n[1]], counts, 1, most=most)
+    a.q = np.abs(a.q) * np.float32(1e20)
+    a.dq.upload(a.q.reshape(a.total, -1))
+    got = a.run()
+    assert c.st() == 1 and not np.isfinite(got).any()
