@@ -588,7 +588,9 @@ int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer, int layers
  * weighted scales of 64 keys (magnitudes from 2^-96 on); what it multiplies and
  * sums of them is exact.
  * `work` (dev): pgpu_kv8_attention_bytes(kv, rows, group, max_positions) bytes
- * that no other call uses at the same time; they need no clearing. */
+ * that no other call uses at the same time; they need no clearing. They do for
+ * every call of at most these streams, max_rows and max_positions, with offsets
+ * or without as here (a few streams may need more than many). */
 size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_rows *rows, int group,
                                 int max_positions);
 int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_kv8_rows *rows,

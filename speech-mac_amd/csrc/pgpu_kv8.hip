@@ -1,6 +1,8 @@
 // 8-bit paged KV cache: quantised writes (with the heads' norm and rotation in
 // the same pass), reads, and causal attention over it. The formats and the
 // rules of the stored values are in phonon_gpu.h.
+#include <algorithm>
+
 #include "pgpu_common.hpp"
 #include "phonon_gpu.h"
 
@@ -547,8 +549,9 @@ struct Kv8Decode {
     int group;
     float scale;  // of the scores, times log2 e
     int max_positions, splits, steps;  // a split: steps * W * 64 keys
-    float *part_acc, *part_ml;  // slot (row * query heads + head) * splits + split
-    float *out;                 // splits = 1: the rows themselves (else NULL)
+    // Slot ((s * max_rows + row of the stream) * query heads + head) * splits + split.
+    float *part_acc, *part_ml;
+    float *out;  // splits = 1: the rows themselves (else NULL)
     size_t out_stride;
 };
 
@@ -1307,7 +1310,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     l = xor16_32_sum(l);
     bool bad = false;
     if (i < live) {
-        const size_t at = (row * kv.heads * a.group + qh) * a.splits + split;
+        const size_t at = (((size_t)s * rows.max_rows + r0 + i) * kv.heads * a.group + qh) *
+                              a.splits + split;
         float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
         // A sum of 0 over keys that the row sees: their blocks were left out, which
         // gives zeros, or all scores are -inf, which does not come out finite.
@@ -1354,7 +1358,7 @@ __global__ __launch_bounds__(256) void k_kv8_join(Kv8 kv, Kv8Rows rows, const fl
         return;
     }
     const int n = keys ? (span.first + (int)i) / keys + 1 : splits;
-    const size_t at = (row * wide + qh) * splits;
+    const size_t at = (((size_t)s * rows.max_rows + i) * wide + qh) * splits;
     // Lane j of the M has split j's maximum and sum, and the next M's.
     float mx = -INFINITY, total = 0.0f;
     for (int j = lane; j < n; j += M) mx = fmaxf(mx, part_ml[(at + j) * 2]);
@@ -1655,9 +1659,30 @@ extern "C" size_t pgpu_kv8_attention_bytes(const pgpu_kv8 *kv, const pgpu_kv8_ro
                                            int group, int max_positions) {
     if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
     if (rows->rows == 0) return 0;
-    const Deal d = deal_of(kv, rows, group, max_positions);
-    if (d.splits == 1) return 0;
-    return (size_t)rows->rows * kv->heads * group * d.splits * (kv->head_dim + 2) * sizeof(float);
+    // Fewer streams, rows or positions may be dealt to more work-groups: the most
+    // parts of any of them.
+    size_t parts = 0;
+    if (!rows->offsets) {
+        // More positions never give fewer parts. More streams do, at the numbers of
+        // work-groups where the keys to each change: the streams before those count.
+        const int heads = kv->heads * (group == 1 ? 1 : (group + 3) / 4);
+        for (int n : {rows->streams, 63 / heads, 191 / heads}) {
+            pgpu_kv8_rows fewer = *rows;
+            fewer.streams = n;
+            if (n < 1 || n > rows->streams) continue;
+            const Deal d = deal_of(kv, &fewer, group, max_positions);
+            if (d.splits > 1) parts = std::max(parts, (size_t)n * kv->heads * group * d.splits);
+        }
+    } else {
+        // Splits times work-groups are at most 1024, a work-group has 64 rows.
+        const int chunks = (max_positions - 1) / 64 + 1;
+        const int most = std::min({32, chunks <= 6 ? 1 : chunks / 2,
+                                   1024 / (kv->heads * ((group + 3) / 4))});
+        if (most > 1)
+            parts = std::min((size_t)1024 * 64, (size_t)rows->streams * rows->max_rows *
+                                                    kv->heads * group * most);
+    }
+    return parts * (kv->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
@@ -1675,14 +1700,13 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
     const Deal d = deal_of(kv, rows, group, max_positions);
     // The grid's limit: 16 million positions of one row a stream.
     if (d.splits > 65535) return bad_arguments("pgpu_kv8_attention");
-    const size_t need = pgpu_kv8_attention_bytes(kv, rows, group, max_positions);
-    if (need && (!work || !aligned(work, 16) || work_bytes < need))
+    const size_t parts = d.splits > 1 ? (size_t)rows->streams * rows->max_rows * kv->heads *
+                                            group * d.splits : 0;
+    if (parts && (!work || !aligned(work, 16) ||
+                  work_bytes < parts * (kv->head_dim + 2) * sizeof(float)))
         return bad_arguments("pgpu_kv8_attention (workspace)");
     const Kv8Decode a = {q, q_stride, group, scale * 1.44269504f, max_positions, d.splits, 1,
-                         (float *)work,
-                         (float *)work + (size_t)rows->rows * kv->heads * group * d.splits *
-                                             kv->head_dim,
-                         out, out_stride};
+                         (float *)work, (float *)work + parts * kv->head_dim, out, out_stride};
     const Kv8 c = layer_of(kv, layer);
     return kv->head_dim == 64
                ? attend<64>(stream, c, rows_of(rows), rows->streams, d, a, status)

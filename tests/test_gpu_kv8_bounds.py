@@ -1,4 +1,7 @@
-"""Attention over an 8-bit cache where tables lead outside it."""
+"""Attention over an 8-bit cache at the ends of what it takes: tables that lead outside
+it, numbers that are not finite, a full batch's workspace for a smaller one."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -97,3 +100,18 @@ def test_scores_that_are_all_minus_infinity(cache, counts, most):
     a.dq.upload(a.q.reshape(a.total, -1))
     got = a.run()
     assert c.st() == 1 and not np.isfinite(got).any()
+
+
+@pytest.mark.parametrize("streams,counts,most", [(23, None, 3136), (7, None, 3136), (1, None, 8192),
+                                                 (2, [30, 5], 3136), (1, [1], 8192)])
+def test_a_full_batch_s_workspace_holds_a_smaller_one(cache, streams, counts, most):
+    """Fewer streams may be dealt to more work-groups than 24, or runs of 64 rows."""
+    c = cache(24, 8, 64, positions=130)
+    c.fill([130] * 24)
+    full = c.call_rows([0] * 24, counts and [64] * 24)
+    size = c.lib.pgpu_kv8_attention_bytes(ctypes.byref(c.kv), ctypes.byref(full), 1, most)
+    c.n = streams
+    n = counts or [1] * streams
+    a = Attend(c, [130 - x for x in n], counts, 1, most=most)
+    a.bytes, a.work = size, c.up(np.full(max(16, size), 0xFF, np.uint8))
+    check(c, a, a.run())
