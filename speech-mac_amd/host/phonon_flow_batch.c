@@ -107,7 +107,8 @@ struct PhononFlowBatch {
     int *status;
     /* Over an 8-bit pool: each stream's open slot, the tables by which the
      * projections append to it (every entry the slot), the attention's rows and
-     * workspace; a prefill's projected rows, and zeros for their residual. */
+     * its workspace, made with the batch; a prefill's projected rows, and zeros for
+     * their residual. */
     struct {
         int32_t *slots, *slot_tables;
         float *att, *qkv, *zeros;
@@ -630,6 +631,20 @@ void phonon_flow_batch_destroy(PhononFlowBatch *b) {
     free(b);
 }
 
+/* The attention's workspace over an 8-bit pool: for every step and prefill that
+ * the batch can have. */
+static size_t q8_work_bytes(const PhononFlowBatch *b) {
+    const int most = (int)(b->table_len * 16), n = (int)b->max_streams;
+    const int32_t *any = b->positions; /* not read */
+    pgpu_kv8_rows rows = {.tables = any, .table_stride = (int)b->table_len, .slots = any,
+                          .first = any, .streams = n, .rows = n, .max_rows = 1};
+    const size_t step = pgpu_kv8_attention_bytes(&b->pool->kv8, &rows, 1, most);
+    rows.offsets = any;
+    rows.max_rows = n;
+    const size_t prefill = pgpu_kv8_attention_bytes(&b->pool->kv8, &rows, 1, most);
+    return step > prefill ? step : prefill;
+}
+
 int ph_batch_create_on(const PhononFlowModel *model, PhononKvPool *pool, size_t max_streams,
                        size_t max_positions, void *stream, PhononFlowBatch **batch) {
     if (!batch)
@@ -678,7 +693,11 @@ int ph_batch_create_on(const PhononFlowModel *model, PhononKvPool *pool, size_t 
         b->q8.slots = pgpu_malloc(max_streams * sizeof(int32_t));
         b->q8.slot_tables = pgpu_malloc(max_streams * b->table_len * sizeof(int32_t));
         b->q8.att = pgpu_malloc(rows);
-        ok = ok && b->q8.slots && b->q8.slot_tables && b->q8.att;
+        b->q8.work_bytes = q8_work_bytes(b);
+        if (b->q8.work_bytes)
+            b->q8.work = pgpu_malloc(b->q8.work_bytes);
+        ok = ok && b->q8.slots && b->q8.slot_tables && b->q8.att &&
+             (b->q8.work || !b->q8.work_bytes);
     }
     b->host_positions = calloc(max_streams, sizeof(size_t));
     b->fl.cover = calloc(max_streams, sizeof(size_t));
@@ -849,24 +868,6 @@ static pgpu_kv8_rows q8_rows(const PhononFlowBatch *b) {
 static int q8_positions(const PhononFlowBatch *b) {
     const size_t keys = b->splits * PH_SPLIT_KEYS, most = b->table_len * 16;
     return (int)(keys < most ? keys : most);
-}
-
-/* Room for the attention's parts with b->splits, before any capture. Graphs
- * hold the workspace's address. */
-static int q8_reserve(PhononFlowBatch *b) {
-    if (!b->pool->q8)
-        return 1;
-    const pgpu_kv8_rows rows = q8_rows(b);
-    const size_t need = pgpu_kv8_attention_bytes(&b->pool->kv8, &rows, 1, q8_positions(b));
-    if (need <= b->q8.work_bytes)
-        return 1;
-    if (!pgpu_stream_sync(b->stream))
-        return 0;
-    drop_graphs(b);
-    pgpu_free(b->q8.work);
-    b->q8.work = pgpu_malloc(need);
-    b->q8.work_bytes = b->q8.work ? need : 0;
-    return b->q8.work != NULL;
 }
 
 /* The attention of a layer of an 8-bit pool into the rows q8.att. */
@@ -1731,8 +1732,7 @@ static int prefill_device(PhononFlowBatch *b, size_t streams, const size_t *firs
         return 0;
     if (flow_usable(b, 1))
         return flow_prepare(b, 1) && enqueue_flow(b, inputs, outputs, theta);
-    return (b->splits = splits_for(b, 0)) > 0 && q8_reserve(b) &&
-           enqueue_step(b, inputs, outputs, theta);
+    return (b->splits = splits_for(b, 0)) > 0 && enqueue_step(b, inputs, outputs, theta);
 }
 
 int phonon_flow_batch_prefill_device(PhononFlowBatch *b, size_t streams, const size_t *first,
@@ -1880,8 +1880,6 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
      * and position lag as arguments: it is never captured. */
     if (b->eager || b->time_before || flow) {
         b->splits = splits_for(b, 0);
-        if (!q8_reserve(b))
-            return 0;
         if (!(flow ? enqueue_flow(b, inputs, outputs, theta)
                    : enqueue_step(b, inputs, outputs, theta)))
             return 0;
@@ -1894,9 +1892,6 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
      * context outgrows it. */
     const size_t need = splits_for(b, 0);
     void *exec = NULL;
-    b->splits = splits_for(b, PH_SPLIT_KEYS);
-    if (!q8_reserve(b))
-        return 0;
     for (size_t i = 0; i < 2 && !exec; i++)
         if (b->graphs[i].exec && b->graphs[i].streams == b->streams &&
             b->graphs[i].splits >= need && b->graphs[i].theta == theta &&
@@ -1906,6 +1901,7 @@ int phonon_flow_batch_step_device(PhononFlowBatch *b, const float *inputs, float
         const size_t slot = b->graph_victim;
         pgpu_graph_destroy(b->graphs[slot].exec);
         b->graphs[slot].exec = NULL;
+        b->splits = splits_for(b, PH_SPLIT_KEYS);
         if (!ph_rope_table(theta) || !pgpu_graph_begin(b->stream))
             return 0;
         const int enqueued = enqueue_step(b, inputs, outputs, theta);
