@@ -685,11 +685,13 @@ int ph_batch_create_on(const PhononFlowModel *model, PhononKvPool *pool, size_t 
     b->positions = pgpu_malloc(b->padded_streams * sizeof(int32_t));
     b->tables = pgpu_malloc(max_streams * b->table_len * sizeof(int32_t));
     b->status = pgpu_malloc(sizeof(int));
-    b->scratch.part_acc = pgpu_malloc(slots * 64 * sizeof(float));
-    b->scratch.part_ml = pgpu_malloc(slots * 2 * sizeof(float));
-    b->scratch.max_streams = (int)max_streams;
-    b->scratch.max_splits = (int)b->max_splits;
-    if (pool->q8) {
+    if (!pool->q8) {
+        b->scratch.part_acc = pgpu_malloc(slots * 64 * sizeof(float));
+        b->scratch.part_ml = pgpu_malloc(slots * 2 * sizeof(float));
+        b->scratch.max_streams = (int)max_streams;
+        b->scratch.max_splits = (int)b->max_splits;
+        ok = ok && b->scratch.part_acc && b->scratch.part_ml;
+    } else {
         b->q8.slots = pgpu_malloc(max_streams * sizeof(int32_t));
         b->q8.slot_tables = pgpu_malloc(max_streams * b->table_len * sizeof(int32_t));
         b->q8.att = pgpu_malloc(rows);
@@ -703,8 +705,7 @@ int ph_batch_create_on(const PhononFlowModel *model, PhononKvPool *pool, size_t 
     b->fl.cover = calloc(max_streams, sizeof(size_t));
     b->fl.units = calloc(max_streams, sizeof(size_t));
     ok = ok && b->x && b->r && b->q && b->in && b->out && b->rows && b->xh && b->positions &&
-         b->tables && b->status && b->scratch.part_acc && b->scratch.part_ml &&
-         b->host_positions && b->fl.cover && b->fl.units;
+         b->tables && b->status && b->host_positions && b->fl.cover && b->fl.units;
     /* Zero everything a kernel may read before writing (padding streams of the
      * split fragments, positions, status). */
     ok = ok && pgpu_memset(b->stream, b->xh, 0, split2048) &&
@@ -983,7 +984,7 @@ static int enqueue_group(PhononFlowBatch *b, void *stream, size_t s0, size_t n, 
     if (b->pre.active)
         return enqueue_prefill(b, stream, first, count, pool_offset, input, output, rope);
     const PhononFlowModel *m = b->model;
-    const size_t slot0 = s0 * PH_HEADS * b->splits;
+    const size_t slot0 = b->pool->q8 ? 0 : s0 * PH_HEADS * b->splits; /* an 8-bit pool's: NULL */
     const pgpu_attention_scratch scratch = {b->scratch.part_acc + slot0 * 64,
                                             b->scratch.part_ml + slot0 * 2, (int)n,
                                             (int)b->splits};
