@@ -435,7 +435,8 @@ int pgpu_wide_from_matrix(void *stream, const pgpu_matrix *w, uint16_t *values, 
  * third split term is left out (each activation taken to 16 significant
  * bits, relative error below 2^-16; two thirds of the matrix-core work);
  * terms = PGPU_SPLIT_F16_PAIR: two fp16 terms with the fp16 weights (22
- * significant bits, two thirds of the work; w->values_f16 required). */
+ * significant bits, two thirds of the work; w->values_f16 required).
+ * residual NULL: the projection alone. */
 int pgpu_prefill_gemm_qkv(void *stream, const pgpu_wide_matrix *w, const uint16_t *split,
                           int streams, int terms, const pgpu_paged_kv *kv, int layer,
                           const int32_t *tables, int table_stride, const int32_t *positions,

@@ -166,6 +166,17 @@ __global__ __launch_bounds__(512) void k_rows_split_ln(const float *__restrict__
 // share a position group's operand rows share an L2.
 constexpr int kChain = 8;  // column blocks per summation chain
 
+// Residual rows; none: zeros.
+template <int EPI>
+__device__ inline void load_residual(EpiOperands &e, const GemmArgs &a, int s, int row0, bool live) {
+    if constexpr (EPI == EPI_RESIDUAL)
+        if (!a.residual) {
+            e.add = make_float4(0.f, 0.f, 0.f, 0.f);
+            return;
+        }
+    load_epilogue_dynamic<EPI>(e, a, s >> 4, s, row0, live);
+}
+
 // One 16-byte LDS-DMA load per lane: global bytes [base + off, +16) -> LDS
 // bytes [lds + 16 lane, +16) (base and lds wave-uniform, in SGPRs; off a
 // per-lane byte offset). Issued as inline assembly so that the compiler,
@@ -333,7 +344,7 @@ __global__ __launch_bounds__(kTaskThreads) void k_prefill_gemm(GemmArgs a, int r
                 const int s = (pt0 + wp * PW + p) * 16 + (lane & 15);
                 const int row0 = (rt0 + wr * RW + r) * 16 + (lane >> 4) * 4;
                 load_epilogue_static<EPI>(ep[r][p], a, s, row0, s < a.streams);
-                load_epilogue_dynamic<EPI>(ep[r][p], a, s >> 4, s, row0, s < a.streams);
+                load_residual<EPI>(ep[r][p], a, s, row0, s < a.streams);
             }
     };
     // Late QKV operands: a lane's append position and pool block depend on
@@ -595,7 +606,7 @@ __global__ __launch_bounds__(kTaskThreads) void k_prefill_split(GemmArgs a, int 
         if (f >= kTiles) break;  // uniform
         const int row0 = (rt0 + f / PW) * 16 + (lane >> 4) * 4;
         load_epilogue_static<EPI>(ep[i], a, s, row0, s < a.streams);
-        load_epilogue_dynamic<EPI>(ep[i], a, s >> 4, s, row0, s < a.streams);
+        load_residual<EPI>(ep[i], a, s, row0, s < a.streams);
     }
 #pragma unroll
     for (int r = 0; r < RW; r++)
@@ -1563,7 +1574,7 @@ extern "C" int pgpu_prefill_gemm_qkv(void *stream, const pgpu_wide_matrix *w, co
 extern "C" int pgpu_prefill_gemm_residual(void *stream, const pgpu_wide_matrix *w,
                                           const uint16_t *split, int streams, int terms,
                                           const float *residual, float *out, int *status) {
-    if (!w || !residual || !out) return bad_arguments("pgpu_prefill_gemm_residual");
+    if (!w || !out) return bad_arguments("pgpu_prefill_gemm_residual");
     GemmArgs a = gemm_args(w, split, streams, terms, status);
     a.out = out;
     a.ld_out = (int)w->rows;

@@ -107,11 +107,10 @@ struct PhononFlowBatch {
     int *status;
     /* Over an 8-bit pool: each stream's open slot, the tables by which the
      * projections append to it (every entry the slot), the attention's rows and
-     * its workspace, made with the batch; a prefill's projected rows, and zeros for
-     * their residual. */
+     * its workspace, made with the batch; a prefill's projected rows. */
     struct {
         int32_t *slots, *slot_tables;
-        float *att, *qkv, *zeros;
+        float *att, *qkv;
         void *work;
         size_t work_bytes;
         const int32_t *pre_slots, *pre_first, *pre_offsets; /* (dev) in pre.stage_dev */
@@ -614,8 +613,7 @@ void phonon_flow_batch_destroy(PhononFlowBatch *b) {
                     b->scratch.part_acc, b->scratch.part_ml, b->pre.stage_dev,
                     b->fl.act, b->fl.part_acc, b->fl.part_ml, b->fl.hidden, b->fl.counters,
                     b->fl.rows, b->fl.parts, b->fl.mlp_parts, b->fl.schedule,
-                    b->q8.slots, b->q8.slot_tables, b->q8.att, b->q8.qkv, b->q8.zeros,
-                    b->q8.work};
+                    b->q8.slots, b->q8.slot_tables, b->q8.att, b->q8.qkv, b->q8.work};
     for (size_t i = 0; i < sizeof(bufs) / sizeof(bufs[0]); i++)
         pgpu_free(bufs[i]);
     pgpu_stream_destroy(b->own_stream);
@@ -918,8 +916,8 @@ static int enqueue_prefill(PhononFlowBatch *b, void *stream, size_t first, size_
             const pgpu_kv8_rows rows = q8_rows(b);
             if (!pgpu_rows_split_ln(stream, cur, norm, norm + PH_WIDTH, 1e-5f, n, terms, xs,
                                     b->status) ||
-                !pgpu_prefill_gemm_residual(stream, &m->wide[l * 4], xs, n, terms, b->q8.zeros,
-                                            b->q8.qkv, b->status) ||
+                !pgpu_prefill_gemm_residual(stream, &m->wide[l * 4], xs, n, terms, NULL, b->q8.qkv,
+                                            b->status) ||
                 !pgpu_kv8_rotate_write(stream, &b->pool->kv8, layer, &rows, b->q8.qkv,
                                        3 * PH_WIDTH, 1, NULL, NULL, 0.0f, rope,
                                        PHONON_FLOW_MAX_POSITIONS, 0.125f, b->q, b->status) ||
@@ -1699,12 +1697,8 @@ static int q8_prefill(PhononFlowBatch *b, size_t streams, const size_t *first,
         if (counts[i] > b->q8.pre_rows)
             b->q8.pre_rows = counts[i];
     }
-    const size_t bytes = b->padded_streams * 3 * PH_WIDTH * sizeof(float);
     if (ok && !b->q8.qkv)
-        ok = (b->q8.qkv = pgpu_malloc(bytes)) != NULL;
-    if (ok && !b->q8.zeros)
-        ok = (b->q8.zeros = pgpu_malloc(bytes)) != NULL &&
-             pgpu_memset(b->stream, b->q8.zeros, 0, bytes);
+        ok = (b->q8.qkv = pgpu_malloc(b->padded_streams * 3 * PH_WIDTH * sizeof(float))) != NULL;
     ok = ok && (b->q8.pre_slots = stage_put(b, slots, streams * sizeof(int32_t))) &&
          (b->q8.pre_first = stage_put(b, host, streams * sizeof(int32_t))) &&
          (b->q8.pre_offsets = stage_put(b, at, (streams + 1) * sizeof(int32_t)));

@@ -79,3 +79,23 @@ def test_a_batch_holds_the_attention_parts_of_its_kind_only(lib, pkg, model):
     finally:
         for x in b:
             x.close()
+
+
+def test_the_first_prefill_takes_one_plane_of_projected_rows(lib, pkg, model):
+    """12.6 MB of 2048 rows of queries, keys and values; the same prefill over an fp32
+    pool takes the rest that this one takes."""
+    b = [Batch(lib, pkg, model, q8) for q8 in (False, True)]
+    try:
+        taken = []
+        for x in b:
+            x.prefill()  # what the runtime takes for it
+            x.close()
+        for n, q8 in enumerate((False, True)):
+            b[n] = Batch(lib, pkg, model, q8)
+            before = used()
+            b[n].prefill()
+            taken.append(used() - before)
+        assert taken[1] - taken[0] <= 2048 * 1536 * 4 + (4 << 20)
+    finally:
+        for x in b:
+            x.close()
