@@ -175,7 +175,8 @@ int phonon_flow_batch_set_groups(PhononFlowBatch *batch, size_t groups);
  * decode batch sizes where that measured faster on MI355X (1..224 streams),
  * phase by phase otherwise. Results are identical (both run the same task
  * code). Batches over 4096 streams, models over 63 layers and models mixing
- * Q8 and BF16 matrices always run phase by phase. */
+ * Q8 and BF16 matrices always run phase by phase. Over an 8-bit pool, whose steps
+ * and prefills do too, mode 2 is refused. */
 int phonon_flow_batch_set_pipeline(PhononFlowBatch *batch, int mode);
 /* Placement of the projection chains in the one-launch step's task list
  * (pgpu_flow_placement); NULL restores the default. Results do not depend

@@ -1818,6 +1818,8 @@ size_t phonon_flow_batch_schedule(const PhononFlowBatch *b, uint32_t *schedule,
 int phonon_flow_batch_set_pipeline(PhononFlowBatch *b, int mode) {
     if (!b || mode < 0 || mode > 2)
         return 0;
+    if (mode == 2 && b->pool->q8)
+        return ph_fail("a batch over an 8-bit pool runs phase by phase");
     if (b->flow != mode) {
         drop_graphs(b);
         b->flow = mode;

@@ -141,3 +141,16 @@ def test_steps_allocate_nothing(long_server, pkg, lib):
     for n in (23, 7, 1, 20):
         run(sv, n, 8000)
         assert parts(sv, None, 8192) > 0 and used() == before, n
+
+
+def test_one_launch_steps_are_refused(server, lib):
+    """A mode that the pool's steps cannot have is not taken and then ignored."""
+    sv = server(2)
+    for mode in (0, 1):
+        assert lib.phonon_flow_batch_set_pipeline(sv.batch, mode)
+    assert not lib.phonon_flow_batch_set_pipeline(sv.batch, 2)
+    assert b"8-bit" in lib.pgpu_last_error()
+    sv.hold([5, 16])
+    sv.set()
+    x, y = step(sv)
+    check_step(sv, x, y)
