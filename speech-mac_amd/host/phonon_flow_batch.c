@@ -1659,7 +1659,9 @@ static int set_prefill(PhononFlowBatch *b, size_t streams, const size_t *first,
     const int32_t *pos_dev = NULL;
     ok = ok && (pos_dev = stage_put(b, pos32, total * sizeof(int32_t))) &&
          (b->table_map = stage_put(b, map, total * sizeof(int32_t))) &&
-         prefill_entries(b, streams, first, counts) && prefill_runs(b, streams, first, counts) &&
+         /* Work lists of the fp32 attentions. */
+         (b->pool->q8 || (prefill_entries(b, streams, first, counts) &&
+                          prefill_runs(b, streams, first, counts))) &&
          stage_flush(b) &&
          pgpu_gather_rows_copy(b->stream, b->tables, tables_dev, b->table_map, (int)total,
                                (int)b->table_len, b->positions, pos_dev);
