@@ -1690,11 +1690,12 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
                                   int group, float scale, int max_positions, float *out,
                                   size_t out_stride, void *work, size_t work_bytes,
                                   int *status) {
+    constexpr float kLog2e = 1.44269504f;
     const size_t width = kv ? (size_t)kv->heads * kv->head_dim * group : 0;
     if (!cache_ok(kv) || !rows_ok(rows) || layer < 0 || layer >= kv->layers || !q || !out ||
         !status || !aligned(q, 16) || !aligned(out, 16) || q_stride % 4 != 0 ||
         out_stride % 4 != 0 || group < 1 || group > 16 || q_stride < width ||
-        out_stride < width || max_positions <= 0 || !__builtin_isfinite(scale))
+        out_stride < width || max_positions <= 0 || !__builtin_isfinite(scale * kLog2e))
         return bad_arguments("pgpu_kv8_attention");
     if (rows->rows == 0) return 1;
     const Deal d = deal_of(kv, rows, group, max_positions);
@@ -1705,7 +1706,7 @@ extern "C" int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer,
     if (parts && (!work || !aligned(work, 16) ||
                   work_bytes < parts * (kv->head_dim + 2) * sizeof(float)))
         return bad_arguments("pgpu_kv8_attention (workspace)");
-    const Kv8Decode a = {q, q_stride, group, scale * 1.44269504f, max_positions, d.splits, 1,
+    const Kv8Decode a = {q, q_stride, group, scale * kLog2e, max_positions, d.splits, 1,
                          (float *)work, (float *)work + parts * kv->head_dim, out, out_stride};
     const Kv8 c = layer_of(kv, layer);
     return kv->head_dim == 64

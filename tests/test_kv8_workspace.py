@@ -1,10 +1,10 @@
-"""The attention workspace of the 8-bit cache: what holds a full batch holds every
-smaller one."""
+"""The attention of the 8-bit cache: its workspace (what holds a full batch holds every
+smaller one), and a scale that it cannot take."""
 import ctypes
 
 import pytest
 
-from test_kv8 import Args
+from test_kv8 import Args, call
 
 
 def size(lib, pkg, heads, dim, group, streams, most, max_rows=None):
@@ -42,3 +42,11 @@ def test_runs(pkg, heads, dim, group):
                                 (streams, (rows + 1) // 2, most), (streams, rows, most // 2 + 1),
                                 (max(1, streams - 1), max(1, rows - 1), most)):
                     assert n >= size(lib, pkg, heads, dim, group, s, p, r), (most, streams, rows, s, r)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+def test_a_scale_that_is_not_finite_in_units_of_log_2(pkg, scale):
+    lib = pkg.load()
+    lib.pgpu_record_error(b"")
+    assert not call(lib, "attention", Args(pkg), scale=scale)
+    assert b"invalid arguments" in lib.pgpu_last_error()
