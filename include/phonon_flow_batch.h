@@ -99,7 +99,9 @@ int phonon_flow_batch_set_streams(PhononFlowBatch *batch, size_t streams,
  * holds the rows of the block of position positions[s] before it. Steps run phase
  * by phase, in one group: a step's attention reads each stream's newest block in
  * fp32 and the earlier ones in 8 bits, and a block is stored by the step of its
- * last position. */
+ * last position. A stream's last bits may differ with the number of streams beside
+ * it, with the longest context, and between a captured step and an eager one
+ * (pgpu_kv8_attention deals its work by them). */
 int phonon_flow_batch_set_streams_q8(PhononFlowBatch *batch, size_t streams,
                                      const size_t *positions, const int32_t *tables,
                                      size_t table_len, const int32_t *slots);

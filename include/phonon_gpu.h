@@ -587,7 +587,9 @@ int pgpu_kv8_close(void *stream, const pgpu_kv8 *kv, int first_layer, int layers
  * the row sees (blocks whose value scales differ by up to 2^86). One row a
  * stream holds them to 2^-31 of the largest element of the query, or of the
  * weighted scales of 64 keys (magnitudes from 2^-96 on); what it multiplies and
- * sums of them is exact.
+ * sums of them is exact. The same call gives the same bits; how the keys are
+ * dealt to work-groups goes by the number of streams, max_rows and
+ * max_positions, so that in another batch a stream's last bits may differ.
  * `work` (dev): pgpu_kv8_attention_bytes(kv, rows, group, max_positions) bytes
  * that no other call uses at the same time; they need no clearing. They do for
  * every call of at most these streams, max_rows and max_positions, with offsets

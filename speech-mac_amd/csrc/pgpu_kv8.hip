@@ -584,7 +584,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
                                                                         Kv8Decode a, int *status) {
     constexpr int KB = D / 64;
     __shared__ Kv8DecodeShared<D, W, Q> sh;
-    // Heads vary fastest: with 8 of them a head's passes stay on one XCD.
+    // Heads vary fastest: with 8 of them a head's passes stay on one XCD (4, 5 or 6
+    // heads over as many bytes: 2 to 4% less of them a second, 6.2 TB/s for 6.4).
     const int head = blockIdx.x % kv.heads, j0 = blockIdx.x / kv.heads * Q;
     const int split = blockIdx.y, s = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -882,9 +883,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
 // 2^15 and their low terms normal: with every scale so far within 2^4 of the first
 // block's, one lift for all rows; else each row's own, from the largest weight
 // times scale among the keys that it sees (so no row loses bits to a block that it
-// does not see or hardly weighs). Bound by
-// vector instructions: a run of 8187 rows over 8 heads of 64 takes 165 us (0.42
-// PFLOP/s of the formula's, 0.83 with the terms'), 249 instructions a tile and chunk in
+// does not see or hardly weighs; 8187 rows 227 us where scales are 2^6 apart, 187 in
+// the same run where they are alike). Bound by
+// vector instructions: a run of 8187 rows over 8 heads of 64 takes 167 us (0.41
+// PFLOP/s of the formula's, 0.82 with the terms'), 249 instructions a tile and chunk in
 // 69% of the cycles, the matrix cores busy in 32%. Tiles of 16 rows keep 4 waves a SIMD
 // (two tiles a wave, half the waves: 244); a work-group of 8 waves, which would share
 // the conversion by twice the rows, waits at its barriers (192). Short runs are bound
