@@ -807,7 +807,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
         }
         float w = newest * kBlockPos + i <= p ? c.x * a.scale : -INFINITY;
         // An infinite query's scores may all be -inf.
-        if (!(__shfl(xor16_32_max(top), g * 4) < INFINITY)) w = __builtin_nanf("");
+        if (__any(!(top < INFINITY)) && !(__shfl(xor16_32_max(top), g * 4) < INFINITY))
+            w = __builtin_nanf("");
         const float mx = row16_max(fmaxf(m, w)), shrink = __builtin_amdgcn_exp2f(m - mx);
         m = mx;
         w = __builtin_amdgcn_exp2f(w - m);
