@@ -885,13 +885,13 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv8_decode(Kv8 kv, 
 // block's, one lift for all rows; else each row's own, from the largest weight
 // times scale among the keys that it sees (so no row loses bits to a block that it
 // does not see or hardly weighs; 8187 rows 227 us where scales are 2^6 apart, 187 in
-// the same run where they are alike). Bound by
-// vector instructions: a run of 8187 rows over 8 heads of 64 takes 167 us (0.41
-// PFLOP/s of the formula's, 0.82 with the terms'), 249 instructions a tile and chunk in
-// 69% of the cycles, the matrix cores busy in 32%. Tiles of 16 rows keep 4 waves a SIMD
-// (two tiles a wave, half the waves: 244); a work-group of 8 waves, which would share
-// the conversion by twice the rows, waits at its barriers (192). Short runs are bound
-// by the chain within a chunk, 1.1 to 1.5 us.
+// the same run where they are alike).
+// Bound by vector instructions: a run of 8187 rows over 8 heads of 64 takes 167 us (183
+// on another card; 0.41 PFLOP/s of the formula's, 0.82 with the terms'), 249 instructions
+// a tile and chunk in 69% of the cycles, the matrix cores busy in 32%. Tiles of 16 rows
+// keep 4 waves a SIMD (two tiles a wave, half the waves: 244); a work-group of 8 waves,
+// which would share the conversion by twice the rows, waits at its barriers (192). Short
+// runs are bound by the chain within a chunk, 1.1 to 1.5 us.
 struct Kv8Run {
     const float *q;
     size_t q_stride;
