@@ -601,6 +601,115 @@ int pgpu_kv8_attention(void *stream, const pgpu_kv8 *kv, int layer, const pgpu_k
                        int max_positions, float *out, size_t out_stride, void *work,
                        size_t work_bytes, int *status);
 
+/* -- 4-bit paged KV cache (pgpu_kv4.hip). A position of one head holds its key
+ * and its value as whole numbers q in [-8, 7] with one fp16 scale for every 64
+ * dims of each: s = the larger of max x / 7 and -min x / 8 (fp32 divisions)
+ * rounded up to 8 significant bits, at least 2^-17; q = x / s rounded to
+ * nearest, ties to even; the stored value is q * s, an fp16 number (8 bits of
+ * scale times 3 of a number: exact). (q + 1/2) s is an fp32 number, so x / s is
+ * never rounded onto a tie that x is not on, and q does not depend on the
+ * precision it is computed in. A scale above 8160 (values from about 57000 on)
+ * does not fit: such a row is taken as one that is not finite. Every row is
+ * quantised by itself, when it is written: nothing is quantised twice, the
+ * stored bits do not depend on how rows were dealt to calls, and a row can be
+ * moved as it is (pgpu_kv4_evict). -- */
+/* Sixteen numbers take 8 bytes: number 8 a + b is the low half of byte 4 a + b,
+ * number 8 a + 4 + b its high half (a < 2, b < 4). For each 64 dims of a (block,
+ * head) keys lie by position, [16 positions][64 dims], values by dim, [64
+ * dims][16 positions]. */
+typedef struct {
+    uint8_t *values;  /* (dev) [layers][blocks][heads][keys, values][head_dim / 64][512]; 16-byte aligned */
+    uint16_t *scales; /* (dev) fp16 [layers][blocks][heads][head_dim / 64][16 positions][key, value]; 16-byte aligned */
+    int layers, heads, head_dim; /* heads 1..256; head_dim 64 or 128 */
+    size_t blocks;               /* up to INT32_MAX */
+} pgpu_kv4;
+/* The rows of a call. Stream s has the rows offsets[s] .. offsets[s + 1] - 1
+ * (offsets NULL: row s alone, rows = streams, max_rows = 1), which are its
+ * cache's rows first[s], first[s] + 1, ...; first[s] < 0: the stream is an empty
+ * place of the batch and is passed over. A cache row's index is its place in the
+ * cache: the position in the sequence until the first eviction, less what was
+ * evicted after it. Rows [16 i, 16 i + 16) lie in block tables[s * table_stride
+ * + i]. Blocks that are written are no other stream's. `max_rows` bounds the
+ * rows of a stream and `rows` every row index. A stream outside its bounds
+ * (offsets, table, more than max_rows rows) is left out, a block id outside the
+ * cache likewise, and status bit 2 set. */
+typedef struct {
+    const int32_t *tables;  /* (dev) [streams][table_stride] */
+    int table_stride;
+    const int32_t *first;   /* (dev) [streams] */
+    const int32_t *offsets; /* (dev) [streams + 1] or NULL */
+    int streams;            /* 1..65535 */
+    int rows, max_rows;     /* max_rows up to 65535 */
+} pgpu_kv4_rows;
+/* Writes rows of keys and values, row r's head h at k[r * row_stride + h *
+ * head_dim] (row_stride a multiple of 4, k and v 16-byte aligned). The other
+ * rows of their blocks are left as they are. A row with a value that is not
+ * finite, or too large, sets status bit 1, and its scales become NaN, the key's
+ * and the value's. */
+int pgpu_kv4_write(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_kv4_rows *rows,
+                   const float *k, const float *v, size_t row_stride, int *status);
+/* Reads rows back as fp32 (the layout of pgpu_kv4_write). lengths[s] (dev): the
+ * rows that stream s holds; a row at or past it sets status bit 2 and leaves
+ * its stream out. Rows of a block outside the cache are not written. */
+int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_kv4_rows *rows,
+                  const int32_t *lengths, float *k, float *v, size_t row_stride, int *status);
+/* What the attention's weights add up to, for each stream, key head and cache
+ * row i that the stream holds after the call: after[(s * heads + h) * stride +
+ * i] = before[same] + the sum of the weights that the last `rows` rows of the
+ * call's (of each stream; all, if it has fewer) and the head's queries give it.
+ * The call's own rows are new: they begin from 0. before NULL: all begin from 0;
+ * before = after: in place (no other overlap). A row that does not come out
+ * finite adds nothing. Summed in fp32, always in the same order. */
+typedef struct {
+    const float *before; /* (dev) [streams][heads][stride] or NULL */
+    float *after;        /* (dev) [streams][heads][stride] */
+    size_t stride;       /* at least max_positions */
+    int rows;            /* 1 or more */
+} pgpu_kv4_sums;
+/* Causal attention over the cache: row r's query head h (group query heads to
+ * a key head, 1..16; q[r * q_stride + h * head_dim]) attends the cache rows 0 ..
+ * its own, softmax(scale q k) v, into out[r * out_stride + h * head_dim]. The
+ * cache already holds the call's rows. One row a stream, or runs of rows.
+ * `max_positions` bounds every cache row's index + 1 (a stream past it is left
+ * out, status bit 2). A block whose id is outside the cache weighs nothing
+ * (status bit 2; a row that is left no key gets zeros). A stream with first < 0
+ * gets zero rows. Strides multiples of 4, pointers 16-byte aligned; out must not
+ * overlap q. `sums` NULL: the weights are not added up.
+ * The same call gives the same bits; how the keys are dealt to work-groups goes
+ * by the number of streams, max_rows and max_positions, so that in another batch
+ * a stream's last bits may differ.
+ * `work` (dev, 16-byte aligned): pgpu_kv4_attention_bytes(kv, rows, group,
+ * max_positions, with_sums) bytes that no other call uses at the same time; they
+ * need no clearing. They do for every call of at most these streams, max_rows,
+ * rows and max_positions, with offsets or without as here. */
+size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *rows, int group,
+                                int max_positions, int with_sums);
+int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_kv4_rows *rows,
+                       const float *q, size_t q_stride, int group, float scale,
+                       int max_positions, float *out, size_t out_stride,
+                       const pgpu_kv4_sums *sums, void *work, size_t work_bytes, int *status);
+/* Shrinks every stream that holds more than `keep` rows (lengths[s], dev) to
+ * `keep`, in layers [first_layer, first_layer + layers), each head by itself: the
+ * first `first` rows, the newest `newest` ones, and of the others those with the
+ * largest sums, of equal ones the lowest index. Rows are moved as they are, in
+ * order, to the cache rows 0 .. keep - 1 of table to_tables (tables' stride;
+ * NULL: tables, in place); a stream with keep rows or fewer keeps all. Entry i
+ * of a stream's to_tables is entry i of its tables, or a block that no table of
+ * the call holds; so are blocks that other streams share kept whole. Rows past
+ * the kept ones in their last block hold nothing afterwards.
+ * sums, to_sums (dev) [layers][streams][heads][sums_stride], sums_stride at
+ * least the longest stream's length: to_sums gets the kept rows' sums in order,
+ * and is left as it is past them (to_sums may be sums, no other overlap). NaN
+ * counts as 0. kept (dev) [layers][streams][heads][keep]: the indexes of the rows
+ * kept, -1 past them. lengths[s] < 0, or a table entry outside the cache or
+ * a length past the table or sums_stride (status bit 2): the stream is left as it
+ * is, its kept all -1. The stream's length is min(lengths[s], keep) afterwards. */
+int pgpu_kv4_evict(void *stream, const pgpu_kv4 *kv, int first_layer, int layers,
+                   const int32_t *tables, const int32_t *to_tables, int table_stride,
+                   const int32_t *lengths, int streams, int keep, int first, int newest,
+                   const float *sums, float *to_sums, size_t sums_stride, int32_t *kept,
+                   int *status);
+
 /* -- flow head launches (pgpu_head.hip); BF16 matrices -- */
 /* One launch of three independent parts: silu_split = split fragments of
  * SiLU((cond_w . c + cond_bias) + tsum) (tsum optional); if eos_w (16 rows,

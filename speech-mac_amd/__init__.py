@@ -109,6 +109,23 @@ class PgpuKv8Rows(ctypes.Structure):
                 ("offsets", _vp), ("streams", _i), ("rows", _i), ("max_rows", _i)]
 
 
+class PgpuKv4(ctypes.Structure):
+    """pgpu_kv4 (phonon_gpu.h): the 4-bit paged KV cache."""
+    _fields_ = [("values", _vp), ("scales", _vp), ("layers", _i), ("heads", _i),
+                ("head_dim", _i), ("blocks", _sz)]
+
+
+class PgpuKv4Rows(ctypes.Structure):
+    """pgpu_kv4_rows (phonon_gpu.h): the rows of a call."""
+    _fields_ = [("tables", _vp), ("table_stride", _i), ("first", _vp), ("offsets", _vp),
+                ("streams", _i), ("rows", _i), ("max_rows", _i)]
+
+
+class PgpuKv4Sums(ctypes.Structure):
+    """pgpu_kv4_sums (phonon_gpu.h): where the attention's weights are added up."""
+    _fields_ = [("before", _vp), ("after", _vp), ("stride", _sz), ("rows", _i)]
+
+
 class PgpuGemmInput(ctypes.Structure):
     _fields_ = [("split", _vp), ("ln_rows", _vp), ("ln_weight", _vp), ("ln_bias", _vp),
                 ("ln_epsilon", _f), ("attn_acc", _vp), ("attn_ml", _vp),
@@ -143,6 +160,9 @@ _scp = ctypes.POINTER(PgpuAttentionScratch)
 _gip = ctypes.POINTER(PgpuGemmInput)
 _k8p = ctypes.POINTER(PgpuKv8)
 _k8r = ctypes.POINTER(PgpuKv8Rows)
+_k4p = ctypes.POINTER(PgpuKv4)
+_k4r = ctypes.POINTER(PgpuKv4Rows)
+_k4s = ctypes.POINTER(PgpuKv4Sums)
 _pp = ctypes.POINTER(_vp)
 
 # Every function declared in include/*.h: name -> (restype, argtypes).
@@ -376,6 +396,13 @@ EXPORTS = {
     "pgpu_kv8_attention_bytes": (_sz, [_k8p, _k8r, _i, _i]),
     "pgpu_kv8_attention": (_i, [_vp, _k8p, _i, _k8r, _vp, _sz, _i, _f, _i, _vp, _sz, _vp, _sz,
                                 _vp]),
+    "pgpu_kv4_write": (_i, [_vp, _k4p, _i, _k4r, _vp, _vp, _sz, _vp]),
+    "pgpu_kv4_read": (_i, [_vp, _k4p, _i, _k4r, _vp, _vp, _vp, _sz, _vp]),
+    "pgpu_kv4_attention_bytes": (_sz, [_k4p, _k4r, _i, _i, _i]),
+    "pgpu_kv4_attention": (_i, [_vp, _k4p, _i, _k4r, _vp, _sz, _i, _f, _i, _vp, _sz, _k4s, _vp,
+                                _sz, _vp]),
+    "pgpu_kv4_evict": (_i, [_vp, _k4p, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _sz,
+                            _vp, _vp]),
     "pgpu_head_flow_schedule": (_i, [_vp, _i, _i, _i, _i]),
     "pgpu_head_flow_launch": (_i, [_vp, _vp]),
     "pgpu_head_flow_reset": (_i, [_vp, _vp, _sz, _vp]),

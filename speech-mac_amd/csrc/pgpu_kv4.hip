@@ -1,0 +1,754 @@
+// 4-bit paged KV cache: quantised writes, reads, causal attention over it with
+// the sums of its weights, and eviction by them. The formats and the rules of the
+// stored values are in phonon_gpu.h.
+#include <algorithm>
+
+#include "pgpu_kv.hpp"
+#include "phonon_gpu.h"
+
+namespace pgpu {
+
+constexpr int kSpan = 64;         // dims of a scale
+constexpr int kPlane = 512;       // bytes of a block's 64 dims, of keys or of values
+constexpr float kLeastScale = 0x1p-17f, kMostScale = 8160.0f;
+
+// One layer of the cache, and the rows of a call (pgpu_kv4, pgpu_kv4_rows).
+struct Kv4 {
+    uint8_t *values;
+    uint32_t *scales;  // (key, value) pairs
+    int heads;
+    unsigned blocks;
+};
+
+struct Kv4Rows {
+    const int32_t *tables;
+    int table_stride;
+    const int32_t *first, *offsets;
+    int rows, max_rows;
+};
+
+// A stream's rows, checked: uniform over the work-group.
+struct Kv4Span {
+    int first, count, row0;
+    bool live;
+};
+
+// limit: indexes must be below it. A stream that breaks a bound is flagged (by
+// the thread with `speak`) and left out.
+__device__ inline Kv4Span kv4_span(const Kv4Rows &r, int s, int limit, bool speak, int *status) {
+    Kv4Span x;
+    x.first = uniform_load(r.first + s);
+    x.row0 = r.offsets ? uniform_load(r.offsets + s) : s;
+    const int end = r.offsets ? uniform_load(r.offsets + s + 1) : s + 1;
+    // 64 bits: any int32 may stand in the arrays.
+    const long long count = (long long)end - x.row0;
+    const bool wild = x.row0 < 0 || count < 0 || end > r.rows || count > r.max_rows;
+    x.count = wild ? 0 : (int)count;
+    const long long last = (long long)x.first + x.count;
+    const bool bad = wild || (x.first >= 0 && x.count > 0 &&
+                              (last > limit || last > (long long)r.table_stride * kBlockPos));
+    x.live = !bad && x.first >= 0 && x.count > 0;
+    if (bad && speak) atomicOr(status, 2);
+    return x;
+}
+
+// Bytes of a (block, head); its values start half way. And its scales.
+template <int D>
+__device__ inline uint8_t *kv4_tile(const Kv4 &kv, unsigned block, int head) {
+    return kv.values + ((size_t)block * kv.heads + head) * (D * kBlockPos);
+}
+template <int D>
+__device__ inline uint32_t *kv4_scales(const Kv4 &kv, unsigned block, int head) {
+    return kv.scales + ((size_t)block * kv.heads + head) * (D / kSpan * kBlockPos);
+}
+__device__ inline float key_scale(uint32_t pair) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)pair);
+}
+__device__ inline float value_scale(uint32_t pair) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(pair >> 16));
+}
+// Number i of the eight in a word: 4 h + b is half h of byte b.
+__device__ inline float nibble(uint32_t w, int i) {
+    const int at = (i & 3) * 8 + (i >> 2) * 4;
+    return (float)((int)(w << (28 - at)) >> 28);
+}
+
+// ------------------------------------------------------------------- writing
+
+// max x, max -x of 64 dims -> their scale. Eight significant bits: see phonon_gpu.h.
+__device__ inline float kv4_scale(float top, float bottom) {
+    const uint32_t bits = fbits(fmaxf(fmaxf(top / 7.0f, bottom / 8.0f), 0.0f)) + 0xFFFFu;
+    return fmaxf(bitsf(bits & ~0xFFFFu), kLeastScale);
+}
+
+// Four numbers in [-8, 7] -> the low halves of a word's bytes.
+__device__ inline uint32_t pack_halves(const float *q) {
+    return ((uint32_t)(int)q[0] & 15u) | ((uint32_t)(int)q[1] & 15u) << 8 |
+           ((uint32_t)(int)q[2] & 15u) << 16 | ((uint32_t)(int)q[3] & 15u) << 24;
+}
+
+__device__ inline uint32_t xor1(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false);
+}
+
+// A row's four dims -> whole numbers. x / s by the reciprocal, which is off by less
+// than 2^-20 below 8; where that could decide a rounding, by the division.
+__device__ inline void kv4_round(const float4 &x, float s, float *q) {
+    const float inverse = 1.0f / s;
+    const float f[4] = {x.x, x.y, x.z, x.w};
+    float off = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        const float y = f[d] * inverse;
+        q[d] = rintf(y);
+        off = fmaxf(off, fabsf(y - q[d]));
+    }
+    if (off > 0.5f - 2e-6f)
+#pragma unroll
+        for (int d = 0; d < 4; d++) q[d] = rintf(f[d] / s);
+}
+
+// The bits of 16 numbers' 8 bytes that rows lo .. hi - 1 take.
+__device__ inline uint64_t row_bits(int lo, int hi) {
+    uint64_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kBlockPos; j++)
+        if (j >= lo && j < hi) m |= (uint64_t)15 << ((j >> 3) * 32 + (j & 3) * 8 + (j >> 2 & 1) * 4);
+    return m;
+}
+
+// A wave for each (block of the call's rows, head): lane (g, c) has rows 4 g .. 4 g + 3
+// of the 4 dims from 4 c on of every 64.
+template <int D>
+__global__ __launch_bounds__(256) void k_kv4_write(Kv4 kv, Kv4Rows rows, const float *k,
+                                                   const float *v, size_t row_stride,
+                                                   int *status) {
+    constexpr int N = D / kSpan;
+    __shared__ __align__(16) uint32_t lds[4][kSpan * 2];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int s = blockIdx.z, head = blockIdx.x * 4 + wave, g = lane >> 4, c = lane & 15;
+    const Kv4Span span = kv4_span(rows, s, INT32_MAX - kBlockPos,
+                                  threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+    if (!span.live || head >= kv.heads) return;
+    const int end = span.first + span.count, block = span.first / kBlockPos + (int)blockIdx.y;
+    if (block * kBlockPos >= end) return;
+    const int id = uniform_load(rows.tables + (size_t)s * rows.table_stride + block);
+    if ((unsigned)id >= kv.blocks) {
+        if (lane == 0) atomicOr(status, 2);
+        return;
+    }
+    const int lo = max(span.first - block * kBlockPos, 0), hi = min(end - block * kBlockPos, 16);
+    float4 x[2][N][4];  // keys, values
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int j = g * 4 + r, p = block * kBlockPos + j;
+        const bool in = j >= lo && j < hi;
+        const size_t at = (size_t)(span.row0 + (in ? p - span.first : 0)) * row_stride +
+                          (size_t)head * D + c * 4;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            x[0][n][r] = in ? once_load(k + at + n * kSpan) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[1][n][r] = in ? once_load(v + at + n * kSpan) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+    float scale[2][N][4];
+    bool wild[4] = {false, false, false, false};
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const float4 y = x[p][n][r];
+                wild[r] |= !(y.x == y.x && y.y == y.y && y.z == y.z && y.w == y.w);
+                const float top = row16_max(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+                const float bottom = row16_max(fmaxf(fmaxf(-y.x, -y.y), fmaxf(-y.z, -y.w)));
+                scale[p][n][r] = kv4_scale(top, bottom);
+                wild[r] |= scale[p][n][r] > kMostScale;
+            }
+        wild[r] = (__ballot(wild[r]) >> (g * 16) & 0xFFFFu) != 0;
+    }
+    uint8_t *tile = kv4_tile<D>(kv, (unsigned)id, head);
+    uint32_t *scales = kv4_scales<D>(kv, (unsigned)id, head);
+    const uint64_t mine = row_bits(lo, hi);
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        float q[4][4];
+        // Keys: a row's four dims are half of a word, the next lane's the other half.
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int j = g * 4 + r;
+            kv4_round(x[0][n][r], scale[0][n][r], q[r]);
+            uint32_t w = wild[r] ? 0u : pack_halves(q[r]);
+            w <<= (c & 1) * 4;
+            w |= xor1(w);
+            if (j < lo || j >= hi) continue;  // the same for the row's 16 lanes
+            if ((c & 1) == (r & 1))
+                *(uint32_t *)(tile + n * kPlane + j * (kSpan / 2) + (c >> 1) * 4) = w;
+            if (c == 0) {
+                const auto pair = __builtin_amdgcn_cvt_pkrtz(scale[0][n][r], scale[1][n][r]);
+                scales[n * kBlockPos + j] = wild[r] ? 0x7E007E00u : __builtin_bit_cast(uint32_t, pair);
+            }
+        }
+        // Values: a dim's four rows are half of a word, of the lanes 16 apart.
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            kv4_round(x[1][n][r], scale[1][n][r], q[r]);
+            if (wild[r]) q[r][0] = q[r][1] = q[r][2] = q[r][3] = 0.0f;
+        }
+#pragma unroll
+        for (int z = 0; z < 4; z++) {
+            const float four[4] = {q[0][z], q[1][z], q[2][z], q[3][z]};
+            uint32_t w = pack_halves(four) << ((g & 1) * 4);
+            w |= (uint32_t)__shfl_xor((int)w, 16);
+            if ((z >> 1) == (g & 1)) lds[wave][(c * 4 + z) * 2 + (g >> 1)] = w;
+        }
+        wave_lds_fence();
+        uint64_t *dim = (uint64_t *)(tile + (N + n) * kPlane) + lane;
+        uint64_t w = *(const uint64_t *)&lds[wave][lane * 2];
+        if (mine != ~(uint64_t)0) w = (*dim & ~mine) | (w & mine);
+        *dim = w;
+        wave_lds_fence();
+    }
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < 4; r++) bad |= wild[r];
+    flag_nonfinite(status, bad);
+}
+
+// ------------------------------------------------------------------- reading
+
+// A wave for each (block of the rows read, head).
+template <int D>
+__global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, Kv4Rows rows, const int32_t *lengths,
+                                                  float *k, float *v, size_t row_stride,
+                                                  int *status) {
+    constexpr int N = D / kSpan;
+    __shared__ __align__(16) uint32_t lds[4][kSpan * 2];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int s = blockIdx.z, head = blockIdx.x * 4 + wave, g = lane >> 4, c = lane & 15;
+    const Kv4Span span = kv4_span(rows, s, uniform_load(lengths + s),
+                                  threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+    if (!span.live || head >= kv.heads) return;
+    const int end = span.first + span.count, block = span.first / kBlockPos + (int)blockIdx.y;
+    if (block * kBlockPos >= end) return;
+    const int id = uniform_load(rows.tables + (size_t)s * rows.table_stride + block);
+    if ((unsigned)id >= kv.blocks) {
+        if (lane == 0) atomicOr(status, 2);
+        return;
+    }
+    const uint8_t *tile = kv4_tile<D>(kv, (unsigned)id, head);
+    const uint32_t *scales = kv4_scales<D>(kv, (unsigned)id, head);
+    uint32_t keys[N][4], pairs[N][4];
+    uint64_t dim[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        dim[n] = *((const uint64_t *)(tile + (N + n) * kPlane) + lane);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            keys[n][r] = *(const uint32_t *)(tile + n * kPlane + (g * 4 + r) * (kSpan / 2) + (c >> 1) * 4);
+            pairs[n][r] = scales[n * kBlockPos + g * 4 + r];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        *(uint64_t *)&lds[wave][lane * 2] = dim[n];
+        wave_lds_fence();
+        uint32_t w[4];  // of dim z: the eight rows of which four are this lane's
+#pragma unroll
+        for (int z = 0; z < 4; z++) w[z] = lds[wave][(c * 4 + z) * 2 + (g >> 1)];
+        wave_lds_fence();
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int p = block * kBlockPos + g * 4 + r, kh = (c & 1) * 4, vh = (g & 1) * 4 + r;
+            if (p < span.first || p >= end) continue;
+            const float ks = key_scale(pairs[n][r]), vs = value_scale(pairs[n][r]);
+            const size_t at = (size_t)(span.row0 + p - span.first) * row_stride + (size_t)head * D +
+                              n * kSpan + c * 4;
+            const uint32_t a = keys[n][r];
+            once_store(k + at, make_float4(nibble(a, kh) * ks, nibble(a, kh + 1) * ks,
+                                           nibble(a, kh + 2) * ks, nibble(a, kh + 3) * ks));
+            once_store(v + at, make_float4(nibble(w[0], vh) * vs, nibble(w[1], vh) * vs,
+                                           nibble(w[2], vh) * vs, nibble(w[3], vh) * vs));
+        }
+    }
+}
+
+// ----------------------------------------------------------------- attention
+
+struct Kv4Run {
+    const float *q;
+    size_t q_stride;
+    int group;
+    float scale;  // of the scores, times log2 e
+    int max_positions;
+    float *out;
+    size_t out_stride;
+    float *lse;  // [rows][query heads]: log2 of a row's sum of 2^score, or NULL
+};
+
+// A wave for each (row, query head): a key to a lane, then a dim to a lane.
+template <int D>
+__global__ __launch_bounds__(64) void k_kv4_attend(Kv4 kv, Kv4Rows rows, Kv4Run a, int *status) {
+    constexpr int N = D / kSpan;
+    __shared__ float q[D], w[kSpan][N];
+    const int qh = blockIdx.x, head = qh / a.group, s = blockIdx.z, lane = threadIdx.x;
+    const Kv4Span span = kv4_span(rows, s, a.max_positions,
+                                  lane == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+    if ((int)blockIdx.y >= span.count) return;
+    const size_t row = (size_t)span.row0 + blockIdx.y;
+    float *out = a.out + row * a.out_stride + (size_t)qh * D;
+    if (!span.live) {
+        if (span.first < 0)
+            for (int n = 0; n < N; n++) out[n * 64 + lane] = 0.0f;
+        return;
+    }
+    for (int n = 0; n < N; n++) q[n * 64 + lane] = a.q[row * a.q_stride + (size_t)qh * D + n * 64 + lane];
+    __syncthreads();
+    const int keys = span.first + (int)blockIdx.y + 1;
+    const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
+    float m = kNone, l = 0.0f, acc[N];
+    for (int n = 0; n < N; n++) acc[n] = 0.0f;
+    bool any = false, wild = false;
+    for (int p0 = 0; p0 < keys; p0 += 64) {
+        const int p = p0 + lane;
+        const int id = p < keys ? table[p / kBlockPos] : 0;
+        const bool in = p < keys && (unsigned)id < kv.blocks;
+        wild |= p < keys && !in;
+        any |= __any(in);
+        float score = 0.0f, vs[N];
+        if (in) {
+            for (int n = 0; n < N; n++) {
+                const uint32_t *x = (const uint32_t *)(kv4_tile<D>(kv, id, head) + n * kPlane +
+                                                       p % kBlockPos * (kSpan / 2));
+                float dot = 0.0f;
+                for (int e = 0; e < 8; e++)
+                    for (int i = 0; i < 8; i++) dot = fmaf(nibble(x[e], i), q[n * 64 + e * 8 + i], dot);
+                const uint32_t pair = kv4_scales<D>(kv, id, head)[n * kBlockPos + p % kBlockPos];
+                score = fmaf(dot, key_scale(pair), score);
+                vs[n] = value_scale(pair);
+            }
+            score *= a.scale;
+        }
+        const float mx = fmaxf(m, wave_max(in ? score : kNone));
+        const float shrink = __builtin_amdgcn_exp2f(m - mx);
+        const float e = in ? __builtin_amdgcn_exp2f(score - mx) : 0.0f;
+        m = mx;
+        l = fmaf(l, shrink, wave_sum(e));
+        for (int n = 0; n < N; n++) {
+            w[lane][n] = in ? e * vs[n] : 0.0f;
+            acc[n] *= shrink;
+        }
+        __syncthreads();
+        for (int j = 0; j < 64 && p0 + j < keys; j++) {
+            const int b = __shfl(id, j);
+            if ((unsigned)b >= kv.blocks) continue;
+            const int i = j % kBlockPos;
+            for (int n = 0; n < N; n++) {
+                const uint32_t x = ((const uint32_t *)(kv4_tile<D>(kv, b, head) + (N + n) * kPlane))
+                    [lane * 2 + (i >> 3)];
+                acc[n] = fmaf(nibble(x, i & 7), w[j][n], acc[n]);
+            }
+        }
+        __syncthreads();
+    }
+    if (__any(wild) && lane == 0) atomicOr(status, 2);
+    // Scores that are all -inf do not come out finite; no keys come out as zeros.
+    if (any && l == 0.0f) l = __builtin_nanf("");
+    bool bad = false;
+    for (int n = 0; n < N; n++) {
+        const float o = any ? acc[n] / l : 0.0f;
+        out[n * 64 + lane] = o;
+        bad |= !isfinite(o);
+    }
+    if (a.lse && lane == 0) a.lse[row * gridDim.x + qh] = any ? m + log2f(l) : INFINITY;
+    flag_nonfinite(status, bad);
+}
+
+// A thread for each key of a (stream, key head).
+template <int D>
+__global__ __launch_bounds__(256) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
+                                                  const float *before, float *after,
+                                                  size_t stride, int counted, int *status) {
+    constexpr int N = D / kSpan;
+    const int head = blockIdx.y, s = blockIdx.z, p = blockIdx.x * 256 + threadIdx.x;
+    const Kv4Span span = kv4_span(rows, s, a.max_positions, false, status);
+    if (!span.live || p >= span.first + span.count) return;
+    const size_t at = ((size_t)s * kv.heads + head) * stride + p;
+    float sum = before && p < span.first ? before[at] : 0.0f;
+    const int id = rows.tables[(size_t)s * rows.table_stride + p / kBlockPos];
+    if ((unsigned)id < kv.blocks) {
+        const uint8_t *tile = kv4_tile<D>(kv, id, head);
+        float part = 0.0f;
+        for (int i = max(max(0, span.count - counted), p - span.first); i < span.count; i++)
+            for (int j = 0; j < a.group; j++) {
+                const int qh = head * a.group + j;
+                const size_t row = (size_t)span.row0 + i;
+                const float lse = a.lse[row * kv.heads * a.group + qh];
+                const float *q = a.q + row * a.q_stride + (size_t)qh * D;
+                float score = 0.0f;
+                for (int n = 0; n < N; n++) {
+                    const uint32_t *x = (const uint32_t *)(tile + n * kPlane + p % kBlockPos * (kSpan / 2));
+                    float dot = 0.0f;
+                    for (int e = 0; e < 8; e++)
+                        for (int z = 0; z < 8; z++)
+                            dot = fmaf(nibble(x[e], z), q[n * 64 + e * 8 + z], dot);
+                    score = fmaf(dot, key_scale(kv4_scales<D>(kv, id, head)[n * kBlockPos + p % kBlockPos]), score);
+                }
+                if (isfinite(lse)) part += __builtin_amdgcn_exp2f(score * a.scale - lse);
+            }
+        sum += part;
+    }
+    after[at] = sum;
+}
+
+// ------------------------------------------------------------------ eviction
+
+// Orders like the number; NaN counts as 0, and -0 as 0.
+__device__ inline uint32_t order_of(float x) {
+    const uint32_t u = fbits(x == x ? x + 0.0f : 0.0f);
+    return u ^ ((int)u < 0 ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kBins = 2048;
+
+struct Kv4Evict {
+    const int32_t *tables, *to_tables;
+    int table_stride;
+    const int32_t *lengths;
+    int keep, first, newest;
+    const float *sums;
+    float *to_sums;
+    size_t sums_stride;
+    int32_t *kept;
+};
+
+struct Kv4EvictShared {
+    uint32_t bins[kBins];
+    uint32_t wave_a[kEvictWaves], wave_b[kEvictWaves];
+    uint32_t bin, above;
+    int bad;
+};
+
+// The sum over the waves before this one, and (total) over all, of a number of each wave.
+__device__ inline uint32_t waves_before(uint32_t *share, uint32_t mine, uint32_t &total) {
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) share[wave] = mine;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+    for (int i = 0; i < kEvictWaves; i++) {
+        if (i < wave) before += share[i];
+        total += share[i];
+    }
+    return before;
+}
+
+// A work-group for each (head, layer, stream). The least order that is kept is found
+// digit by digit (11, 11 and 10 bits) from counts in LDS; then the indexes are dealt out
+// in order, and the rows moved, a block to a wave, kEvictWaves blocks between two
+// barriers: a block's rows come from its own place or later ones, and all that are
+// read before a barrier are written after it, so that nothing is read that was written.
+template <int D>
+__global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t layer_values,
+                                                             size_t layer_scales, Kv4Evict a,
+                                                             int *status) {
+    constexpr int N = D / kSpan;
+    __shared__ Kv4EvictShared sh;
+    const int head = blockIdx.x, layer = blockIdx.y, s = blockIdx.z, streams = gridDim.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    kv.values += layer * layer_values;
+    kv.scales += layer * layer_scales;
+    const size_t unit = ((size_t)layer * streams + s) * kv.heads + head;
+    const float *sums = a.sums + unit * a.sums_stride;
+    float *to_sums = a.to_sums + unit * a.sums_stride;
+    int32_t *kept = a.kept + unit * a.keep;
+    const int32_t *table = a.tables + (size_t)s * a.table_stride;
+    const int32_t *to_table = a.to_tables + (size_t)s * a.table_stride;
+    const int n = uniform_load(a.lengths + s), count = min(n, a.keep);
+    const bool long_ = n > 0 && ((size_t)n > a.sums_stride ||
+                                 (n - 1) / kBlockPos >= a.table_stride);
+    if (threadIdx.x == 0) sh.bad = long_;
+    __syncthreads();
+    if (!long_ && n > 0) {
+        bool bad = false;
+        for (int b = threadIdx.x; b * kBlockPos < n; b += kEvictThreads) {
+            bad |= (unsigned)table[b] >= kv.blocks;
+            if (b * kBlockPos < count) bad |= (unsigned)to_table[b] >= kv.blocks;
+        }
+        if (bad) sh.bad = 1;
+    }
+    __syncthreads();
+    if (sh.bad || n <= 0) {
+        for (int j = threadIdx.x; j < a.keep; j += kEvictThreads) kept[j] = -1;
+        if (sh.bad && threadIdx.x == 0) atomicOr(status, 2);
+        return;
+    }
+
+    const int lo = n > a.keep ? a.first : n, hi = n > a.keep ? n - a.newest : n;
+    uint32_t need = n > a.keep ? a.keep - a.first - a.newest : 0, least = 0;
+    // Of the orders equal to `least`, the first `need` are kept; of the others the larger.
+    if (need) {
+        int shift = 32;
+        for (int digit = 0; digit < 3; digit++) {
+            const int width = digit < 2 ? 11 : 10;
+            for (int b = threadIdx.x; b < kBins; b += kEvictThreads) sh.bins[b] = 0;
+            __syncthreads();
+            for (int i = lo + threadIdx.x; i < hi; i += kEvictThreads) {
+                const uint32_t u = order_of(sums[i]);
+                if (shift == 32 || (u >> shift) == (least >> shift))
+                    atomicAdd(&sh.bins[u >> (shift - width) & ((1u << width) - 1)], 1u);
+            }
+            __syncthreads();
+            // Two bins to a thread, from the top.
+            const int b = kBins - 1 - 2 * (int)threadIdx.x;
+            const uint32_t x = sh.bins[b], y = sh.bins[b - 1];
+            uint32_t run = x + y;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t z = __shfl_up(run, o);
+                if (lane >= o) run += z;
+            }
+            uint32_t total;
+            const uint32_t before = waves_before(sh.wave_a, __shfl(run, 63), total) + run - x - y;
+            if (before < need && before + x >= need) {
+                sh.bin = b;
+                sh.above = before;
+            } else if (before + x < need && before + x + y >= need) {
+                sh.bin = b - 1;
+                sh.above = before + x;
+            }
+            __syncthreads();
+            shift -= width;
+            least |= sh.bin << shift;
+            need -= sh.above;
+            __syncthreads();
+        }
+    }
+    // The indexes and their sums, in order.
+    uint32_t equal = 0, at = 0;  // before this round
+    for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
+        const int i = i0 + threadIdx.x;
+        const float x = i < n ? sums[i] : 0.0f;
+        const uint32_t u = order_of(x);
+        const bool middle = i >= lo && i < hi;
+        const bool same = middle && u == least;
+        const uint64_t mask = __ballot(same);
+        uint32_t total;
+        const uint32_t rank = equal + waves_before(sh.wave_a, __popcll(mask), total) +
+                              __popcll(mask & ((1ull << lane) - 1));
+        equal += total;
+        const bool keep = i < n && (!middle || (lo < hi && need && u > least) ||
+                                    (same && rank < need));
+        const uint64_t all = __ballot(keep);
+        const uint32_t to = at + waves_before(sh.wave_b, __popcll(all), total) +
+                            __popcll(all & ((1ull << lane) - 1));
+        at += total;
+        if (keep) {
+            kept[to] = i;
+            to_sums[to] = x == x ? x : 0.0f;
+        }
+    }
+    for (int j = count + threadIdx.x; j < a.keep; j += kEvictThreads) kept[j] = -1;
+    __syncthreads();
+
+    // The rows.
+    for (int b0 = 0; b0 * kBlockPos < count; b0 += kEvictWaves) {
+        const int b = b0 + wave, rows = min(kBlockPos, count - b * kBlockPos);
+        uint64_t key[N], dim[N];
+        uint32_t pair[N];
+        unsigned to = 0;
+        bool stay = rows <= 0;
+        if (!stay) {
+            to = (unsigned)to_table[b];
+            const int j = lane >> 2, src = kept[b * kBlockPos + min(j, rows - 1)];
+            const unsigned id = (unsigned)table[src / kBlockPos];
+            // Rows that are where they belong.
+            stay = __all(id == to && src == b * kBlockPos + min(j, rows - 1));
+#pragma unroll
+            for (int m = 0; m < N; m++) {
+                const uint8_t *tile = kv4_tile<D>(kv, id, head);
+                key[m] = *((const uint64_t *)(tile + m * kPlane + src % kBlockPos * (kSpan / 2)) +
+                           (lane & 3));
+                pair[m] = kv4_scales<D>(kv, id, head)[m * kBlockPos + src % kBlockPos];
+                dim[m] = 0;
+#pragma unroll
+                for (int z = 0; z < kBlockPos; z++) {
+                    const unsigned from = (unsigned)__builtin_amdgcn_readlane((int)id, z * 4);
+                    const int i = __builtin_amdgcn_readlane(src, z * 4) % kBlockPos;
+                    const uint32_t byte = kv4_tile<D>(kv, from, head)[(N + m) * kPlane + lane * 8 +
+                                                                     (i >> 3) * 4 + (i & 3)];
+                    if (z < rows)
+                        dim[m] |= (uint64_t)(byte >> (i & 4) & 15u)
+                                  << ((z >> 3) * 32 + (z & 3) * 8 + (z >> 2 & 1) * 4);
+                }
+            }
+        }
+        __syncthreads();
+        if (!stay) {
+            uint8_t *tile = kv4_tile<D>(kv, to, head);
+            const int j = lane >> 2;
+#pragma unroll
+            for (int m = 0; m < N; m++) {
+                *((uint64_t *)(tile + (N + m) * kPlane) + lane) = dim[m];
+                if (j >= rows) continue;
+                *((uint64_t *)(tile + m * kPlane + j * (kSpan / 2)) + (lane & 3)) = key[m];
+                if ((lane & 3) == 0) kv4_scales<D>(kv, to, head)[m * kBlockPos + j] = pair[m];
+            }
+        }
+    }
+}
+
+}  // namespace pgpu
+
+using namespace pgpu;
+
+// ------------------------------------------------------------- entry points
+
+namespace {
+
+bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+bool cache_ok(const pgpu_kv4 *kv) {
+    return kv && kv->values && kv->scales && aligned(kv->values, 16) && aligned(kv->scales, 16) &&
+           kv->layers > 0 && kv->heads > 0 && kv->heads <= 256 &&
+           (kv->head_dim == 64 || kv->head_dim == 128) && kv->blocks > 0 &&
+           kv->blocks <= INT32_MAX;
+}
+
+bool rows_ok(const pgpu_kv4_rows *r) {
+    return r && r->tables && r->table_stride > 0 && r->first && r->streams > 0 &&
+           r->streams <= 65535 && r->rows >= 0 && r->max_rows >= 0 && r->max_rows <= 65535 &&
+           r->max_rows <= r->rows &&
+           (r->offsets ? (r->max_rows > 0 || r->rows == 0)
+                       : (r->rows == r->streams && r->max_rows == 1));
+}
+
+// Bytes of a layer, and its scale pairs.
+size_t layer_values(const pgpu_kv4 *kv) {
+    return kv->blocks * kv->heads * kv->head_dim * kBlockPos;
+}
+size_t layer_scales(const pgpu_kv4 *kv) {
+    return kv->blocks * kv->heads * (kv->head_dim / kSpan) * kBlockPos;
+}
+
+Kv4 layer_of(const pgpu_kv4 *kv, int layer) {
+    return {kv->values + layer * layer_values(kv), (uint32_t *)kv->scales + layer * layer_scales(kv),
+            kv->heads, (unsigned)kv->blocks};
+}
+
+Kv4Rows rows_of(const pgpu_kv4_rows *r) {
+    return {r->tables, r->table_stride, r->first, r->offsets, r->rows, r->max_rows};
+}
+
+// Blocks that max_rows consecutive rows can lie in.
+int blocks_of(int max_rows) { return (max_rows + 2 * kBlockPos - 2) / kBlockPos; }
+
+}  // namespace
+
+extern "C" int pgpu_kv4_write(void *stream, const pgpu_kv4 *kv, int layer,
+                              const pgpu_kv4_rows *rows, const float *k, const float *v,
+                              size_t row_stride, int *status) {
+    if (!cache_ok(kv) || !rows_ok(rows) || layer < 0 || layer >= kv->layers || !k || !v ||
+        !status || !aligned(k, 16) || !aligned(v, 16) || row_stride % 4 != 0 ||
+        row_stride < (size_t)kv->heads * kv->head_dim)
+        return bad_arguments("pgpu_kv4_write");
+    if (rows->rows == 0) return 1;
+    const dim3 grid((kv->heads + 3) / 4, blocks_of(rows->max_rows), rows->streams);
+    if (kv->head_dim == 64)
+        hipLaunchKernelGGL(k_kv4_write<64>, grid, dim3(256), 0, (hipStream_t)stream,
+                           layer_of(kv, layer), rows_of(rows), k, v, row_stride, status);
+    else
+        hipLaunchKernelGGL(k_kv4_write<128>, grid, dim3(256), 0, (hipStream_t)stream,
+                           layer_of(kv, layer), rows_of(rows), k, v, row_stride, status);
+    return launch_ok("pgpu_kv4_write");
+}
+
+extern "C" int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer,
+                             const pgpu_kv4_rows *rows, const int32_t *lengths, float *k,
+                             float *v, size_t row_stride, int *status) {
+    if (!cache_ok(kv) || !rows_ok(rows) || layer < 0 || layer >= kv->layers || !lengths || !k ||
+        !v || !status || !aligned(k, 16) || !aligned(v, 16) || row_stride % 4 != 0 ||
+        row_stride < (size_t)kv->heads * kv->head_dim)
+        return bad_arguments("pgpu_kv4_read");
+    if (rows->rows == 0) return 1;
+    const dim3 grid((kv->heads + 3) / 4, blocks_of(rows->max_rows), rows->streams);
+    if (kv->head_dim == 64)
+        hipLaunchKernelGGL(k_kv4_read<64>, grid, dim3(256), 0, (hipStream_t)stream,
+                           layer_of(kv, layer), rows_of(rows), lengths, k, v, row_stride, status);
+    else
+        hipLaunchKernelGGL(k_kv4_read<128>, grid, dim3(256), 0, (hipStream_t)stream,
+                           layer_of(kv, layer), rows_of(rows), lengths, k, v, row_stride, status);
+    return launch_ok("pgpu_kv4_read");
+}
+
+namespace {
+
+template <int D>
+int attend(void *stream, const Kv4 &c, const Kv4Rows &r, int streams, const Kv4Run &a,
+           const pgpu_kv4_sums *sums, int *status) {
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(k_kv4_attend<D>, dim3(c.heads * a.group, r.max_rows, streams), dim3(64), 0,
+                       st, c, r, a, status);
+    if (!launch_ok("pgpu_kv4_attention")) return 0;
+    if (!sums) return 1;
+    hipLaunchKernelGGL(k_kv4_sums<D>, dim3((a.max_positions + 255) / 256, c.heads, streams),
+                       dim3(256), 0, st, c, r, a, sums->before, sums->after, sums->stride,
+                       sums->rows, status);
+    return launch_ok("pgpu_kv4_attention");
+}
+
+}  // namespace
+
+extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *rows,
+                                           int group, int max_positions, int with_sums) {
+    if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
+    return with_sums ? (size_t)rows->rows * kv->heads * group * sizeof(float) : 0;
+}
+
+extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
+                                  const pgpu_kv4_rows *rows, const float *q, size_t q_stride,
+                                  int group, float scale, int max_positions, float *out,
+                                  size_t out_stride, const pgpu_kv4_sums *sums, void *work,
+                                  size_t work_bytes, int *status) {
+    constexpr float kLog2e = 1.44269504f;
+    const size_t width = kv ? (size_t)kv->heads * kv->head_dim * group : 0;
+    if (!cache_ok(kv) || !rows_ok(rows) || layer < 0 || layer >= kv->layers || !q || !out ||
+        !status || !aligned(q, 16) || !aligned(out, 16) || q_stride % 4 != 0 ||
+        out_stride % 4 != 0 || group < 1 || group > 16 || q_stride < width ||
+        out_stride < width || max_positions <= 0 || !__builtin_isfinite(scale * kLog2e) ||
+        (sums && (!sums->after || sums->stride < (size_t)max_positions || sums->rows < 1)))
+        return bad_arguments("pgpu_kv4_attention");
+    if (rows->rows == 0) return 1;
+    const size_t need = pgpu_kv4_attention_bytes(kv, rows, group, max_positions, sums != nullptr);
+    if (need && (!work || !aligned(work, 16) || work_bytes < need))
+        return bad_arguments("pgpu_kv4_attention (workspace)");
+    const Kv4Run a = {q,   q_stride,   group, scale * kLog2e, max_positions, out, out_stride,
+                      sums ? (float *)work : nullptr};
+    return kv->head_dim == 64
+               ? attend<64>(stream, layer_of(kv, layer), rows_of(rows), rows->streams, a, sums, status)
+               : attend<128>(stream, layer_of(kv, layer), rows_of(rows), rows->streams, a, sums, status);
+}
+
+extern "C" int pgpu_kv4_evict(void *stream, const pgpu_kv4 *kv, int first_layer, int layers,
+                              const int32_t *tables, const int32_t *to_tables, int table_stride,
+                              const int32_t *lengths, int streams, int keep, int first,
+                              int newest, const float *sums, float *to_sums,
+                              size_t sums_stride, int32_t *kept, int *status) {
+    if (!cache_ok(kv) || first_layer < 0 || layers <= 0 || first_layer > kv->layers - layers ||
+        layers > 65535 || !tables || table_stride <= 0 || !lengths || streams <= 0 ||
+        streams > 65535 || keep < 1 || first < 0 || newest < 0 || first > keep - newest || !sums ||
+        !to_sums || sums_stride == 0 || !kept || !status)
+        return bad_arguments("pgpu_kv4_evict");
+    const Kv4Evict a = {tables, to_tables ? to_tables : tables, table_stride, lengths, keep, first,
+                        newest, sums, to_sums, sums_stride, kept};
+    const dim3 grid(kv->heads, layers, streams);
+    if (kv->head_dim == 64)
+        hipLaunchKernelGGL(k_kv4_evict<64>, grid, dim3(kEvictThreads), 0, (hipStream_t)stream,
+                           layer_of(kv, first_layer), layer_values(kv), layer_scales(kv), a, status);
+    else
+        hipLaunchKernelGGL(k_kv4_evict<128>, grid, dim3(kEvictThreads), 0, (hipStream_t)stream,
+                           layer_of(kv, first_layer), layer_values(kv), layer_scales(kv), a, status);
+    return launch_ok("pgpu_kv4_evict");
+}
