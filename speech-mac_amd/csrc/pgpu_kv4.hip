@@ -8,6 +8,8 @@
 
 namespace pgpu {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kSpan = 64;         // dims of a scale
 constexpr int kPlane = 512;       // bytes of a block's 64 dims, of keys or of values
 constexpr float kLeastScale = 0x1p-17f, kMostScale = 8160.0f;
@@ -275,6 +277,421 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, Kv4Rows rows, const in
 }
 
 // ----------------------------------------------------------------- attention
+
+// One row a stream multiplies on v_mfma_i32_16x16x64_i8. A byte of the cache gives two
+// of its operand's by a shift and two ANDs: a number in the upper half of a byte is 16
+// times itself as a signed byte. A query (and 64 keys' weights) becomes a fixed-point
+// number of 30 bits, split into four signed bytes that stand in four rows of the other
+// operand: products and sums are exact, and
+//   ((b3 * 2^8 + b2) * 2^16 + (b1 * 2^8 + b0)) * step
+// is rounded to fp32.
+
+// Sixteen numbers of the cache -> an operand, 16 times each.
+__device__ inline i32x4 unpack16(u32x2 x) {
+    return i32x4{(int)(x[0] << 4 & 0xF0F0F0F0u), (int)(x[0] & 0xF0F0F0F0u),
+                 (int)(x[1] << 4 & 0xF0F0F0F0u), (int)(x[1] & 0xF0F0F0F0u)};
+}
+// Bytes of the cache for one row a stream, read once: past the caches.
+__device__ inline u32x2 stream_load8(const uint8_t *p) {
+    return __builtin_nontemporal_load((const u32x2 *)p);
+}
+
+template <int E>
+__device__ inline int row_shift_left(int v) {  // lane i of 16 gets lane i + E's
+    return __builtin_amdgcn_update_dpp(0, v, 0x100 + E, 0xf, 0xf, true);
+}
+
+struct Kv4Decode {
+    const float *q;
+    size_t q_stride;
+    int group;
+    float scale;  // of the scores, times log2 e
+    int max_positions, splits, steps;  // a split: steps * W * 64 keys
+    // Slot (s * query heads + head) * splits + split.
+    float *part_acc, *part_ml;
+    float *out;  // splits = 1: the rows themselves (else NULL)
+    size_t out_stride;
+    float *lse;  // [streams][query heads]: log2 of the sum of 2^score, or NULL
+    float *scores;  // [streams][query heads][max_positions], in units of log 2, or NULL
+};
+
+template <int D, int W, int Q>
+struct Kv4DecodeShared {
+    __align__(16) uint32_t digits[Q == 1 ? 1 : W][16][16];  // [row][block, quad of keys]
+    float acc[W][Q][D];
+    float m[W][Q], l[W][Q];
+};
+
+// One row a stream. A work-group of W waves takes a split's keys of one (stream, key
+// head) for Q (1 or 4) of its queries, W * 64 keys a step: a wave's 64 are 4 blocks,
+// whose bytes it requests together, the next step's as soon as the registers are free:
+// keys after the scores, values after their product. No wave waits for another before
+// the joint of all W.
+//
+// Weights enter their product times their keys' value scales, below 2^m: m is a whole
+// number, the largest of score + exponent of the value scale so far, so that one fixed
+// point serves the running sums, which stay whole numbers as long as m does.
+//
+// A lone query's digits stand in rows 4 t .. 4 t + 3 for block t, zeros elsewhere, so
+// that lane (g, i) gets the score of key i of block g: one key to a lane. Of four
+// queries, lane (g, i) has query g's score of key i of each block.
+template <int D, int W, int Q>
+__global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv4_decode(Kv4 kv, Kv4Rows rows,
+                                                                        Kv4Decode a, int *status) {
+    constexpr int N = D / kSpan, T = D / 16, S = Q == 1 ? 1 : 4;
+    __shared__ Kv4DecodeShared<D, W, Q> sh;
+    // Heads vary fastest: with 8 of them a head's passes stay on one XCD.
+    const int head = blockIdx.x % kv.heads, j0 = blockIdx.x / kv.heads * Q;
+    const int split = blockIdx.y, s = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
+    int b0 = (split * a.steps * W + wave) * 4;  // the wave's blocks: b0 .. b0 + 3
+    const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
+    int ids[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) ids[t] = uniform_load(table + min(b0 + t, rows.table_stride - 1));
+    const Kv4Span span = kv4_span(rows, s, a.max_positions,
+                                  threadIdx.x == 0 && blockIdx.x == 0 && split == 0, status);
+    const int live = min(Q, a.group - j0);  // queries of this work-group
+    const int p = span.first;
+    if (!span.live) {
+        if (a.out && p < 0 && span.count > 0)
+            for (int e = threadIdx.x; e < live * D; e += 64 * W)
+                a.out[(size_t)s * a.out_stride + ((size_t)head * a.group + j0) * D + e] = 0.0f;
+        return;
+    }
+    if (split * a.steps * W * 64 > p) return;
+    const int held = p / kBlockPos + 1;
+    const size_t qh0 = (size_t)s * kv.heads * a.group + (size_t)head * a.group + j0;
+
+    u32x2 kr[4][N], vr[T];
+    uint32_t pair[S][N];
+    bool wild = false;
+    unsigned on = 0, ever = 0;  // bit t: block t of the step whose keys were requested counts
+    // Blocks b .. b + 3; block 0 for one past the last or not in the cache, so that every
+    // step requests alike and waits for no more than it needs.
+    auto load = [&](int b, bool values) {
+        unsigned id[4];
+        if (!values) on = 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const bool there = b + t < held, in = (unsigned)ids[t] < kv.blocks;
+            id[t] = there && in ? (unsigned)ids[t] : 0u;
+            if (!values) {
+                wild |= there && !in;
+                on |= (there && in ? 1u : 0u) << t;
+            }
+        }
+        const unsigned mine = g < 2 ? (g ? id[1] : id[0]) : (g == 2 ? id[2] : id[3]);
+        if (!values) {
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    kr[t][n] = stream_load8(kv4_tile<D>(kv, id[t], head) + n * kPlane + i * 32 + g * 8);
+                if constexpr (Q == 1)
+                    pair[0][n] = __builtin_nontemporal_load(kv4_scales<D>(kv, mine, head) +
+                                                            n * kBlockPos + i);
+                else
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        pair[t][n] = __builtin_nontemporal_load(kv4_scales<D>(kv, id[t], head) +
+                                                                n * kBlockPos + i);
+            }
+        } else {
+            const uint8_t *tile = kv4_tile<D>(kv, mine, head) + N * kPlane + i * 8;
+#pragma unroll
+            for (int t = 0; t < T; t++) vr[t] = stream_load8(tile + t * 128);
+        }
+    };
+
+    // Row i of the operand: byte i % 4 of query j0 + i / 4.
+    const float *q = a.q + (size_t)s * a.q_stride +
+                     ((size_t)head * a.group + min(j0 + (Q == 1 ? 0 : i >> 2), a.group - 1)) * D;
+    const uint32_t byte = row_byte(i & 3), sel = byte | (4u + byte) << 8;
+    i32x4 qd[S == 1 ? 4 : 1][N];
+    float step, top = 0.0f;
+    auto begin = [&] {
+        float4 x[N][4];
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[n][k] = *(const float4 *)(q + n * kSpan + g * 16 + k * 4);
+        // The order of the requests is the order in which they are waited for.
+        __builtin_amdgcn_sched_barrier(0);
+        load(b0, false);
+        __builtin_amdgcn_sched_barrier(0);
+        load(b0, true);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float4 v = x[n][k];
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
+                                       fmaxf(fabsf(v.z), fabsf(v.w))));
+                if (!(v.x == v.x && v.y == v.y && v.z == v.z && v.w == v.w)) top = INFINITY;
+            }
+        top = xor16_32_max(top);
+        const int e = fix_exponent(top);
+        const float mul = power_of_2(e);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            i32x4 d;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                d[k] = (int)pick4(fix_bytes(x[n][k].x, mul), fix_bytes(x[n][k].y, mul),
+                                  fix_bytes(x[n][k].z, mul), fix_bytes(x[n][k].w, mul), sel);
+            if constexpr (Q == 1)
+#pragma unroll
+                for (int t = 0; t < 4; t++) qd[t][n] = i >> 2 == t ? d : i32x4{0, 0, 0, 0};
+            else
+                qd[0][n] = d;
+        }
+        // Fixed point cannot say that a query is infinite. (16: the cache's numbers.)
+        step = top < INFINITY ? a.scale * power_of_2(-e) * 0.0625f : __builtin_nanf("");
+        if (Q != 1) step = __shfl(step, g * 4);  // of query j0 + g
+    };
+    float m = kNone, l = 0.0f, acc[T];
+    i32x4 sum[T];  // whole sums of the values, of dims 16 t + i, times 2^(34 - m)
+    int flushed = 0;
+#pragma unroll
+    for (int t = 0; t < T; t++) acc[t] = 0.0f, sum[t] = i32x4{0, 0, 0, 0};
+    auto flush = [&](float less) {
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const float whole = fmaf((float)sum[t].x, 0x1p24f, fmaf((float)sum[t].y, 0x1p16f,
+                                     fmaf((float)sum[t].z, 0x1p8f, (float)sum[t].w)));
+            acc[t] = fmaf(whole, 0x1p-34f, acc[t]) * less;
+            sum[t] = i32x4{0, 0, 0, 0};
+        }
+    };
+
+    auto attend = [&](bool more) {
+        const unsigned count = on;
+        ever |= on;
+        if (more)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                ids[t] = uniform_load(table + min(b0 + 4 * W + t, rows.table_stride - 1));
+        // Scores, in units of log 2.
+        float w[S], vs[S][N], bound = kNone;
+        i32x4 c[S][N];
+#pragma unroll
+        for (int t = 0; t < S; t++)
+#pragma unroll
+            for (int n = 0; n < N; n++) c[t][n] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                i32x4 &to = c[Q == 1 ? 0 : t][n];
+                to = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[Q == 1 ? t : 0][n], unpack16(kr[t][n]),
+                                                           to, 0, 0, 0);
+            }
+#pragma unroll
+        for (int t = 0; t < S; t++) {
+            const int b = b0 + (Q == 1 ? g : t);
+            const bool seen = (count >> (Q == 1 ? g : t) & 1) && b * kBlockPos + i <= p;
+            float score = 0.0f, large = 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                score = fmaf(fix_sum(c[t][n]), key_scale(pair[t][n]), score);
+                vs[t][n] = seen ? value_scale(pair[t][n]) : 0.0f;
+                large = fmaxf(large, vs[t][n]);
+            }
+            w[t] = seen ? score * step : -INFINITY;
+            if (a.scores && seen && (Q == 1 || g < live))
+                a.scores[(qh0 + (Q == 1 ? 0 : g)) * a.max_positions + b * kBlockPos + i] = w[t];
+            bound = fmaxf(bound, w[t] + (float)((int)(fbits(large) >> 23) - 126));
+        }
+        if (more) load(b0 + 4 * W, false);
+        bound = row16_max(bound);
+        if (Q == 1) bound = xor16_32_max(bound);
+        const float next = fmaxf(m, ceilf(bound));
+        if (__any(next != m) || ++flushed == 1024) {
+            const float less = __builtin_amdgcn_exp2f(m - next);  // m = kNone: 0
+            flush(less);
+            l *= less;
+            m = next;
+            flushed = 0;
+        }
+#pragma unroll
+        for (int t = 0; t < S; t++) {
+            w[t] = __builtin_amdgcn_exp2f(w[t] - m);
+            l += w[t];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            i32x4 pd;
+            if constexpr (Q == 1) {
+                // Row t < 4: digit t of block g's keys, a quad of keys a word.
+                const uint32_t u = fix_bytes(w[0] * vs[0][n], 0x1p30f);
+                const int word = (int)pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u),
+                                            quad_lane<3>(u), sel);
+                pd = i32x4{word, row_shift_left<4>(word), row_shift_left<8>(word),
+                           row_shift_left<12>(word)};
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const uint32_t u = fix_bytes(w[t] * vs[t][n], 0x1p30f);
+                    sh.digits[wave][g * 4 + (i & 3)][t * 4 + (i >> 2)] =
+                        pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u), quad_lane<3>(u), sel);
+                }
+                wave_lds_fence();
+                pd = *(const i32x4 *)&sh.digits[wave][i][g * 4];
+                wave_lds_fence();
+            }
+#pragma unroll
+            for (int t = n * 4; t < n * 4 + 4; t++)
+                sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd, unpack16(vr[t]), sum[t], 0, 0, 0);
+        }
+        b0 += 4 * W;
+        if (more) load(b0, true);
+    };
+    // The last step apart: no branch stands between a request and its wait.
+    int steps = b0 < held ? min(a.steps, (held - b0 - 1) / (4 * W) + 1) : 0;
+    if (steps > 0) {
+        begin();
+        for (; steps > 1; steps--) attend(true);
+        attend(false);
+        flush(1.0f);
+    }
+    if (wild && lane == 0) atomicOr(status, 2);
+    l = row16_sum(l);
+    if (Q == 1) l = xor16_32_sum(l);
+    if (g < Q) {
+#pragma unroll
+        for (int t = 0; t < T; t++) sh.acc[wave][g][t * 16 + i] = acc[t];
+        if (i == 0) {
+            sh.m[wave][g] = ever ? m : -INFINITY;
+            sh.l[wave][g] = l;
+        }
+    }
+    bool bad = !(top < INFINITY);
+    __syncthreads();
+    for (int e = threadIdx.x; e < live * D; e += 64 * W) {
+        const int j = e / D, d = e % D;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < W; n++) mx = fmaxf(mx, sh.m[n][j]);
+        float total = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int n = 0; n < W; n++) {
+            // A wave without a key: m = -inf, l = 0, acc = 0.
+            const float c = __builtin_amdgcn_exp2f(sh.m[n][j] - fmaxf(mx, kNone));
+            total = fmaf(sh.l[n][j], c, total);
+            o = fmaf(sh.acc[n][j][d], c, o);
+        }
+        if (a.out) {
+            // Scores that are all -inf: not finite. No key: zeros.
+            o = mx == -INFINITY ? 0.0f : o / total;
+            a.out[(size_t)s * a.out_stride + ((size_t)head * a.group + j0 + j) * D + d] = o;
+            if (a.lse && d == 0) a.lse[qh0 + j] = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+            bad |= !isfinite(o);
+        } else {
+            const size_t at = (qh0 + j) * a.splits + split;
+            a.part_acc[at * D + d] = o;
+            if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(mx, total);
+        }
+    }
+    flag_nonfinite(status, bad);
+}
+
+// The splits of a row's query head joined: D / 4 lanes for 4 dims each, times G that
+// share the splits. `keys`: of a split, or 0: every split has its part of every row, or
+// says that it has none (a maximum of -inf).
+template <int D, int G>
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const float *part_acc,
+                                                  const float *part_ml, int group,
+                                                  int max_positions, int splits, int keys,
+                                                  float *out, size_t out_stride, float *lse,
+                                                  int *status) {
+    constexpr int L = D / 4, M = L * G;
+    const int s = blockIdx.z, wide = kv.heads * group;
+    const size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int lane = (int)(e % M), share = lane / L, d = lane % L * 4;
+    const int qh = (int)(e / M % wide);
+    const size_t i = e / M / wide;
+    const Kv4Span span = kv4_span(rows, s, max_positions, false, status);
+    if (i >= (size_t)span.count || (!span.live && span.first >= 0)) return;
+    const size_t row = span.row0 + i;
+    float *dst = out + row * out_stride + (size_t)qh * D + d;
+    if (!span.live) {
+        if (share == 0) *(float4 *)dst = make_float4(0.f, 0.f, 0.f, 0.f);
+        return;
+    }
+    const int n = keys ? (span.first + (int)i) / keys + 1 : splits;
+    const size_t at = (((size_t)s * rows.max_rows + i) * wide + qh) * splits;
+    // Lane j of the M has split j's maximum and sum, and the next M's.
+    float mx = -INFINITY, total = 0.0f;
+    for (int j = lane; j < n; j += M) mx = fmaxf(mx, part_ml[(at + j) * 2]);
+#pragma unroll
+    for (int z = 1; z < M; z <<= 1) mx = fmaxf(mx, __shfl_xor(mx, z));
+    const float base = fmaxf(mx, kNone);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 < n; j0 += M) {
+        const int last = min(M, n - j0);
+        const float2 ml = lane < last ? *(const float2 *)(part_ml + (at + j0 + lane) * 2)
+                                      : make_float2(-INFINITY, 0.0f);
+        const float c = __builtin_amdgcn_exp2f(ml.x - base);
+        total = fmaf(ml.y, c, total);
+        for (int j = 0; j < last; j += 8 * G) {
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                x[k] = *(const float4 *)(part_acc +
+                                         (at + j0 + min(j + k * G + share, last - 1)) * D + d);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float w = __shfl(c, min(j + k * G + share, M - 1), M);
+                if (j + k * G + share >= last) continue;
+                o.x = fmaf(x[k].x, w, o.x);
+                o.y = fmaf(x[k].y, w, o.y);
+                o.z = fmaf(x[k].z, w, o.z);
+                o.w = fmaf(x[k].w, w, o.w);
+            }
+        }
+    }
+#pragma unroll
+    for (int z = 1; z < M; z <<= 1) total += __shfl_xor(total, z);
+#pragma unroll
+    for (int z = L; z < M; z <<= 1) {
+        o.x += __shfl_xor(o.x, z);
+        o.y += __shfl_xor(o.y, z);
+        o.z += __shfl_xor(o.z, z);
+        o.w += __shfl_xor(o.w, z);
+    }
+    if (share) return;
+    // No key that counts: zeros. Scores that are all -inf: not finite.
+    if (mx != -INFINITY) o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
+    *(float4 *)dst = o;
+    if (lse && d == 0) lse[row * wide + qh] = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+    flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
+}
+
+// One row a stream's weights, from its scores: a thread for each key of a (stream, key
+// head).
+__global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4Decode a,
+                                                      const float *before, float *after,
+                                                      size_t stride, int *status) {
+    const int head = blockIdx.y, s = blockIdx.z, p = blockIdx.x * 256 + threadIdx.x;
+    const Kv4Span span = kv4_span(rows, s, a.max_positions, false, status);
+    if (!span.live || p > span.first) return;
+    const size_t at = ((size_t)s * kv.heads + head) * stride + p;
+    float sum = before && p < span.first ? before[at] : 0.0f;
+    const int id = rows.tables[(size_t)s * rows.table_stride + p / kBlockPos];
+    if ((unsigned)id < kv.blocks) {
+        const size_t qh0 = ((size_t)s * kv.heads + head) * a.group;
+        float part = 0.0f;
+        for (int j = 0; j < a.group; j++) {
+            const float lse = a.lse[qh0 + j], score = a.scores[(qh0 + j) * a.max_positions + p];
+            if (isfinite(lse)) part += __builtin_amdgcn_exp2f(score - lse);
+        }
+        sum += part;
+    }
+    after[at] = sum;
+}
 
 struct Kv4Run {
     const float *q;
@@ -685,10 +1102,80 @@ extern "C" int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer,
 
 namespace {
 
+// How an attention call of one row a stream deals its work: splits of `keys` keys.
+struct Deal {
+    int splits, keys, tiles, waves, steps;  // tiles: work-groups for a stream and head
+};
+
+Deal deal_of(const pgpu_kv4 *kv, int streams, int group, int max_positions) {
+    Deal d;
+    // A stream's keys whole in one work-group of W waves (no parts to be joined), except
+    // where few work-groups have many keys each: those are dealt to work-groups of 4
+    // waves, more keys to each the more of them there are.
+    d.tiles = group == 1 ? 1 : (group + 3) / 4;
+    const size_t groups = (size_t)kv->heads * d.tiles * streams;
+    const int units = (max_positions - 1) / 64 + 1;
+    const bool wide = kv->head_dim != 64;
+    d.waves = groups > 768 ? (units > 36 ? 8 : 4) : groups > 256 || group > 1 || wide ? 8 : 16;
+    d.steps = (units + d.waves - 1) / d.waves;
+    if (units > (groups < 192 ? 3 * d.waves : wide ? 48 : 80)) {
+        d.waves = 4;
+        d.steps = groups < 64 ? 1 : groups < 192 ? (wide ? 1 : 2) : 3;
+    }
+    d.keys = 64 * d.waves * d.steps;
+    d.splits = (max_positions - 1) / d.keys + 1;
+    return d;
+}
+
+// The workspace of one row a stream: parts of `parts` (row, query head, split), then the
+// rows' log sums and their scores.
+size_t parts_bytes(const pgpu_kv4 *kv, size_t parts) {
+    return parts * (kv->head_dim + 2) * sizeof(float);
+}
+
 template <int D>
-int attend(void *stream, const Kv4 &c, const Kv4Rows &r, int streams, const Kv4Run &a,
+int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
+               const Kv4Decode &a, const pgpu_kv4_sums *sums, int *status) {
+    Kv4Decode one = a;
+    one.steps = d.steps;
+    if (d.splits > 1) one.out = nullptr;
+    const dim3 grid(c.heads * d.tiles, d.splits, streams);
+#define KV4_DECODE(W, Q)                                                                        \
+    hipLaunchKernelGGL((k_kv4_decode<D, W, Q>), grid, dim3(64 * W), 0, st, c, r, one, status)
+    if (a.group == 1 && d.waves == 4)
+        KV4_DECODE(4, 1);
+    else if (a.group == 1 && d.waves == 8)
+        KV4_DECODE(8, 1);
+    else if (a.group == 1) {
+        if constexpr (D == 64) KV4_DECODE(16, 1);
+    } else if (d.waves == 4)
+        KV4_DECODE(4, 4);
+    else
+        KV4_DECODE(8, 4);
+#undef KV4_DECODE
+    if (!launch_ok("pgpu_kv4_attention")) return 0;
+    if (d.splits > 1) {
+        const size_t items = (size_t)c.heads * a.group;
+        if (d.splits >= 8 && items * streams <= 4096)
+            hipLaunchKernelGGL((k_kv4_join<D, 256 / D>), dim3((unsigned)items, 1, streams), dim3(64),
+                               0, st, c, r, a.part_acc, a.part_ml, a.group, a.max_positions,
+                               d.splits, d.keys, a.out, a.out_stride, a.lse, status);
+        else
+            hipLaunchKernelGGL((k_kv4_join<D, 1>),
+                               dim3((unsigned)((items * (D / 4) + 255) / 256), 1, streams),
+                               dim3(256), 0, st, c, r, a.part_acc, a.part_ml, a.group,
+                               a.max_positions, d.splits, d.keys, a.out, a.out_stride, a.lse, status);
+        if (!launch_ok("pgpu_kv4_attention")) return 0;
+    }
+    if (!sums) return 1;
+    hipLaunchKernelGGL(k_kv4_sums_one, dim3((a.max_positions + 255) / 256, c.heads, streams),
+                       dim3(256), 0, st, c, r, one, sums->before, sums->after, sums->stride, status);
+    return launch_ok("pgpu_kv4_attention");
+}
+
+template <int D>
+int attend(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Kv4Run &a,
            const pgpu_kv4_sums *sums, int *status) {
-    hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(k_kv4_attend<D>, dim3(c.heads * a.group, r.max_rows, streams), dim3(64), 0,
                        st, c, r, a, status);
     if (!launch_ok("pgpu_kv4_attention")) return 0;
@@ -704,7 +1191,20 @@ int attend(void *stream, const Kv4 &c, const Kv4Rows &r, int streams, const Kv4R
 extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *rows,
                                            int group, int max_positions, int with_sums) {
     if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
-    return with_sums ? (size_t)rows->rows * kv->heads * group * sizeof(float) : 0;
+    const size_t wide = (size_t)kv->heads * group;
+    if (rows->offsets) return with_sums ? rows->rows * wide * sizeof(float) : 0;
+    // Fewer streams may be dealt to more work-groups: the streams before the numbers of
+    // work-groups where the keys to each change count too. More positions never give
+    // fewer parts.
+    size_t parts = 0;
+    const int groups = kv->heads * (group == 1 ? 1 : (group + 3) / 4);
+    for (int n : {rows->streams, 63 / groups, 191 / groups}) {
+        if (n < 1 || n > rows->streams) continue;
+        const Deal d = deal_of(kv, n, group, max_positions);
+        if (d.splits > 1) parts = std::max(parts, n * wide * d.splits);
+    }
+    return parts_bytes(kv, parts) +
+           (with_sums ? rows->streams * wide * (1 + (size_t)max_positions) * sizeof(float) : 0);
 }
 
 extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
@@ -721,14 +1221,37 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
         (sums && (!sums->after || sums->stride < (size_t)max_positions || sums->rows < 1)))
         return bad_arguments("pgpu_kv4_attention");
     if (rows->rows == 0) return 1;
-    const size_t need = pgpu_kv4_attention_bytes(kv, rows, group, max_positions, sums != nullptr);
+    const Kv4 c = layer_of(kv, layer);
+    const Kv4Rows r = rows_of(rows);
+    const hipStream_t st = (hipStream_t)stream;
+    const size_t wide = (size_t)kv->heads * group;
+    float *floats = (float *)work;
+    if (!rows->offsets) {
+        const Deal d = deal_of(kv, rows->streams, group, max_positions);
+        // The grid's limit: 16 million positions of one row a stream.
+        if (d.splits > 65535) return bad_arguments("pgpu_kv4_attention");
+        const size_t parts = d.splits > 1 ? rows->streams * wide * d.splits : 0;
+        const size_t need = parts_bytes(kv, parts) +
+                            (sums ? rows->streams * wide * (1 + (size_t)max_positions) * sizeof(float)
+                                  : 0);
+        if (need && (!work || !aligned(work, 16) || work_bytes < need))
+            return bad_arguments("pgpu_kv4_attention (workspace)");
+        Kv4Decode a = {q, q_stride, group, scale * kLog2e, max_positions, d.splits, 1,
+                       floats, floats + parts * kv->head_dim, out, out_stride, nullptr, nullptr};
+        if (sums) {
+            a.lse = floats + parts * (kv->head_dim + 2);
+            a.scores = a.lse + rows->streams * wide;
+        }
+        return kv->head_dim == 64 ? attend_one<64>(st, c, r, rows->streams, d, a, sums, status)
+                                  : attend_one<128>(st, c, r, rows->streams, d, a, sums, status);
+    }
+    const size_t need = sums ? rows->rows * wide * sizeof(float) : 0;
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv4_attention (workspace)");
     const Kv4Run a = {q,   q_stride,   group, scale * kLog2e, max_positions, out, out_stride,
-                      sums ? (float *)work : nullptr};
-    return kv->head_dim == 64
-               ? attend<64>(stream, layer_of(kv, layer), rows_of(rows), rows->streams, a, sums, status)
-               : attend<128>(stream, layer_of(kv, layer), rows_of(rows), rows->streams, a, sums, status);
+                      sums ? floats : nullptr};
+    return kv->head_dim == 64 ? attend<64>(st, c, r, rows->streams, a, sums, status)
+                              : attend<128>(st, c, r, rows->streams, a, sums, status);
 }
 
 extern "C" int pgpu_kv4_evict(void *stream, const pgpu_kv4 *kv, int first_layer, int layers,
