@@ -9,6 +9,7 @@
 namespace pgpu {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSpan = 64;         // dims of a scale
 constexpr int kPlane = 512;       // bytes of a block's 64 dims, of keys or of values
@@ -693,92 +694,397 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
     after[at] = sum;
 }
 
+// Runs of rows: a work-group of 4 waves takes 4 tiles of 16 rows of one query head each
+// (the query heads of a key head side by side), and passes over the keys 64 at a time:
+// each wave turns one block into fp16 in LDS (number times scale: exact), where all four
+// read it, while the next 64 keys' bytes are on their way. Scores are taken keys by rows
+// (K Q^T), so that a lane holds 16 of its row's scores and the weights are the next
+// product's operand as they stand (O^T = V^T P^T). A query and a weight are two fp16
+// terms (22 bits). The running maximum is a whole number (in units of log 2), so that
+// rescaling is exact and rare; weights stand 2^14 higher, which keeps their low terms
+// normal.
+//
+// So a weight is held to 2^-38 of the row's largest, which serves while value scales are
+// alike. A block with one that is not within 2^5 of the first block's is far: its values
+// are staged with their scales' exponents made the first block's, and its weights enter
+// the product times the difference, 2^shift; the running maximum is that of score + shift.
+// So no row loses bits to a key that weighs little but whose values are large, nor the
+// other way round.
 struct Kv4Run {
     const float *q;
     size_t q_stride;
     int group;
     float scale;  // of the scores, times log2 e
-    int max_positions;
-    float *out;
+    int max_positions, splits;
+    float *part_acc, *part_ml;
+    float *out;  // splits = 1: the rows themselves
     size_t out_stride;
     float *lse;  // [rows][query heads]: log2 of a row's sum of 2^score, or NULL
 };
 
-// A wave for each (row, query head): a key to a lane, then a dim to a lane.
 template <int D>
-__global__ __launch_bounds__(64) void k_kv4_attend(Kv4 kv, Kv4Rows rows, Kv4Run a, int *status) {
-    constexpr int N = D / kSpan;
-    __shared__ float q[D], w[kSpan][N];
-    const int qh = blockIdx.x, head = qh / a.group, s = blockIdx.z, lane = threadIdx.x;
+struct Kv4RunShared {
+    f16x8 k[2][4][D / 32][64];  // [buffer][block][step][lane]
+    f16x8 v[2][2][D / 16][64];  // [buffer][pair of blocks][16 dims][lane]
+    float shift[2][4][D / kSpan][kBlockPos];  // [buffer][block][64 dims][key], of far blocks
+    uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far
+};
+
+// The low halves of four bytes, numbers + 8 -> fp16 times scales: 0x6400 | n is 1024 + n.
+__device__ inline f16x4 halves_f16(uint32_t n, f16x2 s01, f16x2 s23) {
+    const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+    const uint32_t low = __builtin_amdgcn_perm(0x64646464u, n, 0x04010400u);
+    const uint32_t high = __builtin_amdgcn_perm(0x64646464u, n, 0x04030402u);
+    const f16x2 a = (__builtin_bit_cast(f16x2, low) + off) * s01;
+    const f16x2 b = (__builtin_bit_cast(f16x2, high) + off) * s23;
+    return f16x4{a.x, a.y, b.x, b.y};
+}
+
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Rows rows, Kv4Run a,
+                                                                  int *status) {
+    constexpr int N = D / kSpan, KS = D / 32, T = D / 16;
+    __shared__ Kv4RunShared<D> sh;
+    // Heads fastest (with 8 of them a head's keys stay in one XCD's L2), the longest rows
+    // first, and every second 256 work-groups the other way round: a CU, which gets each
+    // 256th, has long and short ones.
+    const int s = blockIdx.z, head = blockIdx.x % kv.heads, split = blockIdx.x / kv.heads;
+    const int plane = gridDim.x * gridDim.y;
+    int bx = gridDim.y - 1 - blockIdx.y;
+    if (plane <= 256) {
+        if ((int)((size_t)blockIdx.z * plane / 256) & 1) bx = blockIdx.y;
+    } else {
+        const int turn = max(1, 256 / (int)gridDim.x), lap = blockIdx.y / turn;
+        if (lap & 1)
+            bx = gridDim.y - min((lap + 1) * turn, (int)gridDim.y) + (blockIdx.y - lap * turn);
+    }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
     const Kv4Span span = kv4_span(rows, s, a.max_positions,
-                                  lane == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
-    if ((int)blockIdx.y >= span.count) return;
-    const size_t row = (size_t)span.row0 + blockIdx.y;
-    float *out = a.out + row * a.out_stride + (size_t)qh * D;
+                                  threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
+    const int tiles = (span.count + 15) / 16 * a.group;
+    if (bx * 4 >= tiles) return;
+    const int tile = bx * 4 + wave, r0 = tile / a.group * 16;
+    const int qh = head * a.group + tile % a.group, wide = kv.heads * a.group;
+    const int live = tile < tiles ? min(16, span.count - r0) : 0;  // rows of this wave
+    const size_t row = (size_t)(span.row0 + (live > 0 ? r0 + min(i, live - 1) : 0));
     if (!span.live) {
-        if (span.first < 0)
-            for (int n = 0; n < N; n++) out[n * 64 + lane] = 0.0f;
+        if (span.first < 0 && split == 0 && i < live) {
+            float *dst = a.out + row * a.out_stride + (size_t)qh * D;
+            for (int t = 0; t < T; t++)
+                *(float4 *)(dst + t * 16 + g * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         return;
     }
-    for (int n = 0; n < N; n++) q[n * 64 + lane] = a.q[row * a.q_stride + (size_t)qh * D + n * 64 + lane];
-    __syncthreads();
-    const int keys = span.first + (int)blockIdx.y + 1;
+    // Keys to be seen by some row here. Splits take the chunks of 64 in turn, so that each
+    // has its share of every row's.
+    const int keys = span.first +
+                     min(span.count, (min(bx * 4 + 3, tiles - 1) / a.group + 1) * 16);
+    const int c0 = split, stride = a.splits, c1 = (keys + 63) / 64;
+    const int p0 = span.first + r0, p = i < live ? p0 + i : -1;  // this lane's row
+    const int wave_top = p0 + live - 1;
+
+    // The wave's queries, two terms, scaled to a largest element in [2^14, 2^15).
+    const float *q = a.q + row * a.q_stride + (size_t)qh * D;
+    f16x8 qhi[KS], qlo[KS];
+    float qs, biggest = 0.0f;
+    {
+        float4 x[N][4];
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float4 v = *(const float4 *)(q + n * 64 + g * 16 + k * 4);
+                x[n][k] = v;
+                biggest = fmaxf(biggest, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
+                                               fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
+        biggest = xor16_32_max(biggest);
+        const int e = min(126, 141 - (int)(fbits(biggest) >> 23));
+        // The factor of the scores stays above 0, for a scale of 0 too.
+        const float mul = a.scale == 0.0f ? 0.0f : copysignf(power_of_2(e), a.scale);
+        qs = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * power_of_2(-e), 0x1p-126f);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                f16x2 h[4], o[4];
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const float4 v = x[n][k * 2 + z];
+                    split_pair(v.x * mul, v.y * mul, h[z * 2], o[z * 2]);
+                    split_pair(v.z * mul, v.w * mul, h[z * 2 + 1], o[z * 2 + 1]);
+                }
+                qhi[n * 2 + k] = join_pairs(h[0], h[1], h[2], h[3]);
+                qlo[n * 2 + k] = join_pairs(o[0], o[1], o[2], o[3]);
+            }
+    }
+
+    // Chunk c: its bytes requested, then turned into LDS; wave w takes block w. The block's
+    // id of the j-th chunk waits in lane j (j below 64, then the next 64): no chunk waits
+    // for its own. Lane (g, i): 16 dims of key i; keys 4 g .. 4 g + 3 of dims 16 t + i.
+    u32x2 kr[N];
+    uint32_t vr[T], ks[N];
+    u32x4 vs[N];
+    int raw_of = 0, raw = 0;
+    bool wild = false;
     const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
-    float m = kNone, l = 0.0f, acc[N];
-    for (int n = 0; n < N; n++) acc[n] = 0.0f;
-    bool any = false, wild = false;
-    for (int p0 = 0; p0 < keys; p0 += 64) {
-        const int p = p0 + lane;
-        const int id = p < keys ? table[p / kBlockPos] : 0;
-        const bool in = p < keys && (unsigned)id < kv.blocks;
-        wild |= p < keys && !in;
-        any |= __any(in);
-        float score = 0.0f, vs[N];
-        if (in) {
-            for (int n = 0; n < N; n++) {
-                const uint32_t *x = (const uint32_t *)(kv4_tile<D>(kv, id, head) + n * kPlane +
-                                                       p % kBlockPos * (kSpan / 2));
-                float dot = 0.0f;
-                for (int e = 0; e < 8; e++)
-                    for (int i = 0; i < 8; i++) dot = fmaf(nibble(x[e], i), q[n * 64 + e * 8 + i], dot);
-                const uint32_t pair = kv4_scales<D>(kv, id, head)[n * kBlockPos + p % kBlockPos];
-                score = fmaf(dot, key_scale(pair), score);
-                vs[n] = value_scale(pair);
-            }
-            score *= a.scale;
+    const int end = span.first + span.count;
+    // The exponent of the first block's largest value scale (of its first 64 dims).
+    constexpr int kNear = 5;
+    auto exponent = [](float x) { return max((int)(fbits(x) >> 23) - 127, -17); };
+    int usual = -17;
+    uint32_t least_near = 0, past_near = 0;  // scale pairs that are not far
+    auto look_first = [&] {
+        const int front = table[c0 * 4];
+        const float x = value_scale(kv4_scales<D>(kv, (unsigned)front < kv.blocks ? front : 0, head)[i]);
+        const bool in = c0 * 64 + i < end && x >= kLeastScale && x <= kMostScale;
+        usual = __builtin_amdgcn_readfirstlane(exponent(row16_max(in ? x : kLeastScale)));
+    };
+    auto request = [&](int c, int nth) {
+        const int j = nth & 63;
+        if (j == 0) {
+            const int at = c + lane * stride, b = at * 4 + wave;
+            // Past the keys: block 0's bytes, for keys that no row sees.
+            raw_of = at < c1 && b * kBlockPos < keys ? table[b] : 0;
+            wild |= (unsigned)raw_of >= kv.blocks;
         }
-        const float mx = fmaxf(m, wave_max(in ? score : kNone));
-        const float shrink = __builtin_amdgcn_exp2f(m - mx);
-        const float e = in ? __builtin_amdgcn_exp2f(score - mx) : 0.0f;
-        m = mx;
-        l = fmaf(l, shrink, wave_sum(e));
+        raw = __builtin_amdgcn_readlane(raw_of, j);
+        const unsigned id = (unsigned)raw < kv.blocks ? (unsigned)raw : 0u;
+        const uint8_t *tl = kv4_tile<D>(kv, id, head);
+        const uint32_t *sc = kv4_scales<D>(kv, id, head);
+#pragma unroll
         for (int n = 0; n < N; n++) {
-            w[lane][n] = in ? e * vs[n] : 0.0f;
-            acc[n] *= shrink;
+            kr[n] = *(const u32x2 *)(tl + n * kPlane + i * 32 + g * 8);
+            ks[n] = sc[n * kBlockPos + i];
+            vs[n] = *(const u32x4 *)(sc + n * kBlockPos + g * 4);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                vr[n * 4 + t] = *(const uint32_t *)(tl + (N + n) * kPlane + (t * 16 + i) * 8 + (g >> 1) * 4);
         }
-        __syncthreads();
-        for (int j = 0; j < 64 && p0 + j < keys; j++) {
-            const int b = __shfl(id, j);
-            if ((unsigned)b >= kv.blocks) continue;
-            const int i = j % kBlockPos;
-            for (int n = 0; n < N; n++) {
-                const uint32_t x = ((const uint32_t *)(kv4_tile<D>(kv, b, head) + (N + n) * kPlane))
-                    [lane * 2 + (i >> 3)];
-                acc[n] = fmaf(nibble(x, i & 7), w[j][n], acc[n]);
+    };
+    auto stage = [&](int buf, int c) {
+        // Scales order like their bits. Rows that nothing was written to do not count, nor
+        // those that were not finite.
+        uint32_t low = ~0u, high = 0;
+        auto range = [&](int count, uint32_t above) {
+            low = ~0u, high = 0;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const bool in = g * 4 + r < count && vs[n][r] <= above;
+                    low = min(low, in ? vs[n][r] : ~0u);
+                    high = max(high, in ? vs[n][r] : 0u);
+                }
+        };
+        if (c * 64 + wave * 16 + 16 <= end)
+            range(16, ~0u);
+        else
+            range(end - c * 64 - wave * 16, ~0u);
+        if (__any(high >= 0x7C000000u)) range(end - c * 64 - wave * 16, 0x7BFFFFFFu);
+        const bool far = __any(low < least_near || high >= past_near);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(ks[n], ks[n], 0x01000100u));
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t u = kr[n][k] ^ 0x88888888u;
+                const f16x4 x = halves_f16(u & 0x0F0F0F0Fu, s2, s2);
+                const f16x4 y = halves_f16(u >> 4 & 0x0F0F0F0Fu, s2, s2);
+                sh.k[buf][wave][n * 2 + k][lane] =
+                    __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            // Values of rows that nothing was written to, or that were not finite (the
+            // key's scale says so too), stay finite: no weight of theirs reaches a sum.
+            const f16x2 none = {(_Float16)0.0f, (_Float16)0.0f};
+            const f16x2 most = {(_Float16)kMostScale, (_Float16)kMostScale};
+            f16x2 s01 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vs[n][1], vs[n][0], 0x07060302u));
+            f16x2 s23 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vs[n][3], vs[n][2], 0x07060302u));
+            s01 = __builtin_elementwise_min(__builtin_elementwise_max(s01, none), most);
+            s23 = __builtin_elementwise_min(__builtin_elementwise_max(s23, none), most);
+            if (far) {
+                float x[4] = {(float)s01.x, (float)s01.y, (float)s23.x, (float)s23.y};
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int shift = x[r] >= kLeastScale ? exponent(x[r]) - usual : 0;
+                    x[r] = ldexpf(x[r], -shift);
+                    if (i == 0) sh.shift[buf][wave][n][g * 4 + r] = (float)shift;
+                }
+                s01 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+                s23 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const uint32_t u = (vr[n * 4 + t] >> (g & 1) * 4 & 0x0F0F0F0Fu) ^ 0x08080808u;
+                *((f16x4 *)&sh.v[buf][wave >> 1][n * 4 + t][lane] + (wave & 1)) = halves_f16(u, s01, s23);
             }
         }
+        if (lane == 0) sh.kind[buf][wave] = ((unsigned)raw >= kv.blocks ? 1 : 0) | (far ? 2 : 0);
+    };
+
+    float m = kNone, l = 0.0f;  // l: of this lane's keys
+    f32x4 acc[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto attend = [&](int buf, int c, bool masked) {
+        const uint32_t kind = (uint32_t)__builtin_amdgcn_readfirstlane(*(const int *)sh.kind[buf]);
+        f32x4 w[4];
+        // The last key that this lane's row sees, from its own first one on.
+        const int last = p - c * 64 - g * 4;
+#pragma unroll
+        for (int t = 0; t < 4; t++) w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            f16x8 kk[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) kk[t] = sh.k[buf][t][k][lane];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t], qhi[k], w[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t], qlo[k], w[t], 0, 0, 0);
+        }
+        if (masked)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (t * 16 + r > last) w[t][r] = -INFINITY;
+        if (kind & 0x01010101u)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                if (kind >> (8 * t) & 1) w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const bool far = (kind & 0x02020202u) != 0;
+        // NaN (a key that was not finite) does not count.
+        float mx[4], top;
+        if (far) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                mx[t] = kNone;
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+                    if (kind >> (8 * t) & 2) z = *(const f32x4 *)&sh.shift[buf][t][n][g * 4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float x = fmaf(w[t][r], qs, z[r]);
+                        mx[t] = max3(mx[t], x, x);
+                    }
+                }
+            }
+            top = quarters_max(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++) mx[t] = max3(max3(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
+            top = quarters_max(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
+        }
+        const float least = ceilf(top), mn = max3(m, least, least);
+        if (__any(mn != m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - mn);
+            l *= shrink;
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[t][r] *= shrink;
+            m = mn;
+        }
+        const float base = 14.0f - m;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
+                l += w[t][r];
+            }
+        f16x8 ph[2], pl[2];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            if (n == 0 || far) {
+                f16x2 hi[4][2], lo[4][2];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    f32x4 y = w[t];
+                    if (far && (kind >> (8 * t) & 2))
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            y[r] *= __builtin_amdgcn_exp2f(sh.shift[buf][t][n][g * 4 + r]);
+                    split_pair(y[0], y[1], hi[t][0], lo[t][0]);
+                    split_pair(y[2], y[3], hi[t][1], lo[t][1]);
+                }
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    ph[z] = join_pairs(hi[z * 2][0], hi[z * 2][1], hi[z * 2 + 1][0], hi[z * 2 + 1][1]);
+                    pl[z] = join_pairs(lo[z * 2][0], lo[z * 2][1], lo[z * 2 + 1][0], lo[z * 2 + 1][1]);
+                }
+            }
+            const int t0 = n * 4;
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                f16x8 v[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) v[t] = sh.v[buf][z][t0 + t][lane];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], ph[z],
+                                                                         acc[t0 + t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], pl[z],
+                                                                         acc[t0 + t], 0, 0, 0);
+            }
+        }
+    };
+
+    if (c0 < c1) {
+        request(c0, 0);
+        look_first();
+        least_near = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)power_of_2(max(usual - kNear, -17))) << 16;
+        past_near = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)power_of_2(min(usual + kNear + 1, 15))) << 16;
+        stage(0, c0);
         __syncthreads();
+        for (int c = c0, n = 0; c < c1; c += stride, n++) {
+            const int buf = n & 1;
+            const bool more = c + stride < c1;
+            if (more) request(c + stride, n + 1);
+            if (live > 0 && c * 64 <= wave_top)
+                attend(buf, c, c * 64 + 63 > p0 || live < 16);
+            if (more) stage(buf ^ 1, c + stride);
+            __syncthreads();
+        }
     }
     if (__any(wild) && lane == 0) atomicOr(status, 2);
-    // Scores that are all -inf do not come out finite; no keys come out as zeros.
-    if (any && l == 0.0f) l = __builtin_nanf("");
+    l = xor16_32_sum(l);
     bool bad = false;
-    for (int n = 0; n < N; n++) {
-        const float o = any ? acc[n] / l : 0.0f;
-        out[n * 64 + lane] = o;
-        bad |= !isfinite(o);
+    if (i < live) {
+        float base = m - 14.0f;
+        if (l == 0.0f) {
+            // No key of this split counts (zeros), or all scores are -inf (not finite).
+            bool any = false;
+            for (int c = c0; c * 64 <= p; c += stride)
+                for (int b = c * 4; b < c * 4 + 4 && b * kBlockPos <= p; b++)
+                    any |= (unsigned)table[b] < kv.blocks;
+            if (!any) base = -INFINITY;
+        }
+        const size_t at = (((size_t)s * rows.max_rows + r0 + i) * wide + qh) * a.splits + split;
+        float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
+        const float f = a.splits > 1 ? 1.0f : base == -INFINITY ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const float4 o = make_float4(acc[t][0] * f, acc[t][1] * f, acc[t][2] * f, acc[t][3] * f);
+            bad |= !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w));
+            *(float4 *)(dst + t * 16 + g * 4) = o;
+        }
+        if (g == 0) {
+            if (a.splits > 1)
+                *(float2 *)(a.part_ml + at * 2) = make_float2(base, l);
+            else if (a.lse)
+                a.lse[row * wide + qh] = base == -INFINITY ? INFINITY : base + __log2f(l);
+        }
+        bad |= !(biggest < INFINITY);
     }
-    if (a.lse && lane == 0) a.lse[row * gridDim.x + qh] = any ? m + log2f(l) : INFINITY;
     flag_nonfinite(status, bad);
 }
 
@@ -1102,10 +1408,25 @@ extern "C" int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer,
 
 namespace {
 
-// How an attention call of one row a stream deals its work: splits of `keys` keys.
+// How an attention call deals its work: splits of `keys` keys.
 struct Deal {
     int splits, keys, tiles, waves, steps;  // tiles: work-groups for a stream and head
 };
+
+Deal deal_rows(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group, int max_positions) {
+    // Work-groups without splits; where they are few, each row's keys are dealt out until
+    // there are about two for every CU, in chunks of 64 and as many at least to each as
+    // pay for the join.
+    Deal d = {};
+    d.tiles = ((r->max_rows + 15) / 16 * group + 3) / 4;
+    const size_t groups = (size_t)d.tiles * kv->heads * r->streams;
+    const int chunks = (max_positions - 1) / 64 + 1;
+    d.splits = groups >= 512 ? 1 : (int)(1024 / groups);
+    const int least = chunks <= 6 ? chunks : groups <= 64 ? 2 : chunks < 12 ? chunks : 4;
+    if (d.splits > chunks / least) d.splits = chunks / least;
+    if (d.splits > 32) d.splits = 32;
+    return d;
+}
 
 Deal deal_of(const pgpu_kv4 *kv, int streams, int group, int max_positions) {
     Deal d;
@@ -1134,6 +1455,25 @@ size_t parts_bytes(const pgpu_kv4 *kv, size_t parts) {
 }
 
 template <int D>
+int join(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
+         const float *part_acc, const float *part_ml, int group, int max_positions, float *out,
+         size_t out_stride, float *lse, int *status) {
+    // Many splits of few rows: a wave for each, spread over the CUs; else few splits of
+    // many rows.
+    const size_t items = (size_t)r.max_rows * c.heads * group;
+    if (d.splits >= 8 && items * streams <= 4096)
+        hipLaunchKernelGGL((k_kv4_join<D, 256 / D>), dim3((unsigned)items, 1, streams), dim3(64), 0,
+                           st, c, r, part_acc, part_ml, group, max_positions, d.splits, d.keys, out,
+                           out_stride, lse, status);
+    else
+        hipLaunchKernelGGL((k_kv4_join<D, 1>),
+                           dim3((unsigned)((items * (D / 4) + 255) / 256), 1, streams), dim3(256), 0,
+                           st, c, r, part_acc, part_ml, group, max_positions, d.splits, d.keys, out,
+                           out_stride, lse, status);
+    return launch_ok("pgpu_kv4_attention");
+}
+
+template <int D>
 int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
                const Kv4Decode &a, const pgpu_kv4_sums *sums, int *status) {
     Kv4Decode one = a;
@@ -1154,19 +1494,9 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
         KV4_DECODE(8, 4);
 #undef KV4_DECODE
     if (!launch_ok("pgpu_kv4_attention")) return 0;
-    if (d.splits > 1) {
-        const size_t items = (size_t)c.heads * a.group;
-        if (d.splits >= 8 && items * streams <= 4096)
-            hipLaunchKernelGGL((k_kv4_join<D, 256 / D>), dim3((unsigned)items, 1, streams), dim3(64),
-                               0, st, c, r, a.part_acc, a.part_ml, a.group, a.max_positions,
-                               d.splits, d.keys, a.out, a.out_stride, a.lse, status);
-        else
-            hipLaunchKernelGGL((k_kv4_join<D, 1>),
-                               dim3((unsigned)((items * (D / 4) + 255) / 256), 1, streams),
-                               dim3(256), 0, st, c, r, a.part_acc, a.part_ml, a.group,
-                               a.max_positions, d.splits, d.keys, a.out, a.out_stride, a.lse, status);
-        if (!launch_ok("pgpu_kv4_attention")) return 0;
-    }
+    if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
+                                 a.max_positions, a.out, a.out_stride, a.lse, status))
+        return 0;
     if (!sums) return 1;
     hipLaunchKernelGGL(k_kv4_sums_one, dim3((a.max_positions + 255) / 256, c.heads, streams),
                        dim3(256), 0, st, c, r, one, sums->before, sums->after, sums->stride, status);
@@ -1174,11 +1504,14 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
 }
 
 template <int D>
-int attend(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Kv4Run &a,
-           const pgpu_kv4_sums *sums, int *status) {
-    hipLaunchKernelGGL(k_kv4_attend<D>, dim3(c.heads * a.group, r.max_rows, streams), dim3(64), 0,
-                       st, c, r, a, status);
+int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
+                const Kv4Run &a, const pgpu_kv4_sums *sums, int *status) {
+    hipLaunchKernelGGL(k_kv4_run<D>, dim3(c.heads * d.splits, d.tiles, streams), dim3(256), 0, st, c,
+                       r, a, status);
     if (!launch_ok("pgpu_kv4_attention")) return 0;
+    if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
+                                 a.max_positions, a.out, a.out_stride, a.lse, status))
+        return 0;
     if (!sums) return 1;
     hipLaunchKernelGGL(k_kv4_sums<D>, dim3((a.max_positions + 255) / 256, c.heads, streams),
                        dim3(256), 0, st, c, r, a, sums->before, sums->after, sums->stride,
@@ -1192,11 +1525,21 @@ extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_ro
                                            int group, int max_positions, int with_sums) {
     if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
     const size_t wide = (size_t)kv->heads * group;
-    if (rows->offsets) return with_sums ? rows->rows * wide * sizeof(float) : 0;
+    if (rows->rows == 0) return 0;
+    size_t parts = 0;
+    if (rows->offsets) {
+        // Fewer rows or positions may be dealt to more work-groups. Splits times
+        // work-groups are at most 1024, a work-group has 64 rows.
+        const int chunks = (max_positions - 1) / 64 + 1;
+        const int most = std::min({32, chunks <= 6 ? 1 : chunks / 2,
+                                   1024 / (kv->heads * ((group + 3) / 4))});
+        if (most > 1)
+            parts = std::min((size_t)1024 * 64, rows->streams * rows->max_rows * wide * most);
+        return parts_bytes(kv, parts) + (with_sums ? rows->rows * wide * sizeof(float) : 0);
+    }
     // Fewer streams may be dealt to more work-groups: the streams before the numbers of
     // work-groups where the keys to each change count too. More positions never give
     // fewer parts.
-    size_t parts = 0;
     const int groups = kv->heads * (group == 1 ? 1 : (group + 3) / 4);
     for (int n : {rows->streams, 63 / groups, 191 / groups}) {
         if (n < 1 || n > rows->streams) continue;
@@ -1245,13 +1588,16 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
         return kv->head_dim == 64 ? attend_one<64>(st, c, r, rows->streams, d, a, sums, status)
                                   : attend_one<128>(st, c, r, rows->streams, d, a, sums, status);
     }
-    const size_t need = sums ? rows->rows * wide * sizeof(float) : 0;
+    const Deal d = deal_rows(kv, rows, group, max_positions);
+    const size_t parts = d.splits > 1 ? rows->streams * rows->max_rows * wide * d.splits : 0;
+    const size_t need = parts_bytes(kv, parts) + (sums ? rows->rows * wide * sizeof(float) : 0);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv4_attention (workspace)");
-    const Kv4Run a = {q,   q_stride,   group, scale * kLog2e, max_positions, out, out_stride,
-                      sums ? floats : nullptr};
-    return kv->head_dim == 64 ? attend<64>(st, c, r, rows->streams, a, sums, status)
-                              : attend<128>(st, c, r, rows->streams, a, sums, status);
+    const Kv4Run a = {q, q_stride, group, scale * kLog2e, max_positions, d.splits, floats,
+                      floats + parts * kv->head_dim, out, out_stride,
+                      sums ? floats + parts * (kv->head_dim + 2) : nullptr};
+    return kv->head_dim == 64 ? attend_rows<64>(st, c, r, rows->streams, d, a, sums, status)
+                              : attend_rows<128>(st, c, r, rows->streams, d, a, sums, status);
 }
 
 extern "C" int pgpu_kv4_evict(void *stream, const pgpu_kv4 *kv, int first_layer, int layers,
