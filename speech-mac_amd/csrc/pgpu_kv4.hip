@@ -740,6 +740,39 @@ __device__ inline f16x4 halves_f16(uint32_t n, f16x2 s01, f16x2 s23) {
     return f16x4{a.x, a.y, b.x, b.y};
 }
 
+// A wave's queries -> two fp16 terms of 64 dims a step pair, scaled to a largest element
+// in [2^14, 2^15), and the factor of the scores. x: [64 dims][quarter] of dims 16 g on.
+template <int D>
+__device__ inline float kv4_query(const float4 (&x)[D / kSpan][4], float scale, float &biggest,
+                                  f16x8 (&hi)[D / 32], f16x8 (&lo)[D / 32]) {
+    biggest = 0.0f;
+#pragma unroll
+    for (int n = 0; n < D / kSpan; n++)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            biggest = fmaxf(biggest, fmaxf(fmaxf(fabsf(x[n][k].x), fabsf(x[n][k].y)),
+                                           fmaxf(fabsf(x[n][k].z), fabsf(x[n][k].w))));
+    biggest = xor16_32_max(biggest);
+    const int e = min(126, 141 - (int)(fbits(biggest) >> 23));
+    // The factor of the scores stays above 0, for a scale of 0 too.
+    const float mul = scale == 0.0f ? 0.0f : copysignf(power_of_2(e), scale);
+#pragma unroll
+    for (int n = 0; n < D / kSpan; n++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            f16x2 h[4], o[4];
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                const float4 v = x[n][k * 2 + z];
+                split_pair(v.x * mul, v.y * mul, h[z * 2], o[z * 2]);
+                split_pair(v.z * mul, v.w * mul, h[z * 2 + 1], o[z * 2 + 1]);
+            }
+            hi[n * 2 + k] = join_pairs(h[0], h[1], h[2], h[3]);
+            lo[n * 2 + k] = join_pairs(o[0], o[1], o[2], o[3]);
+        }
+    return scale == 0.0f ? 1.0f : fmaxf(fabsf(scale) * power_of_2(-e), 0x1p-126f);
+}
+
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Rows rows, Kv4Run a,
                                                                   int *status) {
@@ -784,40 +817,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     const int p0 = span.first + r0, p = i < live ? p0 + i : -1;  // this lane's row
     const int wave_top = p0 + live - 1;
 
-    // The wave's queries, two terms, scaled to a largest element in [2^14, 2^15).
     const float *q = a.q + row * a.q_stride + (size_t)qh * D;
     f16x8 qhi[KS], qlo[KS];
-    float qs, biggest = 0.0f;
+    float qs, biggest;
     {
         float4 x[N][4];
 #pragma unroll
         for (int n = 0; n < N; n++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float4 v = *(const float4 *)(q + n * 64 + g * 16 + k * 4);
-                x[n][k] = v;
-                biggest = fmaxf(biggest, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)),
-                                               fmaxf(fabsf(v.z), fabsf(v.w))));
-            }
-        biggest = xor16_32_max(biggest);
-        const int e = min(126, 141 - (int)(fbits(biggest) >> 23));
-        // The factor of the scores stays above 0, for a scale of 0 too.
-        const float mul = a.scale == 0.0f ? 0.0f : copysignf(power_of_2(e), a.scale);
-        qs = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale) * power_of_2(-e), 0x1p-126f);
-#pragma unroll
-        for (int n = 0; n < N; n++)
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                f16x2 h[4], o[4];
-#pragma unroll
-                for (int z = 0; z < 2; z++) {
-                    const float4 v = x[n][k * 2 + z];
-                    split_pair(v.x * mul, v.y * mul, h[z * 2], o[z * 2]);
-                    split_pair(v.z * mul, v.w * mul, h[z * 2 + 1], o[z * 2 + 1]);
-                }
-                qhi[n * 2 + k] = join_pairs(h[0], h[1], h[2], h[3]);
-                qlo[n * 2 + k] = join_pairs(o[0], o[1], o[2], o[3]);
-            }
+            for (int k = 0; k < 4; k++) x[n][k] = *(const float4 *)(q + n * kSpan + g * 16 + k * 4);
+        qs = kv4_query<D>(x, a.scale, biggest, qhi, qlo);
     }
 
     // Chunk c: its bytes requested, then turned into LDS; wave w takes block w. The block's
@@ -1088,40 +1097,131 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     flag_nonfinite(status, bad);
 }
 
-// A thread for each key of a (stream, key head).
+// What runs of rows weigh, from their scores once more and the rows' log sums: a
+// work-group of 4 waves for 64 keys of a (stream, key head), which stand in each wave's
+// registers as fp16; the waves take the tiles of 16 rows that see them in turn. A lane
+// adds up its row's weights of 16 keys over the tiles; lanes and waves are added once.
 template <int D>
-__global__ __launch_bounds__(256) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
-                                                  const float *before, float *after,
-                                                  size_t stride, int counted, int *status) {
-    constexpr int N = D / kSpan;
-    const int head = blockIdx.y, s = blockIdx.z, p = blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
+                                                                   const float *before,
+                                                                   float *after, size_t stride,
+                                                                   int counted, int *status) {
+    constexpr int N = D / kSpan, KS = D / 32;
+    __shared__ float parts[4][64];
+    const int head = blockIdx.x % kv.heads, c = blockIdx.x / kv.heads, s = blockIdx.z;
+    const int wide = kv.heads * a.group;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
     const Kv4Span span = kv4_span(rows, s, a.max_positions, false, status);
-    if (!span.live || p >= span.first + span.count) return;
+    const int end = span.first + span.count;
+    if (!span.live || c * 64 >= end) return;
+    const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
+
+    int ids[4];
+    f16x8 kk[4][KS];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const int b = c * 4 + t;
+        ids[t] = b * kBlockPos < end ? uniform_load(table + b) : 0;
+        const unsigned id = (unsigned)ids[t] < kv.blocks ? (unsigned)ids[t] : 0u;
+        const uint8_t *tl = kv4_tile<D>(kv, id, head);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const u32x2 x = *(const u32x2 *)(tl + n * kPlane + i * 32 + g * 8);
+            const uint32_t pair = kv4_scales<D>(kv, id, head)[n * kBlockPos + i];
+            // A key that was not finite: no row that sees it counts.
+            const f16x2 none = {(_Float16)0.0f, (_Float16)0.0f};
+            const f16x2 most = {(_Float16)kMostScale, (_Float16)kMostScale};
+            f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pair, pair, 0x01000100u));
+            s2 = __builtin_elementwise_min(__builtin_elementwise_max(s2, none), most);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t u = x[k] ^ 0x88888888u;
+                kk[t][n * 2 + k] = __builtin_shufflevector(halves_f16(u & 0x0F0F0F0Fu, s2, s2),
+                                                           halves_f16(u >> 4 & 0x0F0F0F0Fu, s2, s2),
+                                                           0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        }
+    }
+
+    // Units: a tile of rows and a query head of the group.
+    const int from = max(max(0, span.count - counted), c * 64 - span.first);
+    const int units = (span.count - from + 15) / 16 * a.group;
+    float4 x[N][4];
+    float lse = INFINITY;
+    auto request = [&](int u) {
+        const int r = from + u / a.group * 16 + i, qh = head * a.group + u % a.group;
+        const size_t row = (size_t)span.row0 + min(r, span.count - 1);
+        const float *q = a.q + row * a.q_stride + (size_t)qh * D;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[n][k] = *(const float4 *)(q + n * kSpan + g * 16 + k * 4);
+        lse = a.lse[row * wide + qh];
+        if (r >= span.count) lse = INFINITY;
+    };
+    f32x4 part[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) part[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (wave < units) request(wave);
+    for (int u = wave; u < units; u += 4) {
+        const int p0 = span.first + from + u / a.group * 16;
+        // Rows that did not come out finite weigh nothing.
+        const bool fine = fabsf(lse) < INFINITY;
+        const float base = fine ? -lse : -INFINITY;
+        if (__any(!fine))
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (!fine) x[n][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        f16x8 qhi[KS], qlo[KS];
+        float biggest;
+        const float qs = kv4_query<D>(x, a.scale, biggest, qhi, qlo);
+        if (u + 4 < units) request(u + 4);
+        f32x4 w[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t][k], qhi[k], w[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t][k], qlo[k], w[t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
+        if (c * 64 + 63 > p0) {
+            const int last = p0 + i - c * 64 - g * 4;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (t * 16 + r > last) w[t][r] = 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) part[t] += w[t];
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float x16 = row16_sum(part[t][r]);
+            if (i == 0) parts[wave][t * 16 + g * 4 + r] = x16;
+        }
+    __syncthreads();
+    const int p = c * 64 + (int)threadIdx.x;
+    if (threadIdx.x >= 64 || p >= end) return;
     const size_t at = ((size_t)s * kv.heads + head) * stride + p;
     float sum = before && p < span.first ? before[at] : 0.0f;
-    const int id = rows.tables[(size_t)s * rows.table_stride + p / kBlockPos];
-    if ((unsigned)id < kv.blocks) {
-        const uint8_t *tile = kv4_tile<D>(kv, id, head);
-        float part = 0.0f;
-        for (int i = max(max(0, span.count - counted), p - span.first); i < span.count; i++)
-            for (int j = 0; j < a.group; j++) {
-                const int qh = head * a.group + j;
-                const size_t row = (size_t)span.row0 + i;
-                const float lse = a.lse[row * kv.heads * a.group + qh];
-                const float *q = a.q + row * a.q_stride + (size_t)qh * D;
-                float score = 0.0f;
-                for (int n = 0; n < N; n++) {
-                    const uint32_t *x = (const uint32_t *)(tile + n * kPlane + p % kBlockPos * (kSpan / 2));
-                    float dot = 0.0f;
-                    for (int e = 0; e < 8; e++)
-                        for (int z = 0; z < 8; z++)
-                            dot = fmaf(nibble(x[e], z), q[n * 64 + e * 8 + z], dot);
-                    score = fmaf(dot, key_scale(kv4_scales<D>(kv, id, head)[n * kBlockPos + p % kBlockPos]), score);
-                }
-                if (isfinite(lse)) part += __builtin_amdgcn_exp2f(score * a.scale - lse);
-            }
-        sum += part;
-    }
+    const int t = threadIdx.x >> 4, id = t < 2 ? (t ? ids[1] : ids[0]) : (t == 2 ? ids[2] : ids[3]);
+    if ((unsigned)id < kv.blocks)
+        sum += (parts[0][threadIdx.x] + parts[1][threadIdx.x]) +
+               (parts[2][threadIdx.x] + parts[3][threadIdx.x]);
     after[at] = sum;
 }
 
@@ -1513,8 +1613,8 @@ int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, con
                                  a.max_positions, a.out, a.out_stride, a.lse, status))
         return 0;
     if (!sums) return 1;
-    hipLaunchKernelGGL(k_kv4_sums<D>, dim3((a.max_positions + 255) / 256, c.heads, streams),
-                       dim3(256), 0, st, c, r, a, sums->before, sums->after, sums->stride,
+    hipLaunchKernelGGL(k_kv4_sums<D>, dim3(c.heads * (unsigned)((a.max_positions + 63) / 64), 1, streams), dim3(256),
+                       0, st, c, r, a, sums->before, sums->after, sums->stride,
                        sums->rows, status);
     return launch_ok("pgpu_kv4_attention");
 }
