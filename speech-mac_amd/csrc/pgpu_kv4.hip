@@ -336,8 +336,8 @@ struct Kv4DecodeShared {
 // A lone query's digits stand in rows 4 t .. 4 t + 3 for block t, zeros elsewhere, so
 // that lane (g, i) gets the score of key i of block g: one key to a lane. Of four
 // queries, lane (g, i) has query g's score of key i of each block.
-template <int D, int W, int Q>
-__global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv4_decode(Kv4 kv, Kv4Rows rows,
+template <int D, int W, int Q, bool SCORES>
+__global__ __launch_bounds__(64 * W, D == 64 ? 5 : 3) void k_kv4_decode(Kv4 kv, Kv4Rows rows,
                                                                         Kv4Decode a, int *status) {
     constexpr int N = D / kSpan, T = D / 16, S = Q == 1 ? 1 : 4;
     __shared__ Kv4DecodeShared<D, W, Q> sh;
@@ -365,6 +365,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv4_decode(Kv4 kv, 
     const int held = p / kBlockPos + 1;
     const size_t qh0 = (size_t)s * kv.heads * a.group + (size_t)head * a.group + j0;
 
+    const uint8_t *values_of = kv.values + head * (D * kBlockPos);
+    const uint32_t *scales_of = kv.scales + head * (N * kBlockPos);
+    const unsigned values_step = kv.heads * (D * kBlockPos), scales_step = kv.heads * (N * kBlockPos);
+    const unsigned key_at = i * 32 + g * 8, pair_at = i, value_at = N * kPlane + i * 8;
     u32x2 kr[4][N], vr[T];
     uint32_t pair[S][N];
     bool wild = false;
@@ -377,7 +381,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv4_decode(Kv4 kv, 
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             const bool there = b + t < held, in = (unsigned)ids[t] < kv.blocks;
-            id[t] = there && in ? (unsigned)ids[t] : 0u;
+            id[t] = (unsigned)__builtin_amdgcn_readfirstlane(there && in ? ids[t] : 0);
             if (!values) {
                 wild |= there && !in;
                 on |= (there && in ? 1u : 0u) << t;
@@ -386,21 +390,20 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv4_decode(Kv4 kv, 
         const unsigned mine = g < 2 ? (g ? id[1] : id[0]) : (g == 2 ? id[2] : id[3]);
         if (!values) {
 #pragma unroll
-            for (int n = 0; n < N; n++) {
+            for (int t = 0; t < 4; t++) {
+                const uint8_t *tile = values_of + (size_t)id[t] * values_step;
 #pragma unroll
-                for (int t = 0; t < 4; t++)
-                    kr[t][n] = stream_load8(kv4_tile<D>(kv, id[t], head) + n * kPlane + i * 32 + g * 8);
-                if constexpr (Q == 1)
-                    pair[0][n] = __builtin_nontemporal_load(kv4_scales<D>(kv, mine, head) +
-                                                            n * kBlockPos + i);
-                else
+                for (int n = 0; n < N; n++) kr[t][n] = stream_load8(tile + (key_at + n * kPlane));
+            }
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
-                        pair[t][n] = __builtin_nontemporal_load(kv4_scales<D>(kv, id[t], head) +
-                                                                n * kBlockPos + i);
+            for (int t = 0; t < S; t++) {
+                const uint32_t *pairs = scales_of + (size_t)(Q == 1 ? mine : id[t]) * scales_step;
+#pragma unroll
+                for (int n = 0; n < N; n++)
+                    pair[t][n] = __builtin_nontemporal_load(pairs + (pair_at + n * kBlockPos));
             }
         } else {
-            const uint8_t *tile = kv4_tile<D>(kv, mine, head) + N * kPlane + i * 8;
+            const uint8_t *tile = values_of + (size_t)mine * values_step + value_at;
 #pragma unroll
             for (int t = 0; t < T; t++) vr[t] = stream_load8(tile + t * 128);
         }
@@ -502,7 +505,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 6 : 4) void k_kv4_decode(Kv4 kv, 
                 large = fmaxf(large, vs[t][n]);
             }
             w[t] = seen ? score * step : -INFINITY;
-            if (a.scores && seen && (Q == 1 || g < live))
+            if (SCORES && seen && (Q == 1 || g < live))
                 a.scores[(qh0 + (Q == 1 ? 0 : g)) * a.max_positions + b * kBlockPos + i] = w[t];
             bound = fmaxf(bound, w[t] + (float)((int)(fbits(large) >> 23) - 126));
         }
@@ -1581,7 +1584,14 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
     if (d.splits > 1) one.out = nullptr;
     const dim3 grid(c.heads * d.tiles, d.splits, streams);
 #define KV4_DECODE(W, Q)                                                                        \
-    hipLaunchKernelGGL((k_kv4_decode<D, W, Q>), grid, dim3(64 * W), 0, st, c, r, one, status)
+    do {                                                                                        \
+        if (sums)                                                                               \
+            hipLaunchKernelGGL((k_kv4_decode<D, W, Q, true>), grid, dim3(64 * W), 0, st, c, r,  \
+                               one, status);                                                    \
+        else                                                                                    \
+            hipLaunchKernelGGL((k_kv4_decode<D, W, Q, false>), grid, dim3(64 * W), 0, st, c, r, \
+                               one, status);                                                    \
+    } while (0)
     if (a.group == 1 && d.waves == 4)
         KV4_DECODE(4, 1);
     else if (a.group == 1 && d.waves == 8)
