@@ -298,8 +298,8 @@ __device__ inline u32x2 stream_load8(const uint8_t *p) {
 }
 
 template <int E>
-__device__ inline int row_shift_left(int v) {  // lane i of 16 gets lane i + E's
-    return __builtin_amdgcn_update_dpp(0, v, 0x100 + E, 0xf, 0xf, true);
+__device__ inline int row_turn(int v) {  // lane i of 16 gets lane (i + E) % 16's
+    return __builtin_amdgcn_update_dpp(0, v, 0x120 + 16 - E, 0xf, 0xf, false);
 }
 
 struct Kv4Decode {
@@ -337,13 +337,15 @@ struct Kv4DecodeShared {
 // that lane (g, i) gets the score of key i of block g: one key to a lane. Of four
 // queries, lane (g, i) has query g's score of key i of each block.
 template <int D, int W, int Q, bool SCORES>
-__global__ __launch_bounds__(64 * W, D == 64 ? 5 : 3) void k_kv4_decode(Kv4 kv, Kv4Rows rows,
-                                                                        Kv4Decode a, int *status) {
-    constexpr int N = D / kSpan, T = D / 16, S = Q == 1 ? 1 : 4;
+__global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_decode(
+    Kv4 kv, Kv4Rows rows, Kv4Decode a, int *status) {
+    constexpr int N = D / kSpan, T = D / 16, S = Q == 1 ? 1 : 4, A = Q == 1 ? N : T;
     __shared__ Kv4DecodeShared<D, W, Q> sh;
     // Heads vary fastest: with 8 of them a head's passes stay on one XCD.
     const int head = blockIdx.x % kv.heads, j0 = blockIdx.x / kv.heads * Q;
-    const int split = blockIdx.y, s = blockIdx.z;
+    // The splits in turn by stream: the first ones, which all contexts have, would else be
+    // dispatched to the same CUs where their number divides 32.
+    const int s = blockIdx.z, split = (blockIdx.y + s) % gridDim.y;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
     int b0 = (split * a.steps * W + wave) * 4;  // the wave's blocks: b0 .. b0 + 3
@@ -456,14 +458,14 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : 3) void k_kv4_decode(Kv4 kv, 
         step = top < INFINITY ? a.scale * power_of_2(-e) * 0.0625f : __builtin_nanf("");
         if (Q != 1) step = __shfl(step, g * 4);  // of query j0 + g
     };
-    float m = kNone, l = 0.0f, acc[T];
-    i32x4 sum[T];  // whole sums of the values, of dims 16 t + i, times 2^(34 - m)
+    float m = kNone, l = 0.0f, acc[A];
+    i32x4 sum[A];  // whole sums of the values, times 2^(34 - m): of dims 16 t + i, or 64 t + lane
     int flushed = 0;
 #pragma unroll
-    for (int t = 0; t < T; t++) acc[t] = 0.0f, sum[t] = i32x4{0, 0, 0, 0};
+    for (int t = 0; t < A; t++) acc[t] = 0.0f, sum[t] = i32x4{0, 0, 0, 0};
     auto flush = [&](float less) {
 #pragma unroll
-        for (int t = 0; t < T; t++) {
+        for (int t = 0; t < A; t++) {
             const float whole = fmaf((float)sum[t].x, 0x1p24f, fmaf((float)sum[t].y, 0x1p16f,
                                      fmaf((float)sum[t].z, 0x1p8f, (float)sum[t].w)));
             acc[t] = fmaf(whole, 0x1p-34f, acc[t]) * less;
@@ -527,14 +529,20 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : 3) void k_kv4_decode(Kv4 kv, 
         }
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            i32x4 pd;
             if constexpr (Q == 1) {
-                // Row t < 4: digit t of block g's keys, a quad of keys a word.
+                // Digit t of block g's keys, a quad of keys a word, in row t of dims 16 j ..
+                // 16 j + 15, which are rows 4 j .. 4 j + 3: their first word is quad j's.
                 const uint32_t u = fix_bytes(w[0] * vs[0][n], 0x1p30f);
                 const int word = (int)pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u),
                                             quad_lane<3>(u), sel);
-                pd = i32x4{word, row_shift_left<4>(word), row_shift_left<8>(word),
-                           row_shift_left<12>(word)};
+                const i32x4 turned = {word, row_turn<4>(word), row_turn<8>(word), row_turn<12>(word)};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const i32x4 x = unpack16(vr[n * 4 + j]);
+                    sum[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                        i >> 2 == j ? turned : i32x4{0, 0, 0, 0},
+                        i32x4{x[j], x[(j + 1) & 3], x[(j + 2) & 3], x[(j + 3) & 3]}, sum[n], 0, 0, 0);
+                }
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -543,12 +551,12 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : 3) void k_kv4_decode(Kv4 kv, 
                         pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u), quad_lane<3>(u), sel);
                 }
                 wave_lds_fence();
-                pd = *(const i32x4 *)&sh.digits[wave][i][g * 4];
+                const i32x4 pd = *(const i32x4 *)&sh.digits[wave][i][g * 4];
                 wave_lds_fence();
-            }
 #pragma unroll
-            for (int t = n * 4; t < n * 4 + 4; t++)
-                sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd, unpack16(vr[t]), sum[t], 0, 0, 0);
+                for (int t = n * 4; t < n * 4 + 4; t++)
+                    sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd, unpack16(vr[t]), sum[t], 0, 0, 0);
+            }
         }
         b0 += 4 * W;
         if (more) load(b0, true);
@@ -564,13 +572,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : 3) void k_kv4_decode(Kv4 kv, 
     if (wild && lane == 0) atomicOr(status, 2);
     l = row16_sum(l);
     if (Q == 1) l = xor16_32_sum(l);
-    if (g < Q) {
 #pragma unroll
-        for (int t = 0; t < T; t++) sh.acc[wave][g][t * 16 + i] = acc[t];
-        if (i == 0) {
-            sh.m[wave][g] = ever ? m : -INFINITY;
-            sh.l[wave][g] = l;
-        }
+    for (int t = 0; t < A; t++) sh.acc[wave][Q == 1 ? 0 : g][Q == 1 ? t * 64 + lane : t * 16 + i] = acc[t];
+    if (g < Q && i == 0) {
+        sh.m[wave][g] = ever ? m : -INFINITY;
+        sh.l[wave][g] = l;
     }
     bool bad = !(top < INFINITY);
     __syncthreads();
@@ -1534,17 +1540,33 @@ Deal deal_rows(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group, int max_po
 Deal deal_of(const pgpu_kv4 *kv, int streams, int group, int max_positions) {
     Deal d;
     // A stream's keys whole in one work-group of W waves (no parts to be joined), except
-    // where few work-groups have many keys each: those are dealt to work-groups of 4
-    // waves, more keys to each the more of them there are.
+    // where few work-groups have many keys each, or contexts are long enough to differ
+    // much: those are dealt to work-groups of 4 waves, in steps of W * 64 keys, more to
+    // each the more of them there are.
+    // us, 8 heads (contexts of one stream as said, of several up to that), whole / dealt
+    // with the steps taken here. Heads of 64: 1 stream of 2048 keys 7.5 / 10.1, of 8187
+    // 16.8 / 10.1; 16 of 4096 10.6 / 11.1, of 8187 17.4 / 13.0; 32 of 4096 11.2 / 14.6, of
+    // 8187 18.9 / 19.2; 64 of 4096 18.8 / 20.5, of 6000 22.6 / 23.7, of 8187 34.0 / 28.8;
+    // 256 of 8187 101.2 / 98.5; 4 queries each: 4 of 4096 13.8 / 10.2, 16 of 2900 11.4 /
+    // 11.5, of 8187 23.4 / 15.5, 64 of 8187 34.9 / 33.2. Heads of 128: 1 of 2048 9.7 / 10.2,
+    // 16 of 8187 29.8 / 19.4, 48 of 4096 29.7 / 24.5, 128 54.2 / 51.3; 4 queries each: 1 of
+    // 2048 12.5 / 10.0, 16 of 2900 16.4 / 15.5, 48 of 4096 34.0 / 28.9, 64 of 2048 21.5 / 31.
+    // Steps of a dealt work-group, 1 / 2 / 3 / 4 / 5: heads of 64, 16 of 8187 15.4 / 13.0 /
+    // 14.4 / 14.7 / 14.0, 64 38.7 / 29.6 / 29.0 / 28.8 / 28.9; heads of 128 with 4 queries,
+    // 4 of 4096 11.2 / 10.9 / 12.3 / 13.7 / 14.9, 16 of 2900 17.0 / 16.2 / 15.5 / 17.3 / 19.0,
+    // 48 of 4096 38.2 / 31.0 / 30.6 / 30.7 / 28.9.
+    // W = 4 / 8: heads of 64, 64 streams of 2048 11.1 / 11.4, of 6000 23.9 / 22.6, 128 of
+    // 2048 18.3 / 19.3, with 4 queries 64 of 2048 14.1 / 13.5; heads of 128, 64 of 600 8.6 /
+    // 9.9, with 4 queries 10.9 / 13.7. (W = 16: 1 of 2048 7.5, 64 of 2048 13.9.)
     d.tiles = group == 1 ? 1 : (group + 3) / 4;
     const size_t groups = (size_t)kv->heads * d.tiles * streams;
     const int units = (max_positions - 1) / 64 + 1;
-    const bool wide = kv->head_dim != 64;
-    d.waves = groups > 768 ? (units > 36 ? 8 : 4) : groups > 256 || group > 1 || wide ? 8 : 16;
+    const bool wide = kv->head_dim != 64, four = group > 1, both = wide && four;
+    d.waves = groups >= 512 && units <= 64 && (wide || !four) ? 4 : 8;
     d.steps = (units + d.waves - 1) / d.waves;
-    if (units > (groups < 192 ? 3 * d.waves : wide ? 48 : 80)) {
+    if (units > (groups >= 192 ? (wide ? 48 : 96) : both ? 24 : wide || four ? 48 : 64)) {
         d.waves = 4;
-        d.steps = groups < 64 ? 1 : groups < 192 ? (wide ? 1 : 2) : 3;
+        d.steps = groups < 64 ? 1 : groups < 192 ? (both ? 3 : 2) : both ? 5 : 4;
     }
     d.keys = 64 * d.waves * d.steps;
     d.splits = (max_positions - 1) / d.keys + 1;
@@ -1594,11 +1616,9 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
     } while (0)
     if (a.group == 1 && d.waves == 4)
         KV4_DECODE(4, 1);
-    else if (a.group == 1 && d.waves == 8)
+    else if (a.group == 1)
         KV4_DECODE(8, 1);
-    else if (a.group == 1) {
-        if constexpr (D == 64) KV4_DECODE(16, 1);
-    } else if (d.waves == 4)
+    else if (d.waves == 4)
         KV4_DECODE(4, 4);
     else
         KV4_DECODE(8, 4);
