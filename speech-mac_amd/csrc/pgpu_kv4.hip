@@ -312,15 +312,19 @@ struct Kv4Decode {
     float *part_acc, *part_ml;
     float *out;  // splits = 1: the rows themselves (else NULL)
     size_t out_stride;
-    float *lse;  // [streams][query heads]: log2 of the sum of 2^score, or NULL
-    float *scores;  // [streams][query heads][max_positions], in units of log 2, or NULL
+    // With sums:
+    float *lse;  // [streams][query heads]: log2 of the sum of 2^score
+    float *scores;  // [streams][query heads][max_positions], in units of log 2
+    const float *before;
+    float *after;  // NULL: another launch adds the weights up
+    size_t stride;
 };
 
 template <int D, int W, int Q>
 struct Kv4DecodeShared {
     __align__(16) uint32_t digits[Q == 1 ? 1 : W][16][16];  // [row][block, quad of keys]
     float acc[W][Q][D];
-    float m[W][Q], l[W][Q];
+    float m[W][Q], l[W][Q], lse[Q];
 };
 
 // One row a stream. A work-group of W waves takes a split's keys of one (stream, key
@@ -507,7 +511,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
                 large = fmaxf(large, vs[t][n]);
             }
             w[t] = seen ? score * step : -INFINITY;
-            if (SCORES && seen && (Q == 1 || g < live))
+            if (SCORES && b * kBlockPos + i <= p && (Q == 1 || g < live))
                 a.scores[(qh0 + (Q == 1 ? 0 : g)) * a.max_positions + b * kBlockPos + i] = w[t];
             bound = fmaxf(bound, w[t] + (float)((int)(fbits(large) >> 23) - 126));
         }
@@ -597,7 +601,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
             // Scores that are all -inf: not finite. No key: zeros.
             o = mx == -INFINITY ? 0.0f : o / total;
             a.out[(size_t)s * a.out_stride + ((size_t)head * a.group + j0 + j) * D + d] = o;
-            if (a.lse && d == 0) a.lse[qh0 + j] = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+            if (SCORES && d == 0) {
+                const float lse = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+                a.lse[qh0 + j] = sh.lse[j] = lse;
+            }
             bad |= !isfinite(o);
         } else {
             const size_t at = (qh0 + j) * a.splits + split;
@@ -606,6 +613,20 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         }
     }
     flag_nonfinite(status, bad);
+    if (!SCORES || !a.after) return;
+    __syncthreads();
+    for (int e = threadIdx.x; e <= p; e += 64 * W) {
+        float part[Q];
+#pragma unroll
+        for (int j = 0; j < Q; j++)
+            part[j] = j < live ? a.scores[(qh0 + j) * a.max_positions + e] : -INFINITY;
+        const size_t at = ((size_t)s * kv.heads + head) * a.stride + e;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < Q; j++)
+            if (j < live && isfinite(sh.lse[j])) sum += __builtin_amdgcn_exp2f(part[j] - sh.lse[j]);
+        a.after[at] = (a.before && e < p ? a.before[at] : 0.0f) + sum;
+    }
 }
 
 // The splits of a row's query head joined: D / 4 lanes for 4 dims each, times G that
@@ -683,24 +704,18 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const fl
 // One row a stream's weights, from its scores: a thread for each key of a (stream, key
 // head).
 __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4Decode a,
-                                                      const float *before, float *after,
-                                                      size_t stride, int *status) {
+                                                      int *status) {
     const int head = blockIdx.y, s = blockIdx.z, p = blockIdx.x * 256 + threadIdx.x;
     const Kv4Span span = kv4_span(rows, s, a.max_positions, false, status);
     if (!span.live || p > span.first) return;
-    const size_t at = ((size_t)s * kv.heads + head) * stride + p;
-    float sum = before && p < span.first ? before[at] : 0.0f;
-    const int id = rows.tables[(size_t)s * rows.table_stride + p / kBlockPos];
-    if ((unsigned)id < kv.blocks) {
-        const size_t qh0 = ((size_t)s * kv.heads + head) * a.group;
-        float part = 0.0f;
-        for (int j = 0; j < a.group; j++) {
-            const float lse = a.lse[qh0 + j], score = a.scores[(qh0 + j) * a.max_positions + p];
-            if (isfinite(lse)) part += __builtin_amdgcn_exp2f(score - lse);
-        }
-        sum += part;
+    const size_t at = ((size_t)s * kv.heads + head) * a.stride + p;
+    const size_t qh0 = ((size_t)s * kv.heads + head) * a.group;
+    float sum = 0.0f;
+    for (int j = 0; j < a.group; j++) {
+        const float lse = a.lse[qh0 + j], score = a.scores[(qh0 + j) * a.max_positions + p];
+        if (isfinite(lse)) sum += __builtin_amdgcn_exp2f(score - lse);
     }
-    after[at] = sum;
+    a.after[at] = (a.before && p < span.first ? a.before[at] : 0.0f) + sum;
 }
 
 // Runs of rows: a work-group of 4 waves takes 4 tiles of 16 rows of one query head each
@@ -1604,6 +1619,8 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
     Kv4Decode one = a;
     one.steps = d.steps;
     if (d.splits > 1) one.out = nullptr;
+    // The weights are added up where a work-group has all of a key's.
+    if (sums && d.splits == 1 && d.tiles == 1) one.after = sums->after;
     const dim3 grid(c.heads * d.tiles, d.splits, streams);
 #define KV4_DECODE(W, Q)                                                                        \
     do {                                                                                        \
@@ -1627,9 +1644,10 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
     if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
                                  a.max_positions, a.out, a.out_stride, a.lse, status))
         return 0;
-    if (!sums) return 1;
+    if (!sums || one.after) return 1;
+    one.after = sums->after;
     hipLaunchKernelGGL(k_kv4_sums_one, dim3((a.max_positions + 255) / 256, c.heads, streams),
-                       dim3(256), 0, st, c, r, one, sums->before, sums->after, sums->stride, status);
+                       dim3(256), 0, st, c, r, one, status);
     return launch_ok("pgpu_kv4_attention");
 }
 
@@ -1709,11 +1727,22 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
                                   : 0);
         if (need && (!work || !aligned(work, 16) || work_bytes < need))
             return bad_arguments("pgpu_kv4_attention (workspace)");
-        Kv4Decode a = {q, q_stride, group, scale * kLog2e, max_positions, d.splits, 1,
-                       floats, floats + parts * kv->head_dim, out, out_stride, nullptr, nullptr};
+        Kv4Decode a = {};
+        a.q = q;
+        a.q_stride = q_stride;
+        a.group = group;
+        a.scale = scale * kLog2e;
+        a.max_positions = max_positions;
+        a.splits = d.splits;
+        a.part_acc = floats;
+        a.part_ml = floats + parts * kv->head_dim;
+        a.out = out;
+        a.out_stride = out_stride;
         if (sums) {
             a.lse = floats + parts * (kv->head_dim + 2);
             a.scores = a.lse + rows->streams * wide;
+            a.before = sums->before;
+            a.stride = sums->stride;
         }
         return kv->head_dim == 64 ? attend_one<64>(st, c, r, rows->streams, d, a, sums, status)
                                   : attend_one<128>(st, c, r, rows->streams, d, a, sums, status);
