@@ -754,15 +754,38 @@ struct Kv4RunShared {
     uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far
 };
 
-// The low halves of four bytes, numbers + 8 -> fp16 times scales: 0x6400 | n is 1024 + n.
-__device__ inline f16x4 halves_f16(uint32_t n, f16x2 s01, f16x2 s23) {
+// Numbers of the cache become fp16 two at a time, numbers b and b + 2 of a word's halves:
+// eight in the order 0, 2, 4, 6, 1, 3, 5, 7, four in the order 0, 2, 1, 3, which the other
+// operands keep to.
+//
+// Four in the low halves of bytes, plus 8, times their scales: 0x6400 | n is 1024 + n.
+__device__ inline f16x4 halves_f16(uint32_t n, f16x2 s02, f16x2 s13) {
     const f16x2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    const uint32_t low = __builtin_amdgcn_perm(0x64646464u, n, 0x04010400u);
-    const uint32_t high = __builtin_amdgcn_perm(0x64646464u, n, 0x04030402u);
-    const f16x2 a = (__builtin_bit_cast(f16x2, low) + off) * s01;
-    const f16x2 b = (__builtin_bit_cast(f16x2, high) + off) * s23;
+    const uint32_t even = __builtin_amdgcn_perm(0x64646464u, n, 0x04020400u);
+    const uint32_t odd = __builtin_amdgcn_perm(0x64646464u, n, 0x04030401u);
+    const f16x2 a = (__builtin_bit_cast(f16x2, even) + off) * s02;
+    const f16x2 b = (__builtin_bit_cast(f16x2, odd) + off) * s13;
     return f16x4{a.x, a.y, b.x, b.y};
 }
+__device__ inline f16x8 word_f16(uint32_t w, f16x2 s2) {
+    const uint32_t u = w ^ 0x88888888u;
+    return __builtin_shufflevector(halves_f16(u & 0x0F0F0F0Fu, s2, s2),
+                                   halves_f16(u >> 4 & 0x0F0F0F0Fu, s2, s2), 0, 1, 4, 5, 2, 3, 6, 7);
+}
+// The same in one multiply-add: a number plus 8 in bits 6 .. 9 (and 22 .. 25) of `shifted`
+// is 1 + n / 16 with an exponent before it; times 16 s, less 24 s, which is exact, as
+// long as 24 s is an fp16 number.
+constexpr uint16_t kMostFast = 0x6950;  // 2720
+struct PairBits {
+    uint32_t mask = 0x03C003C0u, one = 0x3C003C00u;
+    // In registers: an AND-OR takes no literals.
+    __device__ PairBits() { asm("" : "+s"(mask), "+v"(one)); }
+};
+__device__ inline f16x2 pair_f16(uint32_t shifted, f16x2 s16, f16x2 s24, const PairBits &b) {
+    return __builtin_elementwise_fma(
+        __builtin_bit_cast(f16x2, (shifted & b.mask) | b.one), s16, -s24);
+}
+__device__ inline f16x2 times(f16x2 s, float f) { return s * f16x2{(_Float16)f, (_Float16)f}; }
 
 // A wave's queries -> two fp16 terms of 64 dims a step pair, scaled to a largest element
 // in [2^14, 2^15), and the factor of the scores. x: [64 dims][quarter] of dims 16 g on.
@@ -788,13 +811,18 @@ __device__ inline float kv4_query(const float4 (&x)[D / kSpan][4], float scale, 
 #pragma unroll
             for (int z = 0; z < 2; z++) {
                 const float4 v = x[n][k * 2 + z];
-                split_pair(v.x * mul, v.y * mul, h[z * 2], o[z * 2]);
-                split_pair(v.z * mul, v.w * mul, h[z * 2 + 1], o[z * 2 + 1]);
+                split_pair(v.x * mul, v.z * mul, h[z], o[z]);
+                split_pair(v.y * mul, v.w * mul, h[z + 2], o[z + 2]);
             }
             hi[n * 2 + k] = join_pairs(h[0], h[1], h[2], h[3]);
             lo[n * 2 + k] = join_pairs(o[0], o[1], o[2], o[3]);
         }
     return scale == 0.0f ? 1.0f : fmaxf(fabsf(scale) * power_of_2(-e), 0x1p-126f);
+}
+
+// NaN if one is NaN. (No asm: what it reads may come from a matrix instruction.)
+__device__ inline float largest(float a, float b, float c) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 template <int D>
@@ -856,6 +884,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     // Chunk c: its bytes requested, then turned into LDS; wave w takes block w. The block's
     // id of the j-th chunk waits in lane j (j below 64, then the next 64): no chunk waits
     // for its own. Lane (g, i): 16 dims of key i; keys 4 g .. 4 g + 3 of dims 16 t + i.
+    const unsigned key_at = i * 32 + g * 8, value_at = N * kPlane + i * 8 + (g >> 1) * 4;
+    const unsigned scale_at = i, scales_at = g * 4;
     u32x2 kr[N];
     uint32_t vr[T], ks[N];
     u32x4 vs[N];
@@ -867,7 +897,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     constexpr int kNear = 5;
     auto exponent = [](float x) { return max((int)(fbits(x) >> 23) - 127, -17); };
     int usual = -17;
-    uint32_t least_near = 0, past_near = 0;  // scale pairs that are not far
+    uint32_t least_near = 0, range_near = 0;  // scale pairs that are not far
     auto look_first = [&] {
         const int front = table[c0 * 4];
         const float x = value_scale(kv4_scales<D>(kv, (unsigned)front < kv.blocks ? front : 0, head)[i]);
@@ -888,76 +918,94 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         const uint32_t *sc = kv4_scales<D>(kv, id, head);
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            kr[n] = *(const u32x2 *)(tl + n * kPlane + i * 32 + g * 8);
-            ks[n] = sc[n * kBlockPos + i];
-            vs[n] = *(const u32x4 *)(sc + n * kBlockPos + g * 4);
+            kr[n] = *(const u32x2 *)(tl + (key_at + n * kPlane));
+            ks[n] = sc[scale_at + n * kBlockPos];
+            vs[n] = *(const u32x4 *)(sc + (scales_at + n * kBlockPos));
 #pragma unroll
             for (int t = 0; t < 4; t++)
-                vr[n * 4 + t] = *(const uint32_t *)(tl + (N + n) * kPlane + (t * 16 + i) * 8 + (g >> 1) * 4);
+                vr[n * 4 + t] = *(const uint32_t *)(tl + (value_at + n * kPlane + t * 128));
         }
     };
     auto stage = [&](int buf, int c) {
-        // Scales order like their bits. Rows that nothing was written to do not count, nor
-        // those that were not finite.
-        uint32_t low = ~0u, high = 0;
-        auto range = [&](int count, uint32_t above) {
-            low = ~0u, high = 0;
+        // Most blocks are full, and have value scales that are not far and key scales that
+        // pair_f16 takes. Scales order like their bits.
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+            odd |= ks[n] - least_near >= range_near || (uint16_t)ks[n] > kMostFast;
+        odd = c * 64 + wave * 16 + 16 > end || __any(odd);
+        uint32_t kind = (unsigned)raw >= kv.blocks ? 1 : 0;
+        if (!odd) {
+            const PairBits bits;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(ks[n], ks[n], 0x01000100u));
+                const f16x2 k16 = times(s2, 16.0f), k24 = times(s2, 24.0f);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t u = kr[n][k] ^ 0x88888888u;
+                    sh.k[buf][wave][n * 2 + k][lane] =
+                        join_pairs(pair_f16(u << 6, k16, k24, bits), pair_f16(u << 2, k16, k24, bits),
+                                   pair_f16(u >> 2, k16, k24, bits), pair_f16(u >> 6, k16, k24, bits));
+                }
+                const f16x2 s02 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vs[n][2], vs[n][0], 0x07060302u));
+                const f16x2 s13 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vs[n][3], vs[n][1], 0x07060302u));
+                const f16x2 a16 = times(s02, 16.0f), a24 = times(s02, 24.0f);
+                const f16x2 b16 = times(s13, 16.0f), b24 = times(s13, 24.0f);
+                const int left = g & 1 ? 2 : 6, right = g & 1 ? 6 : 2;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const uint32_t u = vr[n * 4 + t] ^ 0x88888888u;
+                    const f16x2 a = pair_f16(u << left, a16, a24, bits),
+                                b = pair_f16(u >> right, b16, b24, bits);
+                    *((f16x4 *)&sh.v[buf][wave >> 1][n * 4 + t][lane] + (wave & 1)) =
+                        f16x4{a.x, a.y, b.x, b.y};
+                }
+            }
+        } else {
+            // Rows that nothing was written to, or that were not finite, are not far.
+            bool far = false;
 #pragma unroll
             for (int n = 0; n < N; n++)
+                far |= c * 64 + wave * 16 + i < end && ks[n] < 0x7C000000u &&
+                       ks[n] - least_near >= range_near;
+            far = __any(far);
+            if (far) kind |= 2;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                const f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(ks[n], ks[n], 0x01000100u));
+#pragma unroll
+                for (int k = 0; k < 2; k++) sh.k[buf][wave][n * 2 + k][lane] = word_f16(kr[n][k], s2);
+                // Their values stay finite (the key's scale says if they were not): no
+                // weight of theirs reaches a sum.
+                float x[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const bool in = g * 4 + r < count && vs[n][r] <= above;
-                    low = min(low, in ? vs[n][r] : ~0u);
-                    high = max(high, in ? vs[n][r] : 0u);
+                    x[r] = value_scale(vs[n][r]);
+                    if (!(x[r] <= kMostScale) || x[r] < 0.0f) x[r] = 0.0f;
+                    if (far) {
+                        const int shift = x[r] >= kLeastScale ? exponent(x[r]) - usual : 0;
+                        x[r] = ldexpf(x[r], -shift);
+                        if (i == 0) sh.shift[buf][wave][n][g * 4 + r] = (float)shift;
+                    }
                 }
-        };
-        if (c * 64 + wave * 16 + 16 <= end)
-            range(16, ~0u);
-        else
-            range(end - c * 64 - wave * 16, ~0u);
-        if (__any(high >= 0x7C000000u)) range(end - c * 64 - wave * 16, 0x7BFFFFFFu);
-        const bool far = __any(low < least_near || high >= past_near);
+                const f16x2 s02 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[0], x[2]));
+                const f16x2 s13 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[1], x[3]));
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(ks[n], ks[n], 0x01000100u));
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const uint32_t u = kr[n][k] ^ 0x88888888u;
-                const f16x4 x = halves_f16(u & 0x0F0F0F0Fu, s2, s2);
-                const f16x4 y = halves_f16(u >> 4 & 0x0F0F0F0Fu, s2, s2);
-                sh.k[buf][wave][n * 2 + k][lane] =
-                    __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-            // Values of rows that nothing was written to, or that were not finite (the
-            // key's scale says so too), stay finite: no weight of theirs reaches a sum.
-            const f16x2 none = {(_Float16)0.0f, (_Float16)0.0f};
-            const f16x2 most = {(_Float16)kMostScale, (_Float16)kMostScale};
-            f16x2 s01 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vs[n][1], vs[n][0], 0x07060302u));
-            f16x2 s23 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(vs[n][3], vs[n][2], 0x07060302u));
-            s01 = __builtin_elementwise_min(__builtin_elementwise_max(s01, none), most);
-            s23 = __builtin_elementwise_min(__builtin_elementwise_max(s23, none), most);
-            if (far) {
-                float x[4] = {(float)s01.x, (float)s01.y, (float)s23.x, (float)s23.y};
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int shift = x[r] >= kLeastScale ? exponent(x[r]) - usual : 0;
-                    x[r] = ldexpf(x[r], -shift);
-                    if (i == 0) sh.shift[buf][wave][n][g * 4 + r] = (float)shift;
+                for (int t = 0; t < 4; t++) {
+                    const uint32_t u = (vr[n * 4 + t] >> (g & 1) * 4 & 0x0F0F0F0Fu) ^ 0x08080808u;
+                    *((f16x4 *)&sh.v[buf][wave >> 1][n * 4 + t][lane] + (wave & 1)) =
+                        halves_f16(u, s02, s13);
                 }
-                s01 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
-                s23 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
-            }
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const uint32_t u = (vr[n * 4 + t] >> (g & 1) * 4 & 0x0F0F0F0Fu) ^ 0x08080808u;
-                *((f16x4 *)&sh.v[buf][wave >> 1][n * 4 + t][lane] + (wave & 1)) = halves_f16(u, s01, s23);
             }
         }
-        if (lane == 0) sh.kind[buf][wave] = ((unsigned)raw >= kv.blocks ? 1 : 0) | (far ? 2 : 0);
+        if (lane == 0) sh.kind[buf][wave] = (uint8_t)kind;
     };
 
-    float m = kNone, l = 0.0f;  // l: of this lane's keys
-    f32x4 acc[T];
+    // The weights' sums: the row's, taken with the values on the matrix cores (all elements
+    // are the same); where blocks are far, of this lane's keys on the vector units.
+    float m = kNone, l = 0.0f;
+    f32x4 acc[T], total = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -986,33 +1034,27 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (t * 16 + r > last) w[t][r] = -INFINITY;
-        if (kind & 0x01010101u)
+        float mx[4], top;
+        if (kind == 0) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
-                if (kind >> (8 * t) & 1) w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const bool far = (kind & 0x02020202u) != 0;
-        // NaN (a key that was not finite) does not count.
-        float mx[4], top;
-        if (far) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                mx[t] = kNone;
-#pragma unroll
-                for (int n = 0; n < N; n++) {
-                    f32x4 z = {0.f, 0.f, 0.f, 0.f};
-                    if (kind >> (8 * t) & 2) z = *(const f32x4 *)&sh.shift[buf][t][n][g * 4];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float x = fmaf(w[t][r], qs, z[r]);
-                        mx[t] = max3(mx[t], x, x);
-                    }
-                }
-            }
-            top = quarters_max(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
+                mx[t] = largest(largest(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
+            top = quarters_max(largest(largest(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
         } else {
 #pragma unroll
-            for (int t = 0; t < 4; t++) mx[t] = max3(max3(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
-            top = quarters_max(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
+            for (int t = 0; t < 4; t++) {
+                if (kind >> (8 * t) & 1) w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                mx[t] = kNone;
+#pragma unroll
+                for (int n = 0; n < N; n++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float z = kind >> (8 * t) & 2 ? sh.shift[buf][t][n][g * 4 + r] : 0.0f;
+                        const float x = fmaf(w[t][r], qs, z);
+                        mx[t] = max3(mx[t], x, x);
+                    }
+            }
+            top = quarters_max(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
         }
         const float least = ceilf(top), mn = max3(m, least, least);
         if (__any(mn != m)) {
@@ -1022,6 +1064,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
             for (int t = 0; t < T; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) acc[t][r] *= shrink;
+#pragma unroll
+            for (int r = 0; r < 4; r++) total[r] *= shrink;
             m = mn;
         }
         const float base = 14.0f - m;
@@ -1030,22 +1074,31 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
-                l += w[t][r];
             }
+        const bool far = (kind & 0x02020202u) != 0;
+        if (far)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) l += w[t][r];
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int n = 0; n < N; n++) {
+            if (far)  // from the last 64 dims' shifts to these
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    if (kind >> (8 * t) & 2)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            w[t][r] *= __builtin_amdgcn_exp2f(
+                                sh.shift[buf][t][n][g * 4 + r] -
+                                (n ? sh.shift[buf][t][n - 1][g * 4 + r] : 0.0f));
             if (n == 0 || far) {
                 f16x2 hi[4][2], lo[4][2];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    f32x4 y = w[t];
-                    if (far && (kind >> (8 * t) & 2))
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            y[r] *= __builtin_amdgcn_exp2f(sh.shift[buf][t][n][g * 4 + r]);
-                    split_pair(y[0], y[1], hi[t][0], lo[t][0]);
-                    split_pair(y[2], y[3], hi[t][1], lo[t][1]);
+                    split_pair(w[t][0], w[t][2], hi[t][0], lo[t][0]);
+                    split_pair(w[t][1], w[t][3], hi[t][1], lo[t][1]);
                 }
 #pragma unroll
                 for (int z = 0; z < 2; z++) {
@@ -1059,6 +1112,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
                 f16x8 v[4];
 #pragma unroll
                 for (int t = 0; t < 4; t++) v[t] = sh.v[buf][z][t0 + t][lane];
+                if (n == 0) {
+                    const int one = far ? 0 : 0x3C003C00;
+                    const f16x8 ones = __builtin_bit_cast(f16x8, i32x4{one, one, one, one});
+                    total = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[z], total, 0, 0, 0);
+                    total = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[z], total, 0, 0, 0);
+                }
 #pragma unroll
                 for (int t = 0; t < 4; t++)
                     acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], ph[z],
@@ -1074,8 +1133,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     if (c0 < c1) {
         request(c0, 0);
         look_first();
-        least_near = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)power_of_2(max(usual - kNear, -17))) << 16;
-        past_near = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)power_of_2(min(usual + kNear + 1, 15))) << 16;
+        const uint16_t least = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(max(usual - kNear, -17)));
+        const uint16_t past = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(min(usual + kNear + 1, 15)));
+        least_near = (uint32_t)least << 16;
+        range_near = ((uint32_t)min(past, kMostFast) << 16) - least_near;
         stage(0, c0);
         __syncthreads();
         for (int c = c0, n = 0; c < c1; c += stride, n++) {
@@ -1089,7 +1150,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         }
     }
     if (__any(wild) && lane == 0) atomicOr(status, 2);
-    l = xor16_32_sum(l);
+    l = xor16_32_sum(l) + total[0];
     bool bad = false;
     if (i < live) {
         float base = m - 14.0f;
@@ -1159,12 +1220,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Ro
             f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pair, pair, 0x01000100u));
             s2 = __builtin_elementwise_min(__builtin_elementwise_max(s2, none), most);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const uint32_t u = x[k] ^ 0x88888888u;
-                kk[t][n * 2 + k] = __builtin_shufflevector(halves_f16(u & 0x0F0F0F0Fu, s2, s2),
-                                                           halves_f16(u >> 4 & 0x0F0F0F0Fu, s2, s2),
-                                                           0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            for (int k = 0; k < 2; k++) kk[t][n * 2 + k] = word_f16(x[k], s2);
         }
     }
 
