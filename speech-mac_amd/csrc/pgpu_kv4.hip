@@ -1326,38 +1326,44 @@ struct Kv4Evict {
     int32_t *kept;
 };
 
+constexpr int kEvictList = 8192;  // indexes that wait in LDS
+
 struct Kv4EvictShared {
     uint32_t bins[kBins];
-    uint32_t wave_a[kEvictWaves], wave_b[kEvictWaves];
+    uint32_t share[2][kEvictWaves];
     uint32_t bin, above;
     int bad;
+    int32_t list[kEvictList];
 };
 
 // The sum over the waves before this one, and (total) over all, of a number of each wave.
+// One barrier: `share` is another's until the one after.
 __device__ inline uint32_t waves_before(uint32_t *share, uint32_t mine, uint32_t &total) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane == 0) share[wave] = mine;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) share[wave] = mine;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-    for (int i = 0; i < kEvictWaves; i++) {
-        if (i < wave) before += share[i];
-        total += share[i];
+    uint32_t run = share[lane & 15];
+#pragma unroll
+    for (int o = 1; o < kEvictWaves; o <<= 1) {
+        const uint32_t z = __shfl_up(run, o, 16);
+        if ((lane & 15) >= o) run += z;
     }
-    return before;
+    total = __shfl(run, kEvictWaves - 1);
+    const uint32_t before = __shfl(run, (wave - 1) & 15);
+    return wave ? before : 0;
 }
 
-// A work-group for each (head, layer, stream). The least order that is kept is found
-// digit by digit (11, 11 and 10 bits) from counts in LDS; then the indexes are dealt out
-// in order, and the rows moved, a block to a wave, kEvictWaves blocks between two
-// barriers: a block's rows come from its own place or later ones, and all that are
-// read before a barrier are written after it, so that nothing is read that was written.
+// A work-group for each (head, layer, stream). The least order that is kept is found digit
+// by digit (11, 11 and 10 bits) from counts in LDS; then the indexes are dealt out in
+// order, and the rows moved, two blocks to a wave between two barriers: a block's rows
+// come from its own place or later ones, and all that are read before a barrier are
+// written after it, so that nothing is read that was written. Values lie by dim: for each
+// row a lane takes the word that has its dim's number, all 16 on their way at once.
 template <int D>
-__global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t layer_values,
+__global__ __launch_bounds__(kEvictThreads, D == 64 ? 8 : 4) void k_kv4_evict(Kv4 kv, size_t layer_values,
                                                              size_t layer_scales, Kv4Evict a,
                                                              int *status) {
-    constexpr int N = D / kSpan;
+    constexpr int N = D / kSpan, R = 1, H = 8;  // blocks to a wave; sums that a thread holds
     __shared__ Kv4EvictShared sh;
     const int head = blockIdx.x, layer = blockIdx.y, s = blockIdx.z, streams = gridDim.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1370,11 +1376,17 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t laye
     const int32_t *table = a.tables + (size_t)s * a.table_stride;
     const int32_t *to_table = a.to_tables + (size_t)s * a.table_stride;
     const int n = uniform_load(a.lengths + s), count = min(n, a.keep);
-    const bool long_ = n > 0 && ((size_t)n > a.sums_stride ||
-                                 (n - 1) / kBlockPos >= a.table_stride);
-    if (threadIdx.x == 0) sh.bad = long_;
+    const bool past = n > 0 && ((size_t)n > a.sums_stride || (n - 1) / kBlockPos >= a.table_stride);
+    if (threadIdx.x == 0) sh.bad = past;
     __syncthreads();
-    if (!long_ && n > 0) {
+    // The sums of rows threadIdx.x + 1024 k.
+    float held[H];
+#pragma unroll
+    for (int k = 0; k < H; k++) {
+        const int i = threadIdx.x + k * kEvictThreads;
+        held[k] = !past && i < n ? sums[i] : 0.0f;
+    }
+    if (!past && n > 0) {
         bool bad = false;
         for (int b = threadIdx.x; b * kBlockPos < n; b += kEvictThreads) {
             bad |= (unsigned)table[b] >= kv.blocks;
@@ -1391,6 +1403,11 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t laye
 
     const int lo = n > a.keep ? a.first : n, hi = n > a.keep ? n - a.newest : n;
     uint32_t need = n > a.keep ? a.keep - a.first - a.newest : 0, least = 0;
+    auto count_digit = [&](int i, float x, int shift, int width) {
+        const uint32_t u = order_of(x);
+        if (i >= lo && i < hi && (shift == 32 || (u >> shift) == (least >> shift)))
+            atomicAdd(&sh.bins[u >> (shift - width) & ((1u << width) - 1)], 1u);
+    };
     // Of the orders equal to `least`, the first `need` are kept; of the others the larger.
     if (need) {
         int shift = 32;
@@ -1398,11 +1415,11 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t laye
             const int width = digit < 2 ? 11 : 10;
             for (int b = threadIdx.x; b < kBins; b += kEvictThreads) sh.bins[b] = 0;
             __syncthreads();
-            for (int i = lo + threadIdx.x; i < hi; i += kEvictThreads) {
-                const uint32_t u = order_of(sums[i]);
-                if (shift == 32 || (u >> shift) == (least >> shift))
-                    atomicAdd(&sh.bins[u >> (shift - width) & ((1u << width) - 1)], 1u);
-            }
+#pragma unroll
+            for (int k = 0; k < H; k++)
+                if (k * kEvictThreads < n) count_digit(threadIdx.x + k * kEvictThreads, held[k], shift, width);
+            for (int i = threadIdx.x + H * kEvictThreads; i < hi; i += kEvictThreads)
+                count_digit(i, sums[i], shift, width);
             __syncthreads();
             // Two bins to a thread, from the top.
             const int b = kBins - 1 - 2 * (int)threadIdx.x;
@@ -1414,7 +1431,8 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t laye
                 if (lane >= o) run += z;
             }
             uint32_t total;
-            const uint32_t before = waves_before(sh.wave_a, __shfl(run, 63), total) + run - x - y;
+            const uint32_t before =
+                waves_before(sh.share[digit & 1], __shfl(run, 63), total) + run - x - y;
             if (before < need && before + x >= need) {
                 sh.bin = b;
                 sh.above = before;
@@ -1426,78 +1444,103 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_evict(Kv4 kv, size_t laye
             shift -= width;
             least |= sh.bin << shift;
             need -= sh.above;
-            __syncthreads();
         }
+        __syncthreads();
     }
-    // The indexes and their sums, in order.
-    uint32_t equal = 0, at = 0;  // before this round
-    for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
-        const int i = i0 + threadIdx.x;
-        const float x = i < n ? sums[i] : 0.0f;
+    // The indexes and their sums, in order. A row comes after those before it that are
+    // larger (or not to be chosen among) and as many of the equal ones as are kept.
+    uint32_t larger = 0, equal = 0;
+    auto place = [&](int round, float x) {
+        const int i = threadIdx.x + round * kEvictThreads;
         const uint32_t u = order_of(x);
         const bool middle = i >= lo && i < hi;
-        const bool same = middle && u == least;
-        const uint64_t mask = __ballot(same);
+        const bool more = i < n && (!middle || (need && u > least)), same = need && middle && u == least;
+        const uint64_t up = __ballot(more), eq = __ballot(same), below = (1ull << lane) - 1;
         uint32_t total;
-        const uint32_t rank = equal + waves_before(sh.wave_a, __popcll(mask), total) +
-                              __popcll(mask & ((1ull << lane) - 1));
-        equal += total;
-        const bool keep = i < n && (!middle || (lo < hi && need && u > least) ||
-                                    (same && rank < need));
-        const uint64_t all = __ballot(keep);
-        const uint32_t to = at + waves_before(sh.wave_b, __popcll(all), total) +
-                            __popcll(all & ((1ull << lane) - 1));
-        at += total;
-        if (keep) {
+        const uint32_t before = waves_before(sh.share[round & 1],
+                                             (uint32_t)(__popcll(up) | __popcll(eq) << 16), total);
+        const uint32_t rank = equal + (before >> 16) + __popcll(eq & below);
+        if (more || (same && rank < need)) {
+            const uint32_t to = larger + (before & 0xFFFFu) + __popcll(up & below) + min(rank, need);
             kept[to] = i;
+            if (to < kEvictList) sh.list[to] = i;
             to_sums[to] = x == x ? x : 0.0f;
         }
+        larger += total & 0xFFFFu;
+        equal += total >> 16;
+    };
+#pragma unroll
+    for (int k = 0; k < H; k++)
+        if (k * kEvictThreads < n) place(k, held[k]);
+    for (int k = H; k * kEvictThreads < n; k++) {
+        const int i = threadIdx.x + k * kEvictThreads;
+        place(k, i < n ? sums[i] : 0.0f);
     }
     for (int j = count + threadIdx.x; j < a.keep; j += kEvictThreads) kept[j] = -1;
     __syncthreads();
 
-    // The rows.
-    for (int b0 = 0; b0 * kBlockPos < count; b0 += kEvictWaves) {
-        const int b = b0 + wave, rows = min(kBlockPos, count - b * kBlockPos);
-        uint64_t key[N], dim[N];
-        uint32_t pair[N];
-        unsigned to = 0;
-        bool stay = rows <= 0;
-        if (!stay) {
-            to = (unsigned)to_table[b];
-            const int j = lane >> 2, src = kept[b * kBlockPos + min(j, rows - 1)];
-            const unsigned id = (unsigned)table[src / kBlockPos];
-            // Rows that are where they belong.
-            stay = __all(id == to && src == b * kBlockPos + min(j, rows - 1));
+    // The rows: lane (j, piece) has row j's key, lane d dim d's values. Past the last row:
+    // the last one again.
+    for (int b0 = 0; b0 * kBlockPos < count; b0 += kEvictWaves * R) {
+        const int j = lane >> 2;
+        int src[R], at[R];
+        unsigned id[R], to[R];
+#pragma unroll
+        for (int e = 0; e < R; e++) {
+            at[e] = min((b0 + e * kEvictWaves + wave) * kBlockPos + j, count - 1);
+            src[e] = at[e] < kEvictList ? sh.list[at[e]] : kept[at[e]];
+            to[e] = (unsigned)to_table[at[e] / kBlockPos];
+        }
+#pragma unroll
+        for (int e = 0; e < R; e++) id[e] = (unsigned)table[src[e] / kBlockPos];
+        uint64_t key[R][N];
+        uint32_t pair[R][N], w[R][N][kBlockPos];
+#pragma unroll
+        for (int e = 0; e < R; e++) {
+            const int row = src[e] % kBlockPos;
+            const uint8_t *tile = kv4_tile<D>(kv, id[e], head);
+            const uint64_t half = (uint64_t)(tile + N * kPlane + (row >> 3) * 4);
 #pragma unroll
             for (int m = 0; m < N; m++) {
-                const uint8_t *tile = kv4_tile<D>(kv, id, head);
-                key[m] = *((const uint64_t *)(tile + m * kPlane + src % kBlockPos * (kSpan / 2)) +
-                           (lane & 3));
-                pair[m] = kv4_scales<D>(kv, id, head)[m * kBlockPos + src % kBlockPos];
-                dim[m] = 0;
+                key[e][m] = *((const uint64_t *)(tile + m * kPlane + row * (kSpan / 2)) + (lane & 3));
+                pair[e][m] = kv4_scales<D>(kv, id[e], head)[m * kBlockPos + row];
+            }
 #pragma unroll
-                for (int z = 0; z < kBlockPos; z++) {
-                    const unsigned from = (unsigned)__builtin_amdgcn_readlane((int)id, z * 4);
-                    const int i = __builtin_amdgcn_readlane(src, z * 4) % kBlockPos;
-                    const uint32_t byte = kv4_tile<D>(kv, from, head)[(N + m) * kPlane + lane * 8 +
-                                                                     (i >> 3) * 4 + (i & 3)];
-                    if (z < rows)
-                        dim[m] |= (uint64_t)(byte >> (i & 4) & 15u)
-                                  << ((z >> 3) * 32 + (z & 3) * 8 + (z >> 2 & 1) * 4);
-                }
+            for (int r = 0; r < kBlockPos; r++) {
+                const uint64_t low = (uint32_t)__builtin_amdgcn_readlane((int)half, r * 4);
+                const uint64_t high = (uint32_t)__builtin_amdgcn_readlane((int)(half >> 32), r * 4);
+                const uint8_t *dims = (const uint8_t *)(high << 32 | low);
+#pragma unroll
+                for (int m = 0; m < N; m++)
+                    w[e][m][r] = *(const uint32_t *)(dims + ((unsigned)lane * 8 + m * kPlane));
+            }
+        }
+        uint32_t dim[R][N][2];
+#pragma unroll
+        for (int e = 0; e < R; e++) {
+            const int shift = (src[e] & 3) * 8 + (src[e] & 4);
+#pragma unroll
+            for (int m = 0; m < N; m++) dim[e][m][0] = dim[e][m][1] = 0;
+#pragma unroll
+            for (int r = 0; r < kBlockPos; r++) {
+                const int from = __builtin_amdgcn_readlane(shift, r * 4);
+#pragma unroll
+                for (int m = 0; m < N; m++)
+                    dim[e][m][r >> 3] |= (w[e][m][r] >> from & 15u) << ((r & 3) * 8 + (r & 4));
             }
         }
         __syncthreads();
-        if (!stay) {
-            uint8_t *tile = kv4_tile<D>(kv, to, head);
-            const int j = lane >> 2;
+#pragma unroll
+        for (int e = 0; e < R; e++) {
+            const int first = (b0 + e * kEvictWaves + wave) * kBlockPos;
+            if (first >= count || __all(id[e] == to[e] && src[e] == at[e])) continue;  // in place
+            uint8_t *tile = kv4_tile<D>(kv, to[e], head);
 #pragma unroll
             for (int m = 0; m < N; m++) {
-                *((uint64_t *)(tile + (N + m) * kPlane) + lane) = dim[m];
-                if (j >= rows) continue;
-                *((uint64_t *)(tile + m * kPlane + j * (kSpan / 2)) + (lane & 3)) = key[m];
-                if ((lane & 3) == 0) kv4_scales<D>(kv, to, head)[m * kBlockPos + j] = pair[m];
+                *((uint2 *)(tile + (N + m) * kPlane) + lane) = make_uint2(dim[e][m][0], dim[e][m][1]);
+                if (first + j >= count) continue;
+                *((uint64_t *)(tile + m * kPlane + j * (kSpan / 2)) + (lane & 3)) = key[e][m];
+                if ((lane & 3) == 0) kv4_scales<D>(kv, to[e], head)[m * kBlockPos + j] = pair[e][m];
             }
         }
     }
