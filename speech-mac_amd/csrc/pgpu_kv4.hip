@@ -743,8 +743,18 @@ struct Kv4Run {
     float *part_acc, *part_ml;
     float *out;  // splits = 1: the rows themselves
     size_t out_stride;
-    float *lse;  // [rows][query heads]: log2 of a row's sum of 2^score, or NULL
+    // With sums: log2 of a row's sum of 2^score, [rows][query heads]; and the last `counted`
+    // rows' queries as operands and their factors, tile by tile (tile_at).
+    float *lse;
+    uint4 *queries;
+    float *factors;
+    int counted;
 };
+
+// Where a tile of 16 rows and a query head stand among rows + 16 * streams rows.
+__device__ inline size_t tile_at(const Kv4Span &span, int s, int r0, int qh, int wide) {
+    return (size_t)(span.row0 + 16 * s + r0) * wide + (size_t)qh * 16;
+}
 
 template <int D>
 struct Kv4RunShared {
@@ -879,6 +889,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
             for (int k = 0; k < 4; k++) x[n][k] = *(const float4 *)(q + n * kSpan + g * 16 + k * 4);
         qs = kv4_query<D>(x, a.scale, biggest, qhi, qlo);
+    }
+    if (a.queries && split == 0 && live > 0 && r0 + 16 > span.count - a.counted) {
+        const size_t at = tile_at(span, s, r0, qh, wide);
+        uint4 *to = a.queries + at * (D / 4) + lane;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            to[k * 128] = __builtin_bit_cast(uint4, qhi[k]);
+            to[k * 128 + 64] = __builtin_bit_cast(uint4, qlo[k]);
+        }
+        if (g == 0) a.factors[at + i] = qs;
     }
 
     // Chunk c: its bytes requested, then turned into LDS; wave w takes block w. The block's
@@ -1183,16 +1203,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 }
 
 // What runs of rows weigh, from their scores once more and the rows' log sums: a
-// work-group of 4 waves for 64 keys of a (stream, key head), which stand in each wave's
+// work-group of W waves for 64 keys of a (stream, key head), which stand in each wave's
 // registers as fp16; the waves take the tiles of 16 rows that see them in turn. A lane
 // adds up its row's weights of 16 keys over the tiles; lanes and waves are added once.
-template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
-                                                                   const float *before,
-                                                                   float *after, size_t stride,
-                                                                   int counted, int *status) {
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
+                                                                      const float *before,
+                                                                      float *after, size_t stride,
+                                                                      int counted, int *status) {
     constexpr int N = D / kSpan, KS = D / 32;
-    __shared__ float parts[4][64];
+    __shared__ float parts[W][64];
     const int head = blockIdx.x % kv.heads, c = blockIdx.x / kv.heads, s = blockIdx.z;
     const int wide = kv.heads * a.group;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1224,41 +1244,44 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Ro
         }
     }
 
-    // Units: a tile of rows and a query head of the group.
-    const int from = max(max(0, span.count - counted), c * 64 - span.first);
+    // Units: a tile of rows, as the attention left it, and a query head of the group.
+    const int late = max(0, span.count - counted);  // rows before it do not count
+    const int from = max(late, c * 64 - span.first) / 16 * 16;
     const int units = (span.count - from + 15) / 16 * a.group;
-    float4 x[N][4];
-    float lse = INFINITY;
+    f16x8 nexthi[KS], nextlo[KS];
+    float lse = INFINITY, factor = 0.0f;
     auto request = [&](int u) {
-        const int r = from + u / a.group * 16 + i, qh = head * a.group + u % a.group;
-        const size_t row = (size_t)span.row0 + min(r, span.count - 1);
-        const float *q = a.q + row * a.q_stride + (size_t)qh * D;
+        const int r0 = from + u / a.group * 16, r = r0 + i, qh = head * a.group + u % a.group;
+        const size_t at = tile_at(span, s, r0, qh, wide);
+        const uint4 *q = a.queries + at * (D / 4) + lane;
 #pragma unroll
-        for (int n = 0; n < N; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[n][k] = *(const float4 *)(q + n * kSpan + g * 16 + k * 4);
-        lse = a.lse[row * wide + qh];
-        if (r >= span.count) lse = INFINITY;
+        for (int k = 0; k < KS; k++) {
+            nexthi[k] = __builtin_bit_cast(f16x8, q[k * 128]);
+            nextlo[k] = __builtin_bit_cast(f16x8, q[k * 128 + 64]);
+        }
+        factor = a.factors[at + i];
+        lse = a.lse[((size_t)span.row0 + min(r, span.count - 1)) * wide + qh];
+        if (r < late || r >= span.count) lse = INFINITY;
     };
     f32x4 part[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) part[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (wave < units) request(wave);
-    for (int u = wave; u < units; u += 4) {
+    for (int u = wave; u < units; u += W) {
         const int p0 = span.first + from + u / a.group * 16;
         // Rows that did not come out finite weigh nothing.
         const bool fine = fabsf(lse) < INFINITY;
-        const float base = fine ? -lse : -INFINITY;
-        if (__any(!fine))
-#pragma unroll
-            for (int n = 0; n < N; n++)
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (!fine) x[n][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float base = fine ? -lse : -INFINITY, qs = factor;
         f16x8 qhi[KS], qlo[KS];
-        float biggest;
-        const float qs = kv4_query<D>(x, a.scale, biggest, qhi, qlo);
-        if (u + 4 < units) request(u + 4);
+#pragma unroll
+        for (int k = 0; k < KS; k++) qhi[k] = nexthi[k], qlo[k] = nextlo[k];
+        if (__any(!fine)) {
+            const i32x4 none = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+                if (!fine) qhi[k] = qlo[k] = __builtin_bit_cast(f16x8, none);
+        }
+        if (u + W < units) request(u + W);
         f32x4 w[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1299,9 +1322,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Ro
     const size_t at = ((size_t)s * kv.heads + head) * stride + p;
     float sum = before && p < span.first ? before[at] : 0.0f;
     const int t = threadIdx.x >> 4, id = t < 2 ? (t ? ids[1] : ids[0]) : (t == 2 ? ids[2] : ids[3]);
-    if ((unsigned)id < kv.blocks)
-        sum += (parts[0][threadIdx.x] + parts[1][threadIdx.x]) +
-               (parts[2][threadIdx.x] + parts[3][threadIdx.x]);
+    if ((unsigned)id < kv.blocks) {
+        float part = 0.0f;
+#pragma unroll
+        for (int z = 0; z < W; z++) part += parts[z][threadIdx.x];
+        sum += part;
+    }
     after[at] = sum;
 }
 
@@ -1693,6 +1719,14 @@ size_t parts_bytes(const pgpu_kv4 *kv, size_t parts) {
     return parts * (kv->head_dim + 2) * sizeof(float);
 }
 
+// What a run's sums need: the queries as operands, factors and log sums (and room to align
+// what follows).
+size_t run_sums_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group) {
+    const size_t wide = (size_t)kv->heads * group;
+    return ((r->rows + (size_t)16 * r->streams) * wide * (kv->head_dim + 1) + r->rows * wide + 4) *
+           sizeof(float);
+}
+
 template <int D>
 int join(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
          const float *part_acc, const float *part_ml, int group, int max_positions, float *out,
@@ -1760,8 +1794,10 @@ int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, con
                                  a.max_positions, a.out, a.out_stride, a.lse, status))
         return 0;
     if (!sums) return 1;
-    hipLaunchKernelGGL(k_kv4_sums<D>, dim3(c.heads * (unsigned)((a.max_positions + 63) / 64), 1, streams), dim3(256),
-                       0, st, c, r, a, sums->before, sums->after, sums->stride,
+    constexpr int W = D == 64 ? 16 : 8;
+    hipLaunchKernelGGL((k_kv4_sums<D, W>), dim3(c.heads * (unsigned)((a.max_positions + 63) / 64), 1,
+                                                streams),
+                       dim3(64 * W), 0, st, c, r, a, sums->before, sums->after, sums->stride,
                        sums->rows, status);
     return launch_ok("pgpu_kv4_attention");
 }
@@ -1782,7 +1818,7 @@ extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_ro
                                    1024 / (kv->heads * ((group + 3) / 4))});
         if (most > 1)
             parts = std::min((size_t)1024 * 64, rows->streams * rows->max_rows * wide * most);
-        return parts_bytes(kv, parts) + (with_sums ? rows->rows * wide * sizeof(float) : 0);
+        return parts_bytes(kv, parts) + (with_sums ? run_sums_bytes(kv, rows, group) : 0);
     }
     // Fewer streams may be dealt to more work-groups: the streams before the numbers of
     // work-groups where the keys to each change count too. More positions never give
@@ -1848,12 +1884,28 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
     }
     const Deal d = deal_rows(kv, rows, group, max_positions);
     const size_t parts = d.splits > 1 ? rows->streams * rows->max_rows * wide * d.splits : 0;
-    const size_t need = parts_bytes(kv, parts) + (sums ? rows->rows * wide * sizeof(float) : 0);
+    const size_t need = parts_bytes(kv, parts) + (sums ? run_sums_bytes(kv, rows, group) : 0);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv4_attention (workspace)");
-    const Kv4Run a = {q, q_stride, group, scale * kLog2e, max_positions, d.splits, floats,
-                      floats + parts * kv->head_dim, out, out_stride,
-                      sums ? floats + parts * (kv->head_dim + 2) : nullptr};
+    Kv4Run a = {};
+    a.q = q;
+    a.q_stride = q_stride;
+    a.group = group;
+    a.scale = scale * kLog2e;
+    a.max_positions = max_positions;
+    a.splits = d.splits;
+    a.out = out;
+    a.out_stride = out_stride;
+    if (sums) {
+        const size_t slots = (rows->rows + (size_t)16 * rows->streams) * wide;
+        a.queries = (uint4 *)floats;
+        a.factors = floats + slots * kv->head_dim;
+        a.lse = a.factors + slots;
+        a.counted = sums->rows;
+        floats = a.lse + rows->rows * wide;
+    }
+    a.part_acc = floats + (-(uintptr_t)floats / sizeof(float) & 3);
+    a.part_ml = a.part_acc + parts * kv->head_dim;
     return kv->head_dim == 64 ? attend_rows<64>(st, c, r, rows->streams, d, a, sums, status)
                               : attend_rows<128>(st, c, r, rows->streams, d, a, sums, status);
 }

@@ -40,7 +40,10 @@ def test_runs(pkg, heads, dim, group, sums):
         for streams in (1, 2, 3, 7, 16, 63, 64, 200):
             for rows in (1, 5, 16, 17, 100, 300, 4096):
                 n = size(lib, pkg, heads, dim, group, streams, most, rows, sums)
-                assert n <= (1024 * 64 * (dim + 2) + sums * streams * rows * heads * group) * 4
+                # Parts of 64 rows by 1024 work-groups; with sums, the queries as operands, a
+                # factor and a log sum for each, by tiles of 16 rows.
+                kept = sums * heads * group * streams * ((rows + 16) * (dim + 1) + rows) + 4
+                assert n <= (1024 * 64 * (dim + 2) + kept) * 4
                 for s, r, p in ((1, rows, most), (streams, 1, most), ((streams + 1) // 2, rows, most),
                                 (streams, (rows + 1) // 2, most), (streams, rows, most // 2 + 1),
                                 (max(1, streams - 1), max(1, rows - 1), most)):
