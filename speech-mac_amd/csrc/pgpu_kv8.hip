@@ -1019,6 +1019,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
             for (int t = 0; t < 4; t++)
                 w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t], qlo[k], w[t], 0, 0, 0);
         }
+        // max3 is asm: the compiler does not place the waits that it needs behind a matrix
+        // instruction (11 states; 16 here).
+        asm("s_nop 7\n\ts_nop 7" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));
         if (masked)
 #pragma unroll
             for (int t = 0; t < 4; t++)
