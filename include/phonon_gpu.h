@@ -631,7 +631,7 @@ typedef struct {
  * evicted after it. Rows [16 i, 16 i + 16) lie in block tables[s * table_stride
  * + i]. Blocks that are written are no other stream's. `max_rows` bounds the
  * rows of a stream and `rows` every row index. A stream outside its bounds
- * (offsets, table, more than max_rows rows) is left out, a block id outside the
+ * (offsets, table, more than max_rows rows, an index of 2^30) is left out, a block id outside the
  * cache likewise, and status bit 2 set. */
 typedef struct {
     const int32_t *tables;  /* (dev) [streams][table_stride] */
@@ -658,7 +658,8 @@ int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_kv4_ro
  * i] = before[same] + the sum of the weights that the last `rows` rows of the
  * call's (of each stream; all, if it has fewer) and the head's queries give it.
  * The call's own rows are new: they begin from 0. before NULL: all begin from 0;
- * before = after: in place (no other overlap). A row that does not come out
+ * before = after: in place (no other overlap). A stream without rows in the
+ * call, or left out, has its `after` left as it is. A row that does not come out
  * finite adds nothing. Summed in fp32, always in the same order. */
 typedef struct {
     const float *before; /* (dev) [streams][heads][stride] or NULL */
@@ -670,11 +671,17 @@ typedef struct {
  * a key head, 1..16; q[r * q_stride + h * head_dim]) attends the cache rows 0 ..
  * its own, softmax(scale q k) v, into out[r * out_stride + h * head_dim]. The
  * cache already holds the call's rows. One row a stream, or runs of rows.
- * `max_positions` bounds every cache row's index + 1 (a stream past it is left
- * out, status bit 2). A block whose id is outside the cache weighs nothing
+ * `max_positions` (up to 2^30; with runs' sums, less than 2^28 over heads)
+ * bounds every cache row's index + 1 (a stream past it is left out, status bit
+ * 2). A block whose id is outside the cache weighs nothing
  * (status bit 2; a row that is left no key gets zeros). A stream with first < 0
  * gets zero rows. Strides multiples of 4, pointers 16-byte aligned; out must not
  * overlap q. `sums` NULL: the weights are not added up.
+ * A run holds a query's elements and a key's weight in two fp16 terms: to 2^-21
+ * of themselves, or 2^-27 of the row's largest element, or of the largest weight
+ * times value scale that it sees. One row a stream holds them to 2^-29 of those
+ * largest ones; what it multiplies and sums of them is exact within 64 keys and
+ * as long as no larger one comes.
  * The same call gives the same bits; how the keys are dealt to work-groups goes
  * by the number of streams, max_rows and max_positions, so that in another batch
  * a stream's last bits may differ.
@@ -701,9 +708,10 @@ int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_k
  * least the longest stream's length: to_sums gets the kept rows' sums in order,
  * and is left as it is past them (to_sums may be sums, no other overlap). NaN
  * counts as 0. kept (dev) [layers][streams][heads][keep]: the indexes of the rows
- * kept, -1 past them. lengths[s] < 0, or a table entry outside the cache or
- * a length past the table or sums_stride (status bit 2): the stream is left as it
- * is, its kept all -1. The stream's length is min(lengths[s], keep) afterwards. */
+ * kept, -1 past them. lengths[s] < 0, or a table entry outside the cache or a
+ * length past the table, sums_stride or 2^30 (status bit 2): the stream is left
+ * as it is, its kept all -1. The stream's length is min(lengths[s], keep)
+ * afterwards. */
 int pgpu_kv4_evict(void *stream, const pgpu_kv4 *kv, int first_layer, int layers,
                    const int32_t *tables, const int32_t *to_tables, int table_stride,
                    const int32_t *lengths, int streams, int keep, int first, int newest,

@@ -14,6 +14,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kSpan = 64;         // dims of a scale
 constexpr int kPlane = 512;       // bytes of a block's 64 dims, of keys or of values
 constexpr float kLeastScale = 0x1p-17f, kMostScale = 8160.0f;
+constexpr int kMostRows = 1 << 30;  // of a stream: a block past its last is an int32 still
 
 // One layer of the cache, and the rows of a call (pgpu_kv4, pgpu_kv4_rows).
 struct Kv4 {
@@ -36,7 +37,7 @@ struct Kv4Span {
     bool live;
 };
 
-// limit: indexes must be below it. A stream that breaks a bound is flagged (by
+// limit: indexes must be below it, and below kMostRows. A stream that breaks a bound is flagged (by
 // the thread with `speak`) and left out.
 __device__ inline Kv4Span kv4_span(const Kv4Rows &r, int s, int limit, bool speak, int *status) {
     Kv4Span x;
@@ -49,7 +50,7 @@ __device__ inline Kv4Span kv4_span(const Kv4Rows &r, int s, int limit, bool spea
     x.count = wild ? 0 : (int)count;
     const long long last = (long long)x.first + x.count;
     const bool bad = wild || (x.first >= 0 && x.count > 0 &&
-                              (last > limit || last > (long long)r.table_stride * kBlockPos));
+                              (last > min(limit, kMostRows) || last > (long long)r.table_stride * kBlockPos));
     x.live = !bad && x.first >= 0 && x.count > 0;
     if (bad && speak) atomicOr(status, 2);
     return x;
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256) void k_kv4_write(Kv4 kv, Kv4Rows rows, const f
     __shared__ __align__(16) uint32_t lds[4][kSpan * 2];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int s = blockIdx.z, head = blockIdx.x * 4 + wave, g = lane >> 4, c = lane & 15;
-    const Kv4Span span = kv4_span(rows, s, INT32_MAX - kBlockPos,
+    const Kv4Span span = kv4_span(rows, s, kMostRows,
                                   threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
     if (!span.live || head >= kv.heads) return;
     const int end = span.first + span.count, block = span.first / kBlockPos + (int)blockIdx.y;
@@ -463,8 +464,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         if (Q != 1) step = __shfl(step, g * 4);  // of query j0 + g
     };
     float m = kNone, l = 0.0f, acc[A];
-    i32x4 sum[A];  // whole sums of the values, times 2^(34 - m): of dims 16 t + i, or 64 t + lane
-    int flushed = 0;
+    // Whole sums of the values, times 2^(34 - m): of dims 16 t + i, or 64 t + lane. A step
+    // adds 2^20 at most, and a work-group has 16 steps at most.
+    i32x4 sum[A];
 #pragma unroll
     for (int t = 0; t < A; t++) acc[t] = 0.0f, sum[t] = i32x4{0, 0, 0, 0};
     auto flush = [&](float less) {
@@ -519,12 +521,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         bound = row16_max(bound);
         if (Q == 1) bound = xor16_32_max(bound);
         const float next = fmaxf(m, ceilf(bound));
-        if (__any(next != m) || ++flushed == 1024) {
+        if (__any(next != m)) {
             const float less = __builtin_amdgcn_exp2f(m - next);  // m = kNone: 0
             flush(less);
             l *= less;
             m = next;
-            flushed = 0;
         }
 #pragma unroll
         for (int t = 0; t < S; t++) {
@@ -1392,7 +1393,8 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_select(int heads, unsigne
     const int32_t *table = a.tables + (size_t)s * a.table_stride;
     const int32_t *to_table = a.to_tables + (size_t)s * a.table_stride;
     const int n = uniform_load(a.lengths + s), count = min(n, a.keep);
-    const bool past = n > 0 && ((size_t)n > a.sums_stride || (n - 1) / kBlockPos >= a.table_stride);
+    const bool past = n > kMostRows || (n > 0 && ((size_t)n > a.sums_stride ||
+                                                  (n - 1) / kBlockPos >= a.table_stride));
     if (threadIdx.x == 0) sh.bad = past;
     __syncthreads();
     // The sums of rows threadIdx.x + 1024 k.
@@ -1850,7 +1852,9 @@ int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, con
 
 extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *rows,
                                            int group, int max_positions, int with_sums) {
-    if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0) return 0;
+    if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0 ||
+        max_positions > kMostRows)
+        return 0;
     const size_t wide = (size_t)kv->heads * group;
     if (rows->rows == 0) return 0;
     size_t parts = 0;
@@ -1887,7 +1891,7 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
     if (!cache_ok(kv) || !rows_ok(rows) || layer < 0 || layer >= kv->layers || !q || !out ||
         !status || !aligned(q, 16) || !aligned(out, 16) || q_stride % 4 != 0 ||
         out_stride % 4 != 0 || group < 1 || group > 16 || q_stride < width ||
-        out_stride < width || max_positions <= 0 || !__builtin_isfinite(scale * kLog2e) ||
+        out_stride < width || max_positions <= 0 || max_positions > kMostRows || !__builtin_isfinite(scale * kLog2e) ||
         (sums && (!sums->after || sums->stride < (size_t)max_positions || sums->rows < 1)))
         return bad_arguments("pgpu_kv4_attention");
     if (rows->rows == 0) return 1;
@@ -1927,6 +1931,9 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
                                   : attend_one<128>(st, c, r, rows->streams, d, a, sums, status);
     }
     const Deal d = deal_rows(kv, rows, group, max_positions);
+    // The grid's limit: 2^32 threads.
+    if (sums && kv->heads * (size_t)((max_positions + 63) / 64) >= (size_t)1 << 22)
+        return bad_arguments("pgpu_kv4_attention");
     const size_t parts = d.splits > 1 ? rows->streams * rows->max_rows * wide * d.splits : 0;
     const size_t need = parts_bytes(kv, parts) + (sums ? run_sums_bytes(kv, rows, group) : 0);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
