@@ -85,31 +85,43 @@ __device__ inline float kv4_scale(float top, float bottom) {
     return fmaxf(bitsf(bits & ~0xFFFFu), kLeastScale);
 }
 
-// Four numbers in [-8, 7] -> the low halves of a word's bytes.
-__device__ inline uint32_t pack_halves(const float *q) {
-    return ((uint32_t)(int)q[0] & 15u) | ((uint32_t)(int)q[1] & 15u) << 8 |
-           ((uint32_t)(int)q[2] & 15u) << 16 | ((uint32_t)(int)q[3] & 15u) << 24;
-}
-
 __device__ inline uint32_t xor1(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false);
 }
+// The largest of a quad's lanes; NaN if one is NaN.
+__device__ inline float quad_largest(float x) {
+    x = __builtin_elementwise_maximum(x, bitsf(xor1(fbits(x))));
+    return __builtin_elementwise_maximum(
+        x, bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(x), 0x4E, 0xf, 0xf, false)));
+}
+// Of 8 lanes, the first four get the last ones' and the other way round.
+__device__ inline float other_quad(float x) {
+    return bitsf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fbits(x), 0x141, 0xf, 0xf, false));
+}
 
-// A row's four dims -> whole numbers. x / s by the reciprocal, which is off by less
-// than 2^-20 below 8; where that could decide a rounding, by the division.
-__device__ inline void kv4_round(const float4 &x, float s, float *q) {
-    const float inverse = 1.0f / s;
-    const float f[4] = {x.x, x.y, x.z, x.w};
+// Eight dims of a row -> whole numbers, the low bytes of q. x / s by the reciprocal, which
+// is off by less than 2^-20 below 8; where that could decide a rounding, by the division.
+__device__ inline void kv4_round(const float4 (&x)[2], float s, float inverse, uint32_t (&q)[2][4]) {
+    constexpr float kWhole = 0x1.8p23f;  // a sum with it is a whole number in the last bits
     float off = 0.0f;
 #pragma unroll
-    for (int d = 0; d < 4; d++) {
-        const float y = f[d] * inverse;
-        q[d] = rintf(y);
-        off = fmaxf(off, fabsf(y - q[d]));
-    }
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int z = 0; z < 4; z++) {
+            const float f = (&x[e].x)[z], sum = fmaf(f, inverse, kWhole);
+            off = fmaxf(off, fabsf(fmaf(f, inverse, -(sum - kWhole))));
+            q[e][z] = fbits(sum);
+        }
     if (off > 0.5f - 2e-6f)
 #pragma unroll
-        for (int d = 0; d < 4; d++) q[d] = rintf(f[d] / s);
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int z = 0; z < 4; z++) q[e][z] = fbits((&x[e].x)[z] / s + kWhole);
+}
+
+// Four low bytes side by side.
+__device__ inline uint32_t low_bytes(const uint32_t (&q)[4]) {
+    return __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000C0Cu);
 }
 
 // The bits of 16 numbers' 8 bytes that rows lo .. hi - 1 take.
@@ -121,103 +133,139 @@ __device__ inline uint64_t row_bits(int lo, int hi) {
     return m;
 }
 
-// A wave for each (block of the call's rows, head): lane (g, c) has rows 4 g .. 4 g + 3
-// of the 4 dims from 4 c on of every 64.
+// A wave for each (block of the call's rows, head). Lane (g, c) has rows 2 g and 2 g + 1,
+// of every 64 dims 4 c .. 4 c + 3 and 32 + those: eight lanes share a row, and each half
+// of them finds one of the two rows' scales. Keys are packed as they lie. Values change
+// from rows to dims through LDS, four numbers a word. Bound by the rows' bytes: 64 streams
+// of up to 2048 rows, 8 heads of 64, 277 MB in 54 us. A row's 128 bytes to an instruction
+// are whole cache lines (64, with 4 lanes a row: 76 us); 256 with 16 lanes a row, each with
+// its scales, are bound by the vector units (65). 211 rows of 1 stream 3.8 us, 5.9 so.
 template <int D>
 __global__ __launch_bounds__(256) void k_kv4_write(Kv4 kv, Kv4Rows rows, const float *k,
                                                    const float *v, size_t row_stride,
                                                    int *status) {
     constexpr int N = D / kSpan;
-    __shared__ __align__(16) uint32_t lds[4][kSpan * 2];
+    __shared__ __align__(16) uint32_t lds[4][N][16][kBlockPos];  // [wave][64 dims][4 dims][row]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int s = blockIdx.z, head = blockIdx.x * 4 + wave, g = lane >> 4, c = lane & 15;
+    const int s = blockIdx.z, head = blockIdx.x * 4 + wave, g = lane >> 3, c = lane & 7;
     const Kv4Span span = kv4_span(rows, s, kMostRows,
                                   threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0, status);
     if (!span.live || head >= kv.heads) return;
     const int end = span.first + span.count, block = span.first / kBlockPos + (int)blockIdx.y;
     if (block * kBlockPos >= end) return;
     const int id = uniform_load(rows.tables + (size_t)s * rows.table_stride + block);
+    const int lo = max(span.first - block * kBlockPos, 0), hi = min(end - block * kBlockPos, 16);
+    float4 x[2][N][2][2];  // keys, values; 64 dims; row; 32 dims
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int j = g * 2 + r;
+        const bool in = j >= lo && j < hi;
+        const size_t at = (size_t)(span.row0 + (in ? block * kBlockPos + j - span.first : 0)) *
+                              row_stride + (size_t)head * D + c * 4;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+                x[0][n][r][e] = in ? once_load(k + at + n * kSpan + e * 32) : none;
+                x[1][n][r][e] = in ? once_load(v + at + n * kSpan + e * 32) : none;
+            }
+    }
     if ((unsigned)id >= kv.blocks) {
         if (lane == 0) atomicOr(status, 2);
         return;
     }
-    const int lo = max(span.first - block * kBlockPos, 0), hi = min(end - block * kBlockPos, 16);
-    float4 x[2][N][4];  // keys, values
+    const int half = c >> 2;  // this lane finds row 2 g + half's scales
+    float mine[2][N];
+    bool wild = false;
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const int j = g * 4 + r, p = block * kBlockPos + j;
-        const bool in = j >= lo && j < hi;
-        const size_t at = (size_t)(span.row0 + (in ? p - span.first : 0)) * row_stride +
-                          (size_t)head * D + c * 4;
+    for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            x[0][n][r] = in ? once_load(k + at + n * kSpan) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[1][n][r] = in ? once_load(v + at + n * kSpan) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    }
-    float scale[2][N][4];
-    bool wild[4] = {false, false, false, false};
+            float top[2], bottom[2];
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
+            for (int r = 0; r < 2; r++) {
+                top[r] = -INFINITY, bottom[r] = INFINITY;
 #pragma unroll
-        for (int p = 0; p < 2; p++)
+                for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int n = 0; n < N; n++) {
-                const float4 y = x[p][n][r];
-                wild[r] |= !(y.x == y.x && y.y == y.y && y.z == y.z && y.w == y.w);
-                const float top = row16_max(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
-                const float bottom = row16_max(fmaxf(fmaxf(-y.x, -y.y), fmaxf(-y.z, -y.w)));
-                scale[p][n][r] = kv4_scale(top, bottom);
-                wild[r] |= scale[p][n][r] > kMostScale;
+                    for (int z = 0; z < 4; z++) {
+                        const float f = (&x[p][n][r][e].x)[z];
+                        top[r] = __builtin_elementwise_maximum(top[r], f);
+                        bottom[r] = __builtin_elementwise_minimum(bottom[r], f);
+                    }
             }
-        wild[r] = (__ballot(wild[r]) >> (g * 16) & 0xFFFFu) != 0;
-    }
+            const float t = quad_largest(__builtin_elementwise_maximum(
+                half ? top[1] : top[0], other_quad(half ? top[0] : top[1])));
+            const float b = -quad_largest(-__builtin_elementwise_minimum(
+                half ? bottom[1] : bottom[0], other_quad(half ? bottom[0] : bottom[1])));
+            mine[p][n] = kv4_scale(t, -b);
+            wild |= !(t < INFINITY && b > -INFINITY && mine[p][n] <= kMostScale);
+        }
     uint8_t *tile = kv4_tile<D>(kv, (unsigned)id, head);
     uint32_t *scales = kv4_scales<D>(kv, (unsigned)id, head);
-    const uint64_t mine = row_bits(lo, hi);
+    const float keep = wild ? 0.0f : 1.0f, keep2 = other_quad(keep);
+    const uint32_t nibbles[2] = {(half ? keep2 : keep) != 0.0f ? 0x0F0F0F0Fu : 0u,
+                                 (half ? keep : keep2) != 0.0f ? 0x0F0F0F0Fu : 0u};
+    const int odd = c & 1;
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        float q[4][4];
-        // Keys: a row's four dims are half of a word, the next lane's the other half.
+        uint32_t w[2][2][2];  // keys, values; row; 32 dims
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int j = g * 4 + r;
-            kv4_round(x[0][n][r], scale[0][n][r], q[r]);
-            uint32_t w = wild[r] ? 0u : pack_halves(q[r]);
-            w <<= (c & 1) * 4;
-            w |= xor1(w);
-            if (j < lo || j >= hi) continue;  // the same for the row's 16 lanes
-            if ((c & 1) == (r & 1))
-                *(uint32_t *)(tile + n * kPlane + j * (kSpan / 2) + (c >> 1) * 4) = w;
-            if (c == 0) {
-                const auto pair = __builtin_amdgcn_cvt_pkrtz(scale[0][n][r], scale[1][n][r]);
-                scales[n * kBlockPos + j] = wild[r] ? 0x7E007E00u : __builtin_bit_cast(uint32_t, pair);
+        for (int p = 0; p < 2; p++) {
+            const float inverse = 1.0f / mine[p][n];
+            const float s2 = other_quad(mine[p][n]), inverse2 = other_quad(inverse);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                uint32_t q[2][4];
+                kv4_round(x[p][n][r], half == r ? mine[p][n] : s2, half == r ? inverse : inverse2, q);
+#pragma unroll
+                for (int e = 0; e < 2; e++) w[p][r][e] = low_bytes(q[e]) & nibbles[r];
             }
         }
-        // Values: a dim's four rows are half of a word, of the lanes 16 apart.
+        // Keys: four dims are half of a word, the next lane's the other half.
+        const int j = g * 2 + odd;
+        const bool in = j >= lo && j < hi;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            kv4_round(x[1][n][r], scale[1][n][r], q[r]);
-            if (wild[r]) q[r][0] = q[r][1] = q[r][2] = q[r][3] = 0.0f;
+        for (int e = 0; e < 2; e++) {
+            const uint32_t w0 = w[0][0][e] << (odd * 4), w1 = w[0][1][e] << (odd * 4);
+            const uint32_t word = (odd ? w1 : w0) | xor1(odd ? w0 : w1);
+            if (in) *(uint32_t *)(tile + n * kPlane + j * (kSpan / 2) + e * 16 + (c >> 1) * 4) = word;
+            *(uint2 *)&lds[wave][n][e * 8 + c][g * 2] = make_uint2(w[1][0][e], w[1][1][e]);
         }
-#pragma unroll
-        for (int z = 0; z < 4; z++) {
-            const float four[4] = {q[0][z], q[1][z], q[2][z], q[3][z]};
-            uint32_t w = pack_halves(four) << ((g & 1) * 4);
-            w |= (uint32_t)__shfl_xor((int)w, 16);
-            if ((z >> 1) == (g & 1)) lds[wave][(c * 4 + z) * 2 + (g >> 1)] = w;
+        if ((c & 3) == 0 && g * 2 + half >= lo && g * 2 + half < hi) {
+            const auto pair = __builtin_amdgcn_cvt_pkrtz(mine[0][n], mine[1][n]);
+            scales[n * kBlockPos + g * 2 + half] =
+                wild ? 0x7E007E00u : __builtin_bit_cast(uint32_t, pair);
         }
-        wave_lds_fence();
-        uint64_t *dim = (uint64_t *)(tile + (N + n) * kPlane) + lane;
-        uint64_t w = *(const uint64_t *)&lds[wave][lane * 2];
-        if (mine != ~(uint64_t)0) w = (*dim & ~mine) | (w & mine);
-        *dim = w;
-        wave_lds_fence();
     }
-    bool bad = false;
+    wave_lds_fence();
+    // Values: lane (d, a) has rows 4 a .. 4 a + 3 of dims 4 d .. 4 d + 3, half of a word, the
+    // next lane's the other half.
+    const int d = lane >> 2, a = lane & 3;
+    const uint64_t there = row_bits(lo, hi);
+    const uint32_t bits = (uint32_t)(a < 2 ? there : there >> 32);
 #pragma unroll
-    for (int r = 0; r < 4; r++) bad |= wild[r];
-    flag_nonfinite(status, bad);
+    for (int n = 0; n < N; n++) {
+        const uint4 r = *(const uint4 *)&lds[wave][n][d][a * 4];
+        const uint32_t a0 = __builtin_amdgcn_perm(r.y, r.x, 0x05010400u);
+        const uint32_t a1 = __builtin_amdgcn_perm(r.y, r.x, 0x07030602u);
+        const uint32_t b0 = __builtin_amdgcn_perm(r.w, r.z, 0x05010400u);
+        const uint32_t b1 = __builtin_amdgcn_perm(r.w, r.z, 0x07030602u);
+        const uint32_t dim[4] = {__builtin_amdgcn_perm(b0, a0, 0x05040100u),
+                                 __builtin_amdgcn_perm(b0, a0, 0x07060302u),
+                                 __builtin_amdgcn_perm(b1, a1, 0x05040100u),
+                                 __builtin_amdgcn_perm(b1, a1, 0x07060302u)};
+        uint32_t *to = (uint32_t *)(tile + (N + n) * kPlane + (d * 4 + odd * 2) * 8) + (a >> 1);
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+            const uint32_t w0 = dim[z] << (odd * 4), w1 = dim[z + 2] << (odd * 4);
+            uint32_t word = (odd ? w1 : w0) | xor1(odd ? w0 : w1);
+            if (~bits) word = (to[z * 2] & ~bits) | (word & bits);
+            to[z * 2] = word;
+        }
+    }
+    flag_nonfinite(status, wild);
 }
 
 // ------------------------------------------------------------------- reading
