@@ -166,3 +166,19 @@ def test_evict_refuses_bad_streams(pkg, field, value):
 @pytest.mark.parametrize("name", ("write", "read", "attention"))
 def test_a_call_of_no_rows_does_nothing(pkg, name):
     assert call(pkg.load(), name, Args(pkg, rows=0)) == 1
+
+
+def test_attention_refuses_more_positions_than_it_can_count(pkg):
+    """2^30 of a stream; with runs' sums, 2^28 over the heads."""
+    lib = pkg.load()
+    for sums, offsets, most in ((False, True, 2 ** 30 + 1), (False, False, 2 ** 30 + 1),
+                                (True, True, 2 ** 28 // 8), (True, False, 2 ** 30 + 1)):
+        a = Args(pkg, *(() if offsets else (2, 2)))
+        if not offsets:
+            a.rows.offsets, a.rows.max_rows = None, 1
+        a.sums.stride = 2 ** 31
+        assert not call(lib, "attention", a, max_positions=most, work_bytes=1 << 62,
+                        **({} if sums else {"sums": None}))
+        assert b"invalid arguments" in lib.pgpu_last_error()
+        if most > 2 ** 30:
+            assert lib.pgpu_kv4_attention_bytes(ctypes.byref(a.kv), ctypes.byref(a.rows), 1, most, sums) == 0
