@@ -672,11 +672,11 @@ typedef struct {
  * its own, softmax(scale q k) v, into out[r * out_stride + h * head_dim]. The
  * cache already holds the call's rows. One row a stream, or runs of rows.
  * `max_positions` (less than 2^24 with one row a stream; with runs up to 2^30,
- * with their sums less than 2^28 over heads) bounds every cache row's index + 1 (a stream past it is left out, status bit
- * 2). A block whose id is outside the cache weighs nothing
- * (status bit 2; a row that is left no key gets zeros). A stream with first < 0
- * gets zero rows. Strides multiples of 4, pointers 16-byte aligned; out must not
- * overlap q. `sums` NULL: the weights are not added up.
+ * with their sums less than 2^28 over heads) bounds every cache row's index + 1
+ * (a stream past it is left out, status bit 2). A block whose id is outside the
+ * cache weighs nothing (status bit 2; a row that is left no key gets zeros). A
+ * stream with first < 0 gets zero rows. Strides multiples of 4, pointers 16-byte
+ * aligned; out must not overlap q. `sums` NULL: the weights are not added up.
  * A run holds a query's elements and a key's weight in two fp16 terms: to 2^-21
  * of themselves, or 2^-27 of the row's largest element, or of the largest weight
  * times value scale that it sees. One row a stream holds them to 2^-29 of those
