@@ -1404,30 +1404,44 @@ struct Kv4Evict {
 struct Kv4SelectShared {
     uint32_t bins[kBins];
     uint32_t share[2][kEvictWaves];
-    uint32_t bin, above;
+    uint32_t bin, above, count;
     int bad;
 };
+
+// Lane i gets lane i - E's within 16 lanes, the first ones 0; then sums over the lanes up
+// to this one, of 16 and of all.
+template <int E>
+__device__ inline uint32_t row_before(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x110 + E, 0xf, 0xf, false);
+}
+__device__ inline uint32_t row_scan(uint32_t v) {
+    v += row_before<1>(v);
+    v += row_before<2>(v);
+    v += row_before<4>(v);
+    return v + row_before<8>(v);
+}
+__device__ inline uint32_t wave_scan(uint32_t v) {
+    v = row_scan(v);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+}
 
 // The sum over the waves before this one, and (total) over all, of a number of each wave.
 // One barrier: `share` is another's until the one after.
 __device__ inline uint32_t waves_before(uint32_t *share, uint32_t mine, uint32_t &total) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (lane == 0) share[wave] = mine;
     __syncthreads();
-    uint32_t run = share[lane & 15];
-#pragma unroll
-    for (int o = 1; o < kEvictWaves; o <<= 1) {
-        const uint32_t z = __shfl_up(run, o, 16);
-        if ((lane & 15) >= o) run += z;
-    }
-    total = __shfl(run, kEvictWaves - 1);
-    const uint32_t before = __shfl(run, (wave - 1) & 15);
-    return wave ? before : 0;
+    const uint32_t run = row_scan(share[lane & 15]);
+    total = (uint32_t)__builtin_amdgcn_readlane((int)run, kEvictWaves - 1);
+    return wave ? (uint32_t)__builtin_amdgcn_readlane((int)run, (wave - 1) & 15) : 0;
 }
 
 // What stays: a work-group for each (head, layer, stream). The least order that is kept is
-// found digit by digit (11, 11 and 10 bits) from counts in LDS; then the indexes and
-// their sums are dealt out in order.
+// found digit by digit (11, 11 and 10 bits) from counts in LDS, as far as it takes; then
+// the indexes and their sums are dealt out in order. Bound by its chain of barriers and
+// what lies between two: 1 stream of 2011 rows 6.0 us, 64 of 600 to 2048 8.9 (8.5 and
+// 15.7 with all three digits and sums over the lanes through LDS).
 __global__ __launch_bounds__(kEvictThreads) void k_kv4_select(int heads, unsigned blocks,
                                                               Kv4Evict a, int *status) {
     constexpr int H = 8;  // sums that a thread holds
@@ -1444,6 +1458,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_select(int heads, unsigne
     const bool past = n > kMostRows || (n > 0 && ((size_t)n > a.sums_stride ||
                                                   (n - 1) / kBlockPos >= a.table_stride));
     if (threadIdx.x == 0) sh.bad = past;
+    for (int b = threadIdx.x; b < kBins; b += kEvictThreads) sh.bins[b] = 0;
     __syncthreads();
     // The sums of rows threadIdx.x + 1024 k.
     float held[H];
@@ -1469,49 +1484,53 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_select(int heads, unsigne
 
     const int lo = n > a.keep ? a.first : n, hi = n > a.keep ? n - a.newest : n;
     uint32_t need = n > a.keep ? a.keep - a.first - a.newest : 0, least = 0;
+    const bool choose = need != 0;
     auto count_digit = [&](int i, float x, int shift, int width) {
         const uint32_t u = order_of(x);
         if (i >= lo && i < hi && (shift == 32 || (u >> shift) == (least >> shift)))
             atomicAdd(&sh.bins[u >> (shift - width) & ((1u << width) - 1)], 1u);
     };
-    // Of the orders equal to `least`, the first `need` are kept; of the others the larger.
-    if (need) {
+    // Orders from `from` on are kept, and of those equal to `least` the first `need`.
+    uint32_t from = 0;
+    if (choose) {
         int shift = 32;
         for (int digit = 0; digit < 3; digit++) {
             const int width = digit < 2 ? 11 : 10;
-            for (int b = threadIdx.x; b < kBins; b += kEvictThreads) sh.bins[b] = 0;
-            __syncthreads();
 #pragma unroll
             for (int k = 0; k < H; k++)
                 if (k * kEvictThreads < n) count_digit(threadIdx.x + k * kEvictThreads, held[k], shift, width);
             for (int i = threadIdx.x + H * kEvictThreads; i < hi; i += kEvictThreads)
                 count_digit(i, sums[i], shift, width);
             __syncthreads();
-            // Two bins to a thread, from the top.
+            // Two bins to a thread, from the top; cleared for the next digit.
             const int b = kBins - 1 - 2 * (int)threadIdx.x;
             const uint32_t x = sh.bins[b], y = sh.bins[b - 1];
-            uint32_t run = x + y;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t z = __shfl_up(run, o);
-                if (lane >= o) run += z;
-            }
+            sh.bins[b] = sh.bins[b - 1] = 0;
+            const uint32_t run = wave_scan(x + y);
             uint32_t total;
             const uint32_t before =
-                waves_before(sh.share[digit & 1], __shfl(run, 63), total) + run - x - y;
+                waves_before(sh.share[digit & 1], __builtin_amdgcn_readlane((int)run, 63), total) +
+                run - x - y;
             if (before < need && before + x >= need) {
                 sh.bin = b;
                 sh.above = before;
+                sh.count = x;
             } else if (before + x < need && before + x + y >= need) {
                 sh.bin = b - 1;
                 sh.above = before + x;
+                sh.count = y;
             }
             __syncthreads();
             shift -= width;
             least |= sh.bin << shift;
             need -= sh.above;
+            from = least + 1;  // not past 2^32: orders end at infinity's
+            if (need == sh.count) {  // the whole bin
+                from = least;
+                need = 0;
+                break;
+            }
         }
-        __syncthreads();
     }
     // The indexes and their sums, in order. A row comes after those before it that are
     // larger (or not to be chosen among) and as many of the equal ones as are kept.
@@ -1520,7 +1539,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_kv4_select(int heads, unsigne
         const int i = threadIdx.x + round * kEvictThreads;
         const uint32_t u = order_of(x);
         const bool middle = i >= lo && i < hi;
-        const bool more = i < n && (!middle || (need && u > least)), same = need && middle && u == least;
+        const bool more = i < n && (!middle || (choose && u >= from)), same = need && middle && u == least;
         const uint64_t up = __ballot(more), eq = __ballot(same), below = (1ull << lane) - 1;
         uint32_t total;
         const uint32_t before = waves_before(sh.share[round & 1],
@@ -1554,7 +1573,7 @@ __device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0xF70); }
 // was written. Past the last row: the last one again. A row's 32 bytes of keys are four
 // lanes' words. Values lie by dim: a lane takes its dim's 16 numbers of each source block,
 // once where rows side by side are of one, and picks those that stay. Bound by memory
-// where there is much to move: 64 streams of 600 to 2048 rows shrunk to 1024, 100 MB by
+// where there is much to move: 64 streams of 600 to 2048 rows shrunk to 1024, 86 MB by
 // the counters, 25 us (41 with a word loaded for each row, 13 cycles of the L1 cache each;
 // 4 blocks at a time of each source block in a loop: 36).
 template <int D>
