@@ -270,7 +270,8 @@ __global__ __launch_bounds__(256) void k_kv4_write(Kv4 kv, Kv4Rows rows, const f
 
 // ------------------------------------------------------------------- reading
 
-// A wave for each (block of the rows read, head).
+// A wave for each (block of the rows read, head). Bound by the fp32 rows that it writes: 64
+// streams of up to 1024 rows, 8 heads of 64, 258 MB in 43 us.
 template <int D>
 __global__ __launch_bounds__(256) void k_kv4_read(Kv4 kv, Kv4Rows rows, const int32_t *lengths,
                                                   float *k, float *v, size_t row_stride,
@@ -389,6 +390,11 @@ struct Kv4DecodeShared {
 // A lone query's digits stand in rows 4 t .. 4 t + 3 for block t, zeros elsewhere, so
 // that lane (g, i) gets the score of key i of block g: one key to a lane. Of four
 // queries, lane (g, i) has query g's score of key i of each block.
+//
+// Bound by the cache's bytes where contexts are long: 256 streams of up to 8187 keys, 567
+// MB in 93 us, 6.1 TB/s (a plain read reaches 6.5). Else by the chain of a few steps: 64
+// of up to 2048 10.1 us (34 MB; with the scores stored and added up 13.2), one key 3.9, a
+// launch. Heads of 128 with 4 queries, 48 streams of up to 4096: 105 MB in 24 us.
 template <int D, int W, int Q, bool SCORES>
 __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_decode(
     Kv4 kv, Kv4Rows rows, Kv4Decode a, int *status) {
@@ -680,7 +686,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
 
 // The splits of a row's query head joined: D / 4 lanes for 4 dims each, times G that
 // share the splits. `keys`: of a split, or 0: every split has its part of every row, or
-// says that it has none (a maximum of -inf).
+// says that it has none (a maximum of -inf). Bound by its launch: 4.5 us for 256 streams
+// of up to 8 splits, 8 heads of 64; 3.8 for 48 of 4 splits, 32 query heads of 128.
 template <int D, int G>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const float *part_acc,
                                                   const float *part_ml, int group,
@@ -783,6 +790,14 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // the product times the difference, 2^shift; the running maximum is that of score + shift.
 // So no row loses bits to a key that weighs little but whose values are large, nor the
 // other way round.
+//
+// Bound by vector and matrix instructions, which overlap in part: for a tile and 64 keys
+// about 800 cycles of a SIMD's vector units (256 of them the exponentials) and 576 of its
+// matrix cores, 1376 one after the other. 8187 rows of one prompt, 8 heads of 64: 180 us,
+// 137 GFLOP with the two terms, 0.76 PFLOP/s (a library product: 1.3). Eight waves that
+// share a block's staging 193; two copies of the loop's body, masked and not, 346 (they
+// spill). 5 prompts of up to 1777 rows 74 us, 3 of up to 300 13.6: 5 to 8 chunks, one
+// after the other.
 struct Kv4Run {
     const float *q;
     size_t q_stride;
@@ -1255,6 +1270,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 // work-group of W waves for 64 keys of a (stream, key head), which stand in each wave's
 // registers as fp16; the waves take the tiles of 16 rows that see them in turn. A lane
 // adds up its row's weights of 16 keys over the tiles; lanes and waves are added once.
+// Bound by the exponentials and the matrix cores: 5 prompts of up to 1777 rows, 8 heads of
+// 64, 44 us (18 GFLOP with the two terms). 16 waves and queries as the attention's
+// operands; 4 waves that turned the queries themselves took 76.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
                                                                       const float *before,
@@ -1588,8 +1606,9 @@ __global__ __launch_bounds__(kEvictThreads, 8) void k_kv4_move(Kv4 kv, size_t la
     const int32_t *kept = a.kept + (((size_t)layer * streams + s) * kv.heads + head) * a.keep;
     const int32_t *table = a.tables + (size_t)s * a.table_stride;
     const int32_t *to_table = a.to_tables + (size_t)s * a.table_stride;
-    const int count = min(uniform_load(a.lengths + s), a.keep);
-    if (count <= 0 || uniform_load(kept) < 0) return;  // left out
+    const int n = uniform_load(a.lengths + s), count = min(n, a.keep);
+    // Left out, or whole and in place.
+    if (count <= 0 || uniform_load(kept) < 0 || (n <= a.keep && a.to_tables == a.tables)) return;
     const int j = lane >> 2;
 
     // Row j of a wave's e-th block of the round from block b0 on.
