@@ -796,8 +796,8 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // matrix cores, 1376 one after the other. 8187 rows of one prompt, 8 heads of 64: 180 us,
 // 137 GFLOP with the two terms, 0.76 PFLOP/s (a library product: 1.3). Eight waves that
 // share a block's staging 193; two copies of the loop's body, masked and not, 346 (they
-// spill). 5 prompts of up to 1777 rows 74 us, 3 of up to 300 13.6: 5 to 8 chunks, one
-// after the other.
+// spill). 5 prompts of up to 1777 rows and 16 query heads 74 us; 3 of up to 300, behind
+// 200, 13.6: up to 8 chunks, one after the other.
 struct Kv4Run {
     const float *q;
     size_t q_stride;
@@ -1270,9 +1270,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 // work-group of W waves for 64 keys of a (stream, key head), which stand in each wave's
 // registers as fp16; the waves take the tiles of 16 rows that see them in turn. A lane
 // adds up its row's weights of 16 keys over the tiles; lanes and waves are added once.
-// Bound by the exponentials and the matrix cores: 5 prompts of up to 1777 rows, 8 heads of
-// 64, 44 us (18 GFLOP with the two terms). 16 waves and queries as the attention's
-// operands; 4 waves that turned the queries themselves took 76.
+// Bound by the exponentials and the matrix cores: 5 prompts of up to 1777 rows, 16 query
+// heads of 64, 44 us, 19 GFLOP with the two terms (4 waves that turned the queries into
+// operands themselves: 40 us more).
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
                                                                       const float *before,
@@ -1795,17 +1795,28 @@ struct Deal {
 };
 
 Deal deal_rows(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group, int max_positions) {
-    // Work-groups without splits; where they are few, each row's keys are dealt out until
-    // there are about two for every CU, in chunks of 64 and as many at least to each as
-    // pay for the join.
+    // Work-groups without splits. Where they are few, and the keys enough to pay for the
+    // join, each row's keys are dealt out in chunks of 64: of 64 work-groups at most to
+    // 1024 of them, of more to 4 splits (or 512 work-groups).
+    // us, 8 heads, whole / dealt. Few rows, heads of 64 and of 128: 60 of 1 stream behind 180
+    // keys 9.4 / 9.6, 12.7 / 11.1; behind 320 11.9 / 9.6, 16.5 / 11.4; behind 1000 25.5 / 9.5,
+    // 36.3 / 11.9; behind 8000 159 / 13.4, 230 / 19.3; 8 streams behind 4000 83.6 / 25.2, 120 /
+    // 39.6; 1 of 300 rows 10.4 / 11.0, 14.3 / 14.7. More: 16 streams of 64 behind 450 15.4 /
+    // 18.1, 21.8 / 22.8, behind 700 19.0 / 18.0, 27.2 / 23.1, behind 2000 44.0 / 25.9, 63.7 /
+    // 37.7; 1 of 600 rows 16.6 / 14.2, 23.3 / 20.4; of 2000 41.1 / 26.1, 60.2 / 43.5.
+    // Splits 1 / 2 / 4 / 8 / 16: 16 streams of 64 behind 2000 44.0 / 30.8 / 25.5 / 26.2 / 34.6;
+    // 1 of 2000 41.1 / 32.3 / 25.7 / 31.1 / 47.1. More than 512 work-groups: 1 of 8187 rows,
+    // 1 / 2 splits 182 / 173, whose parts take 69 MB: not taken; 4 of 2000 56.9 / 67.1.
     Deal d = {};
     d.tiles = ((r->max_rows + 15) / 16 * group + 3) / 4;
     const size_t groups = (size_t)d.tiles * kv->heads * r->streams;
     const int chunks = (max_positions - 1) / 64 + 1;
-    d.splits = groups >= 512 ? 1 : (int)(1024 / groups);
-    const int least = chunks <= 6 ? chunks : groups <= 64 ? 2 : chunks < 12 ? chunks : 4;
-    if (d.splits > chunks / least) d.splits = chunks / least;
-    if (d.splits > 32) d.splits = 32;
+    d.splits = 1;
+    if (groups < 512 && chunks > (groups > 64 ? 9 : groups > 32 || kv->head_dim == 64 ? 5 : 3)) {
+        d.splits = std::min(groups > 32 ? chunks / 2 : chunks, (int)(1024 / groups));
+        if (groups > 64) d.splits = std::min(d.splits, std::max(4, (int)(512 / groups)));
+        if (d.splits > 32) d.splits = 32;
+    }
     return d;
 }
 
@@ -1948,7 +1959,7 @@ extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_ro
         // Fewer rows or positions may be dealt to more work-groups. Splits times
         // work-groups are at most 1024, a work-group has 64 rows.
         const int chunks = (max_positions - 1) / 64 + 1;
-        const int most = std::min({32, chunks <= 6 ? 1 : chunks / 2,
+        const int most = std::min({32, chunks <= 3 ? 1 : chunks,
                                    1024 / (kv->heads * ((group + 3) / 4))});
         if (most > 1)
             parts = std::min((size_t)1024 * 64, rows->streams * rows->max_rows * wide * most);
