@@ -793,8 +793,8 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 //
 // Bound by vector and matrix instructions, which overlap in part: for a tile and 64 keys
 // about 800 cycles of a SIMD's vector units (256 of them the exponentials) and 576 of its
-// matrix cores, 1376 one after the other. 8187 rows of one prompt, 8 heads of 64: 180 us,
-// 137 GFLOP with the two terms, 0.76 PFLOP/s (a library product: 1.3). Eight waves that
+// matrix cores, 1376 one after the other. 8187 rows of one prompt, 8 heads of 64: 183 us,
+// 137 GFLOP with the two terms, 0.75 PFLOP/s (a library product: 1.3). Eight waves that
 // share a block's staging 193; two copies of the loop's body, masked and not, 346 (they
 // spill). 5 prompts of up to 1777 rows and 16 query heads 74 us; 3 of up to 300, behind
 // 200, 13.6: up to 8 chunks, one after the other.
