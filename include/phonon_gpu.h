@@ -702,8 +702,10 @@ int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_k
  * order, to the cache rows 0 .. keep - 1 of table to_tables (tables' stride;
  * NULL: tables, in place); a stream with keep rows or fewer keeps all. Entry i
  * of a stream's to_tables is entry i of its tables, or a block that no table of
- * the call holds; so are blocks that other streams share kept whole. Rows past
- * the kept ones in their last block hold nothing afterwards.
+ * the call holds. A block that stands in several tables is no to_tables entry of
+ * a stream that is shrunk, unless its 16 rows are all among the first ones: such
+ * a block in place is left alone. Rows past the kept ones in their last block
+ * hold nothing afterwards.
  * sums, to_sums (dev) [layers][streams][heads][sums_stride], sums_stride at
  * least the longest stream's length: to_sums gets the kept rows' sums in order,
  * and is left as it is past them (to_sums may be sums, no other overlap). NaN

@@ -242,3 +242,44 @@ def test_a_cache_past_4_gib(cache, counts):
     c.tables.upload(np.where(c.table % 3 == 0, c.table, blocks - 1 - c.table).astype(np.int32))
     for x, y in zip(small, go()):
         assert np.array_equal(x, y)
+
+
+@pytest.mark.parametrize("first", [32, 47])
+def test_evictions_of_streams_that_share_their_first_blocks(cache, first):
+    """Blocks whose rows are all among the first stay where they are, in every table."""
+    c = cache(3, 2, 64, positions=600)
+    k, v = c.random_rows(1500)
+    c.write([0] * 3, [600, 300, 600], k, v)
+    for s, n in ((1, 300), (2, 600)):  # streams 1 and 2 begin as stream 0 does
+        c.table[s, :2] = c.table[0, :2]
+        c.rows[s] = [np.concatenate([a[:32], b[32:]]) for a, b in zip(c.rows[0], c.rows[s])]
+    c.tables.upload(c.table)
+    both_layers(c)
+    e = Evict(c, 300, first, 20, tied_sums(c, 600))
+    shared = [x[:, c.table[0, :2]] for x in c.raw()]
+    assert e.enqueue()
+    assert c.st() == 0
+    check_evicted(c, e, c.table)
+    for x, y in zip(shared, c.raw()):
+        assert np.array_equal(x, y[:, c.table[0, :2]])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_streams_left_with_rows_of_a_block_take_more(cache, dim):
+    """After an eviction that ends inside a block, new rows go behind the kept ones."""
+    c = cache(2, 2, dim, positions=500)
+    c.fill([400, 90])
+    both_layers(c)
+    e = Evict(c, 75, 3, 9, tied_sums(c, 500))
+    assert e.enqueue()
+    kept = check_evicted(c, e, c.table)
+    k, v = c.random_rows(30)
+    c.rows = [[np.stack([x[kept[1, s, h, :75], h] for h in range(2)], 1) for x in r]
+              for s, r in enumerate(c.rows)]
+    c.write([75, 75], [20, 10], k, v)
+    got = c.read([0, 0], c.lengths())
+    for x, r in zip(got, range(2)):
+        assert np.array_equal(x.astype(np.float64), np.concatenate([model.seen(c.rows[s][r]) for s in range(2)]))
+    a = Attend(c, [75, 75], [20, 10], 2, sums=4)
+    a.check(a.run(), added=a.added())
+    assert c.st() == 0
