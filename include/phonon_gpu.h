@@ -695,8 +695,8 @@ int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_k
                        const float *q, size_t q_stride, int group, float scale,
                        int max_positions, float *out, size_t out_stride,
                        const pgpu_kv4_sums *sums, void *work, size_t work_bytes, int *status);
-/* Shrinks every stream that holds more than `keep` rows (lengths[s], dev) to
- * `keep`, in layers [first_layer, first_layer + layers), each head by itself: the
+/* Shrinks every stream that holds more than `keep` rows (1..2^30; lengths[s], dev)
+ * to `keep`, in layers [first_layer, first_layer + layers), each head by itself: the
  * first `first` rows, the newest `newest` ones, and of the others those with the
  * largest sums, of equal ones the lowest index. Rows are moved as they are, in
  * order, to the cache rows 0 .. keep - 1 of table to_tables (tables' stride;

@@ -638,6 +638,18 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         sh.l[wave][g] = l;
     }
     bool bad = !(top < INFINITY);
+    // What U keys weighed before, on its way while the waves are joined.
+    constexpr int U = 8;
+    const size_t sums_at = ((size_t)s * kv.heads + head) * a.stride;
+    float weighed[U];
+    auto load_weighed = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int e = from + u * 64 * W;
+            weighed[u] = a.before && e < p ? a.before[sums_at + e] : 0.0f;
+        }
+    };
+    if (SCORES && a.after) load_weighed(threadIdx.x);
     __syncthreads();
     for (int e = threadIdx.x; e < live * D; e += 64 * W) {
         const int j = e / D, d = e % D;
@@ -670,17 +682,25 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
     flag_nonfinite(status, bad);
     if (!SCORES || !a.after) return;
     __syncthreads();
-    for (int e = threadIdx.x; e <= p; e += 64 * W) {
-        float part[Q];
+    for (int e0 = threadIdx.x; e0 <= p; e0 += 64 * W * U) {
+        float part[U][Q];
 #pragma unroll
-        for (int j = 0; j < Q; j++)
-            part[j] = j < live ? a.scores[(qh0 + j) * a.max_positions + e] : -INFINITY;
-        const size_t at = ((size_t)s * kv.heads + head) * a.stride + e;
-        float sum = 0.0f;
+        for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int j = 0; j < Q; j++)
-            if (j < live && isfinite(sh.lse[j])) sum += __builtin_amdgcn_exp2f(part[j] - sh.lse[j]);
-        a.after[at] = (a.before && e < p ? a.before[at] : 0.0f) + sum;
+            for (int j = 0; j < Q; j++) {
+                const int e = e0 + u * 64 * W;
+                part[u][j] = j < live && e <= p ? a.scores[(qh0 + j) * a.max_positions + e] : -INFINITY;
+            }
+        if (e0 > (int)threadIdx.x) load_weighed(e0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int e = e0 + u * 64 * W;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < Q; j++)
+                if (j < live && isfinite(sh.lse[j])) sum += __builtin_amdgcn_exp2f(part[u][j] - sh.lse[j]);
+            if (e <= p) a.after[sums_at + e] = weighed[u] + sum;
+        }
     }
 }
 
@@ -2067,7 +2087,7 @@ extern "C" int pgpu_kv4_evict(void *stream, const pgpu_kv4 *kv, int first_layer,
                               size_t sums_stride, int32_t *kept, int *status) {
     if (!cache_ok(kv) || first_layer < 0 || layers <= 0 || first_layer > kv->layers - layers ||
         layers > 65535 || !tables || table_stride <= 0 || !lengths || streams <= 0 ||
-        streams > 65535 || keep < 1 || first < 0 || newest < 0 || first > keep - newest || !sums ||
+        streams > 65535 || keep < 1 || keep > kMostRows || first < 0 || newest < 0 || first > keep - newest || !sums ||
         !to_sums || sums_stride == 0 || !kept || !status)
         return bad_arguments("pgpu_kv4_evict");
     const Kv4Evict a = {tables, to_tables ? to_tables : tables, table_stride, lengths, keep, first,

@@ -182,3 +182,9 @@ def test_attention_refuses_more_positions_than_it_can_count(pkg):
         assert b"invalid arguments" in lib.pgpu_last_error()
         if most > 2 ** 30:
             assert lib.pgpu_kv4_attention_bytes(ctypes.byref(a.kv), ctypes.byref(a.rows), 1, most, sums) == 0
+
+
+def test_evict_refuses_to_keep_more_rows_than_it_can_count(pkg):
+    a = Args(pkg)
+    for keep in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert not call(pkg.load(), "evict", a, keep=keep)
