@@ -393,7 +393,7 @@ struct Kv4DecodeShared {
 //
 // Bound by the cache's bytes where contexts are long: 256 streams of up to 8187 keys, 567
 // MB in 93 us, 6.1 TB/s (a plain read reaches 6.5). Else by the chain of a few steps: 64
-// of up to 2048 10.1 us (34 MB; with the scores stored and added up 13.2), one key 3.9, a
+// of up to 2048 10.0 us (34 MB; with the scores stored and added up 12.7), one key 3.7, a
 // launch. Heads of 128 with 4 queries, 48 streams of up to 4096: 105 MB in 24 us.
 template <int D, int W, int Q, bool SCORES>
 __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_decode(
@@ -1613,7 +1613,8 @@ __device__ inline void loads_done() { __builtin_amdgcn_s_waitcnt(0xF70); }
 // once where rows side by side are of one, and picks those that stay. Bound by memory
 // where there is much to move: 64 streams of 600 to 2048 rows shrunk to 1024, 86 MB by
 // the counters, 25 us (41 with a word loaded for each row, 13 cycles of the L1 cache each;
-// 4 blocks at a time of each source block in a loop: 36).
+// 4 blocks at a time of each source block in a loop: 36). With 8 waves evictions of 64
+// streams take as long, of 2 of up to 6156 rows 52 us with the rows read back, not 43.
 template <int D>
 __global__ __launch_bounds__(kEvictThreads, 8) void k_kv4_move(Kv4 kv, size_t layer_values,
                                                                size_t layer_scales, Kv4Evict a) {
