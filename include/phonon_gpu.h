@@ -678,7 +678,7 @@ typedef struct {
  * stream with first < 0 gets zero rows. Strides multiples of 4, pointers 16-byte
  * aligned; out must not overlap q. `sums` NULL: the weights are not added up.
  * A run holds a query's elements and a key's weight in two fp16 terms: to 2^-21
- * of themselves, or 2^-27 of the row's largest element, or of the largest weight
+ * of themselves, or 2^-25 of the row's largest element, or of the largest weight
  * times value scale that it sees. One row a stream holds them to 2^-29 of those
  * largest ones; what it multiplies and sums of them is exact within 64 keys and
  * as long as no larger one comes.

@@ -804,7 +804,7 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // rescaling is exact and rare; weights stand 2^14 higher, which keeps their low terms
 // normal.
 //
-// So a weight is held to 2^-38 of the row's largest, which serves while value scales are
+// So a weight is held to 2^-37 of the row's largest, which serves while value scales are
 // alike. A block with one that is not within 2^5 of the first block's is far: its values
 // are staged with their scales' exponents made the first block's, and its weights enter
 // the product times the difference, 2^shift; the running maximum is that of score + shift.
