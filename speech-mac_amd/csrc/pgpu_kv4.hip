@@ -377,6 +377,11 @@ struct Kv4DecodeShared {
     float m[W][Q], l[W][Q], lse[Q];
 };
 
+// Not below x, a power of two's exponent.
+__device__ inline float exponent_of(float x) { return (float)((int)(fbits(x) >> 23) - 126); }
+// Scores from which on the exponent of a value scale could be lost in a sum with them.
+constexpr float kVast = 0x1p20f;
+
 // One row a stream. A work-group of W waves takes a split's keys of one (stream, key
 // head) for Q (1 or 4) of its queries, W * 64 keys a step: a wave's 64 are 4 blocks,
 // whose bytes it requests together, the next step's as soon as the registers are free:
@@ -385,7 +390,9 @@ struct Kv4DecodeShared {
 //
 // Weights enter their product times their keys' value scales, below 2^m: m is a whole
 // number, the largest of score + exponent of the value scale so far, so that one fixed
-// point serves the running sums, which stay whole numbers as long as m does.
+// point serves the running sums, which stay whole numbers as long as m does. Where scores
+// pass 2^20 their sum with an exponent would round it away: scores and m are then counted
+// from the largest score so far, whose differences to it are exact.
 //
 // A lone query's digits stand in rows 4 t .. 4 t + 3 for block t, zeros elsewhere, so
 // that lane (g, i) gets the score of key i of block g: one key to a lane. Of four
@@ -518,6 +525,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         if (Q != 1) step = __shfl(step, g * 4);  // of query j0 + g
     };
     float m = kNone, l = 0.0f, acc[A];
+    float zero = 0.0f;  // the score that m counts from
+    bool vast = false;
     // Whole sums of the values, times 2^(34 - m): of dims 16 t + i, or 64 t + lane. A step
     // adds 2^20 at most, and a work-group has 16 steps at most.
     i32x4 sum[A];
@@ -569,11 +578,36 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
             w[t] = seen ? score * step : -INFINITY;
             if (SCORES && b * kBlockPos + i <= p && (Q == 1 || g < live))
                 a.scores[(qh0 + (Q == 1 ? 0 : g)) * a.max_positions + b * kBlockPos + i] = w[t];
-            bound = fmaxf(bound, w[t] + (float)((int)(fbits(large) >> 23) - 126));
+            bound = fmaxf(bound, w[t] + exponent_of(large));
         }
         if (more) load(b0 + 4 * W, false);
         bound = row16_max(bound);
         if (Q == 1) bound = xor16_32_max(bound);
+        if (vast || __any(fabsf(bound) >= kVast && bound > kNone)) {
+            const bool none = m <= kNone;  // no key so far
+            float best = kNone;
+#pragma unroll
+            for (int t = 0; t < S; t++) best = fmaxf(best, w[t]);
+            best = row16_max(best);
+            if (Q == 1) best = xor16_32_max(best);
+            best = ceilf(best);
+            if (!vast && !none) zero = m, m = 0.0f;
+            const float last = zero;
+            zero = none ? best : fmaxf(zero, best);
+            if (!none) m -= zero - last;
+            bound = kNone;
+#pragma unroll
+            for (int t = 0; t < S; t++) {
+                float large = 0.0f;
+#pragma unroll
+                for (int n = 0; n < N; n++) large = fmaxf(large, vs[t][n]);
+                w[t] -= zero;
+                bound = fmaxf(bound, w[t] + exponent_of(large));
+            }
+            bound = row16_max(bound);
+            if (Q == 1) bound = xor16_32_max(bound);
+            vast = true;
+        }
         const float next = fmaxf(m, ceilf(bound));
         if (__any(next != m)) {
             const float less = __builtin_amdgcn_exp2f(m - next);  // m = kNone: 0
@@ -626,7 +660,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         begin();
         for (; steps > 1; steps--) attend(true);
         attend(false);
-        flush(1.0f);
+        // Where scores are vast m is an exponent by itself, below 2^6.
+        const float unit = vast ? __builtin_amdgcn_exp2f(m) : 1.0f;
+        flush(unit);
+        l *= unit;
+        if (vast) m = zero;
     }
     if (wild && lane == 0) atomicOr(status, 2);
     l = row16_sum(l);

@@ -1,0 +1,83 @@
+"""The 4-bit paged KV cache's attention where magnitudes meet, against 64 bits: scores past
+what fp32 counts in ones, spans of a head whose values differ in size, one large value among
+many ordinary ones, the precision that one row a stream is held to; values, not only
+finiteness, and the sums of weights with them."""
+import numpy as np
+import pytest
+
+import kv4_bounds as bounds
+import kv4_model as model
+from test_gpu_kv4 import Attend, cache  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+U = model.U
+
+
+def attend(c, q, counts, group, **kw):
+    """The last rows of every stream, with these queries -> Attend, its output."""
+    n = counts or [1] * c.n
+    a = Attend(c, [m - x for m, x in zip(c.lengths(), n)], counts, group, **kw)
+    a.q = q.astype(np.float32)
+    a.dq.upload(a.q.reshape(a.total, -1))
+    return a, a.run()
+
+
+def streams_of(c, a):
+    """(stream, its rows of the call, keys and values as held, its first row's index)."""
+    at = 0
+    for s, n in enumerate(a.n):
+        yield s, slice(at, at + n), [model.seen(x) for x in c.rows[s]], a.first[s]
+        at += n
+
+
+def two_kinds(c, counts, group, size, large):
+    """Keys of a stream and head that are all the same, or half of that, at the places that
+    `half` says: any two scores are equal, also when they are rounded, or far apart. Queries
+    along them, every second head against them. `size`: of the scores in units of log 2."""
+    rng, dim = c.rng, c.dim
+    lengths = [1, 1, 40, 70, 300, 17, 130]
+    sign = np.where(rng.integers(0, 2, (c.n, c.heads, dim)), 1.0, -1.0)
+    half = [np.zeros(n, bool) for n in lengths]
+    half[2][:] = True
+    half[2][20] = False      # one of full size among halves, in the middle, late, last
+    half[4][:] = True
+    half[4][250] = False
+    half[5][:] = True
+    half[5][16] = False
+    half[6][100:] = True     # halves at the end
+    k = np.concatenate([np.where(h, 0.5, 1.0)[:, None, None] * sign[s][None] * large
+                        for s, h in enumerate(half)])
+    v = rng.standard_normal((sum(lengths), c.heads, dim))
+    v *= np.exp2(rng.integers(-12, 13, (len(v), c.heads, 1)))
+    v[0] *= 57000 / np.abs(v[0]).max()
+    v[1] *= 2.0 ** -17 / np.abs(v[1]).max()
+    c.write([0] * c.n, lengths, k.astype(np.float32), np.clip(v, -57000, 57000).astype(np.float32))
+    assert c.st() == 0
+    n = counts or [1] * c.n
+    held = np.abs(model.seen(np.float32(large) * np.ones(64, np.float32)))[0]
+    q = rng.uniform(1.0, 2.0, (sum(n), c.heads * group, dim))
+    along = np.repeat(np.concatenate([np.repeat(sign[s][None], m, 0) for s, m in enumerate(n)]),
+                      group, 1)
+    flip = np.where(np.arange(c.heads * group) % 2, -1.0, 1.0)[:, None]
+    return along * flip * q * (size / 1.4427 / (c.dim ** -0.5 * 1.5 * dim * held))
+
+
+@pytest.mark.parametrize("most", [None, 8192])
+@pytest.mark.parametrize("size,large", [(2.0 ** 18, 1.0), (1.3e7, 1e4), (3e8, 1.0), (1.15e9, 1e4),
+                                        (2.0 ** 41, 1e4), (1e30, 1.0)])
+@pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (2, 64, 3), (1, 128, 2), (2, 128, 1)])
+@pytest.mark.parametrize("counts", [None])
+def test_scores_of_any_size(cache, counts, heads, dim, group, large, size, most):
+    """Rows see one key, some that weigh the same, or some that weigh nothing beside others;
+    their values differ by 2^24 and more. A key alone weighs 1, whatever its score is."""
+    c = cache(7, heads, dim, positions=300)
+    q = two_kinds(c, counts, group, size, large)
+    a, got = attend(c, q, counts, group, most=most)
+    assert c.st() == 0
+    one = counts is None
+    for s, rows, (k, v), first in streams_of(c, a):
+        x, w = bounds.weights(a.q[rows], k, first, a.scale)
+        assert (np.abs(x[np.isfinite(x)]).max() * 1.4427 > size / 4)
+        out, off = bounds.output(w, v, np.zeros((len(w), heads * group, 1)), one)
+        miss = np.abs(got[rows] - out) - off
+        assert (miss <= 0).all(), (s, miss.max())
