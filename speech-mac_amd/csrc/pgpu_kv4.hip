@@ -377,10 +377,27 @@ struct Kv4DecodeShared {
     float m[W][Q], l[W][Q], lse[Q];
 };
 
-// Not below x, a power of two's exponent.
-__device__ inline float exponent_of(float x) { return (float)((int)(fbits(x) >> 23) - 126); }
-// Scores from which on the exponent of a value scale could be lost in a sum with them.
-constexpr float kVast = 0x1p20f;
+// The exponent of a power of two above |x|; 0 for 0 and for what is not finite.
+__device__ inline float exponent_of(float x) { return (float)__builtin_amdgcn_frexp_expf(x); }
+// Scores from which on the exponent of a value scale could be lost in a sum with them; what
+// stands for all that are larger, and for no key.
+constexpr int kVast = 1 << 20;
+constexpr float kMostBound = 0x1p30f;
+
+// The largest of 16 lanes, and over those 16 and 32 apart. Of whole numbers: a maximum of
+// floats takes four instructions for each lane moved, to quiet NaN, of these one.
+__device__ inline int row16_most(int v) {
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x124, 0xf, 0xf, true));
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true));
+    return max(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true));
+}
+__device__ inline int xor16_32_most(int v) {
+    const auto a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    v = max((int)a[0], (int)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    return max((int)b[0], (int)b[1]);
+}
 
 // One row a stream. A work-group of W waves takes a split's keys of one (stream, key
 // head) for Q (1 or 4) of its queries, W * 64 keys a step: a wave's 64 are 4 blocks,
@@ -390,7 +407,8 @@ constexpr float kVast = 0x1p20f;
 //
 // Weights enter their product times their keys' value scales, below 2^m: m is a whole
 // number, the largest of score + exponent of the value scale so far, so that one fixed
-// point serves the running sums, which stay whole numbers as long as m does. Where scores
+// point serves the running sums, which stay whole numbers as long as m does. Each 64 dims
+// have theirs: a span of small values keeps its bits beside one of large ones. Where scores
 // pass 2^20 their sum with an exponent would round it away: scores and m are then counted
 // from the largest score so far, whose differences to it are exact.
 //
@@ -524,20 +542,23 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         step = top < INFINITY ? a.scale * power_of_2(-e) * 0.0625f : __builtin_nanf("");
         if (Q != 1) step = __shfl(step, g * 4);  // of query j0 + g
     };
-    float m = kNone, l = 0.0f, acc[A];
-    float zero = 0.0f;  // the score that m counts from
+    // l counts in units of 2^m[0], the sums of 64 dims n in units of 2^m[n].
+    float m[N], l = 0.0f, acc[A];
+#pragma unroll
+    for (int n = 0; n < N; n++) m[n] = -kMostBound;
+    float zero = 0.0f;  // the score that m counts from, where scores are vast
     bool vast = false;
-    // Whole sums of the values, times 2^(34 - m): of dims 16 t + i, or 64 t + lane. A step
+    // Whole sums of the values, times 2^34 in their units: of dims 16 t + i, or 64 t + lane. A step
     // adds 2^20 at most, and a work-group has 16 steps at most.
     i32x4 sum[A];
 #pragma unroll
     for (int t = 0; t < A; t++) acc[t] = 0.0f, sum[t] = i32x4{0, 0, 0, 0};
-    auto flush = [&](float less) {
+    auto flush = [&](const float (&less)[N]) {
 #pragma unroll
         for (int t = 0; t < A; t++) {
             const float whole = fmaf((float)sum[t].x, 0x1p24f, fmaf((float)sum[t].y, 0x1p16f,
                                      fmaf((float)sum[t].z, 0x1p8f, (float)sum[t].w)));
-            acc[t] = fmaf(whole, 0x1p-34f, acc[t]) * less;
+            acc[t] = fmaf(whole, 0x1p-34f, acc[t]) * less[t * N / A];
             sum[t] = i32x4{0, 0, 0, 0};
         }
     };
@@ -550,7 +571,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
             for (int t = 0; t < 4; t++)
                 ids[t] = uniform_load(table + min(b0 + 4 * W + t, rows.table_stride - 1));
         // Scores, in units of log 2.
-        float w[S], vs[S][N], bound = kNone;
+        float w[S], vs[S][N];
         i32x4 c[S][N];
 #pragma unroll
         for (int t = 0; t < S; t++)
@@ -568,64 +589,81 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         for (int t = 0; t < S; t++) {
             const int b = b0 + (Q == 1 ? g : t);
             const bool seen = (count >> (Q == 1 ? g : t) & 1) && b * kBlockPos + i <= p;
-            float score = 0.0f, large = 0.0f;
+            float score = 0.0f;
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 score = fmaf(fix_sum(c[t][n]), key_scale(pair[t][n]), score);
                 vs[t][n] = seen ? value_scale(pair[t][n]) : 0.0f;
-                large = fmaxf(large, vs[t][n]);
             }
             w[t] = seen ? score * step : -INFINITY;
             if (SCORES && b * kBlockPos + i <= p && (Q == 1 || g < live))
                 a.scores[(qh0 + (Q == 1 ? 0 : g)) * a.max_positions + b * kBlockPos + i] = w[t];
-            bound = fmaxf(bound, w[t] + exponent_of(large));
+        }
+        // Whole numbers that no score + exponent of a value scale passes.
+        int bound[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            float b = -kMostBound;
+#pragma unroll
+            for (int t = 0; t < S; t++) b = fmaxf(b, w[t] + exponent_of(vs[t][n]));
+            bound[n] = row16_most((int)ceilf(fminf(b, kMostBound)));
+            if (Q == 1) bound[n] = xor16_32_most(bound[n]);
         }
         if (more) load(b0 + 4 * W, false);
-        bound = row16_max(bound);
-        if (Q == 1) bound = xor16_32_max(bound);
-        if (vast || __any(fabsf(bound) >= kVast && bound > kNone)) {
-            const bool none = m <= kNone;  // no key so far
-            float best = kNone;
+        float next[N], best = kNone;
+        const bool before = vast;
+#pragma unroll
+        for (int n = 0; n < N; n++) next[n] = fmaxf(m[n], (float)bound[n]);
+        if (vast || __any(abs(bound[0]) >= kVast)) {
 #pragma unroll
             for (int t = 0; t < S; t++) best = fmaxf(best, w[t]);
             best = row16_max(best);
             if (Q == 1) best = xor16_32_max(best);
             best = ceilf(best);
-            if (!vast && !none) zero = m, m = 0.0f;
-            const float last = zero;
-            zero = none ? best : fmaxf(zero, best);
-            if (!none) m -= zero - last;
-            bound = kNone;
-#pragma unroll
-            for (int t = 0; t < S; t++) {
-                float large = 0.0f;
-#pragma unroll
-                for (int n = 0; n < N; n++) large = fmaxf(large, vs[t][n]);
-                w[t] -= zero;
-                bound = fmaxf(bound, w[t] + exponent_of(large));
-            }
-            bound = row16_max(bound);
-            if (Q == 1) bound = xor16_32_max(bound);
-            vast = true;
+            vast |= __any(best > kNone && abs(bound[0]) >= kVast);
         }
-        const float next = fmaxf(m, ceilf(bound));
-        if (__any(next != m)) {
-            const float less = __builtin_amdgcn_exp2f(m - next);  // m = kNone: 0
+        if (vast) {
+            const bool none = m[0] <= -kMostBound;  // no key so far
+            const float last = before || none ? zero : m[0], from = before ? 0.0f : last;
+            zero = none ? best : fmaxf(last, best);
+#pragma unroll
+            for (int t = 0; t < S; t++) w[t] -= zero;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                if (!none) m[n] = m[n] - from - (zero - last);
+                float b = kNone;
+#pragma unroll
+                for (int t = 0; t < S; t++) b = fmaxf(b, w[t] + exponent_of(vs[t][n]));
+                b = row16_max(b);
+                if (Q == 1) b = xor16_32_max(b);
+                next[n] = fmaxf(m[n], ceilf(b));
+            }
+        }
+        bool grows = false;
+#pragma unroll
+        for (int n = 0; n < N; n++) grows |= next[n] != m[n];
+        if (__any(grows)) {
+            float less[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                less[n] = __builtin_amdgcn_exp2f(m[n] - next[n]);  // no key so far: 0
+                m[n] = next[n];
+            }
             flush(less);
-            l *= less;
-            m = next;
+            l *= less[0];
         }
 #pragma unroll
         for (int t = 0; t < S; t++) {
-            w[t] = __builtin_amdgcn_exp2f(w[t] - m);
+            w[t] = __builtin_amdgcn_exp2f(w[t] - m[0]);
             l += w[t];
         }
 #pragma unroll
         for (int n = 0; n < N; n++) {
+            const float fix = n ? __builtin_amdgcn_exp2f(m[0] - m[n]) * 0x1p30f : 0x1p30f;
             if constexpr (Q == 1) {
                 // Digit t of block g's keys, a quad of keys a word, in row t of dims 16 j ..
                 // 16 j + 15, which are rows 4 j .. 4 j + 3: their first word is quad j's.
-                const uint32_t u = fix_bytes(w[0] * vs[0][n], 0x1p30f);
+                const uint32_t u = fix_bytes(w[0] * vs[0][n], fix);
                 const int word = (int)pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u),
                                             quad_lane<3>(u), sel);
                 const i32x4 turned = {word, row_turn<4>(word), row_turn<8>(word), row_turn<12>(word)};
@@ -639,7 +677,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const uint32_t u = fix_bytes(w[t] * vs[t][n], 0x1p30f);
+                    const uint32_t u = fix_bytes(w[t] * vs[t][n], fix);
                     sh.digits[wave][g * 4 + (i & 3)][t * 4 + (i >> 2)] =
                         pick4(quad_lane<0>(u), quad_lane<1>(u), quad_lane<2>(u), quad_lane<3>(u), sel);
                 }
@@ -660,11 +698,16 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
         begin();
         for (; steps > 1; steps--) attend(true);
         attend(false);
-        // Where scores are vast m is an exponent by itself, below 2^6.
-        const float unit = vast ? __builtin_amdgcn_exp2f(m) : 1.0f;
+        // All in units of 2^m[0]; where scores are vast, whose m is an exponent below 2^6, of
+        // 2^zero.
+        float unit[N];
+#pragma unroll
+        for (int n = 0; n < N; n++)
+            unit[n] = n || vast ? __builtin_amdgcn_exp2f(vast ? m[n] : m[n] - m[0]) : 1.0f;
         flush(unit);
-        l *= unit;
-        if (vast) m = zero;
+        l *= unit[0];
+        if (m[0] <= -kMostBound) m[0] = kNone;
+        if (vast) m[0] = zero;
     }
     if (wild && lane == 0) atomicOr(status, 2);
     l = row16_sum(l);
@@ -672,7 +715,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
 #pragma unroll
     for (int t = 0; t < A; t++) sh.acc[wave][Q == 1 ? 0 : g][Q == 1 ? t * 64 + lane : t * 16 + i] = acc[t];
     if (g < Q && i == 0) {
-        sh.m[wave][g] = ever ? m : -INFINITY;
+        sh.m[wave][g] = ever ? m[0] : -INFINITY;
         sh.l[wave][g] = l;
     }
     bool bad = !(top < INFINITY);

@@ -30,6 +30,17 @@ def streams_of(c, a):
         at += n
 
 
+def check_sums(c, a, s, w, rel):
+    """A stream's sums against weights [rows][q heads][keys] that may be off by rel."""
+    keys = w.shape[-1]
+    w = w[max(0, len(w) - a.counted):].reshape(-1, c.heads, a.group, keys).sum((0, 2))
+    want = np.zeros((c.heads, keys))
+    want[:, :a.first[s]] = a.before0[s, :, :a.first[s]]
+    count = min(a.n[s], a.counted) * a.group
+    miss = np.abs(a.added()[s, :, :keys] - want - w) - rel * w - (count + 2) * U * (want + w) - 1e-37
+    assert (miss <= 0).all(), (s, miss.max())
+
+
 def two_kinds(c, counts, group, size, large):
     """Keys of a stream and head that are all the same, or half of that, at the places that
     `half` says: any two scores are equal, also when they are rounded, or far apart. Queries
@@ -81,3 +92,52 @@ def test_scores_of_any_size(cache, counts, heads, dim, group, large, size, most)
         out, off = bounds.output(w, v, np.zeros((len(w), heads * group, 1)), one)
         miss = np.abs(got[rows] - out) - off
         assert (miss <= 0).all(), (s, miss.max())
+
+
+@pytest.mark.parametrize("most", [None, 8192])
+@pytest.mark.parametrize("apart", [0, 10, 20, 25, -10, -20, -25])
+@pytest.mark.parametrize("heads,group", [(2, 1), (1, 4), (3, 2)])
+@pytest.mark.parametrize("counts", [None])
+def test_spans_whose_values_differ_in_size(cache, counts, heads, group, apart, most):
+    """A head of 128 whose last 64 dims are 2^apart times its first: each span is held to
+    its own largest weighted value."""
+    c = cache(3, heads, 128, positions=300)
+    k, v = c.random_rows(800)
+    v = c.rng.standard_normal(v.shape) * np.where(np.arange(128) < 64, 1.0, 2.0 ** apart)
+    v *= 2.0 ** (-12 if apart > 0 else 12 if apart < -20 else 5 if apart < -10 else 0)
+    c.write([0] * 3, [300, 201, 299], k, np.clip(v, -5e4, 5e4).astype(np.float32))
+    assert c.st() == 0
+    n = sum(counts or [1] * 3)
+    a, got = attend(c, c.rng.standard_normal((n, heads * group, 128)), counts, group, most=most)
+    assert c.st() == 0
+    check_rows(c, a, got, counts is None)
+
+
+def check_rows(c, a, got, one):
+    for s, rows, (k, v), first in streams_of(c, a):
+        x, w = bounds.weights(a.q[rows], k, first, a.scale)
+        ds = bounds.score_error(a.q[rows], k, x, a.scale, one)
+        # exp2 and its argument, of a score and of the maximum.
+        spread = np.where(np.isfinite(x), x.max(-1, keepdims=True) - x, 0).max(-1, keepdims=True)
+        rel = 2 * ds + 8 * U + 4 * U * spread
+        out, off = bounds.output(w, v, rel, one)
+        miss = np.abs(got[rows] - out) - off
+        assert (miss <= 0).all(), (s, miss.max(), (np.abs(got[rows] - out) / off).max())
+        if a.sums:
+            # And the weight by itself: relative to the row's sum.
+            check_sums(c, a, s, w, 2 * rel.max() + (w.shape[-1] + 16) * U + (0 if one else 2.0 ** -20))
+
+
+@pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (1, 64, 4), (2, 128, 1), (1, 128, 3)])
+@pytest.mark.parametrize("most", [None, 8192])
+def test_one_row_a_stream_is_held_to_2_to_the_minus_29(cache, heads, dim, group, most):
+    """Queries and values whose elements differ by 2^20, in one span or the other."""
+    c = cache(4, heads, dim, positions=900)
+    k, v = c.random_rows(1700)
+    v *= np.exp2(c.rng.integers(-11, 10, (len(v), heads, 1))).astype(np.float32)
+    c.write([0] * 4, [899, 1, 500, 300], k, np.clip(v, -5e4, 5e4))
+    q = c.rng.standard_normal((4, heads * group, dim))
+    q *= np.exp2(c.rng.integers(-20, 1, q.shape))
+    a, got = attend(c, q, None, group, most=most, sums=1)
+    assert c.st() == 0
+    check_rows(c, a, got, True)
