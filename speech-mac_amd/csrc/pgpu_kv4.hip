@@ -888,9 +888,10 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // So a weight is held to 2^-37 of the row's largest, which serves while value scales are
 // alike. A block with one that is not within 2^5 of the first block's is far: its values
 // are staged with their scales' exponents made the first block's, and its weights enter
-// the product times the difference, 2^shift; the running maximum is that of score + shift.
-// So no row loses bits to a key that weighs little but whose values are large, nor the
-// other way round.
+// the product times the difference, 2^shift. The products are then held to the largest
+// weight times 2^shift, 2^lift times the largest weight by itself, which the row's sum of
+// weights is held to; that is taken in fp32 as long as the two differ. So no row loses
+// bits to a key that weighs little but whose values are large, nor the other way round.
 //
 // Bound by vector and matrix instructions, which overlap in part: for a tile and 64 keys
 // about 800 cycles of a SIMD's vector units (256 of them the exponentials) and 576 of its
@@ -925,8 +926,9 @@ template <int D>
 struct Kv4RunShared {
     f16x8 k[2][4][D / 32][64];  // [buffer][block][step][lane]
     f16x8 v[2][2][D / 16][64];  // [buffer][pair of blocks][16 dims][lane]
-    float shift[2][4][D / kSpan][kBlockPos];  // [buffer][block][64 dims][key], of far blocks
+    __align__(16) float shift[2][4][D / kSpan][kBlockPos];  // [buffer][block][64 dims][key], of far blocks
     uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far
+    float lift[4][16];          // [wave][row]
 };
 
 // Numbers of the cache become fp16 two at a time, numbers b and b + 2 of a word's halves:
@@ -1188,8 +1190,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     };
 
     // The weights' sums: the row's, taken with the values on the matrix cores (all elements
-    // are the same); where blocks are far, of this lane's keys on the vector units.
+    // are the same); where blocks are far, or a row is lifted (apart), of this lane's keys on
+    // the vector units.
     float m = kNone, l = 0.0f;
+    bool apart = false;
     f32x4 acc[T], total = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1219,36 +1223,51 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (t * 16 + r > last) w[t][r] = -INFINITY;
-        float mx[4], top;
-        if (kind == 0) {
+        const bool rare = kind != 0 || apart;
+        auto shifts = [&](int t, int n) {
+            f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            if (kind >> (8 * t) & 2) z = *(const f32x4 *)&sh.shift[buf][t][n][g * 4];
+            return z;
+        };
+        if (rare)
 #pragma unroll
             for (int t = 0; t < 4; t++)
-                mx[t] = largest(largest(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
-            top = quarters_max(largest(largest(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
-        } else {
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
                 if (kind >> (8 * t) & 1) w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                mx[t] = kNone;
+        float mx[4];
 #pragma unroll
-                for (int n = 0; n < N; n++)
+        for (int t = 0; t < 4; t++)
+            mx[t] = largest(largest(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
+        const float top = quarters_max(largest(largest(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
+        const float least = ceilf(top), mn = max3(m, least, least);
+        bool grows = mn != m;
+        float lower = 1.0f;
+        if (rare) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    const f32x4 z = shifts(t, n);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float z = kind >> (8 * t) & 2 ? sh.shift[buf][t][n][g * 4 + r] : 0.0f;
-                        const float x = fmaf(w[t][r], qs, z);
-                        mx[t] = max3(mx[t], x, x);
+                        const float y = fmaf(w[t][r], qs, -mn) + z[r];
+                        x = max3(x, y, y);
                     }
-            }
-            top = quarters_max(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
+                }
+            const float old = sh.lift[wave][i];
+            const float lift = fmaxf(old + (m - mn), ceilf(quarters_max(x)));
+            sh.lift[wave][i] = lift;
+            lower = __builtin_amdgcn_exp2f(old - lift);
+            grows |= lift != old;
+            apart = __any(lift != 0.0f);
         }
-        const float least = ceilf(top), mn = max3(m, least, least);
-        if (__any(mn != m)) {
-            const float shrink = __builtin_amdgcn_exp2f(m - mn);
+        if (__any(grows)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - mn), both = shrink * lower;
             l *= shrink;
 #pragma unroll
             for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[t][r] *= shrink;
+                for (int r = 0; r < 4; r++) acc[t][r] *= both;
 #pragma unroll
             for (int r = 0; r < 4; r++) total[r] *= shrink;
             m = mn;
@@ -1260,8 +1279,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
             for (int r = 0; r < 4; r++) {
                 w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
             }
-        const bool far = (kind & 0x02020202u) != 0;
-        if (far)
+        if (rare)
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -1269,16 +1287,15 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            if (far)  // from the last 64 dims' shifts to these
+            if (rare)  // from the last 64 dims' shifts to these
 #pragma unroll
-                for (int t = 0; t < 4; t++)
-                    if (kind >> (8 * t) & 2)
+                for (int t = 0; t < 4; t++) {
+                    const f32x4 z = shifts(t, n), y = shifts(t, n ? n - 1 : 0);
 #pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            w[t][r] *= __builtin_amdgcn_exp2f(
-                                sh.shift[buf][t][n][g * 4 + r] -
-                                (n ? sh.shift[buf][t][n - 1][g * 4 + r] : 0.0f));
-            if (n == 0 || far) {
+                    for (int r = 0; r < 4; r++)
+                        w[t][r] *= __builtin_amdgcn_exp2f(z[r] - (n ? y[r] : sh.lift[wave][i]));
+                }
+            if (n == 0 || rare) {
                 f16x2 hi[4][2], lo[4][2];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -1298,7 +1315,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int t = 0; t < 4; t++) v[t] = sh.v[buf][z][t0 + t][lane];
                 if (n == 0) {
-                    const int one = far ? 0 : 0x3C003C00;
+                    const int one = rare ? 0 : 0x3C003C00;
                     const f16x8 ones = __builtin_bit_cast(f16x8, i32x4{one, one, one, one});
                     total = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[z], total, 0, 0, 0);
                     total = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[z], total, 0, 0, 0);
@@ -1317,6 +1334,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 
     if (c0 < c1) {
         request(c0, 0);
+        sh.lift[wave][i] = 0.0f;
         look_first();
         const uint16_t least = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(max(usual - kNear, -17)));
         const uint16_t past = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(min(usual + kNear + 1, 15)));
@@ -1349,7 +1367,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         }
         const size_t at = (((size_t)s * rows.max_rows + r0 + i) * wide + qh) * a.splits + split;
         float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
-        const float f = a.splits > 1 ? 1.0f : base == -INFINITY ? 0.0f : 1.0f / l;
+        const float unit = apart ? __builtin_amdgcn_exp2f(sh.lift[wave][i]) : 1.0f;
+        const float f = a.splits > 1 ? unit : base == -INFINITY ? 0.0f : unit / l;
 #pragma unroll
         for (int t = 0; t < T; t++) {
             const float4 o = make_float4(acc[t][0] * f, acc[t][1] * f, acc[t][2] * f, acc[t][3] * f);

@@ -141,3 +141,69 @@ def test_one_row_a_stream_is_held_to_2_to_the_minus_29(cache, heads, dim, group,
     a, got = attend(c, q, None, group, most=most, sums=1)
     assert c.st() == 0
     check_rows(c, a, got, True)
+
+
+CALLS = {"one": (None, 2, 2, [2100, 1300]), "runs": ([40, 100], 2, 2, [2100, 1300]),
+         # So many work-groups that each has all of its rows' keys.
+         "whole": ([512, 500], 8, 4, [900, 1000])}
+
+
+@pytest.mark.parametrize("above", [0.0, 8.0])
+@pytest.mark.parametrize("larger", [12, 20, 28])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("call", CALLS)
+def test_one_large_value_among_ordinary_ones(cache, call, dim, larger, above):
+    """One key with values 2^larger times the others' and a score `above` the others' (in
+    units of log 2): it raises what the products are held to, not what the row's sum of
+    weights is. All of a row's weights together are 1."""
+    counts, heads, group, lengths = CALLS[call]
+    c = cache(2, heads, dim, positions=max(lengths))
+    rng = c.rng
+    at, n = [70, 133], counts or [1, 1]
+    k, v = c.random_rows(sum(lengths))
+    v = rng.standard_normal(v.shape) * 2.0 ** (-14 if larger > 12 else 0)
+    way = rng.standard_normal((2, heads, dim))  # queries and the large keys lie along it
+    way /= np.sqrt((way ** 2).sum(-1, keepdims=True))
+    for s in range(2):
+        row = at[s] + (lengths[0] if s else 0)
+        v[row] *= 2.0 ** larger
+        if above:
+            k[row] = way[s] * (above / 1.4427 * dim ** 0.5)
+    c.write([0, 0], lengths, k.astype(np.float32), np.clip(v, -5e4, 5e4).astype(np.float32))
+    assert c.st() == 0
+    q = np.concatenate([np.repeat(np.repeat(way[s][None], m, 0), group, 1) for s, m in enumerate(n)])
+    q = q + 0.02 * rng.standard_normal(q.shape)
+    a, got = attend(c, q, counts, group, sums=1)
+    assert c.st() == 0
+    check_rows(c, a, got, counts is None)
+    # With before all zeros: the weights of the last row's queries.
+    a.before.upload(np.zeros_like(a.before0))
+    a.run()
+    total = a.added()
+    for s in range(2):
+        # 16 roundings of a weight. The row's sum of weights: of one row a stream a lane adds
+        # 16, then 6 and 8 levels; in runs each of 33 chunks takes 4 products, of weights in
+        # two truncated terms.
+        t = total[s, :, :lengths[s]].astype(np.float64).sum(-1) / group
+        off = 48 * U if counts is None else 2.0 ** -21 + 150 * U
+        assert (np.abs(t - 1) <= off).all(), (s, t - 1)
+
+
+@pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (1, 64, 3), (2, 128, 2)])
+def test_ordinary_rows_after_large_ones(cache, heads, dim, group):
+    """Blocks of large and of ordinary values in turn, scores that rise and fall along the
+    keys: what the products are held to rises with the ones and falls behind the others."""
+    c = cache(3, heads, dim, positions=1000)
+    k, v = c.random_rows(2600)
+    v = c.rng.standard_normal(v.shape)
+    place = np.arange(2600)
+    v *= np.exp2(np.where(place // 48 % 3 == 1, 12.0, np.where(place // 48 % 3 == 2, -8.0, 0.0)))[:, None, None]
+    k *= np.float32(0.3) + (np.abs(place % 400 - 200) / 200).astype(np.float32)[:, None, None]
+    c.write([0] * 3, [1000, 700, 900], k, np.clip(v, -5e4, 5e4).astype(np.float32))
+    for counts in (None, [100, 700, 60]):
+        n = sum(counts or [1] * 3)
+        for most in (None, 8192):
+            a, got = attend(c, 2 * c.rng.standard_normal((n, heads * group, dim)), counts, group,
+                            most=most, sums=50)
+            assert c.st() == 0
+            check_rows(c, a, got, counts is None)
