@@ -679,9 +679,9 @@ typedef struct {
  * aligned; out must not overlap q. `sums` NULL: the weights are not added up.
  * A run holds a query's elements and a key's weight in two fp16 terms: to 2^-21
  * of themselves, or 2^-25 of the row's largest element, or of the largest weight
- * times value scale that it sees. One row a stream holds them to 2^-29 of those
- * largest ones, each 64 dims to their own; what it multiplies and sums of them is
- * exact within 64 keys and as long as no larger one comes.
+ * times value scale that it sees (of the same 64 dims). One row a stream holds them
+ * to 2^-29 of those largest ones; what it multiplies and sums of them is exact
+ * within 64 keys and as long as no larger one comes.
  * The same call gives the same bits; how the keys are dealt to work-groups goes
  * by the number of streams, max_rows and max_positions, so that in another batch
  * a stream's last bits may differ.

@@ -892,6 +892,7 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // weight times 2^shift, 2^lift times the largest weight by itself, which the row's sum of
 // weights is held to; that is taken in fp32 as long as the two differ. So no row loses
 // bits to a key that weighs little but whose values are large, nor the other way round.
+// Each 64 dims have a first block's exponent, shifts and a lift of their own.
 //
 // Bound by vector and matrix instructions, which overlap in part: for a tile and 64 keys
 // about 800 cycles of a SIMD's vector units (256 of them the exponentials) and 576 of its
@@ -928,7 +929,7 @@ struct Kv4RunShared {
     f16x8 v[2][2][D / 16][64];  // [buffer][pair of blocks][16 dims][lane]
     __align__(16) float shift[2][4][D / kSpan][kBlockPos];  // [buffer][block][64 dims][key], of far blocks
     uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far
-    float lift[4][16];          // [wave][row]
+    float lift[4][D / kSpan][16];  // [wave][64 dims][row]
 };
 
 // Numbers of the cache become fp16 two at a time, numbers b and b + 2 of a word's halves:
@@ -1080,16 +1081,24 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     bool wild = false;
     const int32_t *table = rows.tables + (size_t)s * rows.table_stride;
     const int end = span.first + span.count;
-    // The exponent of the first block's largest value scale (of its first 64 dims).
+    // The exponents of the first block's largest value scales.
     constexpr int kNear = 5;
     auto exponent = [](float x) { return max((int)(fbits(x) >> 23) - 127, -17); };
-    int usual = -17;
-    uint32_t least_near = 0, range_near = 0;  // scale pairs that are not far
+    int usual[N];
+    uint32_t least_near[N], range_near[N];  // scale pairs that are not far
     auto look_first = [&] {
         const int front = table[c0 * 4];
-        const float x = value_scale(kv4_scales<D>(kv, (unsigned)front < kv.blocks ? front : 0, head)[i]);
-        const bool in = c0 * 64 + i < end && x >= kLeastScale && x <= kMostScale;
-        usual = __builtin_amdgcn_readfirstlane(exponent(row16_max(in ? x : kLeastScale)));
+        const uint32_t *sc = kv4_scales<D>(kv, (unsigned)front < kv.blocks ? front : 0, head);
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const float x = value_scale(sc[n * kBlockPos + i]);
+            const bool in = c0 * 64 + i < end && x >= kLeastScale && x <= kMostScale;
+            usual[n] = __builtin_amdgcn_readfirstlane(exponent(row16_max(in ? x : kLeastScale)));
+            const uint16_t least = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(max(usual[n] - kNear, -17)));
+            const uint16_t past = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(min(usual[n] + kNear + 1, 15)));
+            least_near[n] = (uint32_t)least << 16;
+            range_near[n] = ((uint32_t)min(past, kMostFast) << 16) - least_near[n];
+        }
     };
     auto request = [&](int c, int nth) {
         const int j = nth & 63;
@@ -1119,7 +1128,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         bool odd = false;
 #pragma unroll
         for (int n = 0; n < N; n++)
-            odd |= ks[n] - least_near >= range_near || (uint16_t)ks[n] > kMostFast;
+            odd |= ks[n] - least_near[n] >= range_near[n] || (uint16_t)ks[n] > kMostFast;
         odd = c * 64 + wave * 16 + 16 > end || __any(odd);
         uint32_t kind = (unsigned)raw >= kv.blocks ? 1 : 0;
         if (!odd) {
@@ -1155,7 +1164,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
             for (int n = 0; n < N; n++)
                 far |= c * 64 + wave * 16 + i < end && ks[n] < 0x7C000000u &&
-                       ks[n] - least_near >= range_near;
+                       ks[n] - least_near[n] >= range_near[n];
             far = __any(far);
             if (far) kind |= 2;
 #pragma unroll
@@ -1171,7 +1180,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
                     x[r] = value_scale(vs[n][r]);
                     if (!(x[r] <= kMostScale) || x[r] < 0.0f) x[r] = 0.0f;
                     if (far) {
-                        const int shift = x[r] >= kLeastScale ? exponent(x[r]) - usual : 0;
+                        const int shift = x[r] >= kLeastScale ? exponent(x[r]) - usual[n] : 0;
                         x[r] = ldexpf(x[r], -shift);
                         if (i == 0) sh.shift[buf][wave][n][g * 4 + r] = (float)shift;
                     }
@@ -1240,13 +1249,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         const float top = quarters_max(largest(largest(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
         const float least = ceilf(top), mn = max3(m, least, least);
         bool grows = mn != m;
-        float lower = 1.0f;
+        float lower[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) lower[n] = 1.0f;
         if (rare) {
-            float x = -INFINITY;
+            bool lifted = false;
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int n = 0; n < N; n++) {
+                float x = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < N; n++) {
+                for (int t = 0; t < 4; t++) {
                     const f32x4 z = shifts(t, n);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
@@ -1254,20 +1266,22 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
                         x = max3(x, y, y);
                     }
                 }
-            const float old = sh.lift[wave][i];
-            const float lift = fmaxf(old + (m - mn), ceilf(quarters_max(x)));
-            sh.lift[wave][i] = lift;
-            lower = __builtin_amdgcn_exp2f(old - lift);
-            grows |= lift != old;
-            apart = __any(lift != 0.0f);
+                const float old = sh.lift[wave][n][i];
+                const float lift = fmaxf(old + (m - mn), ceilf(quarters_max(x)));
+                sh.lift[wave][n][i] = lift;
+                lower[n] = __builtin_amdgcn_exp2f(old - lift);
+                grows |= lift != old;
+                lifted |= lift != 0.0f;
+            }
+            apart = __any(lifted);
         }
         if (__any(grows)) {
-            const float shrink = __builtin_amdgcn_exp2f(m - mn), both = shrink * lower;
+            const float shrink = __builtin_amdgcn_exp2f(m - mn);
             l *= shrink;
 #pragma unroll
             for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[t][r] *= both;
+                for (int r = 0; r < 4; r++) acc[t][r] *= shrink * lower[t / 4];
 #pragma unroll
             for (int r = 0; r < 4; r++) total[r] *= shrink;
             m = mn;
@@ -1287,14 +1301,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            if (rare)  // from the last 64 dims' shifts to these
+            if (rare) {  // from the last 64 dims' shifts and lift to these
+                const float down = sh.lift[wave][n][i] - (n ? sh.lift[wave][n - 1][i] : 0.0f);
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const f32x4 z = shifts(t, n), y = shifts(t, n ? n - 1 : 0);
+                    f32x4 z = shifts(t, n);
+                    if (n) z -= shifts(t, n - 1);
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        w[t][r] *= __builtin_amdgcn_exp2f(z[r] - (n ? y[r] : sh.lift[wave][i]));
+                    for (int r = 0; r < 4; r++) w[t][r] *= __builtin_amdgcn_exp2f(z[r] - down);
                 }
+            }
             if (n == 0 || rare) {
                 f16x2 hi[4][2], lo[4][2];
 #pragma unroll
@@ -1334,12 +1350,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 
     if (c0 < c1) {
         request(c0, 0);
-        sh.lift[wave][i] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++) sh.lift[wave][n][i] = 0.0f;
         look_first();
-        const uint16_t least = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(max(usual - kNear, -17)));
-        const uint16_t past = __builtin_bit_cast(uint16_t, (_Float16)power_of_2(min(usual + kNear + 1, 15)));
-        least_near = (uint32_t)least << 16;
-        range_near = ((uint32_t)min(past, kMostFast) << 16) - least_near;
         stage(0, c0);
         __syncthreads();
         for (int c = c0, n = 0; c < c1; c += stride, n++) {
@@ -1367,11 +1380,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         }
         const size_t at = (((size_t)s * rows.max_rows + r0 + i) * wide + qh) * a.splits + split;
         float *dst = a.splits == 1 ? a.out + row * a.out_stride + (size_t)qh * D : a.part_acc + at * D;
-        const float unit = apart ? __builtin_amdgcn_exp2f(sh.lift[wave][i]) : 1.0f;
-        const float f = a.splits > 1 ? unit : base == -INFINITY ? 0.0f : unit / l;
+        float f[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const float unit = apart ? __builtin_amdgcn_exp2f(sh.lift[wave][n][i]) : 1.0f;
+            f[n] = a.splits > 1 ? unit : base == -INFINITY ? 0.0f : unit / l;
+        }
 #pragma unroll
         for (int t = 0; t < T; t++) {
-            const float4 o = make_float4(acc[t][0] * f, acc[t][1] * f, acc[t][2] * f, acc[t][3] * f);
+            const float4 o = make_float4(acc[t][0] * f[t / 4], acc[t][1] * f[t / 4], acc[t][2] * f[t / 4],
+                                         acc[t][3] * f[t / 4]);
             bad |= !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w));
             *(float4 *)(dst + t * 16 + g * 4) = o;
         }

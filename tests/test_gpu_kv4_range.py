@@ -97,7 +97,7 @@ def test_scores_of_any_size(cache, counts, heads, dim, group, large, size, most)
 @pytest.mark.parametrize("most", [None, 8192])
 @pytest.mark.parametrize("apart", [0, 10, 20, 25, -10, -20, -25])
 @pytest.mark.parametrize("heads,group", [(2, 1), (1, 4), (3, 2)])
-@pytest.mark.parametrize("counts", [None])
+@pytest.mark.parametrize("counts", [None, [40, 33, 150]], ids=["one", "runs"])
 def test_spans_whose_values_differ_in_size(cache, counts, heads, group, apart, most):
     """A head of 128 whose last 64 dims are 2^apart times its first: each span is held to
     its own largest weighted value."""
