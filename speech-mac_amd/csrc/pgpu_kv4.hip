@@ -883,7 +883,9 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // product's operand as they stand (O^T = V^T P^T). A query and a weight are two fp16
 // terms (22 bits). The running maximum is a whole number (in units of log 2), so that
 // rescaling is exact and rare; weights stand 2^14 higher, which keeps their low terms
-// normal.
+// normal. A score less the maximum is one multiply-add, which is
+// within 1/4 of what the rounded score less the maximum is, up to 2^23; where queries or
+// keys are so large that scores can pass that, they are rounded as the maximum is.
 //
 // So a weight is held to 2^-37 of the row's largest, which serves while value scales are
 // alike. A block with one that is not within 2^5 of the first block's is far: its values
@@ -928,7 +930,7 @@ struct Kv4RunShared {
     f16x8 k[2][4][D / 32][64];  // [buffer][block][step][lane]
     f16x8 v[2][2][D / 16][64];  // [buffer][pair of blocks][16 dims][lane]
     __align__(16) float shift[2][4][D / kSpan][kBlockPos];  // [buffer][block][64 dims][key], of far blocks
-    uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far
+    uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far; bit 2: of large keys
     float lift[4][D / kSpan][16];  // [wave][64 dims][row]
 };
 
@@ -954,6 +956,10 @@ __device__ inline f16x8 word_f16(uint32_t w, f16x2 s2) {
 // is 1 + n / 16 with an exponent before it; times 16 s, less 24 s, which is exact, as
 // long as 24 s is an fp16 number.
 constexpr uint16_t kMostFast = 0x6950;  // 2720
+// Key scales up to 64 are ordinary: a score is less than the query's largest element, 2^15,
+// times 8 * 64 in each dim.
+constexpr uint16_t kOrdinary = 0x5400;
+constexpr float kMostFused = 0x1p23f;  // of scores that are not vast
 struct PairBits {
     uint32_t mask = 0x03C003C0u, one = 0x3C003C00u;
     // In registers: an AND-OR takes no literals.
@@ -1123,12 +1129,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         }
     };
     auto stage = [&](int buf, int c) {
-        // Most blocks are full, and have value scales that are not far and key scales that
-        // pair_f16 takes. Scales order like their bits.
+        // Most blocks are full, and have value scales that are not far and key scales of
+        // ordinary size. Scales order like their bits.
         bool odd = false;
 #pragma unroll
         for (int n = 0; n < N; n++)
-            odd |= ks[n] - least_near[n] >= range_near[n] || (uint16_t)ks[n] > kMostFast;
+            odd |= ks[n] - least_near[n] >= range_near[n] || (uint16_t)ks[n] > kOrdinary;
         odd = c * 64 + wave * 16 + 16 > end || __any(odd);
         uint32_t kind = (unsigned)raw >= kv.blocks ? 1 : 0;
         if (!odd) {
@@ -1160,13 +1166,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
             }
         } else {
             // Rows that nothing was written to, or that were not finite, are not far.
-            bool far = false;
+            const bool held = c * 64 + wave * 16 + i < end;
+            bool far = false, large = false;
 #pragma unroll
-            for (int n = 0; n < N; n++)
-                far |= c * 64 + wave * 16 + i < end && ks[n] < 0x7C000000u &&
-                       ks[n] - least_near[n] >= range_near[n];
+            for (int n = 0; n < N; n++) {
+                large |= held && (uint16_t)ks[n] > kOrdinary && (uint16_t)ks[n] < 0x7C00;
+                far |= held && ks[n] < 0x7C000000u && ks[n] - least_near[n] >= range_near[n];
+            }
             far = __any(far);
             if (far) kind |= 2;
+            if (__any(large)) kind |= 4;
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 const f16x2 s2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(ks[n], ks[n], 0x01000100u));
@@ -1203,6 +1212,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     // the vector units.
     float m = kNone, l = 0.0f;
     bool apart = false;
+    // Queries so large that scores of keys of ordinary size can be vast.
+    const bool hot = __any(qs * (D * 0x1p24f) >= kMostFused && biggest < INFINITY);
     f32x4 acc[T], total = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < T; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1232,7 +1243,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (t * 16 + r > last) w[t][r] = -INFINITY;
-        const bool rare = kind != 0 || apart;
+        const bool rare = kind != 0 || apart || hot;
         auto shifts = [&](int t, int n) {
             f32x4 z = {0.f, 0.f, 0.f, 0.f};
             if (kind >> (8 * t) & 2) z = *(const f32x4 *)&sh.shift[buf][t][n][g * 4];
@@ -1262,7 +1273,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
                     const f32x4 z = shifts(t, n);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float y = fmaf(w[t][r], qs, -mn) + z[r];
+                        const float y = (w[t][r] * qs - mn) + z[r];
                         x = max3(x, y, y);
                     }
                 }
@@ -1287,17 +1298,20 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
             m = mn;
         }
         const float base = 14.0f - m;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
-            }
-        if (rare)
+        if (!rare) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) l += w[t][r];
+                for (int r = 0; r < 4; r++) w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    w[t][r] = __builtin_amdgcn_exp2f((w[t][r] * qs - m) + 14.0f);
+                    l += w[t][r];
+                }
+        }
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int n = 0; n < N; n++) {
@@ -1369,7 +1383,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     l = xor16_32_sum(l) + total[0];
     bool bad = false;
     if (i < live) {
-        float base = m - 14.0f;
+        float base = m;
         if (l == 0.0f) {
             // No key of this split counts (zeros), or all scores are -inf (not finite).
             bool any = false;
@@ -1384,7 +1398,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
         for (int n = 0; n < N; n++) {
             const float unit = apart ? __builtin_amdgcn_exp2f(sh.lift[wave][n][i]) : 1.0f;
-            f[n] = a.splits > 1 ? unit : base == -INFINITY ? 0.0f : unit / l;
+            f[n] = a.splits > 1 ? unit * 0x1p-14f : base == -INFINITY ? 0.0f : unit / l;
         }
 #pragma unroll
         for (int t = 0; t < T; t++) {
@@ -1395,9 +1409,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         }
         if (g == 0) {
             if (a.splits > 1)
-                *(float2 *)(a.part_ml + at * 2) = make_float2(base, l);
+                *(float2 *)(a.part_ml + at * 2) = make_float2(base, l * 0x1p-14f);
             else if (a.lse)
-                a.lse[row * wide + qh] = base == -INFINITY ? INFINITY : base + __log2f(l);
+                a.lse[row * wide + qh] = base == -INFINITY ? INFINITY : base + (__log2f(l) - 14.0f);
         }
         bad |= !(biggest < INFINITY);
     }

@@ -77,7 +77,7 @@ def two_kinds(c, counts, group, size, large):
 @pytest.mark.parametrize("size,large", [(2.0 ** 18, 1.0), (1.3e7, 1e4), (3e8, 1.0), (1.15e9, 1e4),
                                         (2.0 ** 41, 1e4), (1e30, 1.0)])
 @pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (2, 64, 3), (1, 128, 2), (2, 128, 1)])
-@pytest.mark.parametrize("counts", [None])
+@pytest.mark.parametrize("counts", [None, [1, 1, 25, 60, 55, 17, 40]], ids=["one", "runs"])
 def test_scores_of_any_size(cache, counts, heads, dim, group, large, size, most):
     """Rows see one key, some that weigh the same, or some that weigh nothing beside others;
     their values differ by 2^24 and more. A key alone weighs 1, whatever its score is."""
