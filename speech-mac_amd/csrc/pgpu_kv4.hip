@@ -363,18 +363,30 @@ struct Kv4Decode {
     float *out;  // splits = 1: the rows themselves (else NULL)
     size_t out_stride;
     // With sums:
-    float *lse;  // [streams][query heads]: log2 of the sum of 2^score
+    // [streams][query heads]: a weight is 2^(score - top) * share; top is infinite where the
+    // row did not come out finite. One number, the logarithm of the sum, would be rounded in
+    // units of the score.
+    float *tops, *shares;
     float *scores;  // [streams][query heads][max_positions], in units of log 2
     const float *before;
     float *after;  // NULL: another launch adds the weights up
     size_t stride;
 };
 
+// A row's top and share, from its sum of weights in units of 2^m: the top is near the sum's
+// logarithm, so that the share is near 1 (or m, where that is too large to be added to).
+// (The reciprocal is off by one step.)
+__device__ inline float2 kv4_share(float m, float total) {
+    const bool fine = total > 0.0f && total < INFINITY && fabsf(m) < INFINITY;
+    const float top = m + (float)__builtin_amdgcn_frexp_expf(total);
+    return make_float2(fine ? top : INFINITY, __builtin_amdgcn_exp2f(top - m) * __builtin_amdgcn_rcpf(total));
+}
+
 template <int D, int W, int Q>
 struct Kv4DecodeShared {
     __align__(16) uint32_t digits[Q == 1 ? 1 : W][16][16];  // [row][block, quad of keys]
     float acc[W][Q][D];
-    float m[W][Q], l[W][Q], lse[Q];
+    float m[W][Q], l[W][Q], top[Q], share[Q];
 };
 
 // The exponent of a power of two above |x|; 0 for 0 and for what is not finite.
@@ -750,8 +762,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
             o = mx == -INFINITY ? 0.0f : o / total;
             a.out[(size_t)s * a.out_stride + ((size_t)head * a.group + j0 + j) * D + d] = o;
             if (SCORES && d == 0) {
-                const float lse = mx == -INFINITY ? INFINITY : mx + __log2f(total);
-                a.lse[qh0 + j] = sh.lse[j] = lse;
+                const float2 x = kv4_share(mx, total);
+                a.tops[qh0 + j] = sh.top[j] = x.x;
+                a.shares[qh0 + j] = sh.share[j] = x.y;
             }
             bad |= !isfinite(o);
         } else {
@@ -779,7 +792,8 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < Q; j++)
-                if (j < live && isfinite(sh.lse[j])) sum += __builtin_amdgcn_exp2f(part[u][j] - sh.lse[j]);
+                if (j < live && sh.top[j] < INFINITY)
+                    sum = fmaf(__builtin_amdgcn_exp2f(part[u][j] - sh.top[j]), sh.share[j], sum);
             if (e <= p) a.after[sums_at + e] = weighed[u] + sum;
         }
     }
@@ -794,7 +808,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const fl
                                                   const float *part_ml, int group,
                                                   int max_positions, int splits, int keys,
                                                   float *out, size_t out_stride, float *lse,
-                                                  int *status) {
+                                                  float *shares, int *status) {
     constexpr int L = D / 4, M = L * G;
     const int s = blockIdx.z, wide = kv.heads * group;
     const size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -854,7 +868,13 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const fl
     // No key that counts: zeros. Scores that are all -inf: not finite.
     if (mx != -INFINITY) o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
     *(float4 *)dst = o;
-    if (lse && d == 0) lse[row * wide + qh] = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+    if (shares && d == 0) {
+        const float2 x = kv4_share(mx, total);
+        lse[row * wide + qh] = x.x;
+        shares[row * wide + qh] = x.y;
+    } else if (lse && d == 0) {
+        lse[row * wide + qh] = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+    }
     flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
 }
 
@@ -869,8 +889,8 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
     const size_t qh0 = ((size_t)s * kv.heads + head) * a.group;
     float sum = 0.0f;
     for (int j = 0; j < a.group; j++) {
-        const float lse = a.lse[qh0 + j], score = a.scores[(qh0 + j) * a.max_positions + p];
-        if (isfinite(lse)) sum += __builtin_amdgcn_exp2f(score - lse);
+        const float top = a.tops[qh0 + j], score = a.scores[(qh0 + j) * a.max_positions + p];
+        if (top < INFINITY) sum = fmaf(__builtin_amdgcn_exp2f(score - top), a.shares[qh0 + j], sum);
     }
     a.after[at] = (a.before && p < span.first ? a.before[at] : 0.0f) + sum;
 }
@@ -2010,7 +2030,7 @@ Deal deal_of(const pgpu_kv4 *kv, int streams, int group, int max_positions) {
 }
 
 // The workspace of one row a stream: parts of `parts` (row, query head, split), then the
-// rows' log sums and their scores.
+// rows' tops and shares, and their scores.
 size_t parts_bytes(const pgpu_kv4 *kv, size_t parts) {
     return parts * (kv->head_dim + 2) * sizeof(float);
 }
@@ -2026,7 +2046,7 @@ size_t run_sums_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group) {
 template <int D>
 int join(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
          const float *part_acc, const float *part_ml, int group, int max_positions, float *out,
-         size_t out_stride, float *lse, int *status) {
+         size_t out_stride, float *lse, float *shares, int *status) {
     // Many splits of few rows: a wave for each, spread over the CUs; else few splits of
     // many rows. us with the attention, 8 heads of 64: 60 rows behind 8000 keys 13.2 / 17.6, 8
     // streams of them behind 4000 24.0 / 25.7, a row behind 8186 9.4 / 9.9; 2000 rows (4
@@ -2035,12 +2055,12 @@ int join(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal
     if (d.splits >= 8 && items * streams <= 4096)
         hipLaunchKernelGGL((k_kv4_join<D, 256 / D>), dim3((unsigned)items, 1, streams), dim3(64), 0,
                            st, c, r, part_acc, part_ml, group, max_positions, d.splits, d.keys, out,
-                           out_stride, lse, status);
+                           out_stride, lse, shares, status);
     else
         hipLaunchKernelGGL((k_kv4_join<D, 1>),
                            dim3((unsigned)((items * (D / 4) + 255) / 256), 1, streams), dim3(256), 0,
                            st, c, r, part_acc, part_ml, group, max_positions, d.splits, d.keys, out,
-                           out_stride, lse, status);
+                           out_stride, lse, shares, status);
     return launch_ok("pgpu_kv4_attention");
 }
 
@@ -2073,7 +2093,7 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
 #undef KV4_DECODE
     if (!launch_ok("pgpu_kv4_attention")) return 0;
     if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
-                                 a.max_positions, a.out, a.out_stride, a.lse, status))
+                                 a.max_positions, a.out, a.out_stride, a.tops, a.shares, status))
         return 0;
     if (!sums || one.after) return 1;
     one.after = sums->after;
@@ -2089,7 +2109,7 @@ int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, con
                        r, a, status);
     if (!launch_ok("pgpu_kv4_attention")) return 0;
     if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
-                                 a.max_positions, a.out, a.out_stride, a.lse, status))
+                                 a.max_positions, a.out, a.out_stride, a.lse, nullptr, status))
         return 0;
     if (!sums) return 1;
     constexpr int W = D == 64 ? 16 : 8;
@@ -2130,7 +2150,7 @@ extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_ro
         if (d.splits > 1) parts = std::max(parts, n * wide * d.splits);
     }
     return parts_bytes(kv, parts) +
-           (with_sums ? rows->streams * wide * (1 + (size_t)max_positions) * sizeof(float) : 0);
+           (with_sums ? rows->streams * wide * (2 + (size_t)max_positions) * sizeof(float) : 0);
 }
 
 extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
@@ -2158,7 +2178,7 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
         if (d.splits > 65535) return bad_arguments("pgpu_kv4_attention");
         const size_t parts = d.splits > 1 ? rows->streams * wide * d.splits : 0;
         const size_t need = parts_bytes(kv, parts) +
-                            (sums ? rows->streams * wide * (1 + (size_t)max_positions) * sizeof(float)
+                            (sums ? rows->streams * wide * (2 + (size_t)max_positions) * sizeof(float)
                                   : 0);
         if (need && (!work || !aligned(work, 16) || work_bytes < need))
             return bad_arguments("pgpu_kv4_attention (workspace)");
@@ -2174,8 +2194,9 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
         a.out = out;
         a.out_stride = out_stride;
         if (sums) {
-            a.lse = floats + parts * (kv->head_dim + 2);
-            a.scores = a.lse + rows->streams * wide;
+            a.tops = floats + parts * (kv->head_dim + 2);
+            a.shares = a.tops + rows->streams * wide;
+            a.scores = a.shares + rows->streams * wide;
             a.before = sums->before;
             a.stride = sums->stride;
         }

@@ -95,6 +95,28 @@ def test_scores_of_any_size(cache, counts, heads, dim, group, large, size, most)
 
 
 @pytest.mark.parametrize("most", [None, 8192])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 18, 1.3e7, 3e8, 1.15e9, 2.0 ** 41, 1e30])
+@pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (2, 64, 3), (1, 128, 2), (1, 128, 8)])
+@pytest.mark.parametrize("counts", [None])
+def test_sums_of_weights_of_scores_of_any_size(cache, counts, heads, dim, group, size, most):
+    """The same keys' weights: 1, or one part of as many as weigh the same. Runs hold a row's
+    sum of weights to 2^-23, or to 2^-16 where the scores pass 2^23."""
+    c = cache(7, heads, dim, positions=300)
+    q = two_kinds(c, counts, group, size, 1.0)
+    a, _ = attend(c, q, counts, group, most=most, sums=30)
+    assert c.st() == 0
+    for s, rows, (k, _), first in streams_of(c, a):
+        x, w = bounds.weights(a.q[rows], k, first, a.scale)
+        if size < 2000:  # halves weigh something: only rows that see one kind are exact
+            w = np.where(w < 2.0 ** -100, 0, w)
+        # exp2 twice and a logarithm or a division: 16 roundings; a row's sum: one for
+        # every key, and in runs two truncated terms of each weight.
+        rel = (w.shape[-1] + 16) * U + (0 if counts is None else
+                                        2.0 ** -20 if size < 2.0 ** 22 else 2.0 ** -15)
+        check_sums(c, a, s, w, rel)
+
+
+@pytest.mark.parametrize("most", [None, 8192])
 @pytest.mark.parametrize("apart", [0, 10, 20, 25, -10, -20, -25])
 @pytest.mark.parametrize("heads,group", [(2, 1), (1, 4), (3, 2)])
 @pytest.mark.parametrize("counts", [None, [40, 33, 150]], ids=["one", "runs"])
