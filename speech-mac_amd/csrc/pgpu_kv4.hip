@@ -799,6 +799,32 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_de
     }
 }
 
+// Where a tile of 16 rows and a query head stand among rows + 16 * streams rows.
+__device__ inline size_t tile_at(const Kv4Span &span, int s, int r0, int qh, int wide) {
+    return (size_t)(span.row0 + 16 * s + r0) * wide + (size_t)qh * 16;
+}
+
+constexpr float kMostFused = 0x1p23f;  // of scores that are not vast
+constexpr uint32_t kExponent = 0x7F800000, kVastRow = 0x80000000;
+
+// A run's row as its sums read it: a weight is 2^(score - top) * share, from its sum of
+// weights in units of 2^m. The share, a number in [1/2, 1), stands in the last 23 bits of the
+// row's word, whose exponent is that of the scores' factor. A vast row's top is m, and 16 bits
+// of the share stand behind 7 of the sum's exponent.
+__device__ inline uint32_t kv4_factor(float m, float total, uint32_t factor, float &top) {
+    const bool fine = total > 0.0f && total < INFINITY && fabsf(m) < INFINITY;
+    const float f = bitsf((fbits(total) & ~kExponent) | 0x3F800000u);  // [1, 2)
+    int e = (int)(fbits(total) >> 23) - 127;
+    uint32_t share = 0;  // of 1 / 2
+    if (f == 1.0f)
+        e--;
+    else
+        share = fbits(1.0f / f) & ~kExponent;
+    const bool vast = fabsf(m) >= kMostFused;
+    top = fine ? (vast ? m : m + (float)e) : INFINITY;
+    return (factor & kExponent) | (vast ? kVastRow | (uint32_t)((e + 64) & 127) << 16 | share >> 7 : share);
+}
+
 // The splits of a row's query head joined: D / 4 lanes for 4 dims each, times G that
 // share the splits. `keys`: of a split, or 0: every split has its part of every row, or
 // says that it has none (a maximum of -inf). Bound by its launch: 4.5 us for 256 streams
@@ -807,8 +833,9 @@ template <int D, int G>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const float *part_acc,
                                                   const float *part_ml, int group,
                                                   int max_positions, int splits, int keys,
-                                                  float *out, size_t out_stride, float *lse,
-                                                  float *shares, int *status) {
+                                                  float *out, size_t out_stride, float *tops,
+                                                  float *shares, uint32_t *factors,
+                                                  int *status) {
     constexpr int L = D / 4, M = L * G;
     const int s = blockIdx.z, wide = kv.heads * group;
     const size_t e = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -868,12 +895,13 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4 kv, Kv4Rows rows, const fl
     // No key that counts: zeros. Scores that are all -inf: not finite.
     if (mx != -INFINITY) o = make_float4(o.x / total, o.y / total, o.z / total, o.w / total);
     *(float4 *)dst = o;
-    if (shares && d == 0) {
+    if (d == 0 && shares) {
         const float2 x = kv4_share(mx, total);
-        lse[row * wide + qh] = x.x;
+        tops[row * wide + qh] = x.x;
         shares[row * wide + qh] = x.y;
-    } else if (lse && d == 0) {
-        lse[row * wide + qh] = mx == -INFINITY ? INFINITY : mx + __log2f(total);
+    } else if (d == 0 && factors) {
+        uint32_t &factor = factors[tile_at(span, s, (int)i & ~15, qh, wide) + (i & 15)];
+        factor = kv4_factor(mx, total, factor, tops[row * wide + qh]);
     }
     flag_nonfinite(status, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)));
 }
@@ -932,18 +960,13 @@ struct Kv4Run {
     float *part_acc, *part_ml;
     float *out;  // splits = 1: the rows themselves
     size_t out_stride;
-    // With sums: log2 of a row's sum of 2^score, [rows][query heads]; and the last `counted`
-    // rows' queries as operands and their factors, tile by tile (tile_at).
-    float *lse;
+    // With sums: the rows' tops, [rows][query heads]; and the last `counted` rows' queries as
+    // operands and their words (kv4_factor), tile by tile (tile_at).
+    float *tops;
     uint4 *queries;
-    float *factors;
+    uint32_t *factors;
     int counted;
 };
-
-// Where a tile of 16 rows and a query head stand among rows + 16 * streams rows.
-__device__ inline size_t tile_at(const Kv4Span &span, int s, int r0, int qh, int wide) {
-    return (size_t)(span.row0 + 16 * s + r0) * wide + (size_t)qh * 16;
-}
 
 template <int D>
 struct Kv4RunShared {
@@ -979,7 +1002,6 @@ constexpr uint16_t kMostFast = 0x6950;  // 2720
 // Key scales up to 64 are ordinary: a score is less than the query's largest element, 2^15,
 // times 8 * 64 in each dim.
 constexpr uint16_t kOrdinary = 0x5400;
-constexpr float kMostFused = 0x1p23f;  // of scores that are not vast
 struct PairBits {
     uint32_t mask = 0x03C003C0u, one = 0x3C003C00u;
     // In registers: an AND-OR takes no literals.
@@ -1070,7 +1092,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
     const int keys = span.first +
                      min(span.count, (min(bx * 4 + 3, tiles - 1) / a.group + 1) * 16);
     const int c0 = split, stride = a.splits, c1 = (keys + 63) / 64;
-    const int p0 = span.first + r0, p = i < live ? p0 + i : -1;  // this lane's row
+    const int p0 = span.first + r0;
+    int p = i < live ? p0 + i : -1;  // this lane's row
+    asm("" : "+v"(p));  // else p0 + i takes a register of its own throughout
     const int wave_top = p0 + live - 1;
 
     const float *q = a.q + row * a.q_stride + (size_t)qh * D;
@@ -1092,7 +1116,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
             to[k * 128] = __builtin_bit_cast(uint4, qhi[k]);
             to[k * 128 + 64] = __builtin_bit_cast(uint4, qlo[k]);
         }
-        if (g == 0) a.factors[at + i] = qs;
+        if (g == 0) a.factors[at + i] = fbits(qs) & kExponent;
     }
 
     // Chunk c: its bytes requested, then turned into LDS; wave w takes block w. The block's
@@ -1324,11 +1348,19 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int r = 0; r < 4; r++) w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
         } else {
+            const bool vast = fabsf(m) >= kMostFused;
+            if (__any(vast))
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (vast) w[t][r] = w[t][r] * qs - m;
+            const float f = vast ? 1.0f : qs, b = vast ? 14.0f : base;
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    w[t][r] = __builtin_amdgcn_exp2f((w[t][r] * qs - m) + 14.0f);
+                    w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], f, b));
                     l += w[t][r];
                 }
         }
@@ -1430,15 +1462,16 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
         if (g == 0) {
             if (a.splits > 1)
                 *(float2 *)(a.part_ml + at * 2) = make_float2(base, l * 0x1p-14f);
-            else if (a.lse)
-                a.lse[row * wide + qh] = base == -INFINITY ? INFINITY : base + (__log2f(l) - 14.0f);
+            else if (a.factors)
+                a.factors[tile_at(span, s, r0, qh, wide) + i] =
+                    kv4_factor(base, l * 0x1p-14f, fbits(qs), a.tops[row * wide + qh]);
         }
         bad |= !(biggest < INFINITY);
     }
     flag_nonfinite(status, bad);
 }
 
-// What runs of rows weigh, from their scores once more and the rows' log sums: a
+// What runs of rows weigh, from their scores once more and the rows' tops and shares: a
 // work-group of W waves for 64 keys of a (stream, key head), which stand in each wave's
 // registers as fp16; the waves take the tiles of 16 rows that see them in turn. A lane
 // adds up its row's weights of 16 keys over the tiles; lanes and waves are added once.
@@ -1488,7 +1521,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv
     const int from = max(late, c * 64 - span.first) / 16 * 16;
     const int units = (span.count - from + 15) / 16 * a.group;
     f16x8 nexthi[KS], nextlo[KS];
-    float lse = INFINITY, factor = 0.0f;
+    float next_top = INFINITY;
+    uint32_t next_word = 0;
+    // The scores' factors are the scale times powers of two.
+    const uint32_t fraction =
+        a.scale == 0.0f ? 0 : fbits(fabsf(a.scale) < 1.0f ? a.scale * 0x1p64f : a.scale) & ~(kExponent | kVastRow);
     auto request = [&](int u) {
         const int r0 = from + u / a.group * 16, r = r0 + i, qh = head * a.group + u % a.group;
         const size_t at = tile_at(span, s, r0, qh, wide);
@@ -1498,9 +1535,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv
             nexthi[k] = __builtin_bit_cast(f16x8, q[k * 128]);
             nextlo[k] = __builtin_bit_cast(f16x8, q[k * 128 + 64]);
         }
-        factor = a.factors[at + i];
-        lse = a.lse[((size_t)span.row0 + min(r, span.count - 1)) * wide + qh];
-        if (r < late || r >= span.count) lse = INFINITY;
+        next_word = a.factors[at + i];
+        next_top = a.tops[((size_t)span.row0 + min(r, span.count - 1)) * wide + qh];
+        if (r < late || r >= span.count) next_top = INFINITY;
     };
     f32x4 part[4];
 #pragma unroll
@@ -1509,8 +1546,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv
     for (int u = wave; u < units; u += W) {
         const int p0 = span.first + from + u / a.group * 16;
         // Rows that did not come out finite weigh nothing.
-        const bool fine = fabsf(lse) < INFINITY;
-        const float base = fine ? -lse : -INFINITY, qs = factor;
+        const bool fine = fabsf(next_top) < INFINITY;
+        const uint32_t word = next_word;
+        const float base = fine ? -next_top : -INFINITY;
+        float qs = bitsf((word & kExponent) | fraction);
+        float share = bitsf((word & 0x007FFFFFu) | 0x3F000000u);
         f16x8 qhi[KS], qlo[KS];
 #pragma unroll
         for (int k = 0; k < KS; k++) qhi[k] = nexthi[k], qlo[k] = nextlo[k];
@@ -1519,25 +1559,41 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv
 #pragma unroll
             for (int k = 0; k < KS; k++)
                 if (!fine) qhi[k] = qlo[k] = __builtin_bit_cast(f16x8, none);
+            if (!fine) qs = 0.0f;
         }
         if (u + W < units) request(u + W);
         f32x4 w[4];
+        auto multiply = [&] {
 #pragma unroll
-        for (int t = 0; t < 4; t++) w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < 4; t++) w[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
+            for (int k = 0; k < KS; k++) {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t][k], qhi[k], w[t], 0, 0, 0);
+                for (int t = 0; t < 4; t++)
+                    w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t][k], qhi[k], w[t], 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-                w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t][k], qlo[k], w[t], 0, 0, 0);
-        }
+                for (int t = 0; t < 4; t++)
+                    w[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[t][k], qlo[k], w[t], 0, 0, 0);
+            }
+        };
+        multiply();
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], qs, base));
-        if (c * 64 + 63 > p0) {
+        const bool vast = (int)word < 0, any = __any(vast);
+        if (any || c * 64 + 63 > p0) {
+            if (any) {  // once more, rounded as the attention did
+                multiply();
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        w[t][r] = __builtin_amdgcn_exp2f(vast ? w[t][r] * qs + base : fmaf(w[t][r], qs, base));
+                if (vast)
+                    share = ldexpf(bitsf((word << 7 & 0x007FFFFFu) | 0x3F000000u),
+                                   64 - (int)(word >> 16 & 127));
+            }
             const int last = p0 + i - c * 64 - g * 4;
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -1546,7 +1602,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv
                     if (t * 16 + r > last) w[t][r] = 0.0f;
         }
 #pragma unroll
-        for (int t = 0; t < 4; t++) part[t] += w[t];
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) part[t][r] = fmaf(w[t][r], share, part[t][r]);
     }
 #pragma unroll
     for (int t = 0; t < 4; t++)
@@ -2035,8 +2093,8 @@ size_t parts_bytes(const pgpu_kv4 *kv, size_t parts) {
     return parts * (kv->head_dim + 2) * sizeof(float);
 }
 
-// What a run's sums need: the queries as operands, factors and log sums (and room to align
-// what follows).
+// What a run's sums need: the queries as operands, their words and the rows' tops (and room
+// to align what follows).
 size_t run_sums_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group) {
     const size_t wide = (size_t)kv->heads * group;
     return ((r->rows + (size_t)16 * r->streams) * wide * (kv->head_dim + 1) + r->rows * wide + 4) *
@@ -2046,7 +2104,7 @@ size_t run_sums_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group) {
 template <int D>
 int join(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal &d,
          const float *part_acc, const float *part_ml, int group, int max_positions, float *out,
-         size_t out_stride, float *lse, float *shares, int *status) {
+         size_t out_stride, float *tops, float *shares, uint32_t *factors, int *status) {
     // Many splits of few rows: a wave for each, spread over the CUs; else few splits of
     // many rows. us with the attention, 8 heads of 64: 60 rows behind 8000 keys 13.2 / 17.6, 8
     // streams of them behind 4000 24.0 / 25.7, a row behind 8186 9.4 / 9.9; 2000 rows (4
@@ -2055,12 +2113,12 @@ int join(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, const Deal
     if (d.splits >= 8 && items * streams <= 4096)
         hipLaunchKernelGGL((k_kv4_join<D, 256 / D>), dim3((unsigned)items, 1, streams), dim3(64), 0,
                            st, c, r, part_acc, part_ml, group, max_positions, d.splits, d.keys, out,
-                           out_stride, lse, shares, status);
+                           out_stride, tops, shares, factors, status);
     else
         hipLaunchKernelGGL((k_kv4_join<D, 1>),
                            dim3((unsigned)((items * (D / 4) + 255) / 256), 1, streams), dim3(256), 0,
                            st, c, r, part_acc, part_ml, group, max_positions, d.splits, d.keys, out,
-                           out_stride, lse, shares, status);
+                           out_stride, tops, shares, factors, status);
     return launch_ok("pgpu_kv4_attention");
 }
 
@@ -2093,7 +2151,8 @@ int attend_one(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, cons
 #undef KV4_DECODE
     if (!launch_ok("pgpu_kv4_attention")) return 0;
     if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
-                                 a.max_positions, a.out, a.out_stride, a.tops, a.shares, status))
+                                 a.max_positions, a.out, a.out_stride, a.tops, a.shares, nullptr,
+                                 status))
         return 0;
     if (!sums || one.after) return 1;
     one.after = sums->after;
@@ -2109,7 +2168,8 @@ int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, con
                        r, a, status);
     if (!launch_ok("pgpu_kv4_attention")) return 0;
     if (d.splits > 1 && !join<D>(st, c, r, streams, d, a.part_acc, a.part_ml, a.group,
-                                 a.max_positions, a.out, a.out_stride, a.lse, nullptr, status))
+                                 a.max_positions, a.out, a.out_stride, a.tops, nullptr, a.factors,
+                                 status))
         return 0;
     if (!sums) return 1;
     constexpr int W = D == 64 ? 16 : 8;
@@ -2223,10 +2283,10 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
     if (sums) {
         const size_t slots = (rows->rows + (size_t)16 * rows->streams) * wide;
         a.queries = (uint4 *)floats;
-        a.factors = floats + slots * kv->head_dim;
-        a.lse = a.factors + slots;
+        a.factors = (uint32_t *)(floats + slots * kv->head_dim);
+        a.tops = floats + slots * (kv->head_dim + 1);
         a.counted = sums->rows;
-        floats = a.lse + rows->rows * wide;
+        floats = a.tops + rows->rows * wide;
     }
     a.part_acc = floats + (-(uintptr_t)floats / sizeof(float) & 3);
     a.part_ml = a.part_acc + parts * kv->head_dim;

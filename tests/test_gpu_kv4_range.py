@@ -97,7 +97,7 @@ def test_scores_of_any_size(cache, counts, heads, dim, group, large, size, most)
 @pytest.mark.parametrize("most", [None, 8192])
 @pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 18, 1.3e7, 3e8, 1.15e9, 2.0 ** 41, 1e30])
 @pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (2, 64, 3), (1, 128, 2), (1, 128, 8)])
-@pytest.mark.parametrize("counts", [None])
+@pytest.mark.parametrize("counts", [None, [1, 1, 25, 60, 55, 17, 40]], ids=["one", "runs"])
 def test_sums_of_weights_of_scores_of_any_size(cache, counts, heads, dim, group, size, most):
     """The same keys' weights: 1, or one part of as many as weigh the same. Runs hold a row's
     sum of weights to 2^-23, or to 2^-16 where the scores pass 2^23."""
