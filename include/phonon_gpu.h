@@ -671,7 +671,7 @@ typedef struct {
  * a key head, 1..16; q[r * q_stride + h * head_dim]) attends the cache rows 0 ..
  * its own, softmax(scale q k) v, into out[r * out_stride + h * head_dim]. The
  * cache already holds the call's rows. One row a stream, or runs of rows.
- * `max_positions` (less than 2^24 with one row a stream; with runs up to 2^30,
+ * `max_positions` (up to 65535 * 256 with one row a stream; with runs up to 2^30,
  * with their sums less than 2^28 over heads) bounds every cache row's index + 1
  * (a stream past it is left out, status bit 2). A block whose id is outside the
  * cache weighs nothing (status bit 2; a row that is left no key gets zeros). A

@@ -15,6 +15,8 @@ constexpr int kSpan = 64;         // dims of a scale
 constexpr int kPlane = 512;       // bytes of a block's 64 dims, of keys or of values
 constexpr float kLeastScale = 0x1p-17f, kMostScale = 8160.0f;
 constexpr int kMostRows = 1 << 30;  // of a stream: a block past its last is an int32 still
+// With one row a stream: the grid's 65535 splits of the fewest keys that one has.
+constexpr int kMostOne = 65535 * 256;
 
 // One layer of the cache, and the rows of a call (pgpu_kv4, pgpu_kv4_rows).
 struct Kv4 {
@@ -2020,6 +2022,13 @@ extern "C" int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer,
 
 namespace {
 
+// The cache rows that a call can count. A run's sums: the grid's 2^32 threads.
+bool positions_ok(const pgpu_kv4 *kv, const pgpu_kv4_rows *rows, int max_positions, bool sums) {
+    if (!rows->offsets) return max_positions > 0 && max_positions <= kMostOne;
+    return max_positions > 0 && max_positions <= kMostRows &&
+           !(sums && kv->heads * (size_t)((max_positions + 63) / 64) >= (size_t)1 << 22);
+}
+
 // How an attention call deals its work: splits of `keys` keys.
 struct Deal {
     int splits, keys, tiles, waves, steps;  // tiles: work-groups for a stream and head
@@ -2184,8 +2193,8 @@ int attend_rows(hipStream_t st, const Kv4 &c, const Kv4Rows &r, int streams, con
 
 extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_rows *rows,
                                            int group, int max_positions, int with_sums) {
-    if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 || max_positions <= 0 ||
-        max_positions > kMostRows)
+    if (!cache_ok(kv) || !rows_ok(rows) || group < 1 || group > 16 ||
+        !positions_ok(kv, rows, max_positions, with_sums != 0))
         return 0;
     const size_t wide = (size_t)kv->heads * group;
     if (rows->rows == 0) return 0;
@@ -2223,7 +2232,8 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
     if (!cache_ok(kv) || !rows_ok(rows) || layer < 0 || layer >= kv->layers || !q || !out ||
         !status || !aligned(q, 16) || !aligned(out, 16) || q_stride % 4 != 0 ||
         out_stride % 4 != 0 || group < 1 || group > 16 || q_stride < width ||
-        out_stride < width || max_positions <= 0 || max_positions > kMostRows || !__builtin_isfinite(scale * kLog2e) ||
+        out_stride < width || !positions_ok(kv, rows, max_positions, sums != nullptr) ||
+        !__builtin_isfinite(scale * kLog2e) ||
         (sums && (!sums->after || sums->stride < (size_t)max_positions || sums->rows < 1)))
         return bad_arguments("pgpu_kv4_attention");
     if (rows->rows == 0) return 1;
@@ -2234,8 +2244,6 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
     float *floats = (float *)work;
     if (!rows->offsets) {
         const Deal d = deal_of(kv, rows->streams, group, max_positions);
-        // The grid's limit: 16 million positions of one row a stream.
-        if (d.splits > 65535) return bad_arguments("pgpu_kv4_attention");
         const size_t parts = d.splits > 1 ? rows->streams * wide * d.splits : 0;
         const size_t need = parts_bytes(kv, parts) +
                             (sums ? rows->streams * wide * (2 + (size_t)max_positions) * sizeof(float)
@@ -2264,9 +2272,6 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
                                   : attend_one<128>(st, c, r, rows->streams, d, a, sums, status);
     }
     const Deal d = deal_rows(kv, rows, group, max_positions);
-    // The grid's limit: 2^32 threads.
-    if (sums && kv->heads * (size_t)((max_positions + 63) / 64) >= (size_t)1 << 22)
-        return bad_arguments("pgpu_kv4_attention");
     const size_t parts = d.splits > 1 ? rows->streams * rows->max_rows * wide * d.splits : 0;
     const size_t need = parts_bytes(kv, parts) + (sums ? run_sums_bytes(kv, rows, group) : 0);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
