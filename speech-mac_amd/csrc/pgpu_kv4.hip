@@ -2206,7 +2206,7 @@ extern "C" size_t pgpu_kv4_attention_bytes(const pgpu_kv4 *kv, const pgpu_kv4_ro
         const int most = std::min({32, chunks <= 3 ? 1 : chunks,
                                    1024 / (kv->heads * ((group + 3) / 4))});
         if (most > 1)
-            parts = std::min((size_t)1024 * 64, rows->streams * rows->max_rows * wide * most);
+            parts = std::min((size_t)1024 * 64, (size_t)rows->streams * rows->max_rows * wide * most);
         return parts_bytes(kv, parts) + (with_sums ? run_sums_bytes(kv, rows, group) : 0);
     }
     // Fewer streams may be dealt to more work-groups: the streams before the numbers of
@@ -2272,7 +2272,7 @@ extern "C" int pgpu_kv4_attention(void *stream, const pgpu_kv4 *kv, int layer,
                                   : attend_one<128>(st, c, r, rows->streams, d, a, sums, status);
     }
     const Deal d = deal_rows(kv, rows, group, max_positions);
-    const size_t parts = d.splits > 1 ? rows->streams * rows->max_rows * wide * d.splits : 0;
+    const size_t parts = d.splits > 1 ? (size_t)rows->streams * rows->max_rows * wide * d.splits : 0;
     const size_t need = parts_bytes(kv, parts) + (sums ? run_sums_bytes(kv, rows, group) : 0);
     if (need && (!work || !aligned(work, 16) || work_bytes < need))
         return bad_arguments("pgpu_kv4_attention (workspace)");

@@ -59,3 +59,20 @@ def test_runs_with_sums_have_one_bound_of_positions(pkg, heads):
     assert not call(lib, "attention", a, max_positions=most + 1, work_bytes=1 << 62)
     assert b"workspace" not in lib.pgpu_last_error()
     assert b"invalid arguments" in lib.pgpu_last_error()
+
+
+@pytest.mark.parametrize("sums", [0, 1])
+@pytest.mark.parametrize("heads,dim,group", [(1, 64, 1), (8, 64, 2), (256, 128, 16)])
+@pytest.mark.parametrize("streams,max_rows", [(65535, 65535), (65535, 40000), (32768, 65535)])
+def test_the_workspace_of_the_largest_ragged_batches(pkg, streams, max_rows, heads, dim, group, sums):
+    """streams * max_rows past 2^31: parts of 64 rows by 1024 work-groups, or none where the
+    work-groups are always many, and with sums what `rows` rows need."""
+    lib, rows = pkg.load(), 2 ** 31 - 1
+    a = Args(pkg)
+    a.kv.heads, a.kv.head_dim = heads, dim
+    r = pkg.PgpuKv4Rows(a.ptr, 4, a.ptr, a.ptr, streams, rows, max_rows)
+    n = lib.pgpu_kv4_attention_bytes(ctypes.byref(a.kv), ctypes.byref(r), group, 131072, sums)
+    wide = heads * group
+    parts = 1024 * 64 if 1024 // (heads * ((group + 3) // 4)) > 1 else 0
+    kept = sums * ((rows + 16 * streams) * wide * (dim + 1) + rows * wide + 4)
+    assert n == (parts * (dim + 2) + kept) * 4
