@@ -997,6 +997,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
     // acc holds the values' sums times 2^lift. A scale within 2^kNear: below 2^15.
     int lift = 0;
     bool apart = false;  // a scale so far was not
+    bool vast = false;   // a row of the wave has scores past 2^23
 
     auto attend = [&](int buf, int c, bool masked) {
         float2 bs[4];
@@ -1044,7 +1045,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
 #pragma unroll
         for (int t = 0; t < 4; t++) signs |= fbits(bs[t].y);
         apart |= (int)__builtin_amdgcn_readfirstlane(signs) < 0;
-        if (apart || __any(mn != m)) {
+        float less = mn;
+        if (apart || vast || __any(mn != m)) {
+            // Vast scores are rounded as the maximum is: within a multiply-add they could
+            // pass it by half a step of theirs.
+            const bool far = fabsf(mn) >= 0x1p23f && fabsf(mn) < -kNone;
+            vast = __any(far);
             const float shrink = __builtin_amdgcn_exp2f(m - mn);
             l *= shrink;
             float both = shrink;
@@ -1056,14 +1062,14 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
                 for (int t = 0; t < 4; t++) {
                     const float e = (float)(exponent(bs[t].y) + 1);
                     const float best = max3(max3(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
-                    large = max3(large, fmaf(best, f[t], e), large);
+                    large = max3(large, far ? (best * f[t] - mn) + e : fmaf(best, f[t], e), large);
                     if (!masked || t * 16 <= last) seen = fmaxf(seen, e);
                     if (fbits(bs[t].y) == 0x80000000u) {  // no block
                         w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         f[t] = 1.0f;
                     }
                 }
-                large = ceilf(quarters_max(large)) - mn;
+                large = ceilf(quarters_max(large)) - (far ? 0.0f : mn);
                 const float next = fminf(fminf((float)lift + (mn - m), 14.0f - large),
                                          100.0f - quarters_max(seen));
                 both = __builtin_amdgcn_exp2f((m - mn) + (next - (float)lift));
@@ -1074,12 +1080,21 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv8_run(Kv8 kv, Kv8Row
 #pragma unroll
                 for (int r = 0; r < 4; r++) acc[t][r] *= both;
             m = mn;
+            if (vast && far) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) w[t][r] = w[t][r] * f[t] - mn;
+                    f[t] = 1.0f;
+                }
+                less = 0.0f;
+            }
         }
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], f[t], -m));
+                w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], f[t], -less));
         if (masked)
 #pragma unroll
             for (int t = 0; t < 4; t++)
