@@ -1289,62 +1289,71 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (t * 16 + r > last) w[t][r] = -INFINITY;
-        const bool rare = kind != 0 || apart || hot;
+        const bool lifts = (kind & 0x02020202u) != 0 || apart;
         auto shifts = [&](int t, int n) {
             f32x4 z = {0.f, 0.f, 0.f, 0.f};
             if (kind >> (8 * t) & 2) z = *(const f32x4 *)&sh.shift[buf][t][n][g * 4];
             return z;
         };
-        if (rare)
+        float mn;
+        auto look = [&] {
+            float mx[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                mx[t] = largest(largest(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
+            const float least =
+                ceilf(quarters_max(largest(largest(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs);
+            mn = max3(m, least, least);
+        };
+        if (kind == 0 && !apart) {
+            look();
+        } else {
 #pragma unroll
             for (int t = 0; t < 4; t++)
                 if (kind >> (8 * t) & 1) w[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        float mx[4];
+            look();
+            if (lifts) {
+                bool lifted = false;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-            mx[t] = largest(largest(w[t][0], w[t][1], w[t][2]), w[t][3], w[t][3]);
-        const float top = quarters_max(largest(largest(mx[0], mx[1], mx[2]), mx[3], mx[3])) * qs;
-        const float least = ceilf(top), mn = max3(m, least, least);
-        bool grows = mn != m;
-        float lower[N];
+                for (int n = 0; n < N; n++) {
+                    float x = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < N; n++) lower[n] = 1.0f;
-        if (rare) {
-            bool lifted = false;
+                    for (int t = 0; t < 4; t++) {
+                        const f32x4 z = shifts(t, n);
 #pragma unroll
-            for (int n = 0; n < N; n++) {
-                float x = -INFINITY;
+                        for (int r = 0; r < 4; r++) {
+                            const float y = (w[t][r] * qs - mn) + z[r];
+                            x = max3(x, y, y);
+                        }
+                    }
+                    const float old = sh.lift[wave][n][i];
+                    const float lift = fmaxf(old + (m - mn), ceilf(quarters_max(x)));
+                    sh.lift[wave][n][i] = lift;
+                    lifted |= lift != 0.0f;
+                    if (__any(lift != old)) {
+                        const float lower = __builtin_amdgcn_exp2f(old - lift);
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const f32x4 z = shifts(t, n);
+                        for (int t = n * 4; t < n * 4 + 4; t++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float y = (w[t][r] * qs - mn) + z[r];
-                        x = max3(x, y, y);
+                            for (int r = 0; r < 4; r++) acc[t][r] *= lower;
                     }
                 }
-                const float old = sh.lift[wave][n][i];
-                const float lift = fmaxf(old + (m - mn), ceilf(quarters_max(x)));
-                sh.lift[wave][n][i] = lift;
-                lower[n] = __builtin_amdgcn_exp2f(old - lift);
-                grows |= lift != old;
-                lifted |= lift != 0.0f;
+                apart = __any(lifted);
             }
-            apart = __any(lifted);
         }
-        if (__any(grows)) {
+        if (__any(mn != m)) {
             const float shrink = __builtin_amdgcn_exp2f(m - mn);
             l *= shrink;
 #pragma unroll
             for (int t = 0; t < T; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[t][r] *= shrink * lower[t / 4];
+                for (int r = 0; r < 4; r++) acc[t][r] *= shrink;
 #pragma unroll
             for (int r = 0; r < 4; r++) total[r] *= shrink;
             m = mn;
         }
         const float base = 14.0f - m;
-        if (!rare) {
+        if (!(hot || lifts || (kind & 0x04040404u) != 0)) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -1361,15 +1370,17 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], f, b));
-                    l += w[t][r];
-                }
+                for (int r = 0; r < 4; r++) w[t][r] = __builtin_amdgcn_exp2f(fmaf(w[t][r], f, b));
+            if (lifts)
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) l += w[t][r];
         }
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            if (rare) {  // from the last 64 dims' shifts and lift to these
+            if (lifts) {  // from the last 64 dims' shifts and lift to these
                 const float down = sh.lift[wave][n][i] - (n ? sh.lift[wave][n - 1][i] : 0.0f);
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -1379,7 +1390,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
                     for (int r = 0; r < 4; r++) w[t][r] *= __builtin_amdgcn_exp2f(z[r] - down);
                 }
             }
-            if (n == 0 || rare) {
+            if (n == 0 || lifts) {
                 f16x2 hi[4][2], lo[4][2];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -1399,7 +1410,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 #pragma unroll
                 for (int t = 0; t < 4; t++) v[t] = sh.v[buf][z][t0 + t][lane];
                 if (n == 0) {
-                    const int one = rare ? 0 : 0x3C003C00;
+                    const int one = lifts ? 0 : 0x3C003C00;
                     const f16x8 ones = __builtin_bit_cast(f16x8, i32x4{one, one, one, one});
                     total = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[z], total, 0, 0, 0);
                     total = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[z], total, 0, 0, 0);
