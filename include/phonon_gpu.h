@@ -660,7 +660,9 @@ int pgpu_kv4_read(void *stream, const pgpu_kv4 *kv, int layer, const pgpu_kv4_ro
  * The call's own rows are new: they begin from 0. before NULL: all begin from 0;
  * before = after: in place (no other overlap). A stream without rows in the
  * call, or left out, has its `after` left as it is. A row that does not come out
- * finite adds nothing. Summed in fp32, always in the same order. */
+ * finite adds nothing. Summed in fp32, always in the same order. A weight is
+ * relative to its row's sum of weights, to some roundings; in a run's rows whose
+ * scores pass 2^23 (in units of log 2) to 2^-16. */
 typedef struct {
     const float *before; /* (dev) [streams][heads][stride] or NULL */
     float *after;        /* (dev) [streams][heads][stride] */
@@ -681,10 +683,12 @@ typedef struct {
  * of themselves, or 2^-25 of the row's largest element, or of the largest weight
  * times value scale that it sees (of the same 64 dims). One row a stream holds them
  * to 2^-29 of those largest ones; what it multiplies and sums of them is exact
- * within 64 keys and as long as no larger one comes.
+ * within 64 keys and as long as no larger one comes. Scores are fp32 numbers of any
+ * size: keys whose scores are equal weigh the same, and one that passes all others
+ * weighs 1.
  * The same call gives the same bits; how the keys are dealt to work-groups goes
- * by the number of streams, max_rows and max_positions, so that in another batch
- * a stream's last bits may differ.
+ * by the number of streams, max_rows and max_positions (best near the longest
+ * context of the call), so that in another batch a stream's last bits may differ.
  * `work` (dev, 16-byte aligned): pgpu_kv4_attention_bytes(kv, rows, group,
  * max_positions, with_sums) bytes that no other call uses at the same time; they
  * need no clearing. They do for every call of at most these streams, max_rows,

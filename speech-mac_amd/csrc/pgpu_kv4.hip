@@ -432,8 +432,9 @@ __device__ inline int xor16_32_most(int v) {
 //
 // Bound by the cache's bytes where contexts are long: 256 streams of up to 8187 keys, 567
 // MB in 93 us, 6.1 TB/s (a plain read reaches 6.5). Else by the chain of a few steps: 64
-// of up to 2048 10.0 us (34 MB; with the scores stored and added up 12.7), one key 3.7, a
-// launch. Heads of 128 with 4 queries, 48 streams of up to 4096: 105 MB in 24 us.
+// of up to 2048 9.4 us (34 MB; with the scores stored and added up 13.6), one key 3.7, a
+// launch. Heads of 128 with 4 queries, 48 streams of up to 4096: 105 MB in 25 us, 24 where
+// both halves of a head share m. Vast scores: 64 of up to 2048 11.6.
 template <int D, int W, int Q, bool SCORES>
 __global__ __launch_bounds__(64 * W, D == 64 ? 5 : Q == 1 ? 4 : 3) void k_kv4_decode(
     Kv4 kv, Kv4Rows rows, Kv4Decode a, int *status) {
@@ -946,13 +947,15 @@ __global__ __launch_bounds__(256) void k_kv4_sums_one(Kv4 kv, Kv4Rows rows, Kv4D
 // bits to a key that weighs little but whose values are large, nor the other way round.
 // Each 64 dims have a first block's exponent, shifts and a lift of their own.
 //
-// Bound by vector and matrix instructions, which overlap in part: for a tile and 64 keys
+// Bound by vector and matrix instructions, which hardly overlap: for a tile and 64 keys
 // about 800 cycles of a SIMD's vector units (256 of them the exponentials) and 576 of its
-// matrix cores, 1376 one after the other. 8187 rows of one prompt, 8 heads of 64: 183 us,
-// 137 GFLOP with the two terms, 0.75 PFLOP/s (a library product: 1.3). Eight waves that
-// share a block's staging 193; two copies of the loop's body, masked and not, 346 (they
-// spill). 5 prompts of up to 1777 rows and 16 query heads 74 us; 3 of up to 300, behind
-// 200, 13.6: up to 8 chunks, one after the other.
+// matrix cores, 1376 one after the other; it takes about 1750, as waves whose rows are short
+// end early. 8187 rows of one prompt, 8 heads of 64: 189 us, 137 GFLOP with the two terms,
+// 0.73 PFLOP/s (a library product: 1.3); 295 with every second block far, 193 where queries
+// may give vast scores, 227 where keys may. Eight waves that share a block's staging 193 for
+// 182; two copies of the loop's body, masked and not, 346 (they spill). 5 prompts of up to
+// 1777 rows and 16 query heads 70 us; 3 of up to 300, behind 200, 14.0: up to 8 chunks, one
+// after the other.
 struct Kv4Run {
     const float *q;
     size_t q_stride;
@@ -974,8 +977,10 @@ template <int D>
 struct Kv4RunShared {
     f16x8 k[2][4][D / 32][64];  // [buffer][block][step][lane]
     f16x8 v[2][2][D / 16][64];  // [buffer][pair of blocks][16 dims][lane]
-    __align__(16) float shift[2][4][D / kSpan][kBlockPos];  // [buffer][block][64 dims][key], of far blocks
-    uint8_t kind[2][4];         // [buffer][block]: bit 0: not in the cache; bit 1: far; bit 2: of large keys
+    // [buffer][block][64 dims][key], of far blocks
+    __align__(16) float shift[2][4][D / kSpan][kBlockPos];
+    // [buffer][block]: bit 0: not in the cache; bit 1: far; bit 2: of large keys
+    uint8_t kind[2][4];
     float lift[4][D / kSpan][16];  // [wave][64 dims][row]
 };
 
@@ -1489,7 +1494,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void k_kv4_run(Kv4 kv, Kv4Row
 // registers as fp16; the waves take the tiles of 16 rows that see them in turn. A lane
 // adds up its row's weights of 16 keys over the tiles; lanes and waves are added once.
 // Bound by the exponentials and the matrix cores: 5 prompts of up to 1777 rows, 16 query
-// heads of 64, 44 us, 19 GFLOP with the two terms (4 waves that turned the queries into
+// heads of 64, 42 us, 19 GFLOP with the two terms (4 waves that turned the queries into
 // operands themselves: 40 us more).
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 64 ? 4 : 2) void k_kv4_sums(Kv4 kv, Kv4Rows rows, Kv4Run a,
@@ -2049,8 +2054,8 @@ Deal deal_rows(const pgpu_kv4 *kv, const pgpu_kv4_rows *r, int group, int max_po
     // Work-groups without splits. Where they are few, and the keys enough to pay for the
     // join, each row's keys are dealt out in chunks of 64: of 64 work-groups at most to
     // 1024 of them, of more to 4 splits (or 512 work-groups).
-    // us, 8 heads, whole / dealt. Few rows, heads of 64 and of 128: 60 of 1 stream behind 180
-    // keys 9.4 / 9.6, 12.7 / 11.1; behind 320 11.9 / 9.6, 16.5 / 11.4; behind 1000 25.5 / 9.5,
+    // us a pass (9.5 at least with two launches), 8 heads, whole / dealt. Few rows, heads of 64
+    // and of 128: 60 of 1 stream behind 180 keys 9.4 / 9.6, 12.7 / 11.1; behind 320 11.9 / 9.6, 16.5 / 11.4; behind 1000 25.5 / 9.5,
     // 36.3 / 11.9; behind 8000 159 / 13.4, 230 / 19.3; 8 streams behind 4000 83.6 / 25.2, 120 /
     // 39.6; 1 of 300 rows 10.4 / 11.0, 14.3 / 14.7. More: 16 streams of 64 behind 450 15.4 /
     // 18.1, 21.8 / 22.8, behind 700 19.0 / 18.0, 27.2 / 23.1, behind 2000 44.0 / 25.9, 63.7 /
