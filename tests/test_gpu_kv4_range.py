@@ -229,3 +229,53 @@ def test_ordinary_rows_after_large_ones(cache, heads, dim, group):
                             most=most, sums=50)
             assert c.st() == 0
             check_rows(c, a, got, counts is None)
+
+
+@pytest.mark.parametrize("size", [3e6, 3e8, 2e9])
+@pytest.mark.parametrize("heads,dim,group", [(2, 64, 1), (2, 64, 3), (1, 128, 1), (2, 128, 4)])
+@pytest.mark.parametrize("counts", [None, [130, 70, 33, 200, 100]], ids=["one", "runs"])
+def test_scores_that_pass_what_is_counted_and_come_back(cache, counts, heads, dim, group, size):
+    """Keys of three sizes, all of one size the same, in runs along the context: ordinary
+    scores before and behind vast ones, of both signs; some blocks are not in the cache, and
+    values differ by 2^24."""
+    c = cache(5, heads, dim, positions=1100)
+    rng = c.rng
+    lengths = [1100, 900, 1000, 600, 700]
+    kinds = [np.r_[np.zeros(600), np.full(300, 2), np.zeros(200)],          # ordinary, vast, ordinary
+             np.r_[np.full(300, 2), np.zeros(600)],                         # vast first
+             np.arange(1000) // 70 % 3,                                     # in turn
+             np.r_[np.zeros(590), np.full(10, 1)],                          # vast at the end
+             np.r_[np.full(40, 1), np.zeros(400), np.full(260, 2)]]
+    sign = np.where(rng.integers(0, 2, (5, heads, dim)), 1.0, -1.0)
+    large = 1e4
+    k = np.concatenate([np.array([2.0 ** -20, 0.5, 1.0])[x.astype(int)][:, None, None] * sign[s][None] * large
+                        for s, x in enumerate(kinds)])
+    v = rng.standard_normal(k.shape) * np.exp2(rng.integers(-12, 13, (len(k), heads, 1)))
+    c.write([0] * 5, lengths, k.astype(np.float32), np.clip(v, -5e4, 5e4).astype(np.float32))
+    assert c.st() == 0
+    table = c.table.copy()
+    lost = [[], [3, 40], [7], [], [1, 2, 30]]
+    for s, blocks in enumerate(lost):
+        table[s, blocks] = c.blocks + s
+    n = counts or [1] * 5
+    q = rng.uniform(1.0, 2.0, (sum(n), heads * group, dim))
+    q *= np.repeat(np.concatenate([np.repeat(sign[s][None], m, 0) for s, m in enumerate(n)]), group, 1)
+    q *= np.where(np.arange(heads * group) % 2, -1.0, 1.0)[:, None]
+    q *= size / 1.4427 / (dim ** -0.5 * 1.5 * dim * large)
+    for tables, missing in ((c.table, [[]] * 5), (table, lost)):
+        c.tables.upload(tables)
+        a, got = attend(c, q, counts, group, sums=50)
+        assert c.st() == (2 if tables is table else 0)
+        for s, rows, (kk, vv), first in streams_of(c, a):
+            there = np.ones(len(kk), bool)
+            for b in missing[s]:
+                there[b * 16:b * 16 + 16] = False
+            x, _ = bounds.weights(a.q[rows], kk, first, a.scale)
+            x = np.where(there, x, -np.inf)
+            w = np.exp(x - x.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            # Keys of a size weigh the same, to the roundings of a weight.
+            out, off = bounds.output(w, vv, np.zeros((len(w), heads * group, 1)), counts is None)
+            miss = np.abs(got[rows] - out) - off
+            assert (miss <= 0).all(), (s, miss.max())
+            check_sums(c, a, s, w, (w.shape[-1] + 16) * U + (0 if counts is None else 2.0 ** -15))
